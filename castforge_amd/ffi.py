@@ -95,6 +95,20 @@ class GgufProblem(ctypes.Structure):
     ]
 
 
+class Kv4CacheStruct(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", c_void_p),
+        ("k_groups", c_void_p),
+        ("v_codes", c_void_p),
+        ("v_groups", c_void_p),
+        ("num_pages", c_int64),
+        ("kv_heads", c_int64),
+        ("page_size", c_int64),
+        ("head_dim", c_int64),
+        ("group", c_int64),
+    ]
+
+
 _P = c_void_p
 _E = POINTER(c_char_p)
 # name -> (restype, argtypes) for every entry point of the header
@@ -157,6 +171,18 @@ SIGNATURES = {
     "castforge_hip_gguf_q4_0_to_gemv_planes": (c_int32, [_P, _P, c_int64, c_int64, _P, _P, _P, _E]),
     "castforge_hip_gguf_q4_0_from_gemv_planes": (c_int32, [_P, _P, c_int64, c_int64, _P, _P, _P, _E]),
     "castforge_hip_gemv_gguf_q4_0_planes_batched": (c_int32, [POINTER(GgufProblem), c_int32, c_int64, c_int32, _P, _E]),
+    "castforge_hip_rms_norm_fp8": (c_int32, [_P, c_int32, _P, _P, c_int32, ctypes.c_float, c_int64, c_int64, c_int32,
+                                             _P, _P, _P, _P, _E]),
+    "castforge_hip_quantize_fp8_block": (c_int32, [_P, c_int32, c_int64, c_int64, c_int32, _P, _P, _P, _E]),
+    "castforge_hip_dequantize_fp8_block": (c_int32, [_P, _P, c_int64, c_int64, c_int32, _P, _P, _E]),
+    "castforge_hip_gemm_fp8_block": (c_int32, [_P, _P, c_int64, _P, _P, c_int64, c_int64, _P, c_int32, c_int32, _P, _E]),
+    "castforge_hip_kv4_append": (c_int32, [POINTER(Kv4CacheStruct), _P, c_int64, _P, c_int64, c_int64, _P, _P, _P, _P,
+                                           c_int64, c_int64, c_int32, _P, c_int64, c_int64, _P, _P, _E]),
+    "castforge_hip_kv4_gather": (c_int32, [POINTER(Kv4CacheStruct), _P, c_int64, _P, _P, c_int32, _P, _E]),
+    "castforge_hip_kv4_attention": (c_int32, [POINTER(Kv4CacheStruct), _P, c_int64, c_int64, c_int64, c_int64, _P, _P,
+                                              c_int64, _P, c_int32, ctypes.c_float, _P, _P, _P, c_int64, _P, _E]),
+    "castforge_hip_kv4_attention_workspace": (c_int32, [POINTER(Kv4CacheStruct), c_int64, c_int64, c_int64, c_int64,
+                                                        c_int32, POINTER(c_int64), _E]),
 }
 
 _lib = None
