@@ -21,7 +21,9 @@ namespace {
 // f16 bits of a group's scale: 1 for a range of (nearly) nothing, kept above zero and finite.
 __device__ __forceinline__ uint16_t group_scale_bits(float hi, float lo) {
     const float range = hi - lo;
-    uint16_t h = range >= 1e-12f ? f32_to_f16_rne(range * (1.0f / 15.0f)) : static_cast<uint16_t>(0x3C00);
+    float step = range * (1.0f / 15.0f);
+    asm("" : "+v"(step));  // rounded to f32 before f16: one mixed-precision instruction would round once
+    uint16_t h = range >= 1e-12f ? f32_to_f16_rne(step) : static_cast<uint16_t>(0x3C00);
     if (h == 0) h = 0x0001;
     if (h == 0x7C00) h = 0x7BFF;
     return h;

@@ -66,7 +66,8 @@ def _case(seed, tokens, hkv, hq, d, rot, max_pos=300):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("tokens,hkv,hq,d,group,page,rot", [
     (1, 1, 1, 64, 32, 16, 64), (1, 8, 32, 128, 128, 16, 128), (5, 3, 6, 64, 64, 32, 32), (17, 2, 10, 128, 32, 64, 128),
-    (33, 8, 8, 128, 64, 16, 64), (130, 1, 7, 128, 128, 128, 16), (257, 4, 4, 64, 64, 16, 48), (40, 5, 5, 128, 64, 32, 0)])
+    (33, 8, 8, 128, 64, 16, 64), (130, 1, 7, 128, 128, 128, 16), (257, 4, 4, 64, 64, 16, 48), (40, 5, 5, 128, 64, 32, 0),
+    (2048, 32, 1, 128, 32, 64, 128)])
 def test_append_bits(cuda, tokens, hkv, hq, d, group, page, rot, interleaved):
     pages = tokens // page + 3
     cache = _random_cache(1, pages, hkv, page, d, group, cuda)
