@@ -47,6 +47,147 @@ __device__ __forceinline__ float load_elem(const void *p, int bf16, int64_t i) {
     return bf16 ? bf16_to_f32(static_cast<const uint16_t *>(p)[i]) : static_cast<const float *>(p)[i];
 }
 
+// Eight consecutive elements as f32.
+template <bool kBf16>
+struct Piece;
+template <>
+struct Piece<true> {
+    uint4 u;
+    __device__ __forceinline__ void load(const void *p, int64_t i) { u = static_cast<const uint4 *>(p)[i]; }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t b[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(b[i] << 16), v[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u);
+    }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+        u = make_uint4(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]), f32x2_to_bf16x2_rne(v[4], v[5]), f32x2_to_bf16x2_rne(v[6], v[7]));
+    }
+    __device__ __forceinline__ void store(void *p, int64_t i) const { static_cast<uint4 *>(p)[i] = u; }
+};
+template <>
+struct Piece<false> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const void *p, int64_t i) { a = static_cast<const float4 *>(p)[2 * i], b = static_cast<const float4 *>(p)[2 * i + 1]; }
+    __device__ __forceinline__ void get(float (&v)[8]) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
+    __device__ __forceinline__ void set(const float (&v)[8]) { a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]); }
+    __device__ __forceinline__ void store(void *p, int64_t i) const { static_cast<float4 *>(p)[2 * i] = a, static_cast<float4 *>(p)[2 * i + 1] = b; }
+};
+
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+    return m;
+}
+
+__device__ __forceinline__ uint2 codes8(const Quot &quot, const float (&v)[8]) {
+    return make_uint2(e4m3x4(quot(v[0]), quot(v[1]), quot(v[2]), quot(v[3])), e4m3x4(quot(v[4]), quot(v[5]), quot(v[6]), quot(v[7])));
+}
+
+// Maximum over the 16 lanes of a DPP row: what holds a run of 128 at eight elements a lane.
+__device__ __forceinline__ float max16(float v) {
+    v = fmaxf(v, lane_xor<1>(v));
+    v = fmaxf(v, lane_xor<2>(v));
+    v = fmaxf(v, lane_xor<4>(v));
+    return fmaxf(v, lane_xor<8>(v));
+}
+
+// The norm with a row in registers, so that HBM sees each byte once: TPR threads a row (64: four rows a
+// workgroup and no barrier), VPT pieces of eight elements a thread.  Threads past the row's end load its last
+// piece again (an index clamp, not a branch: a load under a divergent branch waits for itself), leave it out
+// of the sum and the maximum (where h is x, its owner may have written it by then) and store nothing.
+// HBM-bound: 7 bytes an element with a bf16 residual.
+template <bool kXBf16, bool kWBf16, int VPT, int TPR>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_fp8_kernel(const void *x, const void *r, const void *__restrict__ w, float eps,
+                                                                             int64_t rows, int cols, int block, void *h, uint8_t *__restrict__ codes,
+                                                                             float *__restrict__ scales) {
+    constexpr int kWaves = TPR / 64;
+    __shared__ float red[2][kWaves];
+    const int t = threadIdx.x % TPR, nv = cols / 8;
+    const int64_t row = TPR == 64 ? blockIdx.x * 4ll + threadIdx.x / 64 : blockIdx.x;
+    if (TPR == 64 && row >= rows) return;  // whole waves, which share nothing
+    const int64_t base = row * nv;
+    const auto over_row = [&](float v, bool sum, int which) {
+        v = sum ? wave_sum<64>(v) : wave_max<64>(v);
+        if constexpr (kWaves > 1) {
+            if ((threadIdx.x & 63) == 0) red[which][threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = red[which][0];
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) v = sum ? v + red[which][i] : fmaxf(v, red[which][i]);
+        }
+        return v;
+    };
+    Piece<kXBf16> px[VPT], pr[VPT];
+    Piece<kWBf16> pw[VPT];
+    static_for<VPT>([&](auto i) __attribute__((always_inline)) { px[i].load(x, base + min(t + i * TPR, nv - 1)); });
+    if (r) static_for<VPT>([&](auto i) __attribute__((always_inline)) { pr[i].load(r, base + min(t + i * TPR, nv - 1)); });
+    static_for<VPT>([&](auto i) __attribute__((always_inline)) { pw[i].load(w, min(t + i * TPR, nv - 1)); });
+    float ss = 0.f;
+    float v[VPT][8];
+    static_for<VPT>([&](auto i) __attribute__((always_inline)) {
+        px[i].get(v[i]);
+        const bool in = t + i * TPR < nv;
+        if (r) {
+            float q[8];
+            pr[i].get(q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] += q[e];
+            px[i].set(v[i]);
+            if (in) px[i].store(h, base + t + i * TPR);
+            px[i].get(v[i]);
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += v[i][e] * v[i][e];
+        ss += in ? s : 0.f;
+    });
+    const float rstd = 1.0f / sqrtf(over_row(ss, true, 0) / static_cast<float>(cols) + eps);
+    float am[VPT], top = 0.f;
+    static_for<VPT>([&](auto i) __attribute__((always_inline)) {
+        float g[8];
+        pw[i].get(g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * rstd * g[e];
+        am[i] = t + i * TPR < nv ? amax8(v[i]) : 0.f;
+        top = fmaxf(top, am[i]);
+    });
+    if (!block) top = over_row(top, false, 1);
+    const int runs = block ? (cols + kRun - 1) / kRun : 1;
+    if (!block && t == 0) scales[row] = scale_of(top);
+    static_for<VPT>([&](auto i) __attribute__((always_inline)) {
+        const int p = t + i * TPR;
+        const float scale = scale_of(block ? max16(am[i]) : top);
+        const Quot quot(scale);
+        const uint2 c = codes8(quot, v[i]);
+        if (p < nv) {
+            reinterpret_cast<uint2 *>(codes)[base + p] = c;
+            if (block && (t & 15) == 0) scales[row * runs + p / 16] = scale;
+        }
+    });
+}
+
+// Runs of 128 of any rows, without the norm: 16 lanes a run, eight elements a lane.  HBM-bound, 3 bytes an
+// element of bf16.
+template <bool kBf16>
+__global__ __launch_bounds__(256) void quant_fp8_run_kernel(const void *__restrict__ src, int64_t tasks, int nv, int runs,
+                                                            uint8_t *__restrict__ codes, float *__restrict__ scales) {
+    const int sub = threadIdx.x & 15;
+    const int64_t stride = gridDim.x * 16ll;
+    for (int64_t task = blockIdx.x * 16ll + (threadIdx.x >> 4); task < tasks; task += stride) {
+        const int64_t row = task / runs;
+        const int p = static_cast<int>(task - row * runs) * 16 + sub;  // piece of the row
+        Piece<kBf16> x;
+        x.load(src, row * nv + min(p, nv - 1));
+        float v[8];
+        x.get(v);
+        const float scale = scale_of(max16(amax8(v)));
+        const uint2 c = codes8(Quot(scale), v);
+        if (p < nv) reinterpret_cast<uint2 *>(codes)[row * nv + p] = c;
+        if (sub == 0) scales[task] = scale;
+    }
+}
+
 // Any row length and alignment: one workgroup a row, three passes over it.
 __global__ __launch_bounds__(256) void rms_norm_fp8_generic_kernel(const void *x, const void *r, int x_bf16,
                                                                    const void *__restrict__ w, int w_bf16, float eps,
@@ -127,6 +268,34 @@ __global__ __launch_bounds__(256) void dequant_fp8_block_kernel(const uint8_t *_
         out[i] = e4m3fn_to_f32(codes[i]) * scales[i / cols / block_rows * runs + i % cols / kRun];
 }
 
+// The register kernel's shape by the row's length; false: the generic kernel.
+template <bool kXBf16, bool kWBf16>
+bool launch_norm(const void *x, const void *r, const void *w, float eps, int64_t rows, int64_t cols, int block, void *h, uint8_t *codes,
+                 float *scales, hipStream_t st) {
+    const auto go = [&](auto vpt, auto tpr) {
+        constexpr int V = decltype(vpt)::value, T = decltype(tpr)::value;
+        const int64_t grid = T == 64 ? (rows + 3) / 4 : rows;
+        rms_norm_fp8_kernel<kXBf16, kWBf16, V, T><<<dim3(static_cast<unsigned>(grid)), dim3(T < 256 ? 256 : T), 0, st>>>(
+            x, r, w, eps, rows, static_cast<int>(cols), block, h, codes, scales);
+        return true;
+    };
+    typedef std::integral_constant<int, 1> one;
+    typedef std::integral_constant<int, 2> two;
+    typedef std::integral_constant<int, 4> four;
+    typedef std::integral_constant<int, 64> wave;
+    typedef std::integral_constant<int, 256> wg;
+    typedef std::integral_constant<int, 1024> big;
+    const int64_t nv = cols / 8;
+    if (nv <= 64) return go(one{}, wave{});
+    if (nv <= 128) return go(two{}, wave{});
+    if (nv <= 256) return go(one{}, wg{});
+    if (nv <= 512) return go(two{}, wg{});
+    if (nv <= 1024) return go(four{}, wg{});
+    if (nv <= 2048) return go(two{}, big{});
+    if (nv <= 4096) return go(four{}, big{});
+    return false;
+}
+
 void check_dtype(int32_t d, const char *what) {
     require(d == CFH_DTYPE_F32 || d == CFH_DTYPE_BF16, std::string(what) + " must be CFH_DTYPE_F32 or CFH_DTYPE_BF16");
 }
@@ -157,8 +326,19 @@ int32_t castforge_hip_rms_norm_fp8(const void *x, int32_t x_dtype, const void *r
         require(x && weight && codes && scales, "buffers must not be NULL");
         require(rows <= 0x7fffffff, "too many rows for one launch");
         hipStream_t st = static_cast<hipStream_t>(stream);
+        const bool xb = x_dtype == CFH_DTYPE_BF16, wb = weight_dtype == CFH_DTYPE_BF16;
+        if (cols % 8 == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(h, 16) && aligned(weight, 16) && aligned(codes, 8)) {
+            const auto go = [&](auto x_bf16, auto w_bf16) {
+                return launch_norm<decltype(x_bf16)::value, decltype(w_bf16)::value>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st);
+            };
+            if (xb ? (wb ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{}))
+                   : (wb ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{}))) {
+                check_launch("rms_norm_fp8");
+                return;
+            }
+        }
         rms_norm_fp8_generic_kernel<<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, st>>>(
-            x, residual, x_dtype == CFH_DTYPE_BF16, weight, weight_dtype == CFH_DTYPE_BF16, eps, cols, block, h, codes, scales);
+            x, residual, xb, weight, wb, eps, cols, block, h, codes, scales);
         check_launch("rms_norm_fp8");
     });
 }
@@ -173,7 +353,18 @@ int32_t castforge_hip_quantize_fp8_block(const void *src, int32_t src_dtype, int
         require(src && codes && scales, "buffers must not be NULL");
         const int64_t blocks = ((rows + block_rows - 1) / block_rows) * ((cols + kRun - 1) / kRun);
         require(blocks <= 0x7fffffff, "too many blocks for one launch");
-        quant_fp8_block_generic_kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        hipStream_t st = static_cast<hipStream_t>(stream);
+        if (block_rows == 1 && cols % 8 == 0 && cols <= 0x7fffff00 && aligned(src, 16) && aligned(codes, 8)) {
+            const int runs = static_cast<int>((cols + kRun - 1) / kRun);
+            const unsigned grid = static_cast<unsigned>(std::min<int64_t>((blocks + 15) / 16, 32 * cu_count()));
+            if (src_dtype == CFH_DTYPE_BF16)
+                quant_fp8_run_kernel<true><<<dim3(grid), dim3(256), 0, st>>>(src, blocks, static_cast<int>(cols / 8), runs, codes, scales);
+            else
+                quant_fp8_run_kernel<false><<<dim3(grid), dim3(256), 0, st>>>(src, blocks, static_cast<int>(cols / 8), runs, codes, scales);
+            check_launch("quant_fp8_block");
+            return;
+        }
+        quant_fp8_block_generic_kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st>>>(
             src, src_dtype == CFH_DTYPE_BF16, rows, cols, block_rows, codes, scales);
         check_launch("quant_fp8_block");
     });
