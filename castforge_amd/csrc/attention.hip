@@ -16,6 +16,13 @@
 namespace cfh {
 namespace {
 
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr float kNoMax = -3.402823466e38f;  // below every score, finite: exp2(-inf - kNoMax) is 0, not NaN
+
 struct AttnArgs {
     const uint16_t *q;
     int64_t q_stride;
@@ -24,59 +31,601 @@ struct AttnArgs {
     const int32_t *table, *kv_lens;
     uint16_t *out;
     float *lse;
+    float *part;  // splits > 1: [tokens * q heads][splits][D + 2], output sums, reference, sum
     float scale;
-    int tokens, batch, heads, ratio, page_shift, table_cols, num_pages, causal;
+    int tokens, batch, heads, ratio, page_shift, table_cols, num_pages, causal, splits;
 };
 
-// One wave a (query, head): the plain order of the formula.
+// A uniform word through the scalar cache: no vector load, whose wait would take in the tile loads before it.
+__device__ __forceinline__ int32_t scalar_load(const int32_t *p, int64_t i) {
+    return ((const __attribute__((address_space(4))) int32_t *)(p))[i];
+}
+
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// Codes as they stand in a word are f16 denormals: pairs 16 bits apart, code times 2^-24, or 2^-20 where it lies 4 bits
+// higher; a zero point held the same way is subtracted from them exactly.  (Subtracting the zero points'
+// share of a sum instead leaves the sum's rounding, in an f16 MFMA about 2^-18 of its largest product, where a
+// heavy token's codes equal its zero point.)
+__device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, a) - __builtin_bit_cast(halfx2, b));
+}
+
+__device__ __forceinline__ halfx8 eight(uint32_t p0, uint32_t p1, uint32_t p2, uint32_t p3) {
+    return __builtin_bit_cast(halfx8, uintx4{p0, p1, p2, p3});
+}
+
+// A word's eight codes without their zero point zz (both halves), in the order 0 4 1 5 2 6 3 7; those of positions
+// 1, 3, 5, 7 are 16 times the others.
+__device__ __forceinline__ halfx8 codes_f16(uint32_t w, uint32_t zz) {
+    const uint32_t v = w >> 8, z16 = zz << 4;
+    return eight(minus(w & 0x000F000Fu, zz), minus(w & 0x00F000F0u, z16), minus(v & 0x000F000Fu, zz), minus(v & 0x00F000F0u, z16));
+}
+
+__device__ __forceinline__ float sum_over_g(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
+__device__ __forceinline__ float max_over_g(float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); }
+
+// One sequence's share of a workgroup.
+struct Seq {
+    int seq, first, n, len, tile;  // first token of its n queries; cached tokens; row tile
+};
+
+// Tokens that a sequence's table holds, kept so far below 2^31 that offsets past a length do not wrap.
+__device__ __forceinline__ int token_cap(const AttnArgs &a) {
+    return static_cast<int>(min(static_cast<int64_t>(a.table_cols) << a.page_shift, int64_t{0x7ffffe00}));
+}
+
+// Splits that share a sequence of len tokens: at least 128 tokens each.
+__device__ __forceinline__ int splits_of(int len, int splits) { return max(1, min(splits, (len + 127) / 128)); }
+
+// Which sequence's row tile a workgroup has: tiles are dealt to the sequences in order, rows_per_tile rows each.
+// The lanes of a wave look at 64 sequences at once.  Returns seq -1 past the last tile.
+__device__ __forceinline__ Seq find_tile(const AttnArgs &a, int tile, int rows_per_tile) {
+    const int lane = threadIdx.x & 63;
+    const int cap = token_cap(a);
+    if (!a.cu_q) {
+        const int per = (a.ratio + rows_per_tile - 1) / rows_per_tile, s = tile / per;
+        if (s >= a.batch) return Seq{-1, 0, 0, 0, 0};
+        return Seq{s, s, 1, a.num_pages > 0 ? min(max(scalar_load(a.kv_lens, s), 0), cap) : 0, tile - s * per};
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int b = b0 + lane;
+        int first = 0, n = 0;
+        if (b < a.batch) {  // clamped: a malformed list stays inside the rows
+            first = min(max(a.cu_q[b], 0), a.tokens);
+            n = min(max(a.cu_q[b + 1], first), a.tokens) - first;
+        }
+        const int tiles = static_cast<int>((static_cast<int64_t>(n) * a.ratio + rows_per_tile - 1) / rows_per_tile);
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint64_t hit = __ballot(before + upto > tile);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            Seq s;
+            s.seq = b0 + l;
+            s.first = __builtin_amdgcn_readlane(first, l);
+            s.n = __builtin_amdgcn_readlane(n, l);
+            s.tile = tile - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l));
+            s.len = a.num_pages > 0 ? min(max(scalar_load(a.kv_lens, s.seq), 0), cap) : 0;
+            return s;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return Seq{-1, 0, 0, 0, 0};
+}
+
+// Registers of 32 tokens' keys and values of a head, in halves of 16.  n = lane % 16, g = lane / 16.
 template <int D, int G>
-__global__ __launch_bounds__(64) void kv4_attention_simple_kernel(AttnArgs a) {
-    constexpr int E = D / 64;  // channels a lane
-    const int lane = threadIdx.x, hq = a.heads * a.ratio;
-    const int token = blockIdx.x / hq, head = blockIdx.x % hq, kvh = head / a.ratio;
-    int seq = token, first = token, last = token + 1;
+struct KvTile {
+    static constexpr int GR = D / G, W = G / 32;
+    uint32_t kc[2][GR][W];  // token n: words g W .. of each group
+    uint32_t kz[2][GR];      // token n: its group words, for the zero points
+    uint32_t km[2][4 * GR];  // tokens 4 g .. 4 g + 3: theirs, for the scales
+    uint32_t vc[2][4][GR];  // tokens 4 g + r: word n % (G / 8) of each group
+    uint32_t vm[2][4 * GR];
+    bool live[2];           // uniform: the half's page is one of the cache's
+};
+
+template <int D, int G>
+__device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, int head, const int (&page)[2], int at, int end) {
+    constexpr int GR = D / G, W = G / 32, kWords = D / 8;
+    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        t.live[h] = at + 16 * h < end && page[h] >= 0 && page[h] < a.num_pages;
+        const int64_t row = kv4_row(t.live[h] ? page[h] : 0, head, (at + 16 * h) & ((1 << a.page_shift) - 1), a.heads, a.page_shift);
+        const uint32_t *kc = a.k_codes + row * kWords + n * kWords + g * W, *vc = a.v_codes + row * kWords + 4 * g * kWords + n % (G / 8);
+        const uint32_t *kz = a.k_groups + row * GR + n * GR;
+        const uint4 *km = reinterpret_cast<const uint4 *>(a.k_groups + row * GR) + g * GR, *vm = reinterpret_cast<const uint4 *>(a.v_groups + row * GR) + g * GR;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            if constexpr (W == 4) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(kc + gr * (G / 8));
+                t.kc[h][gr][0] = v.x, t.kc[h][gr][1] = v.y, t.kc[h][gr][2] = v.z, t.kc[h][gr][3] = v.w;
+            } else if constexpr (W == 2) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(kc + gr * (G / 8));
+                t.kc[h][gr][0] = v.x, t.kc[h][gr][1] = v.y;
+            } else {
+                t.kc[h][gr][0] = kc[gr * (G / 8)];
+            }
+            t.kz[h][gr] = kz[gr];
+            const uint4 k4 = km[gr], v4 = vm[gr];
+            t.km[h][4 * gr] = k4.x, t.km[h][4 * gr + 1] = k4.y, t.km[h][4 * gr + 2] = k4.z, t.km[h][4 * gr + 3] = k4.w;
+            t.vm[h][4 * gr] = v4.x, t.vm[h][4 * gr + 1] = v4.y, t.vm[h][4 * gr + 2] = v4.z, t.vm[h][4 * gr + 3] = v4.w;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t.vc[h][r][gr] = vc[r * kWords + gr * (G / 8)];
+        }
+    }
+}
+
+// Rows of a wave: 16 MT of the n * ratio (query, head of the group) pairs of a sequence and a head of keys, row = query *
+// ratio + head; the MFMAs' columns.  With S^T = K Q^T a lane holds the scores of one row and four tokens a
+// half, which is the layout that O^T = V^T P^T takes its second operand in: the weights stay in registers.
+template <int D, int G, int MT>
+struct Rows {
+    static constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = 8 / R;  // NT output tiles of 16 channels a group
+    halfx8 q[MT][GR][W];     // the row times a power of two, 2^14 / unit: in the order and by the factors of codes_f16
+    float unit[MT];
+    int limit[MT];           // tokens that the lane's row sees
+    floatx4 o[MT][GR][NT];   // sum of weight * (code - zero point), by code position times 2^-24 or 2^-20
+    float m[MT], l[MT];      // reference and this lane's part of the sum
+};
+
+template <int D, int G, int MT>
+__device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, const Seq &sq, int head, int row0) {
+    constexpr int GR = D / G, W = G / 32;
+    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int row = row0 + 16 * mt + n, i = row / a.ratio;
+        const bool in = i < sq.n;
+        // rows past the sequence's see all: they are not stored, and do not make a tile an edge
+        s.limit[mt] = in ? (a.causal ? min(sq.len, sq.len - sq.n + i + 1) : sq.len) : 0x7fffffff;
+        const uint16_t *p = a.q + (sq.first + (in ? i : 0)) * a.q_stride + (head * a.ratio + (in ? row - i * a.ratio : 0)) * D;
+        float x[GR][W][8], top = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int u = 0; u < W; ++u) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(p + gr * G + (g * W + u) * 8);
+                const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[gr][u][e] = __uint_as_float(e % 2 ? b[e / 2] & 0xffff0000u : b[e / 2] << 16);
+                    top = fmaxf(top, fabsf(x[gr][u][e]));
+                }
+            }
+        // the largest element below 2^14, so that a sixteenth of it keeps bf16's bits down to 2^-24 of the largest
+        const int ex = __builtin_amdgcn_frexp_expf(max_over_g(top)) - 14;
+        s.unit[mt] = __builtin_ldexpf(1.0f, ex);
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+#pragma unroll
+            for (int u = 0; u < W; ++u) {
+                const auto at = [&](int e) { return static_cast<_Float16>(__builtin_ldexpf(x[gr][u][e], -ex - (e % 2 ? 4 : 0))); };
+                s.q[mt][gr][u] = halfx8{at(0), at(4), at(1), at(5), at(2), at(6), at(3), at(7)};
+            }
+#pragma unroll
+            for (int t = 0; t < Rows<D, G, MT>::NT; ++t) s.o[mt][gr][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+        s.m[mt] = kNoMax, s.l[mt] = 0.f;
+    }
+}
+
+// 32 tokens at `at`.  A token's weight is held with the exponent of its values' scale: with s_t = c_t 2^e_t (the largest
+// of its groups', c in [0.5, 1)), exp2(score + e_t - m) times c rounds to f16 as what the token adds to the output, whatever
+// the scales are; the sum takes the 2^-e_t back.  m is 7 below the largest so far when it moves, and it moves only
+// when something exceeds it by 15: weights stay below 2^15, the largest ones above 2^7 (f16 keeps its 11 bits
+// down to 2^-21 of them), and the rescaling is rare.
+template <int D, int G, int MT>
+__device__ __forceinline__ void attend(const AttnArgs &a, const KvTile<D, G> &t, Rows<D, G, MT> &s, int at, int len, int sure, float qk) {
+    constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = 8 / R;
+    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const bool edge = at + 32 > sure || !t.live[0] || !t.live[1];  // uniform: some row does not see some token
+    float y[MT][2][4];            // scores and their tokens' exponents, base 2
+    float c[2][4][GR], back[2][4];  // the scale of the values without its exponent, 2^-exponent
+    uint32_t zp[2][2][GR];        // zero points as f16 denormals, pairs of tokens
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t km[4 * GR], vm[4 * GR];
+#pragma unroll
+        for (int i = 0; i < 4 * GR; ++i) {
+            km[i] = t.km[h][i], vm[i] = t.vm[h][i];
+            // places past the length or of no page may hold anything
+            if (edge && (!t.live[h] || at + 16 * h + 4 * g + i / GR >= len)) km[i] = vm[i] = 0;
+        }
+        float ks[4][GR], e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float v[GR], top = 0.f;
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) {
+                ks[r][gr] = kv4_scale(km[r * GR + gr]) * qk;
+                v[gr] = kv4_scale(vm[r * GR + gr]);
+                top = fmaxf(top, v[gr]);
+            }
+            const int ex = __builtin_amdgcn_frexp_expf(top);
+            e[r] = static_cast<float>(ex);
+            back[h][r] = __builtin_ldexpf(1.0f, -ex);
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) c[h][r][gr] = __builtin_ldexpf(v[gr], -ex);
+        }
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) zp[h][p][gr] = high_halves(vm[2 * p * GR + gr], vm[(2 * p + 1) * GR + gr]) & 0x000F000Fu;
+
+        floatx4 dot[MT][GR];
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            const uint32_t zz = high_halves(t.kz[h][gr], t.kz[h][gr]) & 0x000F000Fu;
+#pragma unroll
+            for (int u = 0; u < W; ++u) {
+                const halfx8 k = codes_f16(t.kc[h][gr][u], zz);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+                    dot[mt][gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, s.q[mt][gr][u], u ? dot[mt][gr] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = dot[mt][0][r] * ks[r][0];
+#pragma unroll
+                for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[r][gr], v);
+                v = __builtin_fmaf(v, s.unit[mt], e[r]);
+                if (edge && (!t.live[h] || at + 16 * h + 4 * g + r >= s.limit[mt])) v = -INFINITY;
+                y[mt][h][r] = v;
+            }
+    }
+    uint32_t p[MT][GR][4];  // weights times c as f16 pairs: tokens (0, 1), (2, 3) of both halves
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        float top = y[mt][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, y[mt][i / 4][i % 4]);
+        if (__any(top > s.m[mt] + 15.f)) {
+            const float m = fmaxf(s.m[mt], max_over_g(top) - 7.f), f = __builtin_amdgcn_exp2f(s.m[mt] - m);
+            s.m[mt] = m;
+            s.l[mt] *= f;
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+                for (int u = 0; u < NT; ++u) s.o[mt][gr][u] *= f;
+        }
+        float w[2][4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            w[i / 4][i % 4] = __builtin_amdgcn_exp2f(y[mt][i / 4][i % 4] - s.m[mt]);
+            s.l[mt] = __builtin_fmaf(w[i / 4][i % 4], back[i / 4][i % 4], s.l[mt]);
+        }
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int h = i / 2, r = i % 2 * 2;
+                const halfx2 v = {static_cast<_Float16>(w[h][r] * c[h][r][gr]), static_cast<_Float16>(w[h][r + 1] * c[h][r + 1][gr])};
+                p[mt][gr][i] = __builtin_bit_cast(uint32_t, v);
+            }
+    }
+#pragma unroll
+    for (int gr = 0; gr < GR; ++gr) {
+        halfx8 pw[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) pw[mt] = eight(p[mt][gr][0], p[mt][gr][1], p[mt][gr][2], p[mt][gr][3]);
+        // a row of V^T is word n % (G / 8), codes from n / (G / 8) on in steps of R
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int h = i / 2, r = i % 2 * 2, sh = R == 1 ? 0 : 4 * (n / (G / 8));
+            lo[i] = low_halves(t.vc[h][r][gr] >> sh, t.vc[h][r + 1][gr] >> sh);
+            hi[i] = high_halves(t.vc[h][r][gr] >> sh, t.vc[h][r + 1][gr] >> sh);
+        }
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const int code = R * u;  // position in the (shifted) word
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t x = code < 4 ? lo[i] : hi[i];
+                const uint32_t y = code % 4 < 2 ? x : x >> 8, z = zp[i / 2][i % 2][gr];
+                v[i] = code % 2 == 0 ? minus(y & 0x000F000Fu, z) : minus(y & 0x00F000F0u, z << 4);
+            }
+            const halfx8 vv = eight(v[0], v[1], v[2], v[3]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s.o[mt][gr][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pw[mt], s.o[mt][gr][u], 0, 0, 0);
+        }
+    }
+}
+
+// Row tile's walk over tokens first, first + step, .. (of 32) below end, the next tile's loads in flight.
+template <int D, int G, int MT>
+__device__ __forceinline__ void walk(const AttnArgs &a, Rows<D, G, MT> &s, const Seq &sq, int head, int first, int step, int end) {
+    if (first >= end) return;
+    int sure = sq.len;  // tokens that every row sees
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) sure = min(sure, s.limit[mt]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sure = min(sure, __shfl_xor(sure, o));
+    sure = __builtin_amdgcn_readfirstlane(sure);
+    const float qk = a.scale * (1.44269504088896341f * 0x1p24f);  // the codes' 2^-24 undone
+    const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
+    const auto pages = [&](int at, int (&p)[2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) p[h] = at + 16 * h < end ? scalar_load(table, (at + 16 * h) >> a.page_shift) : -1;
+    };
+    KvTile<D, G> cur;
+    int page[2];
+    pages(first, page);
+    load_tile<D, G>(a, cur, head, page, first, end);
+    pages(first + step, page);
+    for (int at = first; at < end; at += step) {
+        KvTile<D, G> next;
+        if (at + step < end) {
+            load_tile<D, G>(a, next, head, page, at + step, end);
+            pages(at + 2 * step, page);
+        } else {
+            next = cur;
+        }
+        attend<D, G, MT>(a, cur, s, at, sq.len, sure, qk);
+        cur = next;
+    }
+}
+
+// Channel of element (r of a lane's four, group gr, tile u) of O^T.
+template <int G>
+__device__ __forceinline__ int channel(int g, int r, int gr, int u) {
+    constexpr int R = 128 / G;
+    const int n = 4 * g + r;
+    return gr * G + 8 * (n % (G / 8)) + R * u + n / (G / 8);
+}
+
+// The whole sum, and the outputs without the codes' factors.
+template <int D, int G, int MT>
+__device__ __forceinline__ void settle(Rows<D, G, MT> &s) {
+    typedef Rows<D, G, MT> S;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        s.l[mt] = sum_over_g(s.l[mt]);
+#pragma unroll
+        for (int gr = 0; gr < S::GR; ++gr)
+#pragma unroll
+            for (int u = 0; u < S::NT; ++u) s.o[mt][gr][u] *= (S::R * u) % 2 ? 0x1p20f : 0x1p24f;
+    }
+}
+
+// One workgroup's four waves take the same rows and every fourth 32 tokens of a split's share, and are joined through
+// LDS; splits are joined by kv4_attention_join_kernel.  For few rows a sequence: bound by the cache's bytes.
+template <int D, int G, int MT>
+__global__ __launch_bounds__(256) void kv4_attention_split_kernel(AttnArgs a) {
+    typedef Rows<D, G, MT> S;
+    constexpr int kRow = D + 4;
+    __shared__ __align__(16) float sums[4][16][kRow];
+    __shared__ float ml[2][4][16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits % a.heads;
+    const Seq sq = find_tile(a, blockIdx.x / a.splits / a.heads, 16 * MT);
+    if (sq.seq < 0) return;
+    const int row0 = sq.tile * 16 * MT;
+    // the last row of the tile sees the most
+    const int rows = min(16 * MT, sq.n * a.ratio - row0);
+    const int seen = a.causal ? max(0, min(sq.len, sq.len - sq.n + (row0 + rows - 1) / a.ratio + 1)) : sq.len;
+    const int used = splits_of(sq.len, a.splits);
+    if (split >= used) return;
+    const int share = (sq.len / used + 128) / 128 * 128;  // used * share >= len; whole rounds of the four waves
+    const int first = split * share, end = min(seen, first + share);
+    S s;
+    load_rows<D, G, MT>(a, s, sq, head, row0);
+    walk<D, G, MT>(a, s, sq, head, first + 32 * wave, 128, end);
+    settle<D, G, MT>(s);
+    const int hq = a.heads * a.ratio;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        if (16 * mt >= rows) break;
+        __syncthreads();
+        if (g == 0) ml[0][wave][n] = s.m[mt], ml[1][wave][n] = s.l[mt];
+        __syncthreads();
+        const float m = fmaxf(fmaxf(ml[0][0][n], ml[0][1][n]), fmaxf(ml[0][2][n], ml[0][3][n]));
+        const float f = __builtin_amdgcn_exp2f(s.m[mt] - m);
+#pragma unroll
+        for (int gr = 0; gr < S::GR; ++gr)
+#pragma unroll
+            for (int u = 0; u < S::NT; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sums[wave][n][channel<G>(g, r, gr, u)] = s.o[mt][gr][u][r] * f;
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * (D / 8); i += 256) {
+            const int rl = i / (D / 8), ch = i % (D / 8) * 8, row = row0 + 16 * mt + rl;
+            if (row >= sq.n * a.ratio) continue;
+            const int64_t at = static_cast<int64_t>(sq.first + row / a.ratio) * hq + head * a.ratio + row % a.ratio;
+            const float mm = fmaxf(fmaxf(ml[0][0][rl], ml[0][1][rl]), fmaxf(ml[0][2][rl], ml[0][3][rl]));
+            float l = 0.f, v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                l = __builtin_fmaf(ml[1][w][rl], __builtin_amdgcn_exp2f(ml[0][w][rl] - mm), l);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += sums[w][rl][ch + e];
+            }
+            if (a.splits > 1) {
+                float *p = a.part + (at * a.splits + split) * (D + 4);
+                *reinterpret_cast<float4 *>(p + ch) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4 *>(p + ch + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                if (ch == 0) p[D] = mm, p[D + 1] = l;
+            } else {
+                const float inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
+                uint4 o;
+                o.x = f32x2_to_bf16x2_rne(v[0] * inv, v[1] * inv), o.y = f32x2_to_bf16x2_rne(v[2] * inv, v[3] * inv);
+                o.z = f32x2_to_bf16x2_rne(v[4] * inv, v[5] * inv), o.w = f32x2_to_bf16x2_rne(v[6] * inv, v[7] * inv);
+                *reinterpret_cast<uint4 *>(a.out + at * D + ch) = o;
+                if (a.lse && ch == 0) a.lse[at] = l == 0.f ? -INFINITY : (mm + log2f(l)) * 0.693147180559945309f;
+            }
+        }
+    }
+}
+
+// The splits of a row: a workgroup a (token, query head), D / 8 lanes of eight channels by 2048 / D lanes of splits.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
+    constexpr int kCh = D / 8, kSp = 256 / kCh;
+    __shared__ __align__(16) float sums[kSp][D + 4];
+    __shared__ float red[4], ls[kSp];
+    const int hq = a.heads * a.ratio, token = blockIdx.x / hq;
+    const int64_t at = blockIdx.x;
+    int seq = token;
     if (a.cu_q) {
         seq = -1;
-        for (int b = 0; b < a.batch; ++b) {
-            const int s0 = a.cu_q[b], s1 = a.cu_q[b + 1];
-            if (token >= s0 && token < s1) {
-                seq = b, first = s0, last = s1;
-                break;
-            }
+        for (int b0 = 0; b0 < a.batch && seq < 0; b0 += 64) {
+            const int b = b0 + (threadIdx.x & 63);
+            const uint64_t hit = __ballot(b < a.batch && a.cu_q[min(b, a.batch)] <= token && token < a.cu_q[min(b, a.batch - 1) + 1]);
+            if (hit) seq = b0 + __builtin_ctzll(hit);
         }
         if (seq < 0) return;
     }
-    const int len = min(max(a.kv_lens[seq], 0), a.table_cols << a.page_shift);
-    const int seen = a.causal ? min(len, len - (last - first) + (token - first) + 1) : len;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
+    const int cap = token_cap(a);
+    const int used = splits_of(a.num_pages > 0 ? min(max(a.kv_lens[seq], 0), cap) : 0, a.splits);
+    const float *part = a.part + at * a.splits * (D + 4);
+    float m = kNoMax;
+    for (int s = threadIdx.x; s < used; s += 256) m = fmaxf(m, part[static_cast<int64_t>(s) * (D + 4) + D]);
+    m = wave_max<64>(m);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const int ch = threadIdx.x % kCh * 8, sl = threadIdx.x / kCh;
+    float l = 0.f, v[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = bf16_to_f32(a.q[token * a.q_stride + head * D + E * lane + e]) * a.scale;
-        o[e] = 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (int s = sl; s < used; s += kSp) {
+        const float *p = part + static_cast<int64_t>(s) * (D + 4);
+        const float f = __builtin_amdgcn_exp2f(p[D] - m);
+        const float4 x = *reinterpret_cast<const float4 *>(p + ch), y = *reinterpret_cast<const float4 *>(p + ch + 4);
+        l = __builtin_fmaf(p[D + 1], f, l);
+        v[0] = __builtin_fmaf(x.x, f, v[0]), v[1] = __builtin_fmaf(x.y, f, v[1]), v[2] = __builtin_fmaf(x.z, f, v[2]), v[3] = __builtin_fmaf(x.w, f, v[3]);
+        v[4] = __builtin_fmaf(y.x, f, v[4]), v[5] = __builtin_fmaf(y.y, f, v[5]), v[6] = __builtin_fmaf(y.z, f, v[6]), v[7] = __builtin_fmaf(y.w, f, v[7]);
     }
-    for (int t = 0; t < seen; ++t) {
-        const int page = a.table[static_cast<int64_t>(seq) * a.table_cols + (t >> a.page_shift)];
-        if (page < 0 || page >= a.num_pages) continue;
-        const int64_t row = kv4_row(page, kvh, t & ((1 << a.page_shift) - 1), a.heads, a.page_shift);
-        const int at = E * lane;
-        const auto value = [&](const uint32_t *codes, const uint32_t *groups, int e) {
-            const uint32_t w = codes[row * (D / 8) + at / 8], g = groups[row * (D / G) + at / G];
-            return static_cast<float>(static_cast<int>((w >> (4 * ((at + e) % 8))) & 15u) - static_cast<int>(kv4_zero(g))) * kv4_scale(g);
-        };
-        float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += q[e] * value(a.k_codes, a.k_groups, e);
-        s = wave_sum<64>(s);
-        const float mn = fmaxf(m, s), f = __expf(m - mn), p = __expf(s - mn);
-        l = l * f + p;
+    for (int e = 0; e < 8; ++e) sums[sl][ch + e] = v[e];
+    if (ch == 0) ls[sl] = l;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float t = 0.f, o = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + p * value(a.v_codes, a.v_groups, e);
-        m = mn;
+        for (int i = 0; i < kSp; ++i) t += ls[i], o += sums[i][threadIdx.x];
+        a.out[at * D + threadIdx.x] = f32_to_bf16_rne(t == 0.f ? 0.f : o / t);
+        if (a.lse && threadIdx.x == 0) a.lse[at] = t == 0.f ? -INFINITY : (m + log2f(t)) * 0.693147180559945309f;
     }
-    const int64_t at = (static_cast<int64_t>(token) * hq + head) * D + E * lane;
+}
+
+// Each wave takes rows of its own and all the tokens that they see.  For many rows: bound by the softmax's and the codes' VALU
+// work.  Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row
+// tiles from the last, which see the most tokens.
+template <int D, int G, int MT>
+__global__ __launch_bounds__(256) void kv4_attention_rows_kernel(AttnArgs a, int tiles) {
+    typedef Rows<D, G, MT> S;
+    constexpr int kRow = D + 4;
+    __shared__ __align__(16) float sums[4][16][kRow];
+    __shared__ float ls[4][2][16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const int head = blockIdx.x % a.heads;
+    const Seq sq = find_tile(a, tiles - 1 - blockIdx.x / a.heads, 64 * MT);
+    if (sq.seq < 0) return;
+    const int row0 = sq.tile * 64 * MT + wave * 16 * MT, total = sq.n * a.ratio;
+    if (row0 >= total) return;  // no barrier below
+    const int rows = min(16 * MT, total - row0);
+    const int seen = a.causal ? max(0, min(sq.len, sq.len - sq.n + (row0 + rows - 1) / a.ratio + 1)) : sq.len;
+    S s;
+    load_rows<D, G, MT>(a, s, sq, head, row0);
+    walk<D, G, MT>(a, s, sq, head, 0, 32, seen);
+    settle<D, G, MT>(s);
+    const int hq = a.heads * a.ratio;
 #pragma unroll
-    for (int e = 0; e < E; ++e) a.out[at + e] = f32_to_bf16_rne(m > -INFINITY ? o[e] / l : 0.f);
-    if (a.lse && lane == 0) a.lse[static_cast<int64_t>(token) * hq + head] = m > -INFINITY ? m + logf(l) : -INFINITY;
+    for (int mt = 0; mt < MT; ++mt) {
+        if (16 * mt >= rows) break;
+        // a wave's own part of LDS, in order within the wave
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int gr = 0; gr < S::GR; ++gr)
+#pragma unroll
+            for (int u = 0; u < S::NT; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sums[wave][n][channel<G>(g, r, gr, u)] = s.o[mt][gr][u][r];
+        if (g == 0) ls[wave][0][n] = s.m[mt], ls[wave][1][n] = s.l[mt];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = lane; i < 16 * (D / 8); i += 64) {
+            const int rl = i / (D / 8), ch = i % (D / 8) * 8, row = row0 + 16 * mt + rl;
+            if (row >= total) continue;
+            const int64_t at = static_cast<int64_t>(sq.first + row / a.ratio) * hq + head * a.ratio + row % a.ratio;
+            const float l = ls[wave][1][rl], inv = l == 0.f ? 0.f : 1.0f / l;
+            const float *v = &sums[wave][rl][ch];
+            uint4 o;
+            o.x = f32x2_to_bf16x2_rne(v[0] * inv, v[1] * inv), o.y = f32x2_to_bf16x2_rne(v[2] * inv, v[3] * inv);
+            o.z = f32x2_to_bf16x2_rne(v[4] * inv, v[5] * inv), o.w = f32x2_to_bf16x2_rne(v[6] * inv, v[7] * inv);
+            *reinterpret_cast<uint4 *>(a.out + at * D + ch) = o;
+            if (a.lse && ch == 0) a.lse[at] = l == 0.f ? -INFINITY : (ls[wave][0][rl] + log2f(l)) * 0.693147180559945309f;
+        }
+    }
+}
+
+// How a call is laid out: rows a wave (16 mt), whether waves share rows (splits of the tokens) or have their own, row
+// tiles at most, splits.
+struct Plan {
+    int mt;
+    bool rows;
+    int64_t tiles, splits, bytes;
+};
+
+Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols, bool varlen) {
+    Plan p{1, false, 0, 1, 0};
+    if (tokens == 0 || batch == 0) return p;
+    const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio;
+    const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
+    // enough row tiles of 32 for two waves a SIMD: every wave its own rows
+    p.rows = varlen && rows / 32 * c->kv_heads >= 4 * cus;
+    if (p.rows) {
+        p.mt = 2;
+        p.tiles = tiles(64 * p.mt);
+        return p;
+    }
+    const int64_t each = (rows + batch - 1) / batch;
+    p.mt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
+    p.tiles = tiles(16 * p.mt);
+    const int64_t tasks = p.tiles * c->kv_heads, len = table_cols * c->page_size;
+    p.splits = std::max<int64_t>(1, std::min((8 * cus + tasks - 1) / tasks, (len + 127) / 128));
+    const int64_t row = (c->head_dim + 4) * 4;
+    p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
+    if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
+    return p;
+}
+
+template <int D, int G, int MT>
+void launch_split(const AttnArgs &a, const Plan &p, hipStream_t st) {
+    const int64_t grid = p.tiles * a.heads * p.splits;
+    require(grid <= 0x7fffffff, "too many workgroups for one launch");
+    kv4_attention_split_kernel<D, G, MT><<<dim3(static_cast<unsigned>(grid)), dim3(256), 0, st>>>(a);
+    check_launch("kv4_attention_split");
+    if (p.splits > 1) {
+        kv4_attention_join_kernel<D><<<dim3(static_cast<unsigned>(a.tokens * a.heads * a.ratio)), dim3(256), 0, st>>>(a);
+        check_launch("kv4_attention_join");
+    }
+}
+
+void check_counts(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols) {
+    require(tokens >= 0 && tokens <= 0x7fffffff && batch >= 0 && batch <= 0x7fffffff, "tokens and batch must be in [0, 2^31)");
+    require(q_heads >= 1 && q_heads % c->kv_heads == 0 && q_heads / c->kv_heads <= 64,
+            "q_heads must be a multiple of kv_heads, at most 64 of them a head of keys");
+    require(table_cols >= 0 && table_cols <= 0x7fffffff / c->page_size, "a sequence must be shorter than 2^31 tokens");
+    require(tokens * q_heads <= 0x7fffffff, "tokens * q_heads must be below 2^31");
 }
 
 }  // namespace
@@ -92,6 +641,8 @@ int32_t castforge_hip_kv4_attention_workspace(const cfh_kv4_cache_t *cache, int6
     return guarded(out_error, [&] {
         check_kv4(cache);
         require(out_bytes != nullptr, "out_bytes must not be NULL");
+        check_counts(cache, tokens, q_heads, batch, table_cols);
+        *out_bytes = plan_of(cache, tokens, q_heads, batch, table_cols, varlen != 0).bytes;
     });
 }
 
@@ -101,10 +652,7 @@ int32_t castforge_hip_kv4_attention(const cfh_kv4_cache_t *cache, const uint16_t
                                     float *lse, void *workspace, int64_t workspace_bytes, void *stream, char **out_error) {
     return guarded(out_error, [&] {
         check_kv4(cache);
-        require(tokens >= 0 && tokens <= 0x7fffffff && batch >= 0 && batch <= 0x7fffffff, "tokens and batch must be in [0, 2^31)");
-        require(q_heads >= 1 && q_heads % cache->kv_heads == 0 && q_heads / cache->kv_heads <= 64,
-                "q_heads must be a multiple of kv_heads, at most 64 of them a head of keys");
-        require(table_cols >= 0 && table_cols <= 0x7fffffff / cache->page_size, "a sequence must be shorter than 2^31 tokens");
+        check_counts(cache, tokens, q_heads, batch, table_cols);
         require(causal == 0 || causal == 1, "causal must be 0 or 1");
         require(cu_q != nullptr || tokens == batch, "without cu_q every sequence has one query: tokens must equal batch");
         if (tokens == 0) return;
@@ -112,15 +660,25 @@ int32_t castforge_hip_kv4_attention(const cfh_kv4_cache_t *cache, const uint16_t
         require(aligned(q, 16) && aligned(out, 16), "q and out must be 16-byte aligned");
         require(tokens <= 1 || (q_stride >= q_heads * cache->head_dim && q_stride % 8 == 0),
                 "q's token stride must be a multiple of 8 and at least q_heads * head_dim");
+        if (batch == 0) return;
+        const Plan p = plan_of(cache, tokens, q_heads, batch, table_cols, cu_q != nullptr);
+        require(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 16)),
+                "workspace must be 16-byte aligned and hold the bytes that castforge_hip_kv4_attention_workspace gives");
         AttnArgs a{q, q_stride, cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups, cu_q, page_table, kv_lens, out, lse,
-                   scale, static_cast<int>(tokens), static_cast<int>(batch), static_cast<int>(cache->kv_heads),
-                   static_cast<int>(q_heads / cache->kv_heads), log2_of(cache->page_size), static_cast<int>(table_cols),
-                   static_cast<int>(cache->num_pages), causal};
-        require(tokens * q_heads <= 0x7fffffff, "too many queries for one launch");
-        kv4_by_shape(cache, [&](auto d, auto g) {
-            kv4_attention_simple_kernel<decltype(d)::value, decltype(g)::value><<<dim3(static_cast<unsigned>(tokens * q_heads)), dim3(64), 0, static_cast<hipStream_t>(stream)>>>(a);
+                   static_cast<float *>(workspace), scale, static_cast<int>(tokens), static_cast<int>(batch),
+                   static_cast<int>(cache->kv_heads), static_cast<int>(q_heads / cache->kv_heads), log2_of(cache->page_size),
+                   static_cast<int>(table_cols), static_cast<int>(cache->num_pages), causal, static_cast<int>(p.splits)};
+        hipStream_t st = static_cast<hipStream_t>(stream);
+        kv4_by_shape(cache, [&](auto d, auto gr) {
+            constexpr int D = decltype(d)::value, G = decltype(gr)::value;
+            if (p.rows) {
+                require(p.tiles * a.heads <= 0x7fffffff, "too many workgroups for one launch");
+                kv4_attention_rows_kernel<D, G, 2><<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(256), 0, st>>>(a, static_cast<int>(p.tiles));
+                check_launch("kv4_attention_rows");
+            } else if (p.mt == 1) launch_split<D, G, 1>(a, p, st);
+            else if (p.mt == 2) launch_split<D, G, 2>(a, p, st);
+            else launch_split<D, G, 4>(a, p, st);
         });
-        check_launch("kv4_attention");
     });
 }
 
