@@ -5,6 +5,7 @@ streams; every computation happens in libcastforge_hip.so.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from dataclasses import dataclass
@@ -877,18 +878,26 @@ def matmul_f32(a: torch.Tensor, b: torch.Tensor, packed_rhs: bool = False) -> to
 
 
 # ------------------------------------- a decoder layer around its products: norm, FP8 ----
+# These calls run many times a token, on inputs that take a few microseconds: each checks its arguments in one
+# expression and looks for what was wrong only when that fails.
+_FLOAT_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+
+
 def _float_code(t: torch.Tensor, what: str) -> int:
-    if t.dtype == torch.float32:
-        return DTYPE_F32
-    if t.dtype == torch.bfloat16:
-        return DTYPE_BF16
-    raise ValueError(f"{what} must be float32 or bfloat16")
+    code = _FLOAT_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32 or bfloat16")
+    return code
 
 
-def _same_device(ref: torch.Tensor, *ts: torch.Tensor | None) -> None:
-    for t in ts:
-        if t is not None and t.get_device() != ref.get_device():
-            raise ValueError(f"all tensors must be on {ref.device}")
+def _refuse(ref: torch.Tensor, tensors: dict[str, torch.Tensor | None], message: str):
+    """Raises: a tensor that is not on ref's device or not contiguous if there is one, else `message`."""
+    for what, t in tensors.items():
+        if t is not None:
+            _dev(t)
+            if t.get_device() != ref.get_device():
+                raise ValueError(f"{what} must be on {ref.device}")
+    raise ValueError(message)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -902,63 +911,57 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     x and residual [M, K] and weight [K] are float32 or bfloat16 (x and residual of one type).  Returns
     (codes u8 [M, K], scales f32, h); h is x itself without a residual, and goes to `out` if given (x or
     residual may be passed to update the stream in place)."""
-    x, weight = _dev(x), _dev(weight)
-    if x.dim() != 2 or weight.dim() != 1 or weight.shape[0] != x.shape[1]:
-        raise ValueError("x must be [M, K] and weight [K]")
+    dev, shape = x.get_device(), x.shape
+    if not (dev >= 0 and len(shape) == 2 and x.is_contiguous() and weight.is_contiguous() and weight.get_device() == dev
+            and weight.shape == shape[1:]):
+        _refuse(x, {"x": x, "weight": weight}, "x must be [M, K] and weight [K]")
     xt, wt = _float_code(x, "x"), _float_code(weight, "weight")
     if block not in (0, 128):
         raise ValueError("block must be 0 (a scale per row) or 128")
-    m, k = x.shape
-    h = x
+    m, k = shape
+    h, hp, rp = x, None, None
     if residual is not None:
-        residual = _dev(residual)
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError("residual must have x's shape and dtype")
-        h = torch.empty_like(x) if out is None else _dev(out)
-        if h.shape != x.shape or h.dtype != x.dtype:
-            raise ValueError("out must have x's shape and dtype")
+        h = torch.empty_like(x) if out is None else out
+        if not (residual.shape == shape and residual.dtype == x.dtype and residual.is_contiguous() and residual.get_device() == dev
+                and h.shape == shape and h.dtype == x.dtype and h.is_contiguous() and h.get_device() == dev):
+            _refuse(x, {"residual": residual, "out": h}, "residual and out must have x's shape and dtype")
+        hp, rp = h.data_ptr(), residual.data_ptr()
     elif out is not None:
         raise ValueError("out takes the sum with the residual; there is none")
-    _same_device(x, weight, residual, h)
-    codes = torch.empty((m, k), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((m, (k + 127) // 128) if block else (m,), dtype=torch.float32, device=x.device)
-    ffi.call("castforge_hip_rms_norm_fp8", _ptr(x), xt, _ptr(residual), _ptr(weight), wt, eps, m, k, block,
-             None if residual is None else _ptr(h), _ptr(codes), _ptr(scales), _stream(x))
+    codes = torch.empty_like(x, dtype=torch.uint8)
+    scales = x.new_empty((m, (k + 127) // 128) if block else (m,), dtype=torch.float32)
+    ffi.call("castforge_hip_rms_norm_fp8", x.data_ptr(), xt, rp, weight.data_ptr(), wt, eps, m, k, block, hp, codes.data_ptr(),
+             scales.data_ptr(), _stream(x))
     return codes, scales, h
 
 
 def quantize_fp8_block(v: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
     """E4M3FN with scale absmax * (1 / 448) per block of block_rows x 128 (1: activations, 128: weights); v is float32
     or bfloat16 [R, C].  Returns (codes u8 [R, C], scales f32 [ceil(R / block_rows), ceil(C / 128)])."""
-    v = _dev(v)
-    if v.dim() != 2:
-        raise ValueError("quantize_fp8_block takes a 2-D [rows, cols] tensor")
+    shape = v.shape
+    if not (v.is_cuda and len(shape) == 2 and v.is_contiguous()):
+        _refuse(v, {"v": v}, "quantize_fp8_block takes a 2-D [rows, cols] tensor")
     if block_rows not in (1, 128):
         raise ValueError("block_rows must be 1 or 128")
     dt = _float_code(v, "v")
-    r, c = v.shape
-    codes = torch.empty((r, c), dtype=torch.uint8, device=v.device)
-    scales = torch.empty(((r + block_rows - 1) // block_rows, (c + 127) // 128), dtype=torch.float32, device=v.device)
-    ffi.call("castforge_hip_quantize_fp8_block", _ptr(v), dt, r, c, block_rows, _ptr(codes), _ptr(scales), _stream(v))
+    r, c = shape
+    codes = torch.empty_like(v, dtype=torch.uint8)
+    scales = v.new_empty(((r + block_rows - 1) // block_rows, (c + 127) // 128), dtype=torch.float32)
+    ffi.call("castforge_hip_quantize_fp8_block", v.data_ptr(), dt, r, c, block_rows, codes.data_ptr(), scales.data_ptr(), _stream(v))
     return codes, scales
 
 
-def _check_block_scales(codes: torch.Tensor, scales: torch.Tensor, block_rows: int, what: str) -> None:
-    r, c = codes.shape
-    want = ((r + block_rows - 1) // block_rows, (c + 127) // 128)
-    if scales.dtype != torch.float32 or tuple(scales.shape) != want:
-        raise ValueError(f"{what} must be float32 {list(want)}")
-
-
 def dequantize_fp8_block(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> torch.Tensor:
-    codes, scales = _dev(codes), _dev(scales)
-    if codes.dim() != 2 or codes.dtype != torch.uint8:
-        raise ValueError("codes must be uint8 [rows, cols]")
     if block_rows not in (1, 128):
         raise ValueError("block_rows must be 1 or 128")
-    _check_block_scales(codes, scales, block_rows, "scales")
-    _same_device(codes, scales)
+    dev = codes.get_device()
+    if codes.dim() != 2 or codes.dtype != torch.uint8:
+        raise ValueError("codes must be uint8 [rows, cols]")
     r, c = codes.shape
+    want = ((r + block_rows - 1) // block_rows, (c + 127) // 128)
+    if not (dev >= 0 and codes.is_contiguous() and scales.is_contiguous() and scales.get_device() == dev
+            and scales.dtype == torch.float32 and scales.shape == want):
+        _refuse(codes, {"codes": codes, "scales": scales}, f"scales must be float32 {list(want)}")
     out = torch.empty((r, c), dtype=torch.float32, device=codes.device)
     ffi.call("castforge_hip_dequantize_fp8_block", _ptr(codes), _ptr(scales), r, c, block_rows, _ptr(out), _stream(codes))
     return out
@@ -975,17 +978,22 @@ def gemm_fp8_block(qa: torch.Tensor, sa: torch.Tensor, qw: torch.Tensor, sw: tor
     (its sums start anew every 128 columns, so the error stays near 1e-4 of a result's size: less than a
     bfloat16 output's rounding); exact=True widens the codes to f16 and runs f16 MFMA, with products exact and
     sums in f32, at about half the rate."""
-    qa, sa, qw, sw = _dev(qa), _dev(sa), _dev(qw), _dev(sw)
-    if qa.dim() != 2 or qw.dim() != 2 or qa.shape[1] != qw.shape[1] or qa.dtype != torch.uint8 or qw.dtype != torch.uint8:
-        raise ValueError("qa [M, K] and qw [N, K] must be uint8 E4M3 codes with the same K")
-    _check_block_scales(qa, sa, 1, "sa")
-    _check_block_scales(qw, sw, 128, "sw")
-    (m, k), n = qa.shape, qw.shape[0]
-    if out is not None and (tuple(out.shape) != (m, n) or not out.is_contiguous()):
-        raise ValueError(f"out must be a contiguous [{m}, {n}] tensor on {qa.device}")
-    y = out if out is not None else torch.empty((m, n), dtype=out_dtype, device=qa.device)
-    _same_device(qa, sa, qw, sw, y)
-    ffi.call("castforge_hip_gemm_fp8_block", _ptr(qa), _ptr(sa), m, _ptr(qw), _ptr(sw), n, k, _ptr(y),
+    ashape, wshape, dev = qa.shape, qw.shape, qa.get_device()
+    if not (dev >= 0 and len(ashape) == 2 and len(wshape) == 2 and ashape[1] == wshape[1] and qa.dtype == torch.uint8
+            and qw.dtype == torch.uint8 and qa.is_contiguous() and qw.is_contiguous() and qw.get_device() == dev):
+        _refuse(qa, {"qa": qa, "qw": qw}, "qa [M, K] and qw [N, K] must be uint8 E4M3 codes with the same K")
+    (m, k), n = ashape, wshape[0]
+    runs = (k + 127) // 128
+    if not (sa.shape == (m, runs) and sw.shape == ((n + 127) // 128, runs) and sa.dtype == torch.float32 and sw.dtype == torch.float32
+            and sa.is_contiguous() and sw.is_contiguous() and sa.get_device() == dev and sw.get_device() == dev):
+        _refuse(qa, {"sa": sa, "sw": sw}, f"sa must be float32 {[m, runs]} and sw float32 {[(n + 127) // 128, runs]}")
+    if out is None:
+        y = qa.new_empty((m, n), dtype=out_dtype)
+    else:
+        y = out
+        if not (y.shape == (m, n) and y.is_contiguous() and y.get_device() == dev):
+            raise ValueError(f"out must be a contiguous [{m}, {n}] tensor on {qa.device}")
+    ffi.call("castforge_hip_gemm_fp8_block", qa.data_ptr(), sa.data_ptr(), m, qw.data_ptr(), sw.data_ptr(), n, k, y.data_ptr(),
              _out_dtype(y.dtype), int(exact), _stream(qa))
     return y
 
@@ -1006,19 +1014,20 @@ class Kv4Cache:
     group: int = 128
 
     def __post_init__(self):
-        kc = _dev(self.k_codes)
-        if kc.dim() != 4 or kc.dtype != torch.int32:
-            raise ValueError("k_codes must be int32 [pages, kv_heads, page_size, head_dim / 8]")
-        pages, heads, page, words = kc.shape
-        if self.group not in (32, 64, 128) or words not in (8, 16) or self.group > 8 * words:
-            raise ValueError("head_dim must be 64 or 128 and group 32, 64 or 128, at most head_dim")
-        for t, w, what in ((self.v_codes, words, "v_codes"), (self.k_groups, 8 * words // self.group, "k_groups"),
-                           (self.v_groups, 8 * words // self.group, "v_groups")):
-            if _dev(t).dtype != torch.int32 or t.shape != (pages, heads, page, w):
-                raise ValueError(f"{what} must be int32 {[pages, heads, page, w]}")
-        _same_device(kc, self.k_groups, self.v_codes, self.v_groups)
-        self._struct = ffi.Kv4CacheStruct(_ptr(kc), _ptr(self.k_groups), _ptr(self.v_codes), _ptr(self.v_groups), pages,
-                                          heads, page, 8 * words, self.group)
+        kc, kg, vc, vg, group = self.k_codes, self.k_groups, self.v_codes, self.v_groups, self.group
+        shape, dev, i32 = kc.shape, kc.get_device(), torch.int32
+        if len(shape) != 4 or shape[3] not in (8, 16) or group not in (32, 64, 128) or group > 8 * shape[3]:
+            raise ValueError("codes must be [pages, kv_heads, page_size, head_dim / 8], head_dim 64 or 128, and group 32, 64 or "
+                             "128, at most head_dim")
+        pages, heads, page, words = shape
+        gshape = (pages, heads, page, 8 * words // group)
+        if not (dev >= 0 and vc.shape == shape and kg.shape == gshape and vg.shape == gshape and kc.dtype == i32 and kg.dtype == i32
+                and vc.dtype == i32 and vg.dtype == i32 and kc.is_contiguous() and kg.is_contiguous() and vc.is_contiguous()
+                and vg.is_contiguous() and kg.get_device() == dev and vc.get_device() == dev and vg.get_device() == dev):
+            _refuse(kc, {"k_codes": kc, "k_groups": kg, "v_codes": vc, "v_groups": vg},
+                    f"codes must be int32 {list(shape)} and groups int32 {list(gshape)}")
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim, self._dev = pages, heads, page, 8 * words, dev
+        self._struct = ffi.Kv4CacheStruct(kc.data_ptr(), kg.data_ptr(), vc.data_ptr(), vg.data_ptr(), pages, heads, page, 8 * words, group)
         self._ref = ctypes.byref(self._struct)
 
     @classmethod
@@ -1029,44 +1038,25 @@ class Kv4Cache:
         z = [torch.zeros(shape + (w,), dtype=torch.int32, device=device) for w in (head_dim // 8, head_dim // group) * 2]
         return cls(*z, group=group)
 
-    @property
-    def num_pages(self) -> int:
-        return self._struct.num_pages
-
-    @property
-    def kv_heads(self) -> int:
-        return self._struct.kv_heads
-
-    @property
-    def page_size(self) -> int:
-        return self._struct.page_size
-
-    @property
-    def head_dim(self) -> int:
-        return self._struct.head_dim
-
     def nbytes(self) -> int:
         return 4 * sum(t.numel() for t in (self.k_codes, self.k_groups, self.v_codes, self.v_groups))
 
+    def _rows(self, t: torch.Tensor, heads: int | None, what: str) -> int:
+        """Checks bf16 [T, heads, head_dim] rows, contiguous but for the token stride, which is returned."""
+        shape, stride, d = t.shape, t.stride(), self.head_dim
+        if not (t.get_device() == self._dev and t.dtype == torch.bfloat16 and len(shape) == 3 and shape[2] == d
+                and (heads is None or shape[1] == heads) and stride[2] == 1 and (stride[1] == d or shape[1] <= 1)):
+            if not t.is_cuda:
+                raise ValueError("castforge_amd kernels take device tensors (HIP); got a CPU tensor")
+            raise ValueError(f"{what} must be bfloat16 [tokens, {'heads' if heads is None else heads}, {d}] on {self.k_codes.device}, "
+                             "contiguous within a token")
+        return stride[0]
 
-def _heads(t: torch.Tensor, heads: int | None, cache: Kv4Cache, what: str) -> torch.Tensor:
-    """Checks bf16 [T, heads, head_dim] rows on the cache's device, contiguous but for the token stride."""
-    if not t.is_cuda:
-        raise ValueError("castforge_amd kernels take device tensors (HIP); got a CPU tensor")
-    d = cache.head_dim
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != d or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what} must be bfloat16 [tokens, {'heads' if heads is None else heads}, {d}]")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d):
-        raise ValueError(f"{what} must be contiguous within a token")
-    _same_device(cache.k_codes, t)
-    return t
-
-
-def _vector(t: torch.Tensor, dtype: torch.dtype, n: int, cache: Kv4Cache, what: str) -> torch.Tensor:
-    if _dev(t).dtype != dtype or t.shape != (n,):
-        raise ValueError(f"{what} must be {str(dtype).removeprefix('torch.')} [{n}]")
-    _same_device(cache.k_codes, t)
-    return t
+    def _vector(self, t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> int:
+        """Checks a contiguous [n] of dtype and returns its address."""
+        if not (t.get_device() == self._dev and t.dtype == dtype and t.shape == (n,) and t.is_contiguous()):
+            _refuse(self.k_codes, {what: t}, f"{what} must be {str(dtype).removeprefix('torch.')} [{n}]")
+        return t.data_ptr()
 
 
 def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -1080,30 +1070,30 @@ def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
 
     Rows may be slices of one projection's output: only the token stride is free (a multiple of 8).  Two
     tokens of a call must not share a slot."""
-    _heads(k, cache.kv_heads, cache, "k")
-    _heads(v, cache.kv_heads, cache, "v")
-    n = k.shape[0]
+    ks, vs, n = cache._rows(k, cache.kv_heads, "k"), cache._rows(v, cache.kv_heads, "v"), k.shape[0]
     if v.shape[0] != n:
         raise ValueError("k and v must have the same tokens")
-    _vector(slots, torch.int64, n, cache, "slots")
+    sp = cache._vector(slots, torch.int64, n, "slots")
     rot = max_pos = 0
+    pp = cp = ip = qp = op = None
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             raise ValueError("positions, cos and sin go together")
-        _vector(positions, torch.int64, n, cache, "positions")
-        if _dev(cos).dtype != torch.float32 or _dev(sin).dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape:
-            raise ValueError("cos and sin must be float32 [max_pos, rot / 2]")
-        _same_device(k, cos, sin)
-        max_pos, rot = cos.shape[0], 2 * cos.shape[1]
-    q_out = None
+        pp = cache._vector(positions, torch.int64, n, "positions")
+        shape, dev = cos.shape, cache._dev
+        if not (len(shape) == 2 and sin.shape == shape and cos.dtype == torch.float32 and sin.dtype == torch.float32
+                and cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == dev and sin.get_device() == dev):
+            _refuse(k, {"cos": cos, "sin": sin}, "cos and sin must be float32 [max_pos, rot / 2]")
+        max_pos, rot, cp, ip = shape[0], 2 * shape[1], cos.data_ptr(), sin.data_ptr()
+    q_out, qs, hq = None, 0, 0
     if q is not None:
-        _heads(q, None, cache, "q")
-        if q.shape[0] != n:
+        qs, qshape = cache._rows(q, None, "q"), q.shape
+        if qshape[0] != n:
             raise ValueError("q and k must have the same tokens")
-        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    ffi.call("castforge_hip_kv4_append", cache._ref, _ptr(k), k.stride(0), _ptr(v), v.stride(0), n, _ptr(slots), _ptr(positions),
-             _ptr(cos), _ptr(sin), max_pos, rot, int(interleaved), _ptr(q), 0 if q is None else q.stride(0),
-             0 if q is None else q.shape[1], _ptr(q_out), _stream(k))
+        q_out, hq = q.new_empty(qshape), qshape[1]
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    ffi.call("castforge_hip_kv4_append", cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, n, sp, pp, cp, ip, max_pos, rot,
+             int(interleaved), qp, qs, hq, op, _stream(k))
     return q_out
 
 
@@ -1112,11 +1102,21 @@ def kv4_gather(cache: Kv4Cache, slots: torch.Tensor, out_dtype: torch.dtype = to
     """The keys and values that `slots` (int64 [T]) hold, [T, kv_heads, head_dim] each, rounded once to out_dtype
     (float32: exact); a slot outside the cache gives zeros."""
     n = slots.shape[0] if slots.dim() == 1 else -1
-    _vector(slots, torch.int64, n, cache, "slots")
-    k = torch.empty((n, cache.kv_heads, cache.head_dim), dtype=out_dtype, device=slots.device)
+    sp = cache._vector(slots, torch.int64, n, "slots")
+    k = slots.new_empty((n, cache.kv_heads, cache.head_dim), dtype=out_dtype)
     v = torch.empty_like(k)
-    ffi.call("castforge_hip_kv4_gather", cache._ref, _ptr(slots), n, _ptr(k), _ptr(v), _out_dtype(out_dtype), _stream(slots))
+    ffi.call("castforge_hip_kv4_gather", cache._ref, sp, n, k.data_ptr(), v.data_ptr(), _out_dtype(out_dtype), _stream(slots))
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv4_workspace(device: int, kv_heads: int, page_size: int, head_dim: int, tokens: int, q_heads: int, batch: int, cols: int,
+                   varlen: int) -> int:
+    """castforge_hip_kv4_attention_workspace's bytes, which depend on sizes alone."""
+    size = ctypes.c_int64()
+    shape = ffi.Kv4CacheStruct(None, None, None, None, 0, kv_heads, page_size, head_dim, 32)
+    ffi.call("castforge_hip_kv4_attention_workspace", ctypes.byref(shape), tokens, q_heads, batch, cols, varlen, ctypes.byref(size))
+    return size.value
 
 
 def kv4_attention(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -1128,25 +1128,23 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, kv
     sequence has one.  causal: query i of n sees the tokens up to kv_lens - n + i.  scale defaults to
     head_dim ** -0.5.  Queries that see nothing give zeros.  Returns bf16 [T, q_heads, head_dim], and with
     return_lse the f32 [T, q_heads] logarithms of the sums of exp(scores)."""
-    _heads(q, None, cache, "q")
-    t, hq, d = q.shape
-    if hq % cache.kv_heads:
+    qs = cache._rows(q, None, "q")
+    t, hq, d = shape = q.shape
+    heads, dev = cache.kv_heads, cache._dev
+    if hq % heads:
         raise ValueError("q_heads must be a multiple of the cache's heads")
-    if _dev(page_table).dtype != torch.int32 or page_table.dim() != 2:
-        raise ValueError("page_table must be int32 [sequences, pages]")
+    if not (page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous() and page_table.get_device() == dev):
+        _refuse(q, {"page_table": page_table}, "page_table must be int32 [sequences, pages]")
     b, cols = page_table.shape
-    _vector(kv_lens, torch.int32, b, cache, "kv_lens")
+    lp, cp = cache._vector(kv_lens, torch.int32, b, "kv_lens"), None
     if cu_q is not None:
-        _vector(cu_q, torch.int32, b + 1, cache, "cu_q")
+        cp = cache._vector(cu_q, torch.int32, b + 1, "cu_q")
     elif t != b:
         raise ValueError("without cu_q every sequence has one query: q and page_table must have the same rows")
-    _same_device(q, page_table)
-    out = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty((t, hq), dtype=torch.float32, device=q.device) if return_lse else None
-    size = ctypes.c_int64()
-    ffi.call("castforge_hip_kv4_attention_workspace", cache._ref, t, hq, b, cols, int(cu_q is not None), ctypes.byref(size))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=q.device) if size.value else None
-    ffi.call("castforge_hip_kv4_attention", cache._ref, _ptr(q), q.stride(0), t, hq, b, _ptr(cu_q), _ptr(page_table), cols,
-             _ptr(kv_lens), int(causal), d ** -0.5 if scale is None else scale, _ptr(out), _ptr(lse), _ptr(ws), size.value,
-             _stream(q))
+    out = q.new_empty(shape)
+    lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
+    size = _kv4_workspace(dev, heads, cache.page_size, d, t, hq, b, cols, 0 if cp is None else 1)
+    ws = q.new_empty((size,), dtype=torch.uint8) if size else None  # held until the call returns
+    ffi.call("castforge_hip_kv4_attention", cache._ref, q.data_ptr(), qs, t, hq, b, cp, page_table.data_ptr(), cols, lp, int(causal),
+             d ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse), _ptr(ws), size, _stream(q))
     return (out, lse) if return_lse else out
