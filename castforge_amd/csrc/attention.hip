@@ -125,24 +125,31 @@ template <int D, int G>
 struct KvTile {
     static constexpr int GR = D / G, W = G / 32;
     uint32_t kc[2][GR][W];  // token n: words g W .. of each group
-    uint32_t kz[2][GR];      // token n: its group words, for the zero points
-    uint32_t km[2][4 * GR];  // tokens 4 g .. 4 g + 3: theirs, for the scales
     uint32_t vc[2][4][GR];  // tokens 4 g + r: word n % (G / 8) of each group
-    uint32_t vm[2][4 * GR];
+    uint32_t words[GR];     // group words of one token: lanes 0 .. 31 of the keys, 32 .. 63 of the values
     bool live[2];           // uniform: the half's page is one of the cache's
+};
+
+// What a wave makes of the group words of 32 tokens, once, each lane for one token's keys or values: in LDS, where
+// the lanes that need a token's numbers read them four tokens at a time.
+template <int GR>
+struct TokenTable {
+    float scale[2][GR][32];    // keys: scale times what turns a product into a score; values: scale without its exponent
+    float exponent[32], back[32];  // of the values' largest scale, 2^-exponent
+    uint32_t kz[GR][32];       // zero point in both halves, as f16 denormals
+    uint16_t vz[GR][32];
 };
 
 template <int D, int G>
 __device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, int head, const int (&page)[2], int at, int end) {
     constexpr int GR = D / G, W = G / 32, kWords = D / 8;
-    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    int64_t rows[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         t.live[h] = at + 16 * h < end && page[h] >= 0 && page[h] < a.num_pages;
-        const int64_t row = kv4_row(t.live[h] ? page[h] : 0, head, (at + 16 * h) & ((1 << a.page_shift) - 1), a.heads, a.page_shift);
-        const uint32_t *kc = a.k_codes + row * kWords + n * kWords + g * W, *vc = a.v_codes + row * kWords + 4 * g * kWords + n % (G / 8);
-        const uint32_t *kz = a.k_groups + row * GR + n * GR;
-        const uint4 *km = reinterpret_cast<const uint4 *>(a.k_groups + row * GR) + g * GR, *vm = reinterpret_cast<const uint4 *>(a.v_groups + row * GR) + g * GR;
+        rows[h] = kv4_row(t.live[h] ? page[h] : 0, head, (at + 16 * h) & ((1 << a.page_shift) - 1), a.heads, a.page_shift);
+        const uint32_t *kc = a.k_codes + rows[h] * kWords + n * kWords + g * W, *vc = a.v_codes + rows[h] * kWords + 4 * g * kWords + n % (G / 8);
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
             if constexpr (W == 4) {
@@ -154,14 +161,51 @@ __device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, in
             } else {
                 t.kc[h][gr][0] = kc[gr * (G / 8)];
             }
-            t.kz[h][gr] = kz[gr];
-            const uint4 k4 = km[gr], v4 = vm[gr];
-            t.km[h][4 * gr] = k4.x, t.km[h][4 * gr + 1] = k4.y, t.km[h][4 * gr + 2] = k4.z, t.km[h][4 * gr + 3] = k4.w;
-            t.vm[h][4 * gr] = v4.x, t.vm[h][4 * gr + 1] = v4.y, t.vm[h][4 * gr + 2] = v4.z, t.vm[h][4 * gr + 3] = v4.w;
 #pragma unroll
             for (int r = 0; r < 4; ++r) t.vc[h][r][gr] = vc[r * kWords + gr * (G / 8)];
         }
     }
+    const uint32_t *w = (lane < 32 ? a.k_groups : a.v_groups) + ((lane & 16 ? rows[1] : rows[0]) + n) * GR;
+    if constexpr (GR == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(w);
+        t.words[0] = v.x, t.words[1] = v.y, t.words[2] = v.z, t.words[3] = v.w;
+    } else if constexpr (GR == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(w);
+        t.words[0] = v.x, t.words[1] = v.y;
+    } else {
+        t.words[0] = *w;
+    }
+}
+
+// LDS accesses of one wave keep their order; the compiler must not move them past each other either.
+__device__ __forceinline__ void wave_order() { asm volatile("" ::: "memory"); }
+
+template <int D, int G>
+__device__ __forceinline__ void fill_table(const KvTile<D, G> &t, TokenTable<D / G> &table, int at, int len, bool edge, float qk) {
+    constexpr int GR = D / G;
+    const int lane = threadIdx.x & 63, token = lane & 31;
+    const bool value = lane >= 32;
+    // places past the length or of no page may hold anything
+    const bool off = edge && (!(token < 16 ? t.live[0] : t.live[1]) || at + token >= len);
+    float v[GR], top = 0.f;
+    uint32_t z[GR];
+#pragma unroll
+    for (int gr = 0; gr < GR; ++gr) {
+        const uint32_t w = off ? 0u : t.words[gr];
+        v[gr] = kv4_scale(w);
+        z[gr] = kv4_zero(w);
+        top = fmaxf(top, v[gr]);
+    }
+    const int ex = __builtin_amdgcn_frexp_expf(top);
+    wave_order();
+#pragma unroll
+    for (int gr = 0; gr < GR; ++gr) {
+        table.scale[value][gr][token] = value ? __builtin_ldexpf(v[gr], -ex) : v[gr] * qk;
+        if (value) table.vz[gr][token] = static_cast<uint16_t>(z[gr]);
+        else table.kz[gr][token] = z[gr] * 0x00010001u;
+    }
+    if (value) table.exponent[token] = static_cast<float>(ex), table.back[token] = __builtin_ldexpf(1.0f, -ex);
+    wave_order();
 }
 
 // Rows of a wave: 16 MT of the n * ratio (query, head of the group) pairs of a sequence and a head of keys, row = query *
@@ -224,47 +268,22 @@ __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, 
 // when something exceeds it by 15: weights stay below 2^15, the largest ones above 2^7 (f16 keeps its 11 bits
 // down to 2^-21 of them), and the rescaling is rare.
 template <int D, int G, int MT>
-__device__ __forceinline__ void attend(const AttnArgs &a, const KvTile<D, G> &t, Rows<D, G, MT> &s, int at, int len, int sure, float qk) {
+__device__ __forceinline__ void attend(const KvTile<D, G> &t, TokenTable<D / G> &table, Rows<D, G, MT> &s, int at, int len, int sure, float qk) {
     constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = 8 / R;
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
     const bool edge = at + 32 > sure || !t.live[0] || !t.live[1];  // uniform: some row does not see some token
+    fill_table<D, G>(t, table, at, len, edge, qk);
     float y[MT][2][4];            // scores and their tokens' exponents, base 2
-    float c[2][4][GR], back[2][4];  // the scale of the values without its exponent, 2^-exponent
-    uint32_t zp[2][2][GR];        // zero points as f16 denormals, pairs of tokens
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint32_t km[4 * GR], vm[4 * GR];
+        floatx4 ks[GR];
 #pragma unroll
-        for (int i = 0; i < 4 * GR; ++i) {
-            km[i] = t.km[h][i], vm[i] = t.vm[h][i];
-            // places past the length or of no page may hold anything
-            if (edge && (!t.live[h] || at + 16 * h + 4 * g + i / GR >= len)) km[i] = vm[i] = 0;
-        }
-        float ks[4][GR], e[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float v[GR], top = 0.f;
-#pragma unroll
-            for (int gr = 0; gr < GR; ++gr) {
-                ks[r][gr] = kv4_scale(km[r * GR + gr]) * qk;
-                v[gr] = kv4_scale(vm[r * GR + gr]);
-                top = fmaxf(top, v[gr]);
-            }
-            const int ex = __builtin_amdgcn_frexp_expf(top);
-            e[r] = static_cast<float>(ex);
-            back[h][r] = __builtin_ldexpf(1.0f, -ex);
-#pragma unroll
-            for (int gr = 0; gr < GR; ++gr) c[h][r][gr] = __builtin_ldexpf(v[gr], -ex);
-        }
-#pragma unroll
-        for (int gr = 0; gr < GR; ++gr)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) zp[h][p][gr] = high_halves(vm[2 * p * GR + gr], vm[(2 * p + 1) * GR + gr]) & 0x000F000Fu;
-
+        for (int gr = 0; gr < GR; ++gr) ks[gr] = *reinterpret_cast<const floatx4 *>(&table.scale[0][gr][16 * h + 4 * g]);
+        const floatx4 e = *reinterpret_cast<const floatx4 *>(&table.exponent[16 * h + 4 * g]);
         floatx4 dot[MT][GR];
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
-            const uint32_t zz = high_halves(t.kz[h][gr], t.kz[h][gr]) & 0x000F000Fu;
+            const uint32_t zz = table.kz[gr][16 * h + n];
 #pragma unroll
             for (int u = 0; u < W; ++u) {
                 const halfx8 k = codes_f16(t.kc[h][gr][u], zz);
@@ -277,13 +296,24 @@ __device__ __forceinline__ void attend(const AttnArgs &a, const KvTile<D, G> &t,
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float v = dot[mt][0][r] * ks[r][0];
+                float v = dot[mt][0][r] * ks[0][r];
 #pragma unroll
-                for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[r][gr], v);
+                for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], v);
                 v = __builtin_fmaf(v, s.unit[mt], e[r]);
                 if (edge && (!t.live[h] || at + 16 * h + 4 * g + r >= s.limit[mt])) v = -INFINITY;
                 y[mt][h][r] = v;
             }
+    }
+    floatx4 back[2], c[2][GR];
+    uint2 zp[2][GR];        // zero points of the values, pairs of tokens
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        back[h] = *reinterpret_cast<const floatx4 *>(&table.back[16 * h + 4 * g]);
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            c[h][gr] = *reinterpret_cast<const floatx4 *>(&table.scale[1][gr][16 * h + 4 * g]);
+            zp[h][gr] = *reinterpret_cast<const uint2 *>(&table.vz[gr][16 * h + 4 * g]);
+        }
     }
     uint32_t p[MT][GR][4];  // weights times c as f16 pairs: tokens (0, 1), (2, 3) of both halves
 #pragma unroll
@@ -311,7 +341,7 @@ __device__ __forceinline__ void attend(const AttnArgs &a, const KvTile<D, G> &t,
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int h = i / 2, r = i % 2 * 2;
-                const halfx2 v = {static_cast<_Float16>(w[h][r] * c[h][r][gr]), static_cast<_Float16>(w[h][r + 1] * c[h][r + 1][gr])};
+                const halfx2 v = {static_cast<_Float16>(w[h][r] * c[h][gr][r]), static_cast<_Float16>(w[h][r + 1] * c[h][gr][r + 1])};
                 p[mt][gr][i] = __builtin_bit_cast(uint32_t, v);
             }
     }
@@ -335,7 +365,7 @@ __device__ __forceinline__ void attend(const AttnArgs &a, const KvTile<D, G> &t,
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t x = code < 4 ? lo[i] : hi[i];
-                const uint32_t y = code % 4 < 2 ? x : x >> 8, z = zp[i / 2][i % 2][gr];
+                const uint32_t y = code % 4 < 2 ? x : x >> 8, z = i % 2 ? zp[i / 2][gr].y : zp[i / 2][gr].x;
                 v[i] = code % 2 == 0 ? minus(y & 0x000F000Fu, z) : minus(y & 0x00F000F0u, z << 4);
             }
             const halfx8 vv = eight(v[0], v[1], v[2], v[3]);
@@ -347,7 +377,7 @@ __device__ __forceinline__ void attend(const AttnArgs &a, const KvTile<D, G> &t,
 
 // Row tile's walk over tokens first, first + step, .. (of 32) below end, the next tile's loads in flight.
 template <int D, int G, int MT>
-__device__ __forceinline__ void walk(const AttnArgs &a, Rows<D, G, MT> &s, const Seq &sq, int head, int first, int step, int end) {
+__device__ __forceinline__ void walk(const AttnArgs &a, TokenTable<D / G> &tokens, Rows<D, G, MT> &s, const Seq &sq, int head, int first, int step, int end) {
     if (first >= end) return;
     int sure = sq.len;  // tokens that every row sees
 #pragma unroll
@@ -374,7 +404,7 @@ __device__ __forceinline__ void walk(const AttnArgs &a, Rows<D, G, MT> &s, const
         } else {
             next = cur;
         }
-        attend<D, G, MT>(a, cur, s, at, sq.len, sure, qk);
+        attend<D, G, MT>(cur, tokens, s, at, sq.len, sure, qk);
         cur = next;
     }
 }
@@ -408,6 +438,7 @@ __global__ __launch_bounds__(256) void kv4_attention_split_kernel(AttnArgs a) {
     typedef Rows<D, G, MT> S;
     constexpr int kRow = D + 4;
     __shared__ __align__(16) float sums[4][16][kRow];
+    __shared__ __align__(16) TokenTable<D / G> tokens[4];
     __shared__ float ml[2][4][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
@@ -424,7 +455,7 @@ __global__ __launch_bounds__(256) void kv4_attention_split_kernel(AttnArgs a) {
     const int first = split * share, end = min(seen, first + share);
     S s;
     load_rows<D, G, MT>(a, s, sq, head, row0);
-    walk<D, G, MT>(a, s, sq, head, first + 32 * wave, 128, end);
+    walk<D, G, MT>(a, tokens[wave], s, sq, head, first + 32 * wave, 128, end);
     settle<D, G, MT>(s);
     const int hq = a.heads * a.ratio;
 #pragma unroll
@@ -533,6 +564,7 @@ __global__ __launch_bounds__(256) void kv4_attention_rows_kernel(AttnArgs a, int
     typedef Rows<D, G, MT> S;
     constexpr int kRow = D + 4;
     __shared__ __align__(16) float sums[4][16][kRow];
+    __shared__ __align__(16) TokenTable<D / G> tokens[4];
     __shared__ float ls[4][2][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
@@ -545,7 +577,7 @@ __global__ __launch_bounds__(256) void kv4_attention_rows_kernel(AttnArgs a, int
     const int seen = a.causal ? max(0, min(sq.len, sq.len - sq.n + (row0 + rows - 1) / a.ratio + 1)) : sq.len;
     S s;
     load_rows<D, G, MT>(a, s, sq, head, row0);
-    walk<D, G, MT>(a, s, sq, head, 0, 32, seen);
+    walk<D, G, MT>(a, tokens[wave], s, sq, head, 0, 32, seen);
     settle<D, G, MT>(s);
     const int hq = a.heads * a.ratio;
 #pragma unroll
@@ -577,6 +609,10 @@ __global__ __launch_bounds__(256) void kv4_attention_rows_kernel(AttnArgs a, int
     }
 }
 
+// Row tiles of 16 a wave at most, by its registers: with groups of 32 in 128 channels two of them no longer fit without
+// spilling, and three or four never do.
+constexpr int most_tiles(int64_t d, int64_t g) { return d / g >= 4 ? 1 : 2; }
+
 // How a call is laid out: rows a wave (16 mt), whether waves share rows (splits of the tokens) or have their own, row
 // tiles at most, splits.
 struct Plan {
@@ -593,12 +629,12 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     // enough row tiles of 32 for two waves a SIMD: every wave its own rows
     p.rows = varlen && rows / 32 * c->kv_heads >= 4 * cus;
     if (p.rows) {
-        p.mt = 2;
+        p.mt = most_tiles(c->head_dim, c->group);
         p.tiles = tiles(64 * p.mt);
         return p;
     }
     const int64_t each = (rows + batch - 1) / batch;
-    p.mt = each <= 16 ? 1 : each <= 32 ? 2 : 4;
+    p.mt = each <= 16 ? 1 : most_tiles(c->head_dim, c->group);
     p.tiles = tiles(16 * p.mt);
     const int64_t tasks = p.tiles * c->kv_heads, len = table_cols * c->page_size;
     p.splits = std::max<int64_t>(1, std::min((8 * cus + tasks - 1) / tasks, (len + 127) / 128));
@@ -673,11 +709,13 @@ int32_t castforge_hip_kv4_attention(const cfh_kv4_cache_t *cache, const uint16_t
             constexpr int D = decltype(d)::value, G = decltype(gr)::value;
             if (p.rows) {
                 require(p.tiles * a.heads <= 0x7fffffff, "too many workgroups for one launch");
-                kv4_attention_rows_kernel<D, G, 2><<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(256), 0, st>>>(a, static_cast<int>(p.tiles));
+                kv4_attention_rows_kernel<D, G, most_tiles(D, G)><<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(256), 0, st>>>(a, static_cast<int>(p.tiles));
                 check_launch("kv4_attention_rows");
-            } else if (p.mt == 1) launch_split<D, G, 1>(a, p, st);
-            else if (p.mt == 2) launch_split<D, G, 2>(a, p, st);
-            else launch_split<D, G, 4>(a, p, st);
+            } else if (p.mt == 1) {
+                launch_split<D, G, 1>(a, p, st);
+            } else if constexpr (most_tiles(D, G) > 1) {
+                launch_split<D, G, 2>(a, p, st);
+            }
         });
     });
 }

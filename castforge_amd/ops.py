@@ -1110,11 +1110,11 @@ def kv4_gather(cache: Kv4Cache, slots: torch.Tensor, out_dtype: torch.dtype = to
 
 
 @functools.lru_cache(maxsize=4096)
-def _kv4_workspace(device: int, kv_heads: int, page_size: int, head_dim: int, tokens: int, q_heads: int, batch: int, cols: int,
+def _kv4_workspace(device: int, kv_heads: int, page_size: int, head_dim: int, group: int, tokens: int, q_heads: int, batch: int, cols: int,
                    varlen: int) -> int:
     """castforge_hip_kv4_attention_workspace's bytes, which depend on sizes alone."""
     size = ctypes.c_int64()
-    shape = ffi.Kv4CacheStruct(None, None, None, None, 0, kv_heads, page_size, head_dim, 32)
+    shape = ffi.Kv4CacheStruct(None, None, None, None, 0, kv_heads, page_size, head_dim, group)
     ffi.call("castforge_hip_kv4_attention_workspace", ctypes.byref(shape), tokens, q_heads, batch, cols, varlen, ctypes.byref(size))
     return size.value
 
@@ -1143,7 +1143,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, kv
         raise ValueError("without cu_q every sequence has one query: q and page_table must have the same rows")
     out = q.new_empty(shape)
     lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
-    size = _kv4_workspace(dev, heads, cache.page_size, d, t, hq, b, cols, 0 if cp is None else 1)
+    size = _kv4_workspace(dev, heads, cache.page_size, d, cache.group, t, hq, b, cols, 0 if cp is None else 1)
     ws = q.new_empty((size,), dtype=torch.uint8) if size else None  # held until the call returns
     ffi.call("castforge_hip_kv4_attention", cache._ref, q.data_ptr(), qs, t, hq, b, cp, page_table.data_ptr(), cols, lp, int(causal),
              d ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse), _ptr(ws), size, _stream(q))
