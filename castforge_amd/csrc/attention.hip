@@ -125,17 +125,25 @@ template <int D, int G>
 struct KvTile {
     static constexpr int GR = D / G, W = G / 32;
     uint32_t kc[2][GR][W];  // token n: words g W .. of each group
-    uint32_t vc[2][4][GR];  // tokens 4 g + r: word n % (G / 8) of each group
+    // tokens 4 g + r: word n % (G / 8) of each group; where a row has 16 words in several groups word n alone, from which
+    // attend() deals the groups' out through LDS (a lane would load each word GR times over)
+    static constexpr bool kDeal = D == 128 && GR > 1;
+    static constexpr int VW = kDeal ? 1 : GR;
+    uint32_t vc[2][4][VW];
     uint32_t words[GR];     // group words of one token: lanes 0 .. 31 of the keys, 32 .. 63 of the values
     bool live[2];           // uniform: the half's page is one of the cache's
 };
 
 // What a wave makes of the group words of 32 tokens, once, each lane for one token's keys or values: in LDS, where
 // the lanes that need a token's numbers read them four tokens at a time.
-template <int GR>
+template <int D, int G>
 struct TokenTable {
+    static constexpr int GR = D / G;
+    static constexpr bool kDeal = KvTile<D, G>::kDeal;
     float scale[2][GR][32];    // keys: scale times what turns a product into a score; values: scale without its exponent
     float exponent[32], back[32];  // of the values' largest scale, 2^-exponent
+    static constexpr int kRow = 36;      // tokens a row of `v`, padded for the banks
+    uint32_t v[kDeal ? 16 * kRow : 4];   // the values' codes: word by word, a token each
     uint32_t kz[GR][32];       // zero point in both halves, as f16 denormals
     uint16_t vz[GR][32];
 };
@@ -149,7 +157,8 @@ __device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, in
     for (int h = 0; h < 2; ++h) {
         t.live[h] = at + 16 * h < end && page[h] >= 0 && page[h] < a.num_pages;
         rows[h] = kv4_row(t.live[h] ? page[h] : 0, head, (at + 16 * h) & ((1 << a.page_shift) - 1), a.heads, a.page_shift);
-        const uint32_t *kc = a.k_codes + rows[h] * kWords + n * kWords + g * W, *vc = a.v_codes + rows[h] * kWords + 4 * g * kWords + n % (G / 8);
+        const uint32_t *kc = a.k_codes + rows[h] * kWords + n * kWords + g * W;
+        const uint32_t *vc = a.v_codes + rows[h] * kWords + 4 * g * kWords + (KvTile<D, G>::kDeal ? n : n % (G / 8));
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
             if constexpr (W == 4) {
@@ -161,9 +170,11 @@ __device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, in
             } else {
                 t.kc[h][gr][0] = kc[gr * (G / 8)];
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) t.vc[h][r][gr] = vc[r * kWords + gr * (G / 8)];
         }
+#pragma unroll
+        for (int i = 0; i < KvTile<D, G>::VW; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t.vc[h][r][i] = vc[r * kWords + i * (G / 8)];
     }
     const uint32_t *w = (lane < 32 ? a.k_groups : a.v_groups) + ((lane & 16 ? rows[1] : rows[0]) + n) * GR;
     if constexpr (GR == 4) {
@@ -181,7 +192,7 @@ __device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, in
 __device__ __forceinline__ void wave_order() { asm volatile("" ::: "memory"); }
 
 template <int D, int G>
-__device__ __forceinline__ void fill_table(const KvTile<D, G> &t, TokenTable<D / G> &table, int at, int len, bool edge, float qk) {
+__device__ __forceinline__ void fill_table(const KvTile<D, G> &t, TokenTable<D, G> &table, int at, int len, bool edge, float qk) {
     constexpr int GR = D / G;
     const int lane = threadIdx.x & 63, token = lane & 31;
     const bool value = lane >= 32;
@@ -198,6 +209,12 @@ __device__ __forceinline__ void fill_table(const KvTile<D, G> &t, TokenTable<D /
     }
     const int ex = __builtin_amdgcn_frexp_expf(top);
     wave_order();
+    if constexpr (KvTile<D, G>::kDeal) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<uint4 *>(&table.v[(lane & 15) * TokenTable<D, G>::kRow + 16 * h + 4 * (lane >> 4)]) =
+                make_uint4(t.vc[h][0][0], t.vc[h][1][0], t.vc[h][2][0], t.vc[h][3][0]);
+    }
 #pragma unroll
     for (int gr = 0; gr < GR; ++gr) {
         table.scale[value][gr][token] = value ? __builtin_ldexpf(v[gr], -ex) : v[gr] * qk;
@@ -268,7 +285,7 @@ __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, 
 // when something exceeds it by 15: weights stay below 2^15, the largest ones above 2^7 (f16 keeps its 11 bits
 // down to 2^-21 of them), and the rescaling is rare.
 template <int D, int G, int MT>
-__device__ __forceinline__ void attend(const KvTile<D, G> &t, TokenTable<D / G> &table, Rows<D, G, MT> &s, int at, int len, int sure, float qk) {
+__device__ __forceinline__ void attend(const KvTile<D, G> &t, TokenTable<D, G> &table, Rows<D, G, MT> &s, int at, int len, int sure, float qk) {
     constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = 8 / R;
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
     const bool edge = at + 32 > sure || !t.live[0] || !t.live[1];  // uniform: some row does not see some token
@@ -353,10 +370,18 @@ __device__ __forceinline__ void attend(const KvTile<D, G> &t, TokenTable<D / G> 
         // a row of V^T is word n % (G / 8), codes from n / (G / 8) on in steps of R
         uint32_t lo[4], hi[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int h = i / 2, r = i % 2 * 2, sh = R == 1 ? 0 : 4 * (n / (G / 8));
-            lo[i] = low_halves(t.vc[h][r][gr] >> sh, t.vc[h][r + 1][gr] >> sh);
-            hi[i] = high_halves(t.vc[h][r][gr] >> sh, t.vc[h][r + 1][gr] >> sh);
+        for (int h = 0; h < 2; ++h) {
+            uint4 w;
+            if constexpr (KvTile<D, G>::kDeal)
+                w = *reinterpret_cast<const uint4 *>(&table.v[(gr * (G / 8) + n % (G / 8)) * TokenTable<D, G>::kRow + 16 * h + 4 * g]);
+            else
+                w = make_uint4(t.vc[h][0][gr], t.vc[h][1][gr], t.vc[h][2][gr], t.vc[h][3][gr]);
+            if constexpr (R > 1) {
+                const int sh = 4 * (n / (G / 8));
+                w.x >>= sh, w.y >>= sh, w.z >>= sh, w.w >>= sh;
+            }
+            lo[2 * h] = low_halves(w.x, w.y), lo[2 * h + 1] = low_halves(w.z, w.w);
+            hi[2 * h] = high_halves(w.x, w.y), hi[2 * h + 1] = high_halves(w.z, w.w);
         }
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
@@ -377,7 +402,7 @@ __device__ __forceinline__ void attend(const KvTile<D, G> &t, TokenTable<D / G> 
 
 // Row tile's walk over tokens first, first + step, .. (of 32) below end, the next tile's loads in flight.
 template <int D, int G, int MT>
-__device__ __forceinline__ void walk(const AttnArgs &a, TokenTable<D / G> &tokens, Rows<D, G, MT> &s, const Seq &sq, int head, int first, int step, int end) {
+__device__ __forceinline__ void walk(const AttnArgs &a, TokenTable<D, G> &tokens, Rows<D, G, MT> &s, const Seq &sq, int head, int first, int step, int end) {
     if (first >= end) return;
     int sure = sq.len;  // tokens that every row sees
 #pragma unroll
@@ -434,11 +459,11 @@ __device__ __forceinline__ void settle(Rows<D, G, MT> &s) {
 // One workgroup's four waves take the same rows and every fourth 32 tokens of a split's share, and are joined through
 // LDS; splits are joined by kv4_attention_join_kernel.  For few rows a sequence: bound by the cache's bytes.
 template <int D, int G, int MT>
-__global__ __launch_bounds__(256) void kv4_attention_split_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((D == 128 && G < 128) || MT > 1 ? 2 : 4))) void kv4_attention_split_kernel(AttnArgs a) {
     typedef Rows<D, G, MT> S;
     constexpr int kRow = D + 4;
     __shared__ __align__(16) float sums[4][16][kRow];
-    __shared__ __align__(16) TokenTable<D / G> tokens[4];
+    __shared__ __align__(16) TokenTable<D, G> tokens[4];
     __shared__ float ml[2][4][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
@@ -560,11 +585,11 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
 // work.  Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row
 // tiles from the last, which see the most tokens.
 template <int D, int G, int MT>
-__global__ __launch_bounds__(256) void kv4_attention_rows_kernel(AttnArgs a, int tiles) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void kv4_attention_rows_kernel(AttnArgs a, int tiles) {
     typedef Rows<D, G, MT> S;
     constexpr int kRow = D + 4;
     __shared__ __align__(16) float sums[4][16][kRow];
-    __shared__ __align__(16) TokenTable<D / G> tokens[4];
+    __shared__ __align__(16) TokenTable<D, G> tokens[4];
     __shared__ float ls[4][2][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
@@ -637,7 +662,7 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     p.mt = each <= 16 ? 1 : most_tiles(c->head_dim, c->group);
     p.tiles = tiles(16 * p.mt);
     const int64_t tasks = p.tiles * c->kv_heads, len = table_cols * c->page_size;
-    p.splits = std::max<int64_t>(1, std::min((8 * cus + tasks - 1) / tasks, (len + 127) / 128));
+    p.splits = std::max<int64_t>(1, std::min((2 * cus + tasks - 1) / tasks, (len + 127) / 128));
     const int64_t row = (c->head_dim + 4) * 4;
     p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
     if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
