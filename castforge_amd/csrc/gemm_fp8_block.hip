@@ -230,21 +230,58 @@ __device__ __forceinline__ void tile_stage(const uint8_t *__restrict__ cur, uint
     const int fr = lane & 31, fc = (lane >> 5) * 2;
     const float *scales = reinterpret_cast<const float *>(cur + (T::BN + T::BM) * kRun) + wm + fr;
     int32x8 w[I][2];
+    float f[J];
+    const auto read_a = [&](int j, int32x8 (&a)[2]) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) a[kk] = frag(cur + T::BN * kRun, wm + 32 * j + fr, 4 * kk + fc);
+    };
+    const auto fold = [&](floatx16 &sum, const floatx16 &part, float by) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sum[q] = __builtin_fmaf(part[q], by, sum[q]);
+    };
+    floatx16 zero;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) zero[q] = 0.f;
+    if constexpr (!kExact && J >= 4) {
+        // Tile by tile: the MFMAs of a tile run while the tile before is folded, and the A fragments of the next 32 rows are
+        // read meanwhile.  One wave alone can so keep the matrix unit busy (two MFMAs take 128 cycles, a fold 64): 222 -> 208 us
+        // for 4096 x 11008 x 4096.  Left to itself the scheduler waits for each tile to fold it.
+        int32x8 a[2][2];
+        floatx16 part[2];
+        read_a(0, a[0]);
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) w[i][kk] = frag(cur, wn + 32 * i + fr, 4 * kk + fc);
+#pragma unroll
+        for (int j = 0; j < J; ++j) f[j] = scales[32 * j] * sw;
+        static_for<I * J + 1>([&](auto TT) {
+            constexpr int t = decltype(TT)::value;
+            if constexpr (t < I * J) {
+                constexpr int i = t % I, j = t / I;
+                if constexpr (i == 0 && j + 1 < J) read_a(j + 1, a[(j + 1) & 1]);
+                part[t & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i][0], a[j & 1][0], zero, 0, 0, 0, 0, 0, 0);
+                part[t & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i][1], a[j & 1][1], part[t & 1], 0, 0, 0, 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (t > 0) fold(acc[(t - 1) % I][(t - 1) / I], part[(t - 1) & 1], f[(t - 1) / I]);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        return;
+    }
+    // two workgroups a CU, which fill each other's gaps
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) w[i][kk] = frag(cur, wn + 32 * i + fr, 4 * kk + fc);
     static_for<J>([&](auto JJ) {
         constexpr int j = decltype(JJ)::value;
-        const float f = scales[32 * j] * sw;
+        f[j] = scales[32 * j] * sw;
         int32x8 a[2];
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) a[kk] = frag(cur + T::BN * kRun, wm + 32 * j + fr, 4 * kk + fc);
+        read_a(j, a);
         floatx16 part[I];
 #pragma unroll
-        for (int i = 0; i < I; ++i)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) part[i][q] = 0.f;
+        for (int i = 0; i < I; ++i) part[i] = zero;
         if constexpr (kExact) {
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
@@ -261,9 +298,7 @@ __device__ __forceinline__ void tile_stage(const uint8_t *__restrict__ cur, uint
                     part[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i][kk], a[kk], part[i], 0, 0, 0, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < I; ++i)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(part[i][q], f, acc[i][j][q]);
+        for (int i = 0; i < I; ++i) fold(acc[i][j], part[i], f[j]);
     });
 }
 

@@ -40,71 +40,35 @@ struct AppendArgs {
     uint32_t *k_codes, *k_groups, *v_codes, *v_groups;
 };
 
-// Eight elements a lane, D / 8 lanes a head of a token; the heads of a token in the order K, V, Q.
-template <int D, int G>
-__global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
-    constexpr int kLanes = D / 8;
-    const int64_t per_token = 2 * a.heads + a.q_heads;
-    const int64_t unit = (blockIdx.x * 256ll + threadIdx.x) / kLanes;
-    const int piece = threadIdx.x % kLanes;  // 256 % kLanes == 0
-    if (unit >= a.tokens * per_token) return;  // whole groups of kLanes lanes
-    const int64_t token = unit / per_token;
-    const int u = static_cast<int>(unit % per_token);
-    const int kind = u < a.heads ? 0 : u < 2 * a.heads ? 1 : 2;  // K, V, Q
-    const int head = u - (kind == 0 ? 0 : kind == 1 ? a.heads : 2 * a.heads);
-    const uint16_t *src = kind == 0 ? a.k + token * a.k_stride : kind == 1 ? a.v + token * a.v_stride : a.q + token * a.q_stride;
-    src += head * D;
-    const auto load8 = [&](int p, float (&x)[8]) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(src + 8 * p);
-        const uint32_t b[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(b[i] << 16), x[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u);
+// Least and greatest over G / 8 lanes of a DPP row.
+template <int G>
+__device__ __forceinline__ void range_of(float &lo, float &hi) {
+    lo = fminf(lo, lane_xor<1>(lo)), hi = fmaxf(hi, lane_xor<1>(hi));
+    lo = fminf(lo, lane_xor<2>(lo)), hi = fmaxf(hi, lane_xor<2>(hi));
+    if constexpr (G >= 64) lo = fminf(lo, lane_xor<4>(lo)), hi = fmaxf(hi, lane_xor<4>(hi));
+    if constexpr (G >= 128) lo = fminf(lo, lane_xor<8>(lo)), hi = fmaxf(hi, lane_xor<8>(hi));
+}
+
+// Eight codes of finite numbers whose range and scale are finite.  The quotient is RN(x / scale) from the reciprocal by two
+// fmas; adding 1.5 * 2^23 rounds it to the nearest even integer and med3 clamps it to [-z, 15 - z]; four codes at a time
+// become a 16-bit number in f32, exactly.  A tenth of a division and rint each.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale, float y, float z) {
+    constexpr float kMagic = 12582912.f;
+    const float lo = kMagic - z, hi = kMagic + 15.f - z;
+    const auto code = [&](float v) {
+        const float q0 = v * y;
+        const float q = __builtin_fmaf(__builtin_fmaf(-q0, scale, v), y, q0);
+        return __builtin_amdgcn_fmed3f(q + kMagic, lo, hi) - lo;
     };
-    float x[8];
-    load8(piece, x);
-    if (kind != 1 && 8 * piece < a.rot) {
-        // a position outside the table takes its nearest row
-        const int64_t pos = min(max(a.positions[token], int64_t{0}), a.max_pos - 1);
-        const int half = a.rot / 2;
-        const float *c = a.cos + pos * half, *s = a.sin + pos * half;
-        if (a.interleaved) {
+    uint32_t half[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float cc = c[4 * piece + i], ss = s[4 * piece + i], p = x[2 * i], q = x[2 * i + 1];
-                x[2 * i] = p * cc - q * ss;
-                x[2 * i + 1] = q * cc + p * ss;
-            }
-        } else {
-            const bool low = 8 * piece < half;
-            const int other = low ? piece + half / 8 : piece - half / 8;
-            const int at = low ? 8 * piece : 8 * piece - half;
-            float y[8];
-            load8(other, y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float cc = c[at + i], ss = s[at + i];
-                x[i] = low ? x[i] * cc - y[i] * ss : x[i] * cc + y[i] * ss;
-            }
-        }
-    }
-    if (kind == 2) {
-        uint4 w;
-        w.x = f32x2_to_bf16x2_rne(x[0], x[1]), w.y = f32x2_to_bf16x2_rne(x[2], x[3]);
-        w.z = f32x2_to_bf16x2_rne(x[4], x[5]), w.w = f32x2_to_bf16x2_rne(x[6], x[7]);
-        *reinterpret_cast<uint4 *>(a.q_out + (token * a.q_heads + head) * D + 8 * piece) = w;
-        return;
-    }
-    const int64_t slot = a.slots[token];
-    if (slot < 0 || slot >= a.capacity) return;  // whole groups of lanes: not appended
-    float lo = 0.f, hi = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
-    lo = wave_min<G / 8>(lo);
-    hi = wave_max<G / 8>(hi);
-    const uint16_t h = group_scale_bits(hi, lo);
-    const float scale = f16_to_f32(h);
-    float z = rintf(-lo / scale);
-    z = z != z ? 0.f : fminf(fmaxf(z, 0.f), 15.f);
+    for (int h = 0; h < 2; ++h)
+        half[h] = static_cast<uint32_t>(__builtin_fmaf(code(x[4 * h + 3]), 4096.f, __builtin_fmaf(code(x[4 * h + 2]), 256.f, __builtin_fmaf(code(x[4 * h + 1]), 16.f, code(x[4 * h])))));
+    return half[0] | (half[1] << 16);
+}
+
+// Any numbers: NaN takes the zero point.
+__device__ __forceinline__ uint32_t codes_of_any(const float (&x)[8], float scale, float z) {
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -112,47 +76,156 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
         if (t != t) t = 0.f;
         word |= static_cast<uint32_t>(fminf(fmaxf(t + z, 0.f), 15.f)) << (4 * i);
     }
-    const int64_t row = kv4_row(slot >> a.page_shift, head, static_cast<int>(slot & ((1 << a.page_shift) - 1)), a.heads, a.page_shift);
-    (kind == 0 ? a.k_codes : a.v_codes)[row * kLanes + piece] = word;
-    if (piece % (G / 8) == 0)
-        (kind == 0 ? a.k_groups : a.v_groups)[row * (D / G) + piece / (G / 8)] = static_cast<uint32_t>(h) | (static_cast<uint32_t>(z) << 16);
+    return word;
 }
 
-// Rows of the cache as numbers, eight elements a lane; a slot outside the cache gives zeros.
+// A workgroup has one token (its slot, position and angles are read once) and up to `share` of its heads, in the order K, V, Q:
+// eight elements a lane, D / 8 lanes a head.  HBM-bound where the tokens are many: 4096 tokens of 32 heads of each kind, all in
+// places of their own, move 170 MB with the cache's partial lines.
+template <int D, int G>
+__global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int share) {
+    constexpr int kLanes = D / 8, kUnits = 256 / kLanes;
+    const int64_t token = blockIdx.x;
+    const int piece = threadIdx.x % kLanes, local = threadIdx.x / kLanes;
+    const int64_t slot = a.slots[token];
+    const bool kept = slot >= 0 && slot < a.capacity;
+    const int64_t row0 = kv4_row(kept ? slot >> a.page_shift : 0, 0, static_cast<int>(slot & ((1 << a.page_shift) - 1)), a.heads, a.page_shift);
+    const uint16_t *k = a.k + token * a.k_stride, *v = a.v + token * a.v_stride, *q = a.q_heads ? a.q + token * a.q_stride : nullptr;
+    const int half = a.rot / 2;
+    const bool turns = 8 * piece < a.rot, low = 8 * piece < half;
+    const int other = a.interleaved ? piece : low ? piece + half / 8 : piece - half / 8;
+    float c[8], t[8];  // cosines and sines of the lane's channels, the sine's sign taken in
+    if (turns) {
+        // a position outside the table takes its nearest row
+        const int64_t pos = min(max(a.positions[token], int64_t{0}), a.max_pos - 1);
+        const float *cp = a.cos + pos * half, *sp = a.sin + pos * half;
+        if (a.interleaved) {
+            const float4 cc = *reinterpret_cast<const float4 *>(cp + 4 * piece), ss = *reinterpret_cast<const float4 *>(sp + 4 * piece);
+            c[0] = c[1] = cc.x, c[2] = c[3] = cc.y, c[4] = c[5] = cc.z, c[6] = c[7] = cc.w;
+            t[0] = -ss.x, t[1] = ss.x, t[2] = -ss.y, t[3] = ss.y, t[4] = -ss.z, t[5] = ss.z, t[6] = -ss.w, t[7] = ss.w;
+        } else {
+            const int at = low ? 8 * piece : 8 * piece - half;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 cc = reinterpret_cast<const float4 *>(cp + at)[h], ss = reinterpret_cast<const float4 *>(sp + at)[h];
+                c[4 * h] = cc.x, c[4 * h + 1] = cc.y, c[4 * h + 2] = cc.z, c[4 * h + 3] = cc.w;
+                t[4 * h] = low ? -ss.x : ss.x, t[4 * h + 1] = low ? -ss.y : ss.y, t[4 * h + 2] = low ? -ss.z : ss.z, t[4 * h + 3] = low ? -ss.w : ss.w;
+            }
+        }
+    }
+    const auto unpack = [](const uint4 &w, float (&x)[8]) {
+        const uint32_t b[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(b[i] << 16), x[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u);
+    };
+    const int units = 2 * a.heads + a.q_heads, end = min(units, static_cast<int>(blockIdx.y + 1) * share);
+    const auto source = [&](int u) { return (u < a.heads ? k + u * D : u < 2 * a.heads ? v + (u - a.heads) * D : q + (u - 2 * a.heads) * D); };
+    const auto load = [&](int u, uint4 (&w)[2]) {
+        const uint16_t *src = source(u);
+        w[0] = *reinterpret_cast<const uint4 *>(src + 8 * piece);
+        if (turns && !a.interleaved && (u < a.heads || u >= 2 * a.heads)) w[1] = *reinterpret_cast<const uint4 *>(src + 8 * other);
+    };
+    int u = static_cast<int>(blockIdx.y) * share + local;
+    uint4 w[2], ahead[2];
+    if (u < end) load(u, ahead);
+    for (; u < end; u += kUnits) {
+        w[0] = ahead[0], w[1] = ahead[1];
+        if (u + kUnits < end) load(u + kUnits, ahead);
+        const bool is_v = u >= a.heads && u < 2 * a.heads;
+        float x[8];
+        unpack(w[0], x);
+        if (turns && !is_v) {
+            // (a, b) -> (a c - b s, b c + a s): x c + partner * (+- s), which rounds as the difference does
+            float y[8];
+            if (a.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+            } else {
+                unpack(w[1], y);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + y[i] * t[i];
+        }
+        if (u >= 2 * a.heads) {
+            uint4 o;
+            o.x = f32x2_to_bf16x2_rne(x[0], x[1]), o.y = f32x2_to_bf16x2_rne(x[2], x[3]);
+            o.z = f32x2_to_bf16x2_rne(x[4], x[5]), o.w = f32x2_to_bf16x2_rne(x[6], x[7]);
+            *reinterpret_cast<uint4 *>(a.q_out + (token * a.q_heads + u - 2 * a.heads) * D + 8 * piece) = o;
+            continue;
+        }
+        if (!kept) continue;
+        float lo = 0.f, hi = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
+        // in a group's lanes alike: a NaN leaves the range, an infinity makes it infinite
+        bool odd = __builtin_isunordered(x[0], x[1]) | __builtin_isunordered(x[2], x[3]) | __builtin_isunordered(x[4], x[5]) | __builtin_isunordered(x[6], x[7]);
+        range_of<G>(lo, hi);
+        odd |= !(hi - lo < INFINITY);
+        const uint16_t h = group_scale_bits(hi, lo);
+        const float scale = f16_to_f32(h), inv = 1.0f / scale;
+        uint32_t word, zero;
+        if (odd) {
+            float z = rintf(-lo / scale);
+            z = z != z ? 0.f : fminf(fmaxf(z, 0.f), 15.f);
+            word = codes_of_any(x, scale, z), zero = static_cast<uint32_t>(z);
+        } else {
+            const float z0 = -lo * inv;
+            const float z = __builtin_amdgcn_fmed3f(rintf(__builtin_fmaf(__builtin_fmaf(-z0, scale, -lo), inv, z0)), 0.f, 15.f);
+            word = codes_of(x, scale, inv, z), zero = static_cast<uint32_t>(z);
+        }
+        const int head = is_v ? u - a.heads : u;
+        const int64_t row = row0 + (static_cast<int64_t>(head) << a.page_shift);
+        (is_v ? a.v_codes : a.k_codes)[row * kLanes + piece] = word;
+        if (piece % (G / 8) == 0) (is_v ? a.v_groups : a.k_groups)[row * (D / G) + piece / (G / 8)] = static_cast<uint32_t>(h) | (zero << 16);
+    }
+}
+
+// Rows of the cache as numbers, a workgroup a token, eight elements a lane; a slot outside the cache gives zeros.
 template <int D, int G>
 __global__ __launch_bounds__(256) void kv4_gather_kernel(const uint32_t *__restrict__ k_codes, const uint32_t *__restrict__ k_groups,
                                                          const uint32_t *__restrict__ v_codes, const uint32_t *__restrict__ v_groups,
-                                                         const int64_t *__restrict__ slots, int64_t tokens, int64_t capacity, int heads,
-                                                         int page_shift, void *__restrict__ k_out, void *__restrict__ v_out, int bf16) {
-    constexpr int kLanes = D / 8;
-    const int64_t unit = (blockIdx.x * 256ll + threadIdx.x) / kLanes;
-    const int piece = threadIdx.x % kLanes;
-    if (unit >= 2 * heads * tokens) return;
-    const int64_t token = unit / (2 * heads);
-    const int u = static_cast<int>(unit % (2 * heads)), head = u % heads;
-    const bool is_v = u >= heads;
-    const int64_t slot = slots[token];
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (slot >= 0 && slot < capacity) {
-        const int64_t row = kv4_row(slot >> page_shift, head, static_cast<int>(slot & ((1 << page_shift) - 1)), heads, page_shift);
-        const uint32_t w = (is_v ? v_codes : k_codes)[row * kLanes + piece];
-        const uint32_t g = (is_v ? v_groups : k_groups)[row * (D / G) + piece / (G / 8)];
-        const float scale = kv4_scale(g);
-        const int z = static_cast<int>(kv4_zero(g));
+                                                         const int64_t *__restrict__ slots, int64_t capacity, int heads, int page_shift,
+                                                         void *__restrict__ k_out, void *__restrict__ v_out, int bf16, int share) {
+    constexpr int kLanes = D / 8, kUnits = 256 / kLanes;
+    const int64_t token = blockIdx.x, slot = slots[token];
+    const bool kept = slot >= 0 && slot < capacity;
+    const int piece = threadIdx.x % kLanes, end = min(2 * heads, static_cast<int>(blockIdx.y + 1) * share);
+    const int64_t row0 = kv4_row(kept ? slot >> page_shift : 0, 0, static_cast<int>(slot & ((1 << page_shift) - 1)), heads, page_shift);
+#pragma unroll 2
+    for (int u = static_cast<int>(blockIdx.y) * share + static_cast<int>(threadIdx.x) / kLanes; u < end; u += kUnits) {
+        const bool is_v = u >= heads;
+        const int head = is_v ? u - heads : u;
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (kept) {
+            const int64_t row = row0 + (static_cast<int64_t>(head) << page_shift);
+            const uint32_t w = (is_v ? v_codes : k_codes)[row * kLanes + piece];
+            const uint32_t g = (is_v ? v_groups : k_groups)[row * (D / G) + piece / (G / 8)];
+            const float scale = kv4_scale(g);
+            const int z = static_cast<int>(kv4_zero(g));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - z) * scale;
+            for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - z) * scale;
+        }
+        const int64_t at = (token * heads + head) * D + 8 * piece;
+        if (bf16) {
+            uint4 w;
+            w.x = f32x2_to_bf16x2_rne(x[0], x[1]), w.y = f32x2_to_bf16x2_rne(x[2], x[3]);
+            w.z = f32x2_to_bf16x2_rne(x[4], x[5]), w.w = f32x2_to_bf16x2_rne(x[6], x[7]);
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(is_v ? v_out : k_out) + at) = w;
+        } else {
+            float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(is_v ? v_out : k_out) + at);
+            o[0] = make_float4(x[0], x[1], x[2], x[3]);
+            o[1] = make_float4(x[4], x[5], x[6], x[7]);
+        }
     }
-    const int64_t at = (token * heads + head) * D + 8 * piece;
-    if (bf16) {
-        uint4 w;
-        w.x = f32x2_to_bf16x2_rne(x[0], x[1]), w.y = f32x2_to_bf16x2_rne(x[2], x[3]);
-        w.z = f32x2_to_bf16x2_rne(x[4], x[5]), w.w = f32x2_to_bf16x2_rne(x[6], x[7]);
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(is_v ? v_out : k_out) + at) = w;
-    } else {
-        float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(is_v ? v_out : k_out) + at);
-        o[0] = make_float4(x[0], x[1], x[2], x[3]);
-        o[1] = make_float4(x[4], x[5], x[6], x[7]);
-    }
+}
+
+// Heads a workgroup takes of a token: one round of its lanes where that leaves the card with less than four workgroups a CU, else
+// more of them, for whom the angles and the slot are read once.
+int share_of(int64_t tokens, int units, int lanes) {
+    const int round = 256 / lanes, rounds = (units + round - 1) / round;
+    const int64_t wanted = (4 * cu_count() + tokens - 1) / tokens;  // workgroups a token
+    const int ways = static_cast<int>(std::min<int64_t>(rounds, wanted));
+    return (rounds + ways - 1) / ways * round;
 }
 
 void check_rows(const void *p, int64_t stride, int64_t heads, int64_t d, int64_t tokens, const char *what) {
@@ -193,10 +266,11 @@ int32_t castforge_hip_kv4_append(const cfh_kv4_cache_t *cache, const uint16_t *k
                      cache->num_pages * cache->page_size, max_pos, static_cast<int>(cache->kv_heads),
                      q ? static_cast<int>(q_heads) : 0, log2_of(cache->page_size), static_cast<int>(rot), interleaved,
                      cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups};
-        const int64_t threads = tokens * (2 * a.heads + a.q_heads) * (cache->head_dim / 8), grid = (threads + 255) / 256;
-        require(grid <= 0x7fffffff, "too many tokens for one launch");
+        require(rot == 0 || (aligned(cos, 16) && aligned(sin, 16)), "cos and sin must be 16-byte aligned");
+        const int units = 2 * a.heads + a.q_heads, share = share_of(tokens, units, static_cast<int>(cache->head_dim / 8));
+        const dim3 grid(static_cast<unsigned>(tokens), (units + share - 1) / share);
         kv4_by_shape(cache, [&](auto d, auto g) {
-            kv4_append_kernel<decltype(d)::value, decltype(g)::value><<<dim3(static_cast<unsigned>(grid)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a);
+            kv4_append_kernel<decltype(d)::value, decltype(g)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a, share);
         });
         check_launch("kv4_append");
     });
@@ -211,12 +285,12 @@ int32_t castforge_hip_kv4_gather(const cfh_kv4_cache_t *cache, const int64_t *sl
         if (tokens == 0) return;
         require(slots && k_out && v_out, "buffers must not be NULL");
         require(aligned(k_out, 16) && aligned(v_out, 16), "k_out and v_out must be 16-byte aligned");
-        const int64_t grid = (tokens * 2 * cache->kv_heads * (cache->head_dim / 8) + 255) / 256;
-        require(grid <= 0x7fffffff, "too many tokens for one launch");
+        const int units = static_cast<int>(2 * cache->kv_heads), share = share_of(tokens, units, static_cast<int>(cache->head_dim / 8));
+        const dim3 grid(static_cast<unsigned>(tokens), (units + share - 1) / share);
         kv4_by_shape(cache, [&](auto d, auto g) {
-            kv4_gather_kernel<decltype(d)::value, decltype(g)::value><<<dim3(static_cast<unsigned>(grid)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups, slots, tokens, cache->num_pages * cache->page_size,
-                static_cast<int>(cache->kv_heads), log2_of(cache->page_size), k_out, v_out, out_dtype == CFH_DTYPE_BF16);
+            kv4_gather_kernel<decltype(d)::value, decltype(g)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+                cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups, slots, cache->num_pages * cache->page_size,
+                static_cast<int>(cache->kv_heads), log2_of(cache->page_size), k_out, v_out, out_dtype == CFH_DTYPE_BF16, share);
         });
         check_launch("kv4_gather");
     });
