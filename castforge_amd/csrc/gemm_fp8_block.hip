@@ -12,6 +12,7 @@
 //     value is an f16 normal), exact products and f32 sums at half the MFMA rate.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "../../include/castforge_hip.h"
 #include "cfh_common.hpp"
@@ -43,6 +44,22 @@ __device__ __forceinline__ int32x8 join(const uint4 &lo, const uint4 &hi) {
     return int32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
 }
 
+// LDS panels of 128-byte rows: 16-byte chunk c of row r sits at c ^ ((r >> 1) & 7), so that sixteen rows read at one chunk
+// cover the 256-byte bank window.
+__device__ __forceinline__ int swz(int r, int c) { return c ^ ((r >> 1) & 7); }
+
+__device__ __forceinline__ int32x8 frag(const uint8_t *rows, int r, int c) {
+    return join(*reinterpret_cast<const uint4 *>(rows + r * kRun + swz(r, c) * 16), *reinterpret_cast<const uint4 *>(rows + r * kRun + swz(r, c + 1) * 16));
+}
+
+// A workgroup's panels of W and A and the scales of A's rows as buffers: what lies past a panel's last row reads 0.
+struct Panels {
+    __amdgpu_buffer_rsrc_t w, a, s;
+    // lane i of a load brings 16 bytes of row i / 8 of its eight: their offsets in the panel at K = 0 and in the run, for loads
+    // whose rows start at an even, or odd, multiple of eight (the swizzle repeats every 16 rows)
+    int at[2], in_run[2];
+};
+
 struct GemmArgs {
     const uint8_t *A, *W;
     const float *sa, *sw;
@@ -51,6 +68,26 @@ struct GemmArgs {
     int M, N, K, runs;
     int tiles_m, tiles_n;
 };
+
+__device__ __forceinline__ Panels panels_of(const GemmArgs &g, int n0, int rows_n, int m0, int rows_m, int lane) {
+    Panels p;
+    p.w = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(g.W + static_cast<int64_t>(n0) * g.K), 0, rows_n * g.K, 0x00020000);
+    p.a = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(g.A + static_cast<int64_t>(m0) * g.K), 0, rows_m * g.K, 0x00020000);
+    p.s = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(g.sa + static_cast<int64_t>(m0) * g.runs), 0, rows_m * g.runs * 4, 0x00020000);
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+        p.in_run[o] = swz(8 * o + (lane >> 3), lane & 7) * 16;
+        p.at[o] = (lane >> 3) * g.K + p.in_run[o];
+    }
+    return p;
+}
+
+// One load of eight rows (8 block, ..) of run r into 1 KB of LDS.  The last run's chunks past K read 0 too, sent past the panel.
+__device__ __forceinline__ void panel_load(__amdgpu_buffer_rsrc_t panel, const Panels &p, uint8_t *dst, int block, int odd, int K, int r) {
+    int at = p.at[odd] + (block * 8 * K + r * kRun);
+    if ((r + 1) * kRun > K) at = r * kRun + p.in_run[odd] < K ? at : 0x7fffffff;  // uniform
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (__attribute__((address_space(3))) void *)dst, 16, at, 0, 0, 0);
+}
 
 __device__ __forceinline__ void store4(const GemmArgs &g, int m, int n, const float (&v)[4]) {
     if (m >= g.M || n >= g.N) return;
@@ -70,115 +107,12 @@ __device__ __forceinline__ void store4(const GemmArgs &g, int m, int n, const fl
         }
 }
 
-// ---- few rows of A: a workgroup owns 16 n, its waves split the runs of K --------------------------------
-//
-// Each wave takes runs w, w + NW, ..: both operands go straight to registers (16 rows x 128 bytes of W a run,
-// read once on the card; A stays in the caches), U runs' loads in flight, and the waves' tiles are summed
-// through LDS in wave order.  A lane holds bytes [16 g, 16 g + 16) and [64 + 16 g, + 16) of a row's run
-// (g = lane / 16), so that four lanes read 64 contiguous bytes; A and W share the order, which is all that a
-// sum over K needs.
-template <bool kExact, int J, int NW, int U>
-__global__ __launch_bounds__(64 * NW) void fp8_block_skinny_kernel(GemmArgs g) {
-    extern __shared__ __align__(16) float sums[];
-    const int lane = threadIdx.x & 63, lr = lane & 15, lk = (lane >> 4) * 16;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * J;
-    // rows past the ends read the last one; their products are not stored
-    const uint8_t *wp = g.W + static_cast<int64_t>(min(n0 + lr, g.N - 1)) * g.K + lk;
-    const uint8_t *ap[J];
-    const float *sp[J];
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int64_t m = min(m0 + 16 * j + lr, g.M - 1);
-        ap[j] = g.A + m * g.K + lk;
-        sp[j] = g.sa + m * g.runs;
-    }
-    const float *swp = g.sw + static_cast<int64_t>(n0 / kRun) * g.runs;
-    floatx4 acc[J];
-#pragma unroll
-    for (int j = 0; j < J; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
-
-    // run r of both operands; where `cut`, the pieces past K are zeros (K % 16 == 0: pieces are whole)
-    const auto load = [&](const uint8_t *p, int r, bool cut) {
-        const int k = r * kRun;
-        uint4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-        if (!cut || k + lk < g.K) lo = *reinterpret_cast<const uint4 *>(p + k);
-        if (!cut || k + 64 + lk < g.K) hi = *reinterpret_cast<const uint4 *>(p + k + 64);
-        return join(lo, hi);
-    };
-    const auto fold = [&](const int32x8 &w, const int32x8 (&a)[J], const float (&s)[J], float sw) {
-        half8_t wh[4];
-        if constexpr (kExact) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) wh[c] = e4m3x8_to_f16(w, c);
-        }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            floatx4 part = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (kExact) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[c], e4m3x8_to_f16(a[j], c), part, 0, 0, 0);
-            } else {
-                part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a[j], part, 0, 0, 0, 0, 0, 0);
-            }
-            const float f = s[j] * sw;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) acc[j][q] = __builtin_fmaf(part[q], f, acc[j][q]);
-        }
-    };
-    const int whole = g.K / kRun;  // runs that need no cut
-    int r = wave;
-    for (; r + (U - 1) * NW < whole; r += U * NW) {
-        int32x8 w[U], a[U][J];
-        float s[U][J], sw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) w[u] = load(wp, r + u * NW, false);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                a[u][j] = load(ap[j], r + u * NW, false);
-                s[u][j] = sp[j][r + u * NW];
-            }
-            sw[u] = swp[r + u * NW];
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) fold(w[u], a[u], s[u], sw[u]);
-    }
-    for (; r < g.runs; r += NW) {
-        const int32x8 w = load(wp, r, true);
-        int32x8 a[J];
-        float s[J];
-#pragma unroll
-        for (int j = 0; j < J; ++j) a[j] = load(ap[j], r, true), s[j] = sp[j][r];
-        fold(w, a, s, swp[r]);
-    }
-
-    // acc[j][q] holds n = 4 (lane / 16) + q, m = 16 j + lane % 16
-    constexpr int kRow = 16 + 4;
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-        *reinterpret_cast<floatx4 *>(sums + ((wave * J + j) * 16 + lr) * kRow + (lane >> 4) * 4) = acc[j];
-    __syncthreads();
-    for (int o = threadIdx.x; o < J * 16 * 4; o += 64 * NW) {
-        const int ml = o >> 2, nl = (o & 3) * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const floatx4 p = *reinterpret_cast<const floatx4 *>(sums + (w * J * 16 + ml) * kRow + nl);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] += p[q];
-        }
-        store4(g, m0 + ml, n0 + nl, v);
-    }
-}
-
 // ---- many rows: tiles through LDS ------------------------------------------------------------------------
 //
 // Workgroup tile 32 I WN (n) x 32 J WM (m), WN x WM waves of 32 I x 32 J.  A stage is one run of 128 of both
 // panels and the A rows' scales, brought by buffer loads straight into LDS; two stages, one barrier a stage:
-// a stage is loaded while the other one is computed.  16-byte chunk c of a 128-byte row sits at c ^ ((row >> 1) & 7),
-// so sixteen rows read at one chunk cover the 256-byte bank window.
+// a stage is loaded while the other one is computed.  MFMA-bound in the large: 4096 x 11008 x 4096 208 us, 1.78 PFLOP/s, the matrix
+// unit busy half the time; the rest is the wait at the stage's barrier for loads and fragments.
 template <int I, int J, int WN, int WM>
 struct Tile {
     static constexpr int NW = WN * WM, BN = 32 * I * WN, BM = 32 * J * WM;
@@ -191,42 +125,29 @@ struct Tile {
     static_assert(kRun % (32 * I) == 0, "a wave's n share one scale of W");
 };
 
-__device__ __forceinline__ int swz(int r, int c) { return c ^ ((r >> 1) & 7); }
-
-__device__ __forceinline__ int32x8 frag(const uint8_t *rows, int r, int c) {
-    return join(*reinterpret_cast<const uint4 *>(rows + r * kRun + swz(r, c) * 16), *reinterpret_cast<const uint4 *>(rows + r * kRun + swz(r, c + 1) * 16));
-}
-
-// This wave's loads of run r of both panels and of the A rows' scales into the stage `dst`.  Lane i of a load
-// writes LDS bytes [16 i, + 16): row i / 8, chunk i % 8 of its eight rows.  Rows past the panels' ends read 0, and
-// so do the last run's chunks past K, sent past the end.
+// This wave's loads of run r of both panels and of the A rows' scales into the stage `dst`.
 template <class T>
-__device__ __forceinline__ void tile_issue(__amdgpu_buffer_rsrc_t rw, __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rs,
-                                           uint8_t *__restrict__ dst, int wave, int lane, int K, int runs, int r) {
+__device__ __forceinline__ void tile_issue(const Panels &p, uint8_t *__restrict__ dst, int wave, int lane, int K, int runs, int r) {
 #pragma unroll
     for (int t = 0; t < T::kLoads; ++t) {
-        const int first = (wave * T::kLoads + t) * 8;
-        const bool is_w = first < T::BN;  // uniform: BN is a multiple of 8
-        const int row = first + (lane >> 3), k = r * kRun + swz(row, lane & 7) * 16;
-        const int at = k < K ? (is_w ? row : row - T::BN) * K + k : 0x7fffffff;
-        auto *to = (__attribute__((address_space(3))) void *)(dst + first * kRun);
-        if (is_w) __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, to, 16, at, 0, 0, 0);
-        else __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, to, 16, at, 0, 0, 0);
+        const int first = wave * T::kLoads + t;  // of the stage's loads of eight rows
+        const bool is_w = first * 8 < T::BN;     // uniform
+        panel_load(is_w ? p.w : p.a, p, dst + first * 1024, is_w ? first : first - T::BN / 8, t & 1, K, r);
     }
+    static_assert(T::kLoads % 2 == 0 && T::BN % 16 == 0, "the parity of a load is that of its rows");
     static_assert(T::BM <= 64 * T::NW, "one load of scales a wave");
     if (wave * 64 < T::BM)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(dst + (T::BN + T::BM) * kRun + wave * 256), 4,
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(p.s, (__attribute__((address_space(3))) void *)(dst + (T::BN + T::BM) * kRun + wave * 256), 4,
                                                  ((wave * 64 + lane) * runs + r) * 4, 0, 0, 0);
 }
 
 // One run: loads the next one into `nxt`, computes `cur`.  The pointers are restrict-qualified: the reads of `cur`
 // do not wait for the loads into `nxt`.
 template <bool kExact, int I, int J, int WN, int WM>
-__device__ __forceinline__ void tile_stage(const uint8_t *__restrict__ cur, uint8_t *__restrict__ nxt, __amdgpu_buffer_rsrc_t rw,
-                                           __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rs, int wave, int lane, int K, int runs, int r,
+__device__ __forceinline__ void tile_stage(const uint8_t *__restrict__ cur, uint8_t *__restrict__ nxt, const Panels &panels, int wave, int lane, int K, int runs, int r,
                                            float sw, int wn, int wm, floatx16 (&acc)[I][J]) {
     typedef Tile<I, J, WN, WM> T;
-    if (r + 1 < runs) tile_issue<T>(rw, ra, rs, nxt, wave, lane, K, runs, r + 1);
+    if (r + 1 < runs) tile_issue<T>(panels, nxt, wave, lane, K, runs, r + 1);
     const int fr = lane & 31, fc = (lane >> 5) * 2;
     const float *scales = reinterpret_cast<const float *>(cur + (T::BN + T::BM) * kRun) + wm + fr;
     int32x8 w[I][2];
@@ -318,11 +239,7 @@ void fp8_block_tile_kernel(GemmArgs g) {
     const int m0 = (first_m + pid % span % gm) * T::BM, n0 = pid % span / gm * T::BN;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rows_n = min(T::BN, g.N - n0), rows_m = min(T::BM, g.M - m0);
-    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(g.W + static_cast<int64_t>(n0) * g.K), 0, rows_n * g.K, 0x00020000);
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(g.A + static_cast<int64_t>(m0) * g.K), 0, rows_m * g.K, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(g.sa + static_cast<int64_t>(m0) * g.runs), 0, rows_m * g.runs * 4, 0x00020000);
-
+    const Panels panels = panels_of(g, n0, min(T::BN, g.N - n0), m0, min(T::BM, g.M - m0), lane);
     const int wn = (wave / WM) * 32 * I, wm = (wave % WM) * 32 * J;
     const int fr = lane & 31;
     floatx16 acc[I][J];
@@ -336,7 +253,7 @@ void fp8_block_tile_kernel(GemmArgs g) {
     const auto *swp = (const __attribute__((address_space(4))) float *)(g.sw + static_cast<int64_t>(min(n0 + wn, g.N - 1) / kRun) * g.runs);
 
     float sw = swp[0];
-    tile_issue<T>(rw, ra, rs, lds, wave, lane, g.K, g.runs, 0);
+    tile_issue<T>(panels, lds, wave, lane, g.K, g.runs, 0);
     for (int r = 0; r < g.runs; ++r) {
         const uint8_t *cur = lds + (r & 1) * T::kStage;
         // this wave's loads of the stage have landed, and its reads of the other stage returned; then everyone's
@@ -345,7 +262,7 @@ void fp8_block_tile_kernel(GemmArgs g) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const float sw_next = swp[min(r + 1, g.runs - 1)];
-        tile_stage<kExact, I, J, WN, WM>(cur, lds + ((r + 1) & 1) * T::kStage, rw, ra, rs, wave, lane, g.K, g.runs, r, sw, wn, wm, acc);
+        tile_stage<kExact, I, J, WN, WM>(cur, lds + ((r + 1) & 1) * T::kStage, panels, wave, lane, g.K, g.runs, r, sw, wn, wm, acc);
         sw = sw_next;
     }
 
@@ -392,6 +309,153 @@ void fp8_block_tile_kernel(GemmArgs g) {
     });
 }
 
+// ---- few tiles: K split over the waves --------------------------------------------------------------------
+//
+// Workgroup tile 32 I (n) x 32 J (m).  Each of NW waves computes the whole tile over its own runs (w, w + NW, ..), with an LDS ring
+// of its own (S stages of both panels' rows of 128 bytes and the A rows' scales), so the loop has no barrier and up to NW S
+// runs a workgroup are in flight; the tiles are summed through LDS in wave order.  Bound by the latency of the few runs that
+// each wave walks, and by HBM where N K is large: one row, 4096 x 4096, 5.9 us; one row, 11008 x 4096, 11.4 us (4.0 TB/s).
+template <int I, int J, int NW, int S>
+struct Split {
+    static constexpr int kPanels = 32 * (I + J) * kRun, kStage = kPanels + 256;
+    static constexpr int kLoads = 4 * (I + J) + 1;  // a run: 1 KB each, and the scales
+    static constexpr int kRow = 32 * I + 4;
+    static constexpr int kSums = NW * 32 * J * kRow * 4, kLds = NW * S * kStage > kSums ? NW * S * kStage : kSums;
+    static_assert(kLds <= 160 * 1024 && S * kLoads <= 63 && J <= 2, "LDS budget, vmcnt range, one load of scales");
+};
+
+// Waits until at most N vector-memory loads are outstanding and every LDS read has returned, and keeps memory accesses on
+// their side of the wait.
+template <int N>
+__device__ __forceinline__ void wait_vm_fence() {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(N) & ~(15 << 8));
+    asm volatile("" ::: "memory");
+}
+
+template <int I, int J>
+__device__ __forceinline__ void split_issue(const Panels &p, uint8_t *__restrict__ dst, int lane, int K, int runs, int r) {
+#pragma unroll
+    for (int t = 0; t < 4 * (I + J); ++t) panel_load(t < 4 * I ? p.w : p.a, p, dst + t * 1024, t < 4 * I ? t : t - 4 * I, t & 1, K, r);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(p.s, (__attribute__((address_space(3))) void *)(dst + 32 * (I + J) * kRun), 4, (lane * runs + r) * 4, 0, 0, 0);
+}
+
+// One run: refill `nxt` (read a step ago), wait for `cur`, compute it.  `ahead`: runs issued after this one's.  The slots differ
+// and are restrict-qualified: the reads of `cur` need not wait for the refill.
+template <bool kExact, int I, int J, int NW, int S>
+__device__ __forceinline__ void split_step(const uint8_t *__restrict__ cur, uint8_t *__restrict__ nxt, bool refill, const Panels &panels, int lane,
+                                           int K, int runs, int r_next, float sw, floatx16 (&acc)[I][J]) {
+    typedef Split<I, J, NW, S> P;
+    wait_vm_fence<63>();
+    if (refill) split_issue<I, J>(panels, nxt, lane, K, runs, r_next);
+    if (refill) wait_vm_fence<(S - 1) * P::kLoads>();
+    else wait_vm_fence<0>();
+    const int fr = lane & 31, fc = (lane >> 5) * 2;
+    int32x8 w[I][2], a[J][2];
+    float f[J];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+        for (int i = 0; i < I; ++i) w[i][kk] = frag(cur, 32 * i + fr, 4 * kk + fc);
+#pragma unroll
+        for (int j = 0; j < J; ++j) a[j][kk] = frag(cur + 32 * I * kRun, 32 * j + fr, 4 * kk + fc);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) f[j] = reinterpret_cast<const float *>(cur + P::kPanels)[32 * j + fr] * sw;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        floatx16 part[I];
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) part[i][q] = 0.f;
+        if constexpr (kExact) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const half8_t ah = e4m3x8_to_f16(a[j][c / 4], c % 4);
+#pragma unroll
+                for (int i = 0; i < I; ++i)
+                    part[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(e4m3x8_to_f16(w[i][c / 4], c % 4), ah, part[i], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int i = 0; i < I; ++i)
+                    part[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i][kk], a[j][kk], part[i], 0, 0, 0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = __builtin_fmaf(part[i][q], f[j], acc[i][j][q]);
+    }
+}
+
+template <bool kExact, int I, int J, int NW, int S>
+__global__ __launch_bounds__(64 * NW) void fp8_block_split_kernel(GemmArgs g) {
+    typedef Split<I, J, NW, S> P;
+    constexpr int BN = 32 * I, BM = 32 * J;
+    extern __shared__ __align__(16) uint8_t lds[];
+    // each XCD owns a contiguous run of tiles, in groups of up to 8 m tiles of one W panel
+    int pid = blockIdx.x;
+    {
+        const int per_xcd = g.tiles_m * g.tiles_n / kXcds, full = per_xcd * kXcds;
+        if (pid < full) pid = (pid % kXcds) * per_xcd + pid / kXcds;
+    }
+    const int span = 8 * g.tiles_n, first_m = pid / span * 8, gm = min(8, g.tiles_m - first_m);
+    const int m0 = (first_m + pid % span % gm) * BM, n0 = pid % span / gm * BN;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Panels panels = panels_of(g, n0, min(BN, g.N - n0), m0, min(BM, g.M - m0), lane);
+    const auto *swp = (const __attribute__((address_space(4))) float *)(g.sw + static_cast<int64_t>(n0 / kRun) * g.runs);
+    floatx16 acc[I][J];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+    const int own = g.runs > wave ? (g.runs - wave + NW - 1) / NW : 0;
+    uint8_t *ring = lds + wave * S * P::kStage;
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t)
+        if (t < own) {
+            asm volatile("" ::: "memory");  // the waits count whole runs
+            split_issue<I, J>(panels, ring + t * P::kStage, lane, g.K, g.runs, wave + NW * t);
+        }
+    for (int t0 = 0; t0 < own; t0 += S)
+        static_for<S>([&](auto SI) {
+            constexpr int s = decltype(SI)::value;
+            const int t = t0 + s;
+            if (t < own)
+                split_step<kExact, I, J, NW, S>(ring + s * P::kStage, ring + (s + S - 1) % S * P::kStage, t + S - 1 < own, panels, lane, g.K, g.runs,
+                                                wave + NW * (t + S - 1), swp[wave + NW * t], acc);
+        });
+
+    __syncthreads();  // every wave is done with its ring (all of its loads were waited for)
+    float *sums = reinterpret_cast<float *>(lds);
+    const int fr = lane & 31, fc = (lane >> 5) * 2;
+    static_for<I * J>([&](auto II) {
+        constexpr int i = decltype(II)::value / J, j = decltype(II)::value % J;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            *reinterpret_cast<floatx4 *>(sums + (wave * BM + 32 * j + fr) * P::kRow + 32 * i + 8 * t + 2 * fc) =
+                floatx4{acc[i][j][4 * t], acc[i][j][4 * t + 1], acc[i][j][4 * t + 2], acc[i][j][4 * t + 3]};
+    });
+    __syncthreads();
+#pragma unroll
+    for (int o = threadIdx.x; o < BM * BN / 4; o += 64 * NW) {
+        const int ml = o / (BN / 4), nl = o % (BN / 4) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const floatx4 p = *reinterpret_cast<const floatx4 *>(sums + (w * BM + ml) * P::kRow + nl);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] += p[q];
+        }
+        store4(g, m0 + ml, n0 + nl, v);
+    }
+}
+
 // Any shape and alignment: one thread per output, exact E4M3 decode, f32 sums.
 __global__ __launch_bounds__(256) void fp8_block_gemm_generic_kernel(GemmArgs g) {
     const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -420,13 +484,16 @@ void raise_lds_limit(const void *kern, int bytes, std::atomic<uint64_t> &done) {
     }
 }
 
-template <bool kExact, int J>
-void launch_skinny(const GemmArgs &g, hipStream_t st) {
-    constexpr int NW = 8, U = J == 1 ? 4 : 2;
-    constexpr int lds = NW * J * 16 * 20 * 4;
-    static_assert(lds <= 64 * 1024, "no raised LDS limit needed");
-    fp8_block_skinny_kernel<kExact, J, NW, U><<<dim3((g.N + 15) / 16, (g.M + 16 * J - 1) / (16 * J)), dim3(64 * NW), lds, st>>>(g);
-    check_launch("fp8_block_skinny");
+template <bool kExact, int I, int J, int NW, int S>
+void launch_split(GemmArgs g, hipStream_t st) {
+    typedef Split<I, J, NW, S> P;
+    static std::atomic<uint64_t> attr_devices{0};
+    const auto kern = fp8_block_split_kernel<kExact, I, J, NW, S>;
+    raise_lds_limit(reinterpret_cast<const void *>(kern), P::kLds, attr_devices);
+    g.tiles_m = (g.M + 32 * J - 1) / (32 * J), g.tiles_n = (g.N + 32 * I - 1) / (32 * I);
+    require(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 8, "too many tiles for one launch");
+    kern<<<dim3(g.tiles_m * g.tiles_n), dim3(64 * NW), P::kLds, st>>>(g);
+    check_launch("fp8_block_split");
 }
 
 template <bool kExact, int I, int J, int WN, int WM>
@@ -436,22 +503,32 @@ void launch_tile(GemmArgs g, hipStream_t st) {
     const auto kern = fp8_block_tile_kernel<kExact, I, J, WN, WM>;
     raise_lds_limit(reinterpret_cast<const void *>(kern), T::kLds, attr_devices);
     g.tiles_m = (g.M + T::BM - 1) / T::BM, g.tiles_n = (g.N + T::BN - 1) / T::BN;
+    require(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 8, "too many tiles for one launch");
     kern<<<dim3(g.tiles_m * g.tiles_n), dim3(64 * T::NW), T::kLds, st>>>(g);
     check_launch("fp8_block_tile");
 }
 
+// The cheapest kernel by the rounds of its workgroups over the CUs, in us at K = 4096 (all grow with K alike; measured, fp8 and exact
+// form, beside what the next candidate takes there):
+//   32 x 32, K over 8 waves     4.5 (4.9) a round    M = 1: 5.9 us; M = 64, N = 4096: 7.3 (64 x 64: 12.2)
+//   64 x 64, K over 4 waves     10.3 (12.7) a round  M = 256, N = 4096: 12.8 (128 x 128: 26); M = 64, N = 11008: 12.8 (32 x 32: 16.2)
+//   128 x 128, two a CU         20.5 (35) times tiles over CUs, at least 24.5 (33)
+//                                                    M = 1024, N = 4096: 28.7 (64 x 64: 42); M = 256, N = 11008: 27 (31.5)
+//   256 x 256, fp8 form         70 a round, 54 for one that leaves CUs idle
+//                                                    M = 4096, N = 11008: 208 (128 x 128: 246); M = 1024, N = 11008: 61 (67)
 template <bool kExact>
-void launch_by_shape(const GemmArgs &g, hipStream_t st) {
-    if (g.M <= 16) launch_skinny<kExact, 1>(g, st);
-    else if (g.M <= 32) launch_skinny<kExact, 2>(g, st);
-    else if (g.M <= 64) launch_skinny<kExact, 4>(g, st);
-    else if constexpr (kExact) launch_tile<kExact, 2, 2, 2, 2>(g, st);
-    else {
-        const int64_t cus = cu_count();
-        const int64_t big = static_cast<int64_t>((g.M + 255) / 256) * ((g.N + 255) / 256);
-        if (big * 4 <= cus * 2) launch_tile<kExact, 2, 2, 2, 2>(g, st);
-        else launch_tile<kExact, 2, 4, 4, 2>(g, st);
-    }
+void launch_by_cost(const GemmArgs &g, hipStream_t st) {
+    const double cus = static_cast<double>(cu_count());
+    const auto tiles = [&](int t) { return static_cast<double>((g.M + t - 1) / t) * ((g.N + t - 1) / t); };
+    const auto rounds = [&](int t) { return std::ceil(tiles(t) / cus); };
+    const double c32 = (kExact ? 4.9 : 4.5) * rounds(32), c64 = (kExact ? 12.7 : 10.3) * rounds(64);
+    const double c128 = kExact ? std::max(33.0, 35 * tiles(128) / cus) : std::max(24.5, 20.5 * tiles(128) / cus);
+    const double c256 = kExact ? 1e30 : tiles(256) < 0.9 * cus ? 54 : 70 * rounds(256);
+    const double best = std::min({c32, c64, c128, c256});
+    if (best == c32) launch_split<kExact, 1, 1, 8, 2>(g, st);
+    else if (best == c64) launch_split<kExact, 2, 2, 4, 2>(g, st);
+    else if (kExact || best == c128) launch_tile<kExact, 2, 2, 2, 2>(g, st);
+    else if constexpr (!kExact) launch_tile<false, 2, 4, 4, 2>(g, st);
 }
 
 }  // namespace
@@ -474,8 +551,8 @@ extern "C" int32_t castforge_hip_gemm_fp8_block(const uint8_t *qa, const float *
                    static_cast<int>(n), static_cast<int>(k), static_cast<int>((k + kRun - 1) / kRun), 0, 0};
         // buffer resources address a panel of 256 rows: 256 k bytes must fit in 31 bits
         const bool fast = k > 0 && k % 16 == 0 && k < (1 << 23) && aligned(qa, 16) && aligned(qw, 16);
-        if (fast && (m + 127) / 128 * ((n + 127) / 128) <= 0x7fffffff) {
-            exact ? launch_by_shape<true>(g, st) : launch_by_shape<false>(g, st);
+        if (fast) {
+            exact ? launch_by_cost<true>(g, st) : launch_by_cost<false>(g, st);
             return;
         }
         const int64_t tot = m * n;
