@@ -8,6 +8,7 @@
 //
 // The softmax's maximum and sum, the scores and the output sums are f32.
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/castforge_hip.h"
 #include "cfh_common.hpp"
@@ -134,18 +135,22 @@ struct KvTile {
     bool live[2];           // uniform: the half's page is one of the cache's
 };
 
-// What a wave makes of the group words of 32 tokens, once, each lane for one token's keys or values: in LDS, where
-// the lanes that need a token's numbers read them four tokens at a time.
-template <int D, int G>
-struct TokenTable {
-    static constexpr int GR = D / G;
-    static constexpr bool kDeal = KvTile<D, G>::kDeal;
-    float scale[2][GR][32];    // keys: scale times what turns a product into a score; values: scale without its exponent
-    float exponent[32], back[32];  // of the values' largest scale, 2^-exponent
-    static constexpr int kRow = 36;      // tokens a row of `v`, padded for the banks
-    uint32_t v[kDeal ? 16 * kRow : 4];   // the values' codes: word by word, a token each
-    uint32_t kz[GR][32];       // zero point in both halves, as f16 denormals
-    uint16_t vz[GR][32];
+// What the group words of N tokens say, in LDS: worked out once, each lane for one token's keys or values, and read four tokens
+// at a time.
+template <int GR, int N>
+struct Tokens {
+    float scale[2][GR][N];  // keys: scale times what turns a product into a score; values: scale without its exponent
+    float exponent[N];      // of the values' largest scale; -inf where there is no token
+    float back[N];          // 2^-exponent
+};
+
+// A wave's zero points of N tokens, and its deal of the values' words.
+template <int D, int G, int N>
+struct Zeros {
+    static constexpr int GR = D / G, kRow = N + 4;   // tokens a row of `v`, padded for the banks
+    uint32_t v[KvTile<D, G>::kDeal ? 16 * kRow : 4];  // the values' codes: word by word, a token each
+    uint32_t k[GR][N];  // zero point in both halves, as f16 denormals
+    uint16_t z[GR][N];  // of the values
 };
 
 template <int D, int G>
@@ -191,38 +196,43 @@ __device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, in
 // LDS accesses of one wave keep their order; the compiler must not move them past each other either.
 __device__ __forceinline__ void wave_order() { asm volatile("" ::: "memory"); }
 
-template <int D, int G>
-__device__ __forceinline__ void fill_table(const KvTile<D, G> &t, TokenTable<D, G> &table, int at, int len, bool edge, float qk) {
-    constexpr int GR = D / G;
-    const int lane = threadIdx.x & 63, token = lane & 31;
-    const bool value = lane >= 32;
-    // places past the length or of no page may hold anything
-    const bool off = edge && (!(token < 16 ? t.live[0] : t.live[1]) || at + token >= len);
+// The lane's token (`token` of the table; value: its values' words, else its keys') into the tables.  off: there is no such token,
+// and its words may be anything.
+template <int GR, int N, class Z>
+__device__ __forceinline__ void fill_token(const uint32_t (&words)[GR], bool value, int token, bool off, float qk, Tokens<GR, N> &tokens, Z &zeros, int own) {
     float v[GR], top = 0.f;
-    uint32_t z[GR];
 #pragma unroll
     for (int gr = 0; gr < GR; ++gr) {
-        const uint32_t w = off ? 0u : t.words[gr];
+        const uint32_t w = off ? 0u : words[gr];
         v[gr] = kv4_scale(w);
-        z[gr] = kv4_zero(w);
         top = fmaxf(top, v[gr]);
+        if (value) zeros.z[gr][own] = static_cast<uint16_t>(kv4_zero(w));
+        else zeros.k[gr][own] = kv4_zero(w) * 0x00010001u;
     }
     const int ex = __builtin_amdgcn_frexp_expf(top);
-    wave_order();
-    if constexpr (KvTile<D, G>::kDeal) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<uint4 *>(&table.v[(lane & 15) * TokenTable<D, G>::kRow + 16 * h + 4 * (lane >> 4)]) =
-                make_uint4(t.vc[h][0][0], t.vc[h][1][0], t.vc[h][2][0], t.vc[h][3][0]);
+    for (int gr = 0; gr < GR; ++gr) tokens.scale[value][gr][token] = value ? __builtin_ldexpf(v[gr], -ex) : v[gr] * qk;
+    if (value) tokens.exponent[token] = off ? -INFINITY : static_cast<float>(ex), tokens.back[token] = __builtin_ldexpf(1.0f, -ex);
+}
+
+// Four tokens' words of a row of V^T as pairs of tokens, codes 0 .. 3 and 4 .. 7: the row is word n % (G / 8) of the group, and its
+// codes are those from n / (G / 8) on in steps of R = 128 / G.
+struct Pairs {
+    uint32_t lo[2], hi[2];
+};
+template <int G>
+__device__ __forceinline__ Pairs pairs_of(uint4 w, int n) {
+    if constexpr (G < 128) {
+        const int sh = 4 * (n / (G / 8));
+        w.x >>= sh, w.y >>= sh, w.z >>= sh, w.w >>= sh;
     }
-#pragma unroll
-    for (int gr = 0; gr < GR; ++gr) {
-        table.scale[value][gr][token] = value ? __builtin_ldexpf(v[gr], -ex) : v[gr] * qk;
-        if (value) table.vz[gr][token] = static_cast<uint16_t>(z[gr]);
-        else table.kz[gr][token] = z[gr] * 0x00010001u;
-    }
-    if (value) table.exponent[token] = static_cast<float>(ex), table.back[token] = __builtin_ldexpf(1.0f, -ex);
-    wave_order();
+    return Pairs{{low_halves(w.x, w.y), low_halves(w.z, w.w)}, {high_halves(w.x, w.y), high_halves(w.z, w.w)}};
+}
+
+// Code `code` of pair i without its zero points.
+__device__ __forceinline__ uint32_t pair_code(const Pairs &p, int i, int code, uint32_t z) {
+    const uint32_t x = code < 4 ? p.lo[i] : p.hi[i], y = code % 4 < 2 ? x : x >> 8;
+    return code % 2 == 0 ? minus(y & 0x000F000Fu, z) : minus(y & 0x00F000F0u, z << 4);
 }
 
 // Rows of a wave: 16 MT of the n * ratio (query, head of the group) pairs of a sequence and a head of keys, row = query *
@@ -284,31 +294,30 @@ __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, 
 // the scales are; the sum takes the 2^-e_t back.  m is 7 below the largest so far when it moves, and it moves only
 // when something exceeds it by 15: weights stay below 2^15, the largest ones above 2^7 (f16 keeps its 11 bits
 // down to 2^-21 of them), and the rescaling is rare.
-template <int D, int G, int MT>
-__device__ __forceinline__ void attend(const KvTile<D, G> &t, TokenTable<D, G> &table, Rows<D, G, MT> &s, int at, int len, int sure, float qk) {
-    constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = 8 / R;
-    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-    const bool edge = at + 32 > sure || !t.live[0] || !t.live[1];  // uniform: some row does not see some token
-    fill_table<D, G>(t, table, at, len, edge, qk);
-    float y[MT][2][4];            // scores and their tokens' exponents, base 2
+// keys(h, gr, u): the MFMA operand of half h's 16 tokens and 32 channels; values(gr) prepares a group's rows of V^T and gives what
+// turns u into the operand of 16 channels and 32 tokens.  first: the tokens' place in the table.
+template <int D, int G, int MT, int N, class Keys, class Values>
+__device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first, Rows<D, G, MT> &s, int at, int sure, const Keys &keys, const Values &values) {
+    constexpr int GR = D / G, W = G / 32, NT = G / 16;
+    const int g = (threadIdx.x >> 4) & 3;
+    const bool edge = at + 32 > sure;  // uniform: some row does not see some token
+    const auto four = [&](const float *p, int h) { return *reinterpret_cast<const floatx4 *>(p + first + 16 * h + 4 * g); };
+    float y[MT][2][4];  // scores and their tokens' exponents, base 2
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        floatx4 ks[GR];
+        floatx4 ks[GR], dot[MT][GR];
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) ks[gr] = *reinterpret_cast<const floatx4 *>(&table.scale[0][gr][16 * h + 4 * g]);
-        const floatx4 e = *reinterpret_cast<const floatx4 *>(&table.exponent[16 * h + 4 * g]);
-        floatx4 dot[MT][GR];
+        for (int gr = 0; gr < GR; ++gr) ks[gr] = four(tokens.scale[0][gr], h);
+        const floatx4 e = four(tokens.exponent, h);
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) {
-            const uint32_t zz = table.kz[gr][16 * h + n];
+        for (int gr = 0; gr < GR; ++gr)
 #pragma unroll
             for (int u = 0; u < W; ++u) {
-                const halfx8 k = codes_f16(t.kc[h][gr][u], zz);
+                const halfx8 k = keys(h, gr, u);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
                     dot[mt][gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, s.q[mt][gr][u], u ? dot[mt][gr] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             }
-        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -317,100 +326,85 @@ __device__ __forceinline__ void attend(const KvTile<D, G> &t, TokenTable<D, G> &
 #pragma unroll
                 for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], v);
                 v = __builtin_fmaf(v, s.unit[mt], e[r]);
-                if (edge && (!t.live[h] || at + 16 * h + 4 * g + r >= s.limit[mt])) v = -INFINITY;
+                if (edge && at + 16 * h + 4 * g + r >= s.limit[mt]) v = -INFINITY;
                 y[mt][h][r] = v;
             }
     }
-    floatx4 back[2], c[2][GR];
-    uint2 zp[2][GR];        // zero points of the values, pairs of tokens
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        back[h] = *reinterpret_cast<const floatx4 *>(&table.back[16 * h + 4 * g]);
-#pragma unroll
-        for (int gr = 0; gr < GR; ++gr) {
-            c[h][gr] = *reinterpret_cast<const floatx4 *>(&table.scale[1][gr][16 * h + 4 * g]);
-            zp[h][gr] = *reinterpret_cast<const uint2 *>(&table.vz[gr][16 * h + 4 * g]);
-        }
-    }
     uint32_t p[MT][GR][4];  // weights times c as f16 pairs: tokens (0, 1), (2, 3) of both halves
+    {
+        floatx4 back[2], c[2][GR];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        float top = y[mt][0][0];
+        for (int h = 0; h < 2; ++h) {
+            back[h] = four(tokens.back, h);
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, y[mt][i / 4][i % 4]);
-        if (__any(top > s.m[mt] + 15.f)) {
-            const float m = fmaxf(s.m[mt], max_over_g(top) - 7.f), f = __builtin_amdgcn_exp2f(s.m[mt] - m);
-            s.m[mt] = m;
-            s.l[mt] *= f;
+            for (int gr = 0; gr < GR; ++gr) c[h][gr] = four(tokens.scale[1][gr], h);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float top = y[mt][0][0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) top = fmaxf(top, y[mt][i / 4][i % 4]);
+            if (__any(top > s.m[mt] + 15.f)) {
+                const float m = fmaxf(s.m[mt], max_over_g(top) - 7.f), f = __builtin_amdgcn_exp2f(s.m[mt] - m);
+                s.m[mt] = m;
+                s.l[mt] *= f;
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) s.o[mt][gr][u] *= f;
+            }
+            float w[2][4];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i / 4][i % 4] = __builtin_amdgcn_exp2f(y[mt][i / 4][i % 4] - s.m[mt]);
+                s.l[mt] = __builtin_fmaf(w[i / 4][i % 4], back[i / 4][i % 4], s.l[mt]);
+            }
 #pragma unroll
             for (int gr = 0; gr < GR; ++gr)
 #pragma unroll
-                for (int u = 0; u < NT; ++u) s.o[mt][gr][u] *= f;
+                for (int i = 0; i < 4; ++i) {
+                    const int h = i / 2, r = i % 2 * 2;
+                    const halfx2 v = {static_cast<_Float16>(w[h][r] * c[h][gr][r]), static_cast<_Float16>(w[h][r + 1] * c[h][gr][r + 1])};
+                    p[mt][gr][i] = __builtin_bit_cast(uint32_t, v);
+                }
         }
-        float w[2][4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            w[i / 4][i % 4] = __builtin_amdgcn_exp2f(y[mt][i / 4][i % 4] - s.m[mt]);
-            s.l[mt] = __builtin_fmaf(w[i / 4][i % 4], back[i / 4][i % 4], s.l[mt]);
-        }
-#pragma unroll
-        for (int gr = 0; gr < GR; ++gr)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int h = i / 2, r = i % 2 * 2;
-                const halfx2 v = {static_cast<_Float16>(w[h][r] * c[h][gr][r]), static_cast<_Float16>(w[h][r + 1] * c[h][gr][r + 1])};
-                p[mt][gr][i] = __builtin_bit_cast(uint32_t, v);
-            }
     }
 #pragma unroll
     for (int gr = 0; gr < GR; ++gr) {
         halfx8 pw[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) pw[mt] = eight(p[mt][gr][0], p[mt][gr][1], p[mt][gr][2], p[mt][gr][3]);
-        // a row of V^T is word n % (G / 8), codes from n / (G / 8) on in steps of R
-        uint32_t lo[4], hi[4];
+        const auto operand = values(gr);
+        static_for<NT>([&](auto u) __attribute__((always_inline)) {
+            const halfx8 v = operand(u);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint4 w;
-            if constexpr (KvTile<D, G>::kDeal)
-                w = *reinterpret_cast<const uint4 *>(&table.v[(gr * (G / 8) + n % (G / 8)) * TokenTable<D, G>::kRow + 16 * h + 4 * g]);
-            else
-                w = make_uint4(t.vc[h][0][gr], t.vc[h][1][gr], t.vc[h][2][gr], t.vc[h][3][gr]);
-            if constexpr (R > 1) {
-                const int sh = 4 * (n / (G / 8));
-                w.x >>= sh, w.y >>= sh, w.z >>= sh, w.w >>= sh;
-            }
-            lo[2 * h] = low_halves(w.x, w.y), lo[2 * h + 1] = low_halves(w.z, w.w);
-            hi[2 * h] = high_halves(w.x, w.y), hi[2 * h + 1] = high_halves(w.z, w.w);
-        }
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            const int code = R * u;  // position in the (shifted) word
-            uint32_t v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t x = code < 4 ? lo[i] : hi[i];
-                const uint32_t y = code % 4 < 2 ? x : x >> 8, z = i % 2 ? zp[i / 2][gr].y : zp[i / 2][gr].x;
-                v[i] = code % 2 == 0 ? minus(y & 0x000F000Fu, z) : minus(y & 0x00F000F0u, z << 4);
-            }
-            const halfx8 vv = eight(v[0], v[1], v[2], v[3]);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) s.o[mt][gr][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pw[mt], s.o[mt][gr][u], 0, 0, 0);
-        }
+            for (int mt = 0; mt < MT; ++mt) s.o[mt][gr][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pw[mt], s.o[mt][gr][u], 0, 0, 0);
+        });
     }
 }
 
-// Row tile's walk over tokens first, first + step, .. (of 32) below end, the next tile's loads in flight.
+// The least of the rows' limits: tokens below it are seen by every row of the wave.
 template <int D, int G, int MT>
-__device__ __forceinline__ void walk(const AttnArgs &a, TokenTable<D, G> &tokens, Rows<D, G, MT> &s, const Seq &sq, int head, int first, int step, int end) {
-    if (first >= end) return;
-    int sure = sq.len;  // tokens that every row sees
+__device__ __forceinline__ int seen_by_all(const Rows<D, G, MT> &s, int len) {
+    int sure = len;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) sure = min(sure, s.limit[mt]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sure = min(sure, __shfl_xor(sure, o));
-    sure = __builtin_amdgcn_readfirstlane(sure);
-    const float qk = a.scale * (1.44269504088896341f * 0x1p24f);  // the codes' 2^-24 undone
+    return __builtin_amdgcn_readfirstlane(sure);
+}
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// A wave's walk over tokens first, first + step, .. (of 32) below end, the next tile's loads in flight.
+template <int D, int G, int MT>
+__device__ __forceinline__ void walk(const AttnArgs &a, Tokens<D / G, 32> &tokens, Zeros<D, G, 32> &zeros, Rows<D, G, MT> &s, const Seq &sq, int head,
+                                     int first, int step, int end) {
+    constexpr int R = 128 / G;
+    if (first >= end) return;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int sure = seen_by_all(s, sq.len);
+    const float qk = a.scale * (kLog2e * 0x1p24f);  // the codes' 2^-24 undone
     const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
     const auto pages = [&](int at, int (&p)[2]) {
 #pragma unroll
@@ -429,7 +423,33 @@ __device__ __forceinline__ void walk(const AttnArgs &a, TokenTable<D, G> &tokens
         } else {
             next = cur;
         }
-        attend<D, G, MT>(cur, tokens, s, at, sq.len, sure, qk);
+        const int token = lane & 31;
+        wave_order();
+        fill_token(cur.words, lane >= 32, token, !(token < 16 ? cur.live[0] : cur.live[1]) || at + token >= sq.len, qk, tokens, zeros, token);
+        if constexpr (KvTile<D, G>::kDeal) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<uint4 *>(&zeros.v[n * Zeros<D, G, 32>::kRow + 16 * h + 4 * g]) = make_uint4(cur.vc[h][0][0], cur.vc[h][1][0], cur.vc[h][2][0], cur.vc[h][3][0]);
+        }
+        wave_order();
+        attend<D, G, MT>(
+            tokens, 0, s, at, sure, [&](int h, int gr, int u) { return codes_f16(cur.kc[h][gr][u], zeros.k[gr][16 * h + n]); },
+            [&](int gr) {
+                Pairs p[2];
+                uint2 z[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (KvTile<D, G>::kDeal)
+                        p[h] = pairs_of<G>(*reinterpret_cast<const uint4 *>(&zeros.v[(gr * (G / 8) + n % (G / 8)) * Zeros<D, G, 32>::kRow + 16 * h + 4 * g]), n);
+                    else
+                        p[h] = pairs_of<G>(make_uint4(cur.vc[h][0][gr], cur.vc[h][1][gr], cur.vc[h][2][gr], cur.vc[h][3][gr]), n);
+                    z[h] = *reinterpret_cast<const uint2 *>(&zeros.z[gr][16 * h + 4 * g]);
+                }
+                return [=](int u) {
+                    return eight(pair_code(p[0], 0, R * u, z[0].x), pair_code(p[0], 1, R * u, z[0].y), pair_code(p[1], 0, R * u, z[1].x),
+                                 pair_code(p[1], 1, R * u, z[1].y));
+                };
+            });
         cur = next;
     }
 }
@@ -459,11 +479,12 @@ __device__ __forceinline__ void settle(Rows<D, G, MT> &s) {
 // One workgroup's four waves take the same rows and every fourth 32 tokens of a split's share, and are joined through
 // LDS; splits are joined by kv4_attention_join_kernel.  For few rows a sequence: bound by the cache's bytes.
 template <int D, int G, int MT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((D == 128 && G < 128) || MT > 1 ? 2 : 4))) void kv4_attention_split_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((D == 128 && G < 128) || MT > 1 ? 2 : G == 32 ? 3 : 4))) void kv4_attention_split_kernel(AttnArgs a) {
     typedef Rows<D, G, MT> S;
     constexpr int kRow = D + 4;
     __shared__ __align__(16) float sums[4][16][kRow];
-    __shared__ __align__(16) TokenTable<D, G> tokens[4];
+    __shared__ __align__(16) Tokens<D / G, 32> tokens[4];
+    __shared__ __align__(16) Zeros<D, G, 32> zeros[4];
     __shared__ float ml[2][4][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
@@ -480,7 +501,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((D == 128 &
     const int first = split * share, end = min(seen, first + share);
     S s;
     load_rows<D, G, MT>(a, s, sq, head, row0);
-    walk<D, G, MT>(a, tokens[wave], s, sq, head, first + 32 * wave, 128, end);
+    walk<D, G, MT>(a, tokens[wave], zeros[wave], s, sq, head, first + 32 * wave, 128, end);
     settle<D, G, MT>(s);
     const int hq = a.heads * a.ratio;
 #pragma unroll
@@ -581,55 +602,133 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
     }
 }
 
-// Each wave takes rows of its own and all the tokens that they see.  For many rows: bound by the softmax's and the codes' VALU
-// work.  Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row
-// tiles from the last, which see the most tokens.
+// Many rows: each wave takes 16 MT rows of its own, and the four of a workgroup share the work on the codes.  Of every 64 tokens
+// a wave turns 16 into MFMA operands in LDS (f16, codes less zero points, exactly) and all four read them back; two stages, one
+// barrier a stage: the operands of the next 64 tokens are made while the present ones are used, and the words of those after
+// that are on their way.  Bound by VALU work, the softmax's most of all.
+// Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row tiles from the
+// last, which see the most tokens.
+template <int D, int G>
+struct Stage {
+    static constexpr int GR = D / G, kSteps = D / 32, kTiles = D / 16;
+    uint4 keys[4][kSteps][64];      // 16 tokens, 32 channels: a lane's operand
+    uint4 values[2][kTiles][64];    // 32 tokens, 16 channels
+    Tokens<GR, 64> tokens;
+};
+
 template <int D, int G, int MT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void kv4_attention_rows_kernel(AttnArgs a, int tiles) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void kv4_attention_tile_kernel(AttnArgs a, int tiles) {
     typedef Rows<D, G, MT> S;
-    constexpr int kRow = D + 4;
-    __shared__ __align__(16) float sums[4][16][kRow];
-    __shared__ __align__(16) TokenTable<D, G> tokens[4];
-    __shared__ float ls[4][2][16];
+    constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = G / 16, kWords = D / 8, VW = KvTile<D, G>::VW, kRow = D + 4;
+    extern __shared__ __align__(16) uint8_t lds[];
+    Stage<D, G> *stages = reinterpret_cast<Stage<D, G> *>(lds);
+    __shared__ __align__(16) Zeros<D, G, 16> own[4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const int n = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % a.heads;
     const Seq sq = find_tile(a, tiles - 1 - blockIdx.x / a.heads, 64 * MT);
     if (sq.seq < 0) return;
-    const int row0 = sq.tile * 64 * MT + wave * 16 * MT, total = sq.n * a.ratio;
-    if (row0 >= total) return;  // no barrier below
-    const int rows = min(16 * MT, total - row0);
-    const int seen = a.causal ? max(0, min(sq.len, sq.len - sq.n + (row0 + rows - 1) / a.ratio + 1)) : sq.len;
+    const int total = sq.n * a.ratio, row_of_all = sq.tile * 64 * MT, row0 = row_of_all + wave * 16 * MT;
+    const auto seen = [&](int last_row) { return a.causal ? max(0, min(sq.len, sq.len - sq.n + last_row / a.ratio + 1)) : sq.len; };
+    const int end = seen(min(row_of_all + 64 * MT, total) - 1);  // of the workgroup
+    const int mine = row0 < total ? seen(min(row0 + 16 * MT, total) - 1) : 0;
     S s;
     load_rows<D, G, MT>(a, s, sq, head, row0);
-    walk<D, G, MT>(a, tokens[wave], s, sq, head, 0, 32, seen);
+    const int sure = seen_by_all(s, sq.len);
+    const float qk = a.scale * (kLog2e * 0x1p24f);  // the codes' 2^-24 undone
+    const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
+    Zeros<D, G, 16> &zeros = own[wave];
+
+    // this wave's 16 tokens of a stage
+    struct Part {
+        uint32_t kc[GR][W], vc[4][VW], words[GR];
+        bool live;
+    };
+    const auto page_of = [&](int at) { return at < end ? scalar_load(table, at >> a.page_shift) : -1; };
+    const auto load = [&](Part &t, int page, int at) {
+        t.live = at < end && page >= 0 && page < a.num_pages;
+        const int64_t row = kv4_row(t.live ? page : 0, head, at & ((1 << a.page_shift) - 1), a.heads, a.page_shift);
+        const uint32_t *kc = a.k_codes + row * kWords + n * kWords + g * W;
+        const uint32_t *vc = a.v_codes + row * kWords + 4 * g * kWords + (KvTile<D, G>::kDeal ? n : n % (G / 8));
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) __builtin_memcpy(t.kc[gr], __builtin_assume_aligned(kc + gr * (G / 8), 4 * W), 4 * W);
+#pragma unroll
+        for (int i = 0; i < VW; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t.vc[r][i] = vc[r * kWords + i * (G / 8)];
+        __builtin_memcpy(t.words, __builtin_assume_aligned((lane & 16 ? a.v_groups : a.k_groups) + (row + n) * GR, 4 * GR), 4 * GR);
+    };
+    const auto make = [&](const Part &t, Stage<D, G> &st, int at) {
+        wave_order();
+        if (lane < 32) fill_token(t.words, lane >= 16, 16 * wave + n, !t.live || at + n >= sq.len, qk, st.tokens, zeros, n);
+        if constexpr (KvTile<D, G>::kDeal) *reinterpret_cast<uint4 *>(&zeros.v[n * Zeros<D, G, 16>::kRow + 4 * g]) = make_uint4(t.vc[0][0], t.vc[1][0], t.vc[2][0], t.vc[3][0]);
+        wave_order();
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+            const uint32_t zz = zeros.k[gr][n];
+#pragma unroll
+            for (int u = 0; u < W; ++u) st.keys[wave][gr * W + u][lane] = __builtin_bit_cast(uint4, codes_f16(t.kc[gr][u], zz));
+            uint4 w;
+            if constexpr (KvTile<D, G>::kDeal) w = *reinterpret_cast<const uint4 *>(&zeros.v[(gr * (G / 8) + n % (G / 8)) * Zeros<D, G, 16>::kRow + 4 * g]);
+            else w = make_uint4(t.vc[0][gr], t.vc[1][gr], t.vc[2][gr], t.vc[3][gr]);
+            const Pairs p = pairs_of<G>(w, n);
+            const uint2 z = *reinterpret_cast<const uint2 *>(&zeros.z[gr][4 * g]);
+            static_for<NT>([&](auto u) __attribute__((always_inline)) {
+                reinterpret_cast<uint2 *>(&st.values[wave / 2][gr * NT + u][lane])[wave % 2] = make_uint2(pair_code(p, 0, R * u, z.x), pair_code(p, 1, R * u, z.y));
+            });
+        }
+    };
+    Part part;
+    if (end > 0) {
+        load(part, page_of(16 * wave), 16 * wave);
+        make(part, stages[0], 16 * wave);
+        load(part, page_of(64 + 16 * wave), 64 + 16 * wave);
+    }
+    int page = page_of(128 + 16 * wave);
+    for (int at = 0, i = 0; at < end; at += 64, i ^= 1) {
+        __syncthreads();  // stage i is made, and the other one no longer read
+        if (at + 64 < end) {
+            make(part, stages[i ^ 1], at + 64 + 16 * wave);
+            load(part, page, at + 128 + 16 * wave);
+            page = page_of(at + 192 + 16 * wave);
+        }
+        const Stage<D, G> &st = stages[i];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            if (at + 32 * sub >= mine) break;
+            attend<D, G, MT>(
+                st.tokens, 32 * sub, s, at + 32 * sub, sure, [&](int h, int gr, int u) { return __builtin_bit_cast(halfx8, st.keys[2 * sub + h][gr * W + u][lane]); },
+                [&](int gr) { return [&st, gr, sub, lane](int u) { return __builtin_bit_cast(halfx8, st.values[sub][gr * NT + u][lane]); }; });
+        }
+    }
     settle<D, G, MT>(s);
-    const int hq = a.heads * a.ratio;
+    __syncthreads();  // the stages' LDS now holds outputs, each wave's own part
+    if (row0 >= total) return;
+    float (*sums)[kRow] = reinterpret_cast<float (*)[kRow]>(lds) + 16 * wave;
+    const int hq = a.heads * a.ratio, rows = min(16 * MT, total - row0);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (16 * mt >= rows) break;
-        // a wave's own part of LDS, in order within the wave
+        const float l = s.l[mt], inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int gr = 0; gr < S::GR; ++gr)
+        for (int gr = 0; gr < GR; ++gr)
 #pragma unroll
-            for (int u = 0; u < S::NT; ++u)
+            for (int u = 0; u < NT; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sums[wave][n][channel<G>(g, r, gr, u)] = s.o[mt][gr][u][r];
-        if (g == 0) ls[wave][0][n] = s.m[mt], ls[wave][1][n] = s.l[mt];
+                for (int r = 0; r < 4; ++r) sums[n][channel<G>(g, r, gr, u)] = s.o[mt][gr][u][r] * inv;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int row = row0 + 16 * mt + n;
+        if (a.lse && g == 0 && row < total)
+            a.lse[static_cast<int64_t>(sq.first + row / a.ratio) * hq + head * a.ratio + row % a.ratio] = l == 0.f ? -INFINITY : (s.m[mt] + log2f(l)) * 0.693147180559945309f;
 #pragma unroll
-        for (int i = lane; i < 16 * (D / 8); i += 64) {
-            const int rl = i / (D / 8), ch = i % (D / 8) * 8, row = row0 + 16 * mt + rl;
-            if (row >= total) continue;
-            const int64_t at = static_cast<int64_t>(sq.first + row / a.ratio) * hq + head * a.ratio + row % a.ratio;
-            const float l = ls[wave][1][rl], inv = l == 0.f ? 0.f : 1.0f / l;
-            const float *v = &sums[wave][rl][ch];
-            uint4 o;
-            o.x = f32x2_to_bf16x2_rne(v[0] * inv, v[1] * inv), o.y = f32x2_to_bf16x2_rne(v[2] * inv, v[3] * inv);
-            o.z = f32x2_to_bf16x2_rne(v[4] * inv, v[5] * inv), o.w = f32x2_to_bf16x2_rne(v[6] * inv, v[7] * inv);
-            *reinterpret_cast<uint4 *>(a.out + at * D + ch) = o;
-            if (a.lse && ch == 0) a.lse[at] = l == 0.f ? -INFINITY : (ls[wave][0][rl] + log2f(l)) * 0.693147180559945309f;
+        for (int k = lane; k < 16 * (D / 8); k += 64) {
+            const int rl = k / (D / 8), ch = k % (D / 8) * 8, to = row0 + 16 * mt + rl;
+            if (to >= total) continue;
+            const int64_t out = static_cast<int64_t>(sq.first + to / a.ratio) * hq + head * a.ratio + to % a.ratio;
+            const float *v = &sums[rl][ch];
+            *reinterpret_cast<uint4 *>(a.out + out * D + ch) =
+                make_uint4(f32x2_to_bf16x2_rne(v[0], v[1]), f32x2_to_bf16x2_rne(v[2], v[3]), f32x2_to_bf16x2_rne(v[4], v[5]), f32x2_to_bf16x2_rne(v[6], v[7]));
         }
     }
 }
@@ -667,6 +766,29 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
     if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
     return p;
+}
+
+// Raises a kernel's dynamic-LDS limit once per device (bit = device ordinal < 64).
+void raise_lds_limit(const void *kern, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    check_hip(hipGetDevice(&dev), "hipGetDevice");
+    const uint64_t bit = dev < 64 ? (uint64_t{1} << dev) : 0;
+    if (bit == 0 || !(done.load(std::memory_order_acquire) & bit)) {
+        check_hip(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute(attention)");
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+}
+
+template <int D, int G>
+void launch_tile(const AttnArgs &a, const Plan &p, hipStream_t st) {
+    constexpr int MT = most_tiles(D, G), sums = 64 * (D + 4) * 4, stages = 2 * sizeof(Stage<D, G>), lds = stages > sums ? stages : sums;
+    static_assert(lds + 4 * sizeof(Zeros<D, G, 16>) <= 80 * 1024, "two workgroups a CU");
+    require(p.tiles * a.heads <= 0x7fffffff, "too many workgroups for one launch");
+    static std::atomic<uint64_t> attr_devices{0};
+    const auto kern = kv4_attention_tile_kernel<D, G, MT>;
+    raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
+    kern<<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(256), lds, st>>>(a, static_cast<int>(p.tiles));
+    check_launch("kv4_attention_tile");
 }
 
 template <int D, int G, int MT>
@@ -733,9 +855,7 @@ int32_t castforge_hip_kv4_attention(const cfh_kv4_cache_t *cache, const uint16_t
         kv4_by_shape(cache, [&](auto d, auto gr) {
             constexpr int D = decltype(d)::value, G = decltype(gr)::value;
             if (p.rows) {
-                require(p.tiles * a.heads <= 0x7fffffff, "too many workgroups for one launch");
-                kv4_attention_rows_kernel<D, G, most_tiles(D, G)><<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(256), 0, st>>>(a, static_cast<int>(p.tiles));
-                check_launch("kv4_attention_rows");
+                launch_tile<D, G>(a, p, st);
             } else if (p.mt == 1) {
                 launch_split<D, G, 1>(a, p, st);
             } else if constexpr (most_tiles(D, G) > 1) {

@@ -144,6 +144,33 @@ def test_long_context_and_prompt(cuda, d, group):
     _run(cuda, [6, 2], [6000, 3000], 2, 4, d, group, 32, seed=8)
 
 
+@pytest.mark.parametrize("d,group", SHAPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hkv,ratio,page,lens", [
+    (8, 4, 64, [(1500, 1500), (700, 1203), (1, 65)]), (4, 8, 16, [(1037, 1037), (3, 1), (0, 9), (60, 20)]),
+    (1, 40, 128, [(901, 1000)]), (16, 1, 32, [(2100, 2112)]), (8, 3, 4096, [(1, 5000), (1400, 1399)])])
+def test_whole_prompts(cuda, d, group, causal, hkv, ratio, page, lens):
+    """Enough rows for every wave to have its own."""
+    q, cache, table, kv, cu, ref = _run(cuda, [n for n, _ in lens], [k for _, k in lens], hkv, ratio, d, group, page, causal, seed=30 + hkv)
+    last = lens[0][1] - 1
+    if lens[0][1] % page:  # what lies past the first sequence's last token changes nothing
+        at = table[0, last // page].item()
+        for g in (cache.k_groups, cache.v_groups):
+            g[at, :, lens[0][1] % page:] = torch.tensor([0x7E00] * (d // group), dtype=torch.int32, device=cuda)
+        assert torch.equal(ops.kv4_attention(q, cache, table, kv, cu_q=cu, causal=causal), ref)
+    t = table.clone()
+    t[0, 0] = -1  # a page of no cache is left out
+    got = ops.kv4_attention(q, cache, t, kv, cu_q=cu, causal=causal)
+    want, _, bound, _ = _reference(q, cache, t, [k for _, k in lens], [n for n, _ in lens], causal, d ** -0.5)
+    assert torch.all((got.double() - want).abs() <= bound)
+
+
+@pytest.mark.parametrize("d,group", [(64, 64), (128, 32), (128, 128)])
+@pytest.mark.parametrize("spread,base,q_scale", [(3.0, 0.25, 1.5), (0.3, 2000.0, 1e-5), (0.3, 1e-5, 1e4), (0.3, 0.25, 30.0)])
+def test_whole_prompts_scales_of_any_size(cuda, d, group, spread, base, q_scale):
+    _run(cuda, [1100, 300], [1100, 700], 8, 4, d, group, 16, seed=40, spread=spread, base=base, q_scale=q_scale)
+
+
 @pytest.mark.parametrize("d,group", [(64, 64), (128, 32), (128, 128)])
 @pytest.mark.parametrize("q_lens", [[1, 1], [40, 90]])
 def test_scales_of_any_size(cuda, d, group, q_lens):
