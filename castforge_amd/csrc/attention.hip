@@ -325,10 +325,16 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first
                 float v = dot[mt][0][r] * ks[0][r];
 #pragma unroll
                 for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], v);
-                v = __builtin_fmaf(v, s.unit[mt], e[r]);
-                if (edge && at + 16 * h + 4 * g + r >= s.limit[mt]) v = -INFINITY;
-                y[mt][h][r] = v;
+                y[mt][h][r] = __builtin_fmaf(v, s.unit[mt], e[r]);
             }
+    }
+    if (edge) {
+        asm volatile("");  // a branch: as selects on a uniform condition these were a quarter of the loop
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (at + 16 * (i / 4) + 4 * g + i % 4 >= s.limit[mt]) y[mt][i / 4][i % 4] = -INFINITY;
     }
     uint32_t p[MT][GR][4];  // weights times c as f16 pairs: tokens (0, 1), (2, 3) of both halves
     {
