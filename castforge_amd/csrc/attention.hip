@@ -482,16 +482,25 @@ __device__ __forceinline__ void settle(Rows<D, G, MT> &s) {
     }
 }
 
-// One workgroup's four waves take the same rows and every fourth 32 tokens of a split's share, and are joined through
-// LDS; splits are joined by kv4_attention_join_kernel.  For few rows a sequence: bound by the cache's bytes.
-template <int D, int G, int MT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((D == 128 && G < 128) || MT > 1 ? 2 : G == 32 ? 3 : 4))) void kv4_attention_split_kernel(AttnArgs a) {
+// One workgroup's NW waves take the same rows and every NW-th 32 tokens of a split's share, and are joined through LDS;
+// splits are joined by kv4_attention_join_kernel.  For few rows a sequence: bound by the cache's bytes where they are many (48
+// sequences of up to 8000 tokens, 8 heads: 235 MB in 63 us), by latency where they are few.
+template <int D, int G, int NW>
+struct SplitLds {
+    float sums[NW][16][D + 4];
+    Tokens<D / G, 32> tokens[NW];
+    Zeros<D, G, 32> zeros[NW];
+    float m[NW][16], l[NW][16];
+};
+
+// Waves a SIMD by the registers they take: two where a row tile's are doubled or a token has several group words in 128 channels.
+constexpr int split_waves(int d, int g, int mt) { return (d == 128 && g < 128) || mt > 1 ? 2 : g == 32 ? 3 : 4; }
+
+template <int D, int G, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 ? NW / 4 : split_waves(D, G, MT)))) void kv4_attention_split_kernel(AttnArgs a) {
     typedef Rows<D, G, MT> S;
-    constexpr int kRow = D + 4;
-    __shared__ __align__(16) float sums[4][16][kRow];
-    __shared__ __align__(16) Tokens<D / G, 32> tokens[4];
-    __shared__ __align__(16) Zeros<D, G, 32> zeros[4];
-    __shared__ float ml[2][4][16];
+    extern __shared__ __align__(16) uint8_t lds[];
+    SplitLds<D, G, NW> &sh = *reinterpret_cast<SplitLds<D, G, NW> *>(lds);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
     const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits % a.heads;
@@ -503,41 +512,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu((D == 128 &
     const int seen = a.causal ? max(0, min(sq.len, sq.len - sq.n + (row0 + rows - 1) / a.ratio + 1)) : sq.len;
     const int used = splits_of(sq.len, a.splits);
     if (split >= used) return;
-    const int share = (sq.len / used + 128) / 128 * 128;  // used * share >= len; whole rounds of the four waves
+    const int share = (sq.len / used + 32 * NW) / (32 * NW) * (32 * NW);  // used * share >= len; whole rounds of the waves
     const int first = split * share, end = min(seen, first + share);
     S s;
     load_rows<D, G, MT>(a, s, sq, head, row0);
-    walk<D, G, MT>(a, tokens[wave], zeros[wave], s, sq, head, first + 32 * wave, 128, end);
+    walk<D, G, MT>(a, sh.tokens[wave], sh.zeros[wave], s, sq, head, first + 32 * wave, 32 * NW, end);
     settle<D, G, MT>(s);
     const int hq = a.heads * a.ratio;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (16 * mt >= rows) break;
         __syncthreads();
-        if (g == 0) ml[0][wave][n] = s.m[mt], ml[1][wave][n] = s.l[mt];
+        if (g == 0) sh.m[wave][n] = s.m[mt], sh.l[wave][n] = s.l[mt];
         __syncthreads();
-        const float m = fmaxf(fmaxf(ml[0][0][n], ml[0][1][n]), fmaxf(ml[0][2][n], ml[0][3][n]));
-        const float f = __builtin_amdgcn_exp2f(s.m[mt] - m);
+        const auto top = [&](int row) {
+            float m = sh.m[0][row];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) m = fmaxf(m, sh.m[w][row]);
+            return m;
+        };
+        const float f = __builtin_amdgcn_exp2f(s.m[mt] - top(n));
 #pragma unroll
         for (int gr = 0; gr < S::GR; ++gr)
 #pragma unroll
             for (int u = 0; u < S::NT; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sums[wave][n][channel<G>(g, r, gr, u)] = s.o[mt][gr][u][r] * f;
+                for (int r = 0; r < 4; ++r) sh.sums[wave][n][channel<G>(g, r, gr, u)] = s.o[mt][gr][u][r] * f;
         __syncthreads();
-        for (int i = threadIdx.x; i < 16 * (D / 8); i += 256) {
+        for (int i = threadIdx.x; i < 16 * (D / 8); i += 64 * NW) {
             const int rl = i / (D / 8), ch = i % (D / 8) * 8, row = row0 + 16 * mt + rl;
             if (row >= sq.n * a.ratio) continue;
             const int64_t at = static_cast<int64_t>(sq.first + row / a.ratio) * hq + head * a.ratio + row % a.ratio;
-            const float mm = fmaxf(fmaxf(ml[0][0][rl], ml[0][1][rl]), fmaxf(ml[0][2][rl], ml[0][3][rl]));
+            const float mm = top(rl);
             float l = 0.f, v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll 4
+            for (int w = 0; w < NW; ++w) {
+                l = __builtin_fmaf(sh.l[w][rl], __builtin_amdgcn_exp2f(sh.m[w][rl] - mm), l);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                l = __builtin_fmaf(ml[1][w][rl], __builtin_amdgcn_exp2f(ml[0][w][rl] - mm), l);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += sums[w][rl][ch + e];
+                for (int e = 0; e < 8; ++e) v[e] += sh.sums[w][rl][ch + e];
             }
             if (a.splits > 1) {
                 float *p = a.part + (at * a.splits + split) * (D + 4);
@@ -747,12 +761,15 @@ constexpr int most_tiles(int64_t d, int64_t g) { return d / g >= 4 ? 1 : 2; }
 // tiles at most, splits.
 struct Plan {
     int mt;
-    bool rows;
+    bool rows, wide;  // wide: more waves a workgroup in place of splits
     int64_t tiles, splits, bytes;
 };
 
+// Waves of a wide workgroup: as many as its registers allow.
+constexpr int wide_waves(int64_t d, int64_t g) { return d / g == 1 ? 16 : 8; }
+
 Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols, bool varlen) {
-    Plan p{1, false, 0, 1, 0};
+    Plan p{1, false, false, 0, 1, 0};
     if (tokens == 0 || batch == 0) return p;
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio;
     const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
@@ -767,6 +784,12 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     p.mt = each <= 16 ? 1 : most_tiles(c->head_dim, c->group);
     p.tiles = tiles(16 * p.mt);
     const int64_t tasks = p.tiles * c->kv_heads, len = table_cols * c->page_size;
+    // A short table and few workgroups: one launch of wide workgroups, two rounds of 32 tokens a wave at most, no partial sums.
+    // One sequence of 777 tokens, 8 heads of 128: 11.5 us a call against 15.9 with splits and their join, whose second launch
+    // costs the host more than the longer walk costs the GPU (10.5 against 8.4 us on the GPU); 32 sequences of 1000: 13.9
+    // against 16.3 on the GPU.  At 2000 tokens, four rounds, one sequence takes 16.1 against 8.5 there.
+    p.wide = p.mt == 1 && tasks <= cus && len > 128 && len <= 64 * wide_waves(c->head_dim, c->group);
+    if (p.wide) return p;
     p.splits = std::max<int64_t>(1, std::min((2 * cus + tasks - 1) / tasks, (len + 127) / 128));
     const int64_t row = (c->head_dim + 4) * 4;
     p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
@@ -797,11 +820,16 @@ void launch_tile(const AttnArgs &a, const Plan &p, hipStream_t st) {
     check_launch("kv4_attention_tile");
 }
 
-template <int D, int G, int MT>
+template <int D, int G, int MT, int NW>
 void launch_split(const AttnArgs &a, const Plan &p, hipStream_t st) {
     const int64_t grid = p.tiles * a.heads * p.splits;
     require(grid <= 0x7fffffff, "too many workgroups for one launch");
-    kv4_attention_split_kernel<D, G, MT><<<dim3(static_cast<unsigned>(grid)), dim3(256), 0, st>>>(a);
+    constexpr int lds = sizeof(SplitLds<D, G, NW>);
+    static_assert(lds <= 160 * 1024, "LDS budget");
+    const auto kern = kv4_attention_split_kernel<D, G, MT, NW>;
+    static std::atomic<uint64_t> attr_devices{0};
+    if (lds > 64 * 1024) raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
+    kern<<<dim3(static_cast<unsigned>(grid)), dim3(64 * NW), lds, st>>>(a);
     check_launch("kv4_attention_split");
     if (p.splits > 1) {
         kv4_attention_join_kernel<D><<<dim3(static_cast<unsigned>(a.tokens * a.heads * a.ratio)), dim3(256), 0, st>>>(a);
@@ -862,10 +890,12 @@ int32_t castforge_hip_kv4_attention(const cfh_kv4_cache_t *cache, const uint16_t
             constexpr int D = decltype(d)::value, G = decltype(gr)::value;
             if (p.rows) {
                 launch_tile<D, G>(a, p, st);
+            } else if (p.wide) {
+                launch_split<D, G, 1, wide_waves(D, G)>(a, p, st);
             } else if (p.mt == 1) {
-                launch_split<D, G, 1>(a, p, st);
+                launch_split<D, G, 1, 4>(a, p, st);
             } else if constexpr (most_tiles(D, G) > 1) {
-                launch_split<D, G, 2>(a, p, st);
+                launch_split<D, G, 2, 4>(a, p, st);
             }
         });
     });

@@ -120,6 +120,14 @@ def test_one_query_each(cuda, d, group, hkv, ratio, page, kv_lens):
 
 
 @pytest.mark.parametrize("d,group", SHAPES)
+@pytest.mark.parametrize("q_lens,kv_lens", [([1] * 4, [100, 1, 0, 700]), ([1] * 3, [513, 1024, 97]), ([3, 1, 4], [300, 129, 1000])])
+@pytest.mark.parametrize("cols", [0, 90])
+def test_short_sequences(cuda, d, group, q_lens, kv_lens, cols):
+    """In one launch or, with a table that has room for more, in splits and a join."""
+    _run(cuda, q_lens, kv_lens, 4, 3, d, group, 16, seed=60, extra_cols=cols)
+
+
+@pytest.mark.parametrize("d,group", SHAPES)
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("hkv,ratio,page,lens", [
     (2, 4, 16, [(5, 100), (1, 33), (3, 3)]), (1, 8, 32, [(17, 17), (64, 200), (2, 1000)]), (4, 1, 64, [(130, 130), (33, 65)]),
