@@ -66,6 +66,18 @@ __device__ __forceinline__ halfx8 codes_f16(uint32_t w, uint32_t zz) {
 
 __device__ __forceinline__ float sum_over_g(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
 __device__ __forceinline__ float max_over_g(float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); }
+__device__ __forceinline__ int max_over_wave(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// The instruction itself: fmaxf() quiets each operand first, ten instructions more for a row's eight scores.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
 
 // One sequence's share of a workgroup.
 struct Seq {
@@ -139,18 +151,19 @@ struct KvTile {
 // at a time.
 template <int GR, int N>
 struct Tokens {
-    float scale[2][GR][N];  // keys: scale times what turns a product into a score; values: scale without its exponent
-    float exponent[N];      // of the values' largest scale; -inf where there is no token
-    float back[N];          // 2^-exponent
+    float keys[GR][N];   // scale times what turns a product into a score
+    float exponent[N];   // of the values' largest scale; -inf where there is no token
+    float back[N];       // 2^-exponent
 };
 
-// A wave's zero points of N tokens, and its deal of the values' words.
-template <int D, int G, int N>
-struct Zeros {
+// What a wave keeps to itself of N tokens: zero points, the values' scales, and its deal of their words.
+template <int D, int G, int N, class C>
+struct Own {
     static constexpr int GR = D / G, kRow = N + 4;   // tokens a row of `v`, padded for the banks
     uint32_t v[KvTile<D, G>::kDeal ? 16 * kRow : 4];  // the values' codes: word by word, a token each
     uint32_t k[GR][N];  // zero point in both halves, as f16 denormals
     uint16_t z[GR][N];  // of the values
+    C c[GR][N];         // the values' scales without the exponent, an f16 one times 2^11
 };
 
 template <int D, int G>
@@ -198,20 +211,24 @@ __device__ __forceinline__ void wave_order() { asm volatile("" ::: "memory"); }
 
 // The lane's token (`token` of the table; value: its values' words, else its keys') into the tables.  off: there is no such token,
 // and its words may be anything.
-template <int GR, int N, class Z>
-__device__ __forceinline__ void fill_token(const uint32_t (&words)[GR], bool value, int token, bool off, float qk, Tokens<GR, N> &tokens, Z &zeros, int own) {
+template <int D, int G, int N, int M, class C>
+__device__ __forceinline__ void fill_token(const uint32_t (&words)[D / G], bool value, int token, bool off, float qk, Tokens<D / G, N> &tokens, Own<D, G, M, C> &own, int at) {
+    constexpr int GR = D / G;
     float v[GR], top = 0.f;
 #pragma unroll
     for (int gr = 0; gr < GR; ++gr) {
         const uint32_t w = off ? 0u : words[gr];
         v[gr] = kv4_scale(w);
         top = fmaxf(top, v[gr]);
-        if (value) zeros.z[gr][own] = static_cast<uint16_t>(kv4_zero(w));
-        else zeros.k[gr][own] = kv4_zero(w) * 0x00010001u;
+        if (value) own.z[gr][at] = static_cast<uint16_t>(kv4_zero(w));
+        else own.k[gr][at] = kv4_zero(w) * 0x00010001u;
     }
     const int ex = __builtin_amdgcn_frexp_expf(top);
 #pragma unroll
-    for (int gr = 0; gr < GR; ++gr) tokens.scale[value][gr][token] = value ? __builtin_ldexpf(v[gr], -ex) : v[gr] * qk;
+    for (int gr = 0; gr < GR; ++gr) {
+        if (value) own.c[gr][at] = static_cast<C>(__builtin_ldexpf(v[gr], (sizeof(C) == 2 ? 11 : 0) - ex));  // f16: exact down to 2^-25
+        else tokens.keys[gr][token] = v[gr] * qk;
+    }
     if (value) tokens.exponent[token] = off ? -INFINITY : static_cast<float>(ex), tokens.back[token] = __builtin_ldexpf(1.0f, -ex);
 }
 
@@ -235,23 +252,38 @@ __device__ __forceinline__ uint32_t pair_code(const Pairs &p, int i, int code, u
     return code % 2 == 0 ? minus(y & 0x000F000Fu, z) : minus(y & 0x00F000F0u, z << 4);
 }
 
+// The same with the scales c (f16, times 2^11) taken in, rounded once to f16: codes in the mantissas of 1024 or 64, from which the
+// zero points are subtracted exactly.
+__device__ __forceinline__ uint32_t pair_value(const Pairs &p, int i, int code, uint32_t z, uint32_t c) {
+    const uint32_t x = code < 4 ? p.lo[i] : p.hi[i], y = code % 4 < 2 ? x : x >> 8;
+    const uint32_t v = code % 2 == 0 ? minus((y & 0x000F000Fu) | 0x64006400u, z | 0x64006400u) : minus((y & 0x00F000F0u) | 0x54005400u, (z << 4) | 0x54005400u);
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, v) * __builtin_bit_cast(halfx2, c));
+}
+
 // Rows of a wave: 16 MT of the n * ratio (query, head of the group) pairs of a sequence and a head of keys, row = query *
 // ratio + head; the MFMAs' columns.  With S^T = K Q^T a lane holds the scores of one row and four tokens a
 // half, which is the layout that O^T = V^T P^T takes its second operand in: the weights stay in registers.
 template <int D, int G, int MT>
 struct Rows {
     static constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = 8 / R;  // NT output tiles of 16 channels a group
-    halfx8 q[MT][GR][W];     // the row times a power of two, 2^14 / unit: in the order and by the factors of codes_f16
-    float unit[MT];
+    halfx8 q[MT][GR][W];     // the row by a power of two, in the order and by the factors of codes_f16
+    float rel[MT];           // what undoes the power of two; in the tile kernel, what the tables' share of it leaves
+    bool uneven;             // tile kernel, uniform: rel is not 1 everywhere
     int limit[MT];           // tokens that the lane's row sees
     floatx4 o[MT][GR][NT];   // sum of weight * (code - zero point), by code position times 2^-24 or 2^-20
     float m[MT], l[MT];      // reference and this lane's part of the sum
 };
 
-template <int D, int G, int MT>
-__device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, const Seq &sq, int head, int row0) {
-    constexpr int GR = D / G, W = G / 32;
+// Loads the rows.  A row's power of two takes its largest element below 2^14, so that a sixteenth of it keeps bf16's bits down to
+// 2^-24 of the largest.  kShared: all rows take the greatest one's, whose exponent is returned for the tables to hold: a row
+// 2^10 smaller keeps its bits down to 2^-16 of its largest and loses 2^-25 of that below.  Rows smaller still have their own, and
+// `uneven` is set.  most(v): the greatest v of those who read the tables.
+template <bool kShared, int D, int G, int MT, class Most>
+__device__ __forceinline__ int load_rows(const AttnArgs &a, Rows<D, G, MT> &s, const Seq &sq, int head, int row0, const Most &most) {
+    constexpr int GR = D / G, W = G / 32, kNone = -1000;
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    uint4 raw[MT][GR][W];
+    int ex[MT], greatest = kNone;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int row = row0 + 16 * mt + n, i = row / a.ratio;
@@ -259,27 +291,43 @@ __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, 
         // rows past the sequence's see all: they are not stored, and do not make a tile an edge
         s.limit[mt] = in ? (a.causal ? min(sq.len, sq.len - sq.n + i + 1) : sq.len) : 0x7fffffff;
         const uint16_t *p = a.q + (sq.first + (in ? i : 0)) * a.q_stride + (head * a.ratio + (in ? row - i * a.ratio : 0)) * D;
-        float x[GR][W][8], top = 0.f;
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr)
 #pragma unroll
-            for (int u = 0; u < W; ++u) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(p + gr * G + (g * W + u) * 8);
-                const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+            for (int u = 0; u < W; ++u) raw[mt][gr][u] = *reinterpret_cast<const uint4 *>(p + gr * G + (g * W + u) * 8);
+    }
+    const auto element = [&](int mt, int gr, int u, int e) {
+        const uint4 v = raw[mt][gr][u];
+        const uint32_t b = e / 2 == 0 ? v.x : e / 2 == 1 ? v.y : e / 2 == 2 ? v.z : v.w;
+        return __uint_as_float(e % 2 ? b & 0xffff0000u : b << 16);
+    };
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[gr][u][e] = __uint_as_float(e % 2 ? b[e / 2] & 0xffff0000u : b[e / 2] << 16);
-                    top = fmaxf(top, fabsf(x[gr][u][e]));
-                }
-            }
-        // the largest element below 2^14, so that a sixteenth of it keeps bf16's bits down to 2^-24 of the largest
-        const int ex = __builtin_amdgcn_frexp_expf(max_over_g(top)) - 14;
-        s.unit[mt] = __builtin_ldexpf(1.0f, ex);
+    for (int mt = 0; mt < MT; ++mt) {
+        float top = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+            for (int u = 0; u < W; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(element(mt, gr, u, e)));
+        top = max_over_g(top);
+        ex[mt] = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 14 : kNone;
+        greatest = max(greatest, ex[mt]);
+    }
+    int all = kShared ? most(max_over_wave(greatest)) : 0;
+    if (all == kNone) all = 0;  // rows of zeros
+    bool apart = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const bool own = ex[mt] != kNone && (!kShared || ex[mt] < all - 10);
+        const int at_ex = own ? ex[mt] : all;
+        apart |= own;
+        s.rel[mt] = __builtin_ldexpf(1.0f, at_ex - all);
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
 #pragma unroll
             for (int u = 0; u < W; ++u) {
-                const auto at = [&](int e) { return static_cast<_Float16>(__builtin_ldexpf(x[gr][u][e], -ex - (e % 2 ? 4 : 0))); };
+                const auto at = [&](int e) { return static_cast<_Float16>(__builtin_ldexpf(element(mt, gr, u, e), -at_ex - (e % 2 ? 4 : 0))); };
                 s.q[mt][gr][u] = halfx8{at(0), at(4), at(1), at(5), at(2), at(6), at(3), at(7)};
             }
 #pragma unroll
@@ -287,7 +335,12 @@ __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, 
         }
         s.m[mt] = kNoMax, s.l[mt] = 0.f;
     }
+    s.uneven = __any(apart);
+    return all;
 }
+
+// What turns a product of codes and a row (by 2^-ex) into a score, base 2; the codes' 2^-24 undone.
+__device__ __forceinline__ float score_factor(const AttnArgs &a, int ex) { return __builtin_ldexpf(a.scale * 1.44269504088896341f, ex + 24); }
 
 // 32 tokens at `at`.  A token's weight is held with the exponent of its values' scale: with s_t = c_t 2^e_t (the largest
 // of its groups', c in [0.5, 1)), exp2(score + e_t - m) times c rounds to f16 as what the token adds to the output, whatever
@@ -295,9 +348,10 @@ __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows<D, G, MT> &s, 
 // when something exceeds it by 15: weights stay below 2^15, the largest ones above 2^7 (f16 keeps its 11 bits
 // down to 2^-21 of them), and the rescaling is rare.
 // keys(h, gr, u): the MFMA operand of half h's 16 tokens and 32 channels; values(gr) prepares a group's rows of V^T and gives what
-// turns u into the operand of 16 channels and 32 tokens.  first: the tokens' place in the table.
-template <int D, int G, int MT, int N, class Keys, class Values>
-__device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first, Rows<D, G, MT> &s, int at, int sure, const Keys &keys, const Values &values) {
+// turns u into the operand of 16 channels and 32 tokens.  first: the tokens' place in the table.  kShared: the values hold c
+// already, rounded to f16 with it, and the weights are rounded alone; many rows share that work then.
+template <bool kShared, int D, int G, int MT, int N, class Keys, class Values>
+__device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const float (*scales)[32], int first, Rows<D, G, MT> &s, int at, int sure, const Keys &keys, const Values &values) {
     constexpr int GR = D / G, W = G / 32, NT = G / 16;
     const int g = (threadIdx.x >> 4) & 3;
     const bool edge = at + 32 > sure;  // uniform: some row does not see some token
@@ -307,7 +361,7 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first
     for (int h = 0; h < 2; ++h) {
         floatx4 ks[GR], dot[MT][GR];
 #pragma unroll
-        for (int gr = 0; gr < GR; ++gr) ks[gr] = four(tokens.scale[0][gr], h);
+        for (int gr = 0; gr < GR; ++gr) ks[gr] = four(tokens.keys[gr], h);
         const floatx4 e = four(tokens.exponent, h);
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr)
@@ -318,14 +372,27 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first
                 for (int mt = 0; mt < MT; ++mt)
                     dot[mt][gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, s.q[mt][gr][u], u ? dot[mt][gr] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             }
+        if (kShared && s.uneven) {
+            asm volatile("");  // a branch
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) dot[mt][gr] *= s.rel[mt];
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float v = dot[mt][0][r] * ks[0][r];
+                if constexpr (!kShared) {
+                    float v = dot[mt][0][r] * ks[0][r];
 #pragma unroll
-                for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], v);
-                y[mt][h][r] = __builtin_fmaf(v, s.unit[mt], e[r]);
+                    for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], v);
+                    y[mt][h][r] = __builtin_fmaf(v, s.rel[mt], e[r]);
+                    continue;
+                }
+                y[mt][h][r] = e[r];
+#pragma unroll
+                for (int gr = 0; gr < GR; ++gr) y[mt][h][r] = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], y[mt][h][r]);
             }
     }
     if (edge) {
@@ -336,20 +403,23 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first
             for (int i = 0; i < 8; ++i)
                 if (at + 16 * (i / 4) + 4 * g + i % 4 >= s.limit[mt]) y[mt][i / 4][i % 4] = -INFINITY;
     }
-    uint32_t p[MT][GR][4];  // weights times c as f16 pairs: tokens (0, 1), (2, 3) of both halves
+    constexpr int PG = kShared ? 1 : GR;
+    uint32_t p[MT][PG][4];  // weights, times c, as f16 pairs: tokens (0, 1), (2, 3) of both halves
     {
-        floatx4 back[2], c[2][GR];
+        floatx4 back[2], c[2][PG];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             back[h] = four(tokens.back, h);
 #pragma unroll
-            for (int gr = 0; gr < GR; ++gr) c[h][gr] = four(tokens.scale[1][gr], h);
+            for (int gr = 0; gr < PG; ++gr) {
+                if constexpr (kShared) c[h][gr] = floatx4{1.f, 1.f, 1.f, 1.f};
+                else c[h][gr] = four(scales[gr], h);
+            }
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float top = y[mt][0][0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) top = fmaxf(top, y[mt][i / 4][i % 4]);
+            const float (&v)[2][4] = y[mt];
+            const float top = max3(max3(v[0][0], v[0][1], v[0][2]), max3(v[0][3], v[1][0], v[1][1]), max3(v[1][2], v[1][3], v[1][3]));
             if (__any(top > s.m[mt] + 15.f)) {
                 const float m = fmaxf(s.m[mt], max_over_g(top) - 7.f), f = __builtin_amdgcn_exp2f(s.m[mt] - m);
                 s.m[mt] = m;
@@ -366,7 +436,7 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first
                 s.l[mt] = __builtin_fmaf(w[i / 4][i % 4], back[i / 4][i % 4], s.l[mt]);
             }
 #pragma unroll
-            for (int gr = 0; gr < GR; ++gr)
+            for (int gr = 0; gr < PG; ++gr)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int h = i / 2, r = i % 2 * 2;
@@ -379,7 +449,10 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, int first
     for (int gr = 0; gr < GR; ++gr) {
         halfx8 pw[MT];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) pw[mt] = eight(p[mt][gr][0], p[mt][gr][1], p[mt][gr][2], p[mt][gr][3]);
+        for (int mt = 0; mt < MT; ++mt) {
+            const uint32_t(&w)[4] = p[mt][kShared ? 0 : gr];
+            pw[mt] = eight(w[0], w[1], w[2], w[3]);
+        }
         const auto operand = values(gr);
         static_for<NT>([&](auto u) __attribute__((always_inline)) {
             const halfx8 v = operand(u);
@@ -400,17 +473,16 @@ __device__ __forceinline__ int seen_by_all(const Rows<D, G, MT> &s, int len) {
     return __builtin_amdgcn_readfirstlane(sure);
 }
 
-constexpr float kLog2e = 1.44269504088896341f;
 
 // A wave's walk over tokens first, first + step, .. (of 32) below end, the next tile's loads in flight.
 template <int D, int G, int MT>
-__device__ __forceinline__ void walk(const AttnArgs &a, Tokens<D / G, 32> &tokens, Zeros<D, G, 32> &zeros, Rows<D, G, MT> &s, const Seq &sq, int head,
+__device__ __forceinline__ void walk(const AttnArgs &a, Tokens<D / G, 32> &tokens, Own<D, G, 32, float> &own, Rows<D, G, MT> &s, const Seq &sq, int head,
                                      int first, int step, int end) {
     constexpr int R = 128 / G;
     if (first >= end) return;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int sure = seen_by_all(s, sq.len);
-    const float qk = a.scale * (kLog2e * 0x1p24f);  // the codes' 2^-24 undone
+    const float qk = score_factor(a, 0);
     const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
     const auto pages = [&](int at, int (&p)[2]) {
 #pragma unroll
@@ -431,25 +503,25 @@ __device__ __forceinline__ void walk(const AttnArgs &a, Tokens<D / G, 32> &token
         }
         const int token = lane & 31;
         wave_order();
-        fill_token(cur.words, lane >= 32, token, !(token < 16 ? cur.live[0] : cur.live[1]) || at + token >= sq.len, qk, tokens, zeros, token);
+        fill_token(cur.words, lane >= 32, token, !(token < 16 ? cur.live[0] : cur.live[1]) || at + token >= sq.len, qk, tokens, own, token);
         if constexpr (KvTile<D, G>::kDeal) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<uint4 *>(&zeros.v[n * Zeros<D, G, 32>::kRow + 16 * h + 4 * g]) = make_uint4(cur.vc[h][0][0], cur.vc[h][1][0], cur.vc[h][2][0], cur.vc[h][3][0]);
+                *reinterpret_cast<uint4 *>(&own.v[n * Own<D, G, 32, float>::kRow + 16 * h + 4 * g]) = make_uint4(cur.vc[h][0][0], cur.vc[h][1][0], cur.vc[h][2][0], cur.vc[h][3][0]);
         }
         wave_order();
-        attend<D, G, MT>(
-            tokens, 0, s, at, sure, [&](int h, int gr, int u) { return codes_f16(cur.kc[h][gr][u], zeros.k[gr][16 * h + n]); },
+        attend<false, D, G, MT>(
+            tokens, own.c, 0, s, at, sure, [&](int h, int gr, int u) { return codes_f16(cur.kc[h][gr][u], own.k[gr][16 * h + n]); },
             [&](int gr) {
                 Pairs p[2];
                 uint2 z[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if constexpr (KvTile<D, G>::kDeal)
-                        p[h] = pairs_of<G>(*reinterpret_cast<const uint4 *>(&zeros.v[(gr * (G / 8) + n % (G / 8)) * Zeros<D, G, 32>::kRow + 16 * h + 4 * g]), n);
+                        p[h] = pairs_of<G>(*reinterpret_cast<const uint4 *>(&own.v[(gr * (G / 8) + n % (G / 8)) * Own<D, G, 32, float>::kRow + 16 * h + 4 * g]), n);
                     else
                         p[h] = pairs_of<G>(make_uint4(cur.vc[h][0][gr], cur.vc[h][1][gr], cur.vc[h][2][gr], cur.vc[h][3][gr]), n);
-                    z[h] = *reinterpret_cast<const uint2 *>(&zeros.z[gr][16 * h + 4 * g]);
+                    z[h] = *reinterpret_cast<const uint2 *>(&own.z[gr][16 * h + 4 * g]);
                 }
                 return [=](int u) {
                     return eight(pair_code(p[0], 0, R * u, z[0].x), pair_code(p[0], 1, R * u, z[0].y), pair_code(p[1], 0, R * u, z[1].x),
@@ -469,7 +541,7 @@ __device__ __forceinline__ int channel(int g, int r, int gr, int u) {
 }
 
 // The whole sum, and the outputs without the codes' factors.
-template <int D, int G, int MT>
+template <bool kShared, int D, int G, int MT>
 __device__ __forceinline__ void settle(Rows<D, G, MT> &s) {
     typedef Rows<D, G, MT> S;
 #pragma unroll
@@ -478,7 +550,7 @@ __device__ __forceinline__ void settle(Rows<D, G, MT> &s) {
 #pragma unroll
         for (int gr = 0; gr < S::GR; ++gr)
 #pragma unroll
-            for (int u = 0; u < S::NT; ++u) s.o[mt][gr][u] *= (S::R * u) % 2 ? 0x1p20f : 0x1p24f;
+            for (int u = 0; u < S::NT; ++u) s.o[mt][gr][u] *= kShared ? 0x1p-11f : (S::R * u) % 2 ? 0x1p20f : 0x1p24f;
     }
 }
 
@@ -489,7 +561,7 @@ template <int D, int G, int NW>
 struct SplitLds {
     float sums[NW][16][D + 4];
     Tokens<D / G, 32> tokens[NW];
-    Zeros<D, G, 32> zeros[NW];
+    Own<D, G, 32, float> own[NW];
     float m[NW][16], l[NW][16];
 };
 
@@ -515,9 +587,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 
     const int share = (sq.len / used + 32 * NW) / (32 * NW) * (32 * NW);  // used * share >= len; whole rounds of the waves
     const int first = split * share, end = min(seen, first + share);
     S s;
-    load_rows<D, G, MT>(a, s, sq, head, row0);
-    walk<D, G, MT>(a, sh.tokens[wave], sh.zeros[wave], s, sq, head, first + 32 * wave, 32 * NW, end);
-    settle<D, G, MT>(s);
+    load_rows<false>(a, s, sq, head, row0, [](int v) { return v; });
+    walk<D, G, MT>(a, sh.tokens[wave], sh.own[wave], s, sq, head, first + 32 * wave, 32 * NW, end);
+    settle<false>(s);
     const int hq = a.heads * a.ratio;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -622,42 +694,51 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
     }
 }
 
-// Many rows: each wave takes 16 MT rows of its own, and the four of a workgroup share the work on the codes.  Of every 64 tokens
-// a wave turns 16 into MFMA operands in LDS (f16, codes less zero points, exactly) and all four read them back; two stages, one
-// barrier a stage: the operands of the next 64 tokens are made while the present ones are used, and the words of those after
-// that are on their way.  Bound by VALU work, the softmax's most of all.
+// Many rows: each wave takes 16 MT rows of its own, and the NW of a workgroup share the work on the codes.  Of every 16 NW tokens a
+// wave turns 16 into MFMA operands in LDS (f16: of the keys codes less zero points, exactly; of the values that times c) and all
+// read them back; two stages, one barrier a stage: the operands of the next tokens are made while the present ones are used, and
+// the words of those after that are on their way.
+// A prompt of 4096 tokens, 32 query heads on 8 of 128 channels: 165 us, 137 GFLOP at 834 TFLOP/s.  VALU work and MFMAs hardly overlap on a
+// SIMD (an MFMA of 16 cycles hides one or two instructions), so it is bound by their sum: 37% of the time are MFMAs, 49% the softmax
+// and the making of operands; without the latter it takes 145 us, without LDS reads 7 us less, and the products of
+// the next tokens issued among the present ones' exponentials change nothing.
 // Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row tiles from the
 // last, which see the most tokens.
-template <int D, int G>
+template <int D, int G, int NW>
 struct Stage {
     static constexpr int GR = D / G, kSteps = D / 32, kTiles = D / 16;
-    uint4 keys[4][kSteps][64];      // 16 tokens, 32 channels: a lane's operand
-    uint4 values[2][kTiles][64];    // 32 tokens, 16 channels
-    Tokens<GR, 64> tokens;
+    uint4 keys[NW][kSteps][64];     // 16 tokens, 32 channels: a lane's operand
+    uint4 values[NW / 2][kTiles][64];   // 32 tokens, 16 channels
+    Tokens<GR, 16 * NW> tokens;
 };
 
-template <int D, int G, int MT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void kv4_attention_tile_kernel(AttnArgs a, int tiles) {
+template <int D, int G, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void kv4_attention_tile_kernel(AttnArgs a, int tiles) {
     typedef Rows<D, G, MT> S;
-    constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = G / 16, kWords = D / 8, VW = KvTile<D, G>::VW, kRow = D + 4;
+    constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = G / 16, kWords = D / 8, VW = KvTile<D, G>::VW, kRow = D + 4, kTokens = 16 * NW;
     extern __shared__ __align__(16) uint8_t lds[];
-    Stage<D, G> *stages = reinterpret_cast<Stage<D, G> *>(lds);
-    __shared__ __align__(16) Zeros<D, G, 16> own[4];
+    Stage<D, G, NW> *stages = reinterpret_cast<Stage<D, G, NW> *>(lds);
+    __shared__ __align__(16) Own<D, G, 16, _Float16> all[NW];
+    __shared__ int greatest[NW];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int n = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % a.heads;
-    const Seq sq = find_tile(a, tiles - 1 - blockIdx.x / a.heads, 64 * MT);
+    const Seq sq = find_tile(a, tiles - 1 - blockIdx.x / a.heads, 16 * NW * MT);
     if (sq.seq < 0) return;
-    const int total = sq.n * a.ratio, row_of_all = sq.tile * 64 * MT, row0 = row_of_all + wave * 16 * MT;
+    const int total = sq.n * a.ratio, row_of_all = sq.tile * 16 * NW * MT, row0 = row_of_all + wave * 16 * MT;
     const auto seen = [&](int last_row) { return a.causal ? max(0, min(sq.len, sq.len - sq.n + last_row / a.ratio + 1)) : sq.len; };
-    const int end = seen(min(row_of_all + 64 * MT, total) - 1);  // of the workgroup
+    const int end = seen(min(row_of_all + 16 * NW * MT, total) - 1);  // of the workgroup
     const int mine = row0 < total ? seen(min(row0 + 16 * MT, total) - 1) : 0;
     S s;
-    load_rows<D, G, MT>(a, s, sq, head, row0);
+    const float qk = score_factor(a, load_rows<true>(a, s, sq, head, row0, [&](int v) {
+        if (lane == 0) greatest[wave] = v;
+        __syncthreads();
+        for (int w = 0; w < NW; ++w) v = max(v, greatest[w]);
+        return __builtin_amdgcn_readfirstlane(v);
+    }));
     const int sure = seen_by_all(s, sq.len);
-    const float qk = a.scale * (kLog2e * 0x1p24f);  // the codes' 2^-24 undone
     const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
-    Zeros<D, G, 16> &zeros = own[wave];
+    Own<D, G, 16, _Float16> &own = all[wave];
 
     // this wave's 16 tokens of a stage
     struct Part {
@@ -678,23 +759,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             for (int r = 0; r < 4; ++r) t.vc[r][i] = vc[r * kWords + i * (G / 8)];
         __builtin_memcpy(t.words, __builtin_assume_aligned((lane & 16 ? a.v_groups : a.k_groups) + (row + n) * GR, 4 * GR), 4 * GR);
     };
-    const auto make = [&](const Part &t, Stage<D, G> &st, int at) {
+    const auto make = [&](const Part &t, Stage<D, G, NW> &st, int at) {
         wave_order();
-        if (lane < 32) fill_token(t.words, lane >= 16, 16 * wave + n, !t.live || at + n >= sq.len, qk, st.tokens, zeros, n);
-        if constexpr (KvTile<D, G>::kDeal) *reinterpret_cast<uint4 *>(&zeros.v[n * Zeros<D, G, 16>::kRow + 4 * g]) = make_uint4(t.vc[0][0], t.vc[1][0], t.vc[2][0], t.vc[3][0]);
+        if (lane < 32) fill_token(t.words, lane >= 16, 16 * wave + n, !t.live || at + n >= sq.len, qk, st.tokens, own, n);
+        if constexpr (KvTile<D, G>::kDeal) *reinterpret_cast<uint4 *>(&own.v[n * own.kRow + 4 * g]) = make_uint4(t.vc[0][0], t.vc[1][0], t.vc[2][0], t.vc[3][0]);
         wave_order();
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
-            const uint32_t zz = zeros.k[gr][n];
+            const uint32_t zz = own.k[gr][n];
 #pragma unroll
             for (int u = 0; u < W; ++u) st.keys[wave][gr * W + u][lane] = __builtin_bit_cast(uint4, codes_f16(t.kc[gr][u], zz));
             uint4 w;
-            if constexpr (KvTile<D, G>::kDeal) w = *reinterpret_cast<const uint4 *>(&zeros.v[(gr * (G / 8) + n % (G / 8)) * Zeros<D, G, 16>::kRow + 4 * g]);
+            if constexpr (KvTile<D, G>::kDeal) w = *reinterpret_cast<const uint4 *>(&own.v[(gr * (G / 8) + n % (G / 8)) * own.kRow + 4 * g]);
             else w = make_uint4(t.vc[0][gr], t.vc[1][gr], t.vc[2][gr], t.vc[3][gr]);
             const Pairs p = pairs_of<G>(w, n);
-            const uint2 z = *reinterpret_cast<const uint2 *>(&zeros.z[gr][4 * g]);
+            const uint2 z = *reinterpret_cast<const uint2 *>(&own.z[gr][4 * g]), c = *reinterpret_cast<const uint2 *>(&own.c[gr][4 * g]);
             static_for<NT>([&](auto u) __attribute__((always_inline)) {
-                reinterpret_cast<uint2 *>(&st.values[wave / 2][gr * NT + u][lane])[wave % 2] = make_uint2(pair_code(p, 0, R * u, z.x), pair_code(p, 1, R * u, z.y));
+                reinterpret_cast<uint2 *>(&st.values[wave / 2][gr * NT + u][lane])[wave % 2] = make_uint2(pair_value(p, 0, R * u, z.x, c.x), pair_value(p, 1, R * u, z.y, c.y));
             });
         }
     };
@@ -702,26 +783,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     if (end > 0) {
         load(part, page_of(16 * wave), 16 * wave);
         make(part, stages[0], 16 * wave);
-        load(part, page_of(64 + 16 * wave), 64 + 16 * wave);
+        load(part, page_of(kTokens + 16 * wave), kTokens + 16 * wave);
     }
-    int page = page_of(128 + 16 * wave);
-    for (int at = 0, i = 0; at < end; at += 64, i ^= 1) {
+    int page = page_of(2 * kTokens + 16 * wave);
+    for (int at = 0, i = 0; at < end; at += kTokens, i ^= 1) {
         __syncthreads();  // stage i is made, and the other one no longer read
-        if (at + 64 < end) {
-            make(part, stages[i ^ 1], at + 64 + 16 * wave);
-            load(part, page, at + 128 + 16 * wave);
-            page = page_of(at + 192 + 16 * wave);
+        if (at + kTokens < end) {
+            make(part, stages[i ^ 1], at + kTokens + 16 * wave);
+            load(part, page, at + 2 * kTokens + 16 * wave);
+            page = page_of(at + 3 * kTokens + 16 * wave);
         }
-        const Stage<D, G> &st = stages[i];
+        const Stage<D, G, NW> &st = stages[i];
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
+        for (int sub = 0; sub < NW / 2; ++sub) {
             if (at + 32 * sub >= mine) break;
-            attend<D, G, MT>(
-                st.tokens, 32 * sub, s, at + 32 * sub, sure, [&](int h, int gr, int u) { return __builtin_bit_cast(halfx8, st.keys[2 * sub + h][gr * W + u][lane]); },
+            attend<true, D, G, MT>(
+                st.tokens, nullptr, 32 * sub, s, at + 32 * sub, sure, [&](int h, int gr, int u) { return __builtin_bit_cast(halfx8, st.keys[2 * sub + h][gr * W + u][lane]); },
                 [&](int gr) { return [&st, gr, sub, lane](int u) { return __builtin_bit_cast(halfx8, st.values[sub][gr * NT + u][lane]); }; });
         }
     }
-    settle<D, G, MT>(s);
+    settle<true>(s);
     __syncthreads();  // the stages' LDS now holds outputs, each wave's own part
     if (row0 >= total) return;
     float (*sums)[kRow] = reinterpret_cast<float (*)[kRow]>(lds) + 16 * wave;
@@ -760,7 +841,7 @@ constexpr int most_tiles(int64_t d, int64_t g) { return d / g >= 4 ? 1 : 2; }
 // How a call is laid out: rows a wave (16 mt), whether waves share rows (splits of the tokens) or have their own, row
 // tiles at most, splits.
 struct Plan {
-    int mt;
+    int mt, waves;
     bool rows, wide;  // wide: more waves a workgroup in place of splits
     int64_t tiles, splits, bytes;
 };
@@ -769,7 +850,7 @@ struct Plan {
 constexpr int wide_waves(int64_t d, int64_t g) { return d / g == 1 ? 16 : 8; }
 
 Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols, bool varlen) {
-    Plan p{1, false, false, 0, 1, 0};
+    Plan p{1, 4, false, false, 0, 1, 0};
     if (tokens == 0 || batch == 0) return p;
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio;
     const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
@@ -777,7 +858,11 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     p.rows = varlen && rows / 32 * c->kv_heads >= 4 * cus;
     if (p.rows) {
         p.mt = most_tiles(c->head_dim, c->group);
-        p.tiles = tiles(64 * p.mt);
+        // Eight waves share the making of operands where there are two workgroups of them a CU, the heavy ones to be evened out by the
+        // light ones.  Prompts of 4096 and of 2048 tokens, 8 heads of 128 channels, 4 queries each: 165 and 78 us, with four waves
+        // 186 and 73.  With 64 channels four of them take 109 us and eight 120: their registers leave room for four waves a SIMD.
+        if (c->head_dim == 128 && rows / (128 * p.mt) * c->kv_heads >= 2 * cus) p.waves = 8;
+        p.tiles = tiles(16 * p.waves * p.mt);
         return p;
     }
     const int64_t each = (rows + batch - 1) / batch;
@@ -808,15 +893,15 @@ void raise_lds_limit(const void *kern, int bytes, std::atomic<uint64_t> &done) {
     }
 }
 
-template <int D, int G>
+template <int D, int G, int NW>
 void launch_tile(const AttnArgs &a, const Plan &p, hipStream_t st) {
-    constexpr int MT = most_tiles(D, G), sums = 64 * (D + 4) * 4, stages = 2 * sizeof(Stage<D, G>), lds = stages > sums ? stages : sums;
-    static_assert(lds + 4 * sizeof(Zeros<D, G, 16>) <= 80 * 1024, "two workgroups a CU");
+    constexpr int MT = most_tiles(D, G), sums = 16 * NW * (D + 4) * 4, stages = 2 * sizeof(Stage<D, G, NW>), lds = stages > sums ? stages : sums;
+    static_assert(lds + NW * sizeof(Own<D, G, 16, _Float16>) <= NW * 20 * 1024, "two workgroups a CU");
     require(p.tiles * a.heads <= 0x7fffffff, "too many workgroups for one launch");
     static std::atomic<uint64_t> attr_devices{0};
-    const auto kern = kv4_attention_tile_kernel<D, G, MT>;
+    const auto kern = kv4_attention_tile_kernel<D, G, MT, NW>;
     raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
-    kern<<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(256), lds, st>>>(a, static_cast<int>(p.tiles));
+    kern<<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(64 * NW), lds, st>>>(a, static_cast<int>(p.tiles));
     check_launch("kv4_attention_tile");
 }
 
@@ -888,8 +973,10 @@ int32_t castforge_hip_kv4_attention(const cfh_kv4_cache_t *cache, const uint16_t
         hipStream_t st = static_cast<hipStream_t>(stream);
         kv4_by_shape(cache, [&](auto d, auto gr) {
             constexpr int D = decltype(d)::value, G = decltype(gr)::value;
-            if (p.rows) {
-                launch_tile<D, G>(a, p, st);
+            if (p.rows && p.waves == 4) {
+                launch_tile<D, G, 4>(a, p, st);
+            } else if (p.rows) {
+                if constexpr (D == 128) launch_tile<D, G, 8>(a, p, st);
             } else if (p.wide) {
                 launch_split<D, G, 1, wide_waves(D, G)>(a, p, st);
             } else if (p.mt == 1) {

@@ -179,6 +179,34 @@ def test_whole_prompts_scales_of_any_size(cuda, d, group, spread, base, q_scale)
     _run(cuda, [1100, 300], [1100, 700], 8, 4, d, group, 16, seed=40, spread=spread, base=base, q_scale=q_scale)
 
 
+@pytest.mark.parametrize("d,group", SHAPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts_of_many_heads(cuda, d, group, causal):
+    """Enough row tiles for the largest workgroups."""
+    _run(cuda, [1101, 30, 0, 300], [1101, 500, 9, 299], 8, 16, d, group, 16, causal, seed=50)
+
+
+@pytest.mark.parametrize("d,group", SHAPES)
+@pytest.mark.parametrize("q_lens,kv_lens", [([1037, 30], [1037, 500]), ([20, 9], [300, 700])])
+def test_rows_of_any_size(cuda, d, group, q_lens, kv_lens):
+    """Queries of a tile from 2^-40 to 2^3, and of zeros: a row's products do not suffer from a larger row's."""
+    cache = _cache(51, 200, 8, 16, d, group, cuda)
+    table = _table(51, [-(-n // 16) for n in kv_lens], 200, -(-max(kv_lens) // 16), cuda)
+    g = torch.Generator(device=cuda).manual_seed(52)
+    shape = (sum(q_lens), 32, 1)
+    q = torch.randn((*shape[:2], d), generator=g, device=cuda) * torch.exp2(torch.randint(-40, 4, shape, generator=g, device=cuda).float())
+    q = (q * (torch.rand(shape, generator=g, device=cuda) > 0.1)).bfloat16()
+    lens = torch.tensor(kv_lens, dtype=torch.int32, device=cuda)
+    cu = torch.tensor(np.cumsum([0] + q_lens), dtype=torch.int32, device=cuda)
+    for scale in (d ** -0.5, 2.0 ** 20):  # the second makes scores of the small rows, and one heavy token of the large ones'
+        got, lse = ops.kv4_attention(q, cache, table, lens, cu_q=cu, scale=scale, return_lse=True)
+        want, want_lse, bound, moved = _reference(q, cache, table, kv_lens, q_lens, True, scale)
+        near = 2 * moved < 1  # else the scores' own rounding decides which token is the heavy one
+        assert torch.all(((got.double() - want).abs() <= bound)[near])
+        assert torch.all(((lse.double() - want_lse).abs() <= 1e-5 * (1 + want_lse.abs()) + moved)[near])
+        assert near.double().mean() > 0.5
+
+
 @pytest.mark.parametrize("d,group", [(64, 64), (128, 32), (128, 128)])
 @pytest.mark.parametrize("q_lens", [[1, 1], [40, 90]])
 def test_scales_of_any_size(cuda, d, group, q_lens):
