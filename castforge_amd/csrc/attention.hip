@@ -84,10 +84,8 @@ struct Seq {
     int seq, first, n, len, tile;  // first token of its n queries; cached tokens; row tile
 };
 
-// Tokens that a sequence's table holds, kept so far below 2^31 that offsets past a length do not wrap.
-__device__ __forceinline__ int token_cap(const AttnArgs &a) {
-    return static_cast<int>(min(static_cast<int64_t>(a.table_cols) << a.page_shift, int64_t{0x7ffffe00}));
-}
+// Tokens that a sequence's table holds: so far below 2^31 (check_counts) that offsets past a length do not wrap.
+__device__ __forceinline__ int token_cap(const AttnArgs &a) { return a.table_cols << a.page_shift; }
 
 // Splits that share a sequence of len tokens: at least 128 tokens each.
 __device__ __forceinline__ int splits_of(int len, int splits) { return max(1, min(splits, (len + 127) / 128)); }
@@ -565,7 +563,8 @@ struct SplitLds {
     float m[NW][16], l[NW][16];
 };
 
-// Waves a SIMD by the registers they take: two where a row tile's are doubled or a token has several group words in 128 channels.
+// Waves a SIMD at least, by the registers they take without spilling.  (Fewer registers, for one wave more with several group words in
+// 128 channels, and loads two tiles ahead were no faster: 33 us for a sequence of 131072, 4 heads in groups of 32, against 36 and 36.)
 constexpr int split_waves(int d, int g, int mt) { return (d == 128 && g < 128) || mt > 1 ? 2 : g == 32 ? 3 : 4; }
 
 template <int D, int G, int MT, int NW>
@@ -642,6 +641,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 
     }
 }
 
+// Joins the splits: 2.7 us for one sequence of a few splits, 5.4 us for 128 splits of 28 rows, and the host's second launch.
 // The splits of a row: a workgroup a (token, query head), D / 8 lanes of eight channels by 2048 / D lanes of splits.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
@@ -854,8 +854,9 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     if (tokens == 0 || batch == 0) return p;
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio;
     const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
-    // enough row tiles of 32 for two waves a SIMD: every wave its own rows
-    p.rows = varlen && rows / 32 * c->kv_heads >= 4 * cus;
+    // Enough rows for six waves a CU of 32 rows: every wave its own rows.  8 heads of 128, 4 queries each: prompts of 1024 (four
+    // waves a CU), 1536 and 2048 tokens 39, 57 and 74 us; as splits 32, 56 and 85.
+    p.rows = varlen && rows / 32 * c->kv_heads >= 6 * cus;
     if (p.rows) {
         p.mt = most_tiles(c->head_dim, c->group);
         // Eight waves share the making of operands where there are two workgroups of them a CU, the heavy ones to be evened out by the
@@ -866,7 +867,10 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
         return p;
     }
     const int64_t each = (rows + batch - 1) / batch;
-    p.mt = each <= 16 ? 1 : most_tiles(c->head_dim, c->group);
+    // Two row tiles a wave, where they fit, halve the work on the codes; with few rows a sequence they leave tiles half empty and
+    // sequences of unlike lengths unevenly dealt.  8 heads of 128, 4 queries each: 16 sequences of up to 33 tokens (86 rows on
+    // average) 42 us with one tile and 58 with two, 4 of 16 tokens 30 and 29, 8 of 64 tokens 81 and 64.
+    p.mt = each <= 96 ? 1 : most_tiles(c->head_dim, c->group);
     p.tiles = tiles(16 * p.mt);
     const int64_t tasks = p.tiles * c->kv_heads, len = table_cols * c->page_size;
     // A short table and few workgroups: one launch of wide workgroups, two rounds of 32 tokens a wave at most, no partial sums.
@@ -875,6 +879,8 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     // against 16.3 on the GPU.  At 2000 tokens, four rounds, one sequence takes 16.1 against 8.5 there.
     p.wide = p.mt == 1 && tasks <= cus && len > 128 && len <= 64 * wide_waves(c->head_dim, c->group);
     if (p.wide) return p;
+    // Two workgroups a CU.  With three or four: 512 tokens after 8192 (8 heads of 128, 4 queries each) 118, 148 and 148 us; one sequence
+    // of 32768 18.2, 18.5 and 20.6.
     p.splits = std::max<int64_t>(1, std::min((2 * cus + tasks - 1) / tasks, (len + 127) / 128));
     const int64_t row = (c->head_dim + 4) * 4;
     p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
@@ -926,7 +932,7 @@ void check_counts(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int
     require(tokens >= 0 && tokens <= 0x7fffffff && batch >= 0 && batch <= 0x7fffffff, "tokens and batch must be in [0, 2^31)");
     require(q_heads >= 1 && q_heads % c->kv_heads == 0 && q_heads / c->kv_heads <= 64,
             "q_heads must be a multiple of kv_heads, at most 64 of them a head of keys");
-    require(table_cols >= 0 && table_cols <= 0x7fffffff / c->page_size, "a sequence must be shorter than 2^31 tokens");
+    require(table_cols >= 0 && table_cols <= 0x7ffff000 / c->page_size, "a sequence's table must hold at most 2^31 - 4096 tokens");
     require(tokens * q_heads <= 0x7fffffff, "tokens * q_heads must be below 2^31");
 }
 

@@ -20,7 +20,6 @@
 namespace cfh {
 namespace {
 
-typedef int int32x4 __attribute__((ext_vector_type(4)));
 typedef int int32x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));

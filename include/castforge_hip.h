@@ -558,7 +558,7 @@ typedef struct {
  * The groups' scales are thus finite.
  * q (optional, bf16 [tokens, q_heads, head_dim]) is rotated into q_out (contiguous), rounded once to bf16.
  * k, v, q: bf16, 16-byte aligned, channels and heads contiguous, *_stride elements from token to token (a
- * multiple of 8), so that slices of one projection's output need no copy. */
+ * multiple of 8), so that slices of one projection's output need no copy.  cos, sin and q_out: 16-byte aligned. */
 int32_t castforge_hip_kv4_append(const cfh_kv4_cache_t *cache, const uint16_t *k, int64_t k_stride, const uint16_t *v,
                                  int64_t v_stride, int64_t tokens, const int64_t *slots, const int64_t *positions,
                                  const float *cos, const float *sin, int64_t max_pos, int64_t rot, int32_t interleaved,
@@ -574,7 +574,7 @@ int32_t castforge_hip_kv4_gather(const cfh_kv4_cache_t *cache, const int64_t *sl
  * h / (q_heads / kv_heads) of the keys.  Sequence b has the queries cu_q[b] .. cu_q[b + 1] - 1 (cu_q i32 [batch + 1],
  * rising from 0; NULL: one query each) and kv_lens[b] cached tokens, token t in place t % page_size of page
  * page_table[b][t / page_size] (i32 [batch, table_cols]; entries past a sequence's last page are not read, tokens of a
- * page id outside the cache are left out, and a length past the table is cut).  causal 1: query i of n sees the tokens
+ * page id outside the cache are left out, and a length past the table is cut; table_cols * page_size at most 2^31 - 4096).  causal 1: query i of n sees the tokens
  * t <= kv_lens[b] - n + i; 0: all.  A query that sees nothing gives zeros.  lse (optional, f32 [tokens, q_heads]): the natural
  * logarithm of the sum of exp(scores), -inf there.  Rows of out and lse that belong to no sequence are not written.
  * q: bf16, 16-byte aligned, heads contiguous, q_stride elements from token to token (a multiple of 8).
