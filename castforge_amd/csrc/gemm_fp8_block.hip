@@ -313,7 +313,7 @@ void fp8_block_tile_kernel(GemmArgs g) {
 // Workgroup tile 32 I (n) x 32 J (m).  Each of NW waves computes the whole tile over its own runs (w, w + NW, ..), with an LDS ring
 // of its own (S stages of both panels' rows of 128 bytes and the A rows' scales), so the loop has no barrier and up to NW S
 // runs a workgroup are in flight; the tiles are summed through LDS in wave order.  Bound by the latency of the few runs that
-// each wave walks, and by HBM where N K is large: one row, 4096 x 4096, 5.9 us; one row, 11008 x 4096, 11.4 us (4.0 TB/s).
+// each wave walks, and by HBM where N K is large: one row, 4096 x 4096, 5.9 us; one row, 11008 x 4096, 9.3 us (4.9 TB/s).
 template <int I, int J, int NW, int S>
 struct Split {
     static constexpr int kPanels = 32 * (I + J) * kRun, kStage = kPanels + 256;
@@ -509,22 +509,29 @@ void launch_tile(GemmArgs g, hipStream_t st) {
 
 // The cheapest kernel by the rounds of its workgroups over the CUs, in us at K = 4096 (all grow with K alike; measured, fp8 and exact
 // form, beside what the next candidate takes there):
-//   32 x 32, K over 8 waves     4.5 (4.9) a round    M = 1: 5.9 us; M = 64, N = 4096: 7.3 (64 x 64: 12.2)
-//   64 x 64, K over 4 waves     10.3 (12.7) a round  M = 256, N = 4096: 12.8 (128 x 128: 26); M = 64, N = 11008: 12.8 (32 x 32: 16.2)
-//   128 x 128, two a CU         20.5 (35) times tiles over CUs, at least 24.5 (33)
+//   32 x 32, K over 8 waves      6.5 (7.0) and 4.5 (4.8) for each further round
+//                                                    M = 64, N = 4096: 7.1 (64 n x 32 m: 8.0)
+//   64 n x 32 m, K over 6 waves  8.8 (10.4) and 6.2 (7.6)
+//                                                    M = 1, N = 11008: 9.3 (32 x 32: 10.9); M = 45, N = 5001, exact: 10.0 (11.6)
+//   64 x 64, K over 4 waves      12 (15) and 10.3 (12.7)
+//                                                    M = 256, N = 4096: 12.8 (128 x 128: 26); M = 64, N = 11008: 12.4 (64 n x 32 m: 15.4)
+//   128 x 128, two a CU          20.5 (35) times tiles over CUs, at least 24.5 (33)
 //                                                    M = 1024, N = 4096: 28.7 (64 x 64: 42); M = 256, N = 11008: 27 (31.5)
-//   256 x 256, fp8 form         70 a round, 54 for one that leaves CUs idle
+//   256 x 256, fp8 form          70 a round, 54 for one that leaves CUs idle
 //                                                    M = 4096, N = 11008: 208 (128 x 128: 246); M = 1024, N = 11008: 61 (67)
 template <bool kExact>
 void launch_by_cost(const GemmArgs &g, hipStream_t st) {
     const double cus = static_cast<double>(cu_count());
-    const auto tiles = [&](int t) { return static_cast<double>((g.M + t - 1) / t) * ((g.N + t - 1) / t); };
-    const auto rounds = [&](int t) { return std::ceil(tiles(t) / cus); };
-    const double c32 = (kExact ? 4.9 : 4.5) * rounds(32), c64 = (kExact ? 12.7 : 10.3) * rounds(64);
-    const double c128 = kExact ? std::max(33.0, 35 * tiles(128) / cus) : std::max(24.5, 20.5 * tiles(128) / cus);
-    const double c256 = kExact ? 1e30 : tiles(256) < 0.9 * cus ? 54 : 70 * rounds(256);
-    const double best = std::min({c32, c64, c128, c256});
+    const auto tiles = [&](int tn, int tm) { return static_cast<double>((g.M + tm - 1) / tm) * ((g.N + tn - 1) / tn); };
+    const auto cost = [&](int tn, int tm, double first, double further) { return first + further * (std::ceil(tiles(tn, tm) / cus) - 1); };
+    const double c32 = kExact ? cost(32, 32, 7.0, 4.8) : cost(32, 32, 6.5, 4.5);
+    const double c64n = kExact ? cost(64, 32, 10.4, 7.6) : cost(64, 32, 8.8, 6.2);
+    const double c64 = kExact ? cost(64, 64, 15, 12.7) : cost(64, 64, 12, 10.3);
+    const double c128 = kExact ? std::max(33.0, 35 * tiles(128, 128) / cus) : std::max(24.5, 20.5 * tiles(128, 128) / cus);
+    const double c256 = kExact ? 1e30 : tiles(256, 256) < 0.9 * cus ? 54 : cost(256, 256, 70, 70);
+    const double best = std::min({c32, c64n, c64, c128, c256});
     if (best == c32) launch_split<kExact, 1, 1, 8, 2>(g, st);
+    else if (best == c64n) launch_split<kExact, 2, 1, 6, 2>(g, st);
     else if (best == c64) launch_split<kExact, 2, 2, 4, 2>(g, st);
     else if (kExact || best == c128) launch_tile<kExact, 2, 2, 2, 2>(g, st);
     else if constexpr (!kExact) launch_tile<false, 2, 4, 4, 2>(g, st);
