@@ -47,6 +47,7 @@ __device__ __forceinline__ int32x8 join(const uint4 &lo, const uint4 &hi) {
 // cover the 256-byte bank window.
 __device__ __forceinline__ int swz(int r, int c) { return c ^ ((r >> 1) & 7); }
 
+// Chunks c and c + 1 of row r; `rows` starts at a multiple of 16 rows of its panel.
 __device__ __forceinline__ int32x8 frag(const uint8_t *rows, int r, int c) {
     return join(*reinterpret_cast<const uint4 *>(rows + r * kRun + swz(r, c) * 16), *reinterpret_cast<const uint4 *>(rows + r * kRun + swz(r, c + 1) * 16));
 }
@@ -81,10 +82,11 @@ __device__ __forceinline__ Panels panels_of(const GemmArgs &g, int n0, int rows_
     return p;
 }
 
-// One load of eight rows (8 block, ..) of run r into 1 KB of LDS.  The last run's chunks past K read 0 too, sent past the panel.
+// One load of eight rows (8 block, ..) of run r into 1 KB of LDS.  kTail: the run's chunks past K read 0 too, sent past the panel.
+template <bool kTail>
 __device__ __forceinline__ void panel_load(__amdgpu_buffer_rsrc_t panel, const Panels &p, uint8_t *dst, int block, int odd, int K, int r) {
     int at = p.at[odd] + (block * 8 * K + r * kRun);
-    if ((r + 1) * kRun > K) at = r * kRun + p.in_run[odd] < K ? at : 0x7fffffff;  // uniform
+    if (kTail) at = r * kRun + p.in_run[odd] < K ? at : 0x7fffffff;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(panel, (__attribute__((address_space(3))) void *)dst, 16, at, 0, 0, 0);
 }
 
@@ -110,8 +112,10 @@ __device__ __forceinline__ void store4(const GemmArgs &g, int m, int n, const fl
 //
 // Workgroup tile 32 I WN (n) x 32 J WM (m), WN x WM waves of 32 I x 32 J.  A stage is one run of 128 of both
 // panels and the A rows' scales, brought by buffer loads straight into LDS; two stages, one barrier a stage:
-// a stage is loaded while the other one is computed.  MFMA-bound in the large: 4096 x 11008 x 4096 208 us, 1.78 PFLOP/s, the matrix
-// unit busy half the time; the rest is the wait at the stage's barrier for loads and fragments.
+// a stage is loaded while the other one is computed.  4096 x 11008 x 4096: 206 to 220 us, 1.7 to 1.8 PFLOP/s (2.0 where K is 11008); a
+// third of a CU's last round of tiles is idle, the clock is 2.05 GHz under the load, and of the busy cycles 47% are MFMAs and 35%
+// the folds and addresses, which hardly overlap on a SIMD.  No faster: a run's first fragments read ahead of its barrier; 128 x
+// 128 a wave at one wave a SIMD, whose sums lie where vector instructions cannot reach them (73 -> 90 us for 4096 x 4096 x 4096).
 template <int I, int J, int WN, int WM>
 struct Tile {
     static constexpr int NW = WN * WM, BN = 32 * I * WN, BM = 32 * J * WM;
@@ -127,11 +131,19 @@ struct Tile {
 // This wave's loads of run r of both panels and of the A rows' scales into the stage `dst`.
 template <class T>
 __device__ __forceinline__ void tile_issue(const Panels &p, uint8_t *__restrict__ dst, int wave, int lane, int K, int runs, int r) {
+    const auto load = [&](auto tail) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < T::kLoads; ++t) {
-        const int first = wave * T::kLoads + t;  // of the stage's loads of eight rows
-        const bool is_w = first * 8 < T::BN;     // uniform
-        panel_load(is_w ? p.w : p.a, p, dst + first * 1024, is_w ? first : first - T::BN / 8, t & 1, K, r);
+        for (int t = 0; t < T::kLoads; ++t) {
+            const int first = wave * T::kLoads + t;  // of the stage's loads of eight rows
+            const bool is_w = first * 8 < T::BN;     // uniform
+            panel_load<decltype(tail)::value>(is_w ? p.w : p.a, p, dst + first * 1024, is_w ? first : first - T::BN / 8, t & 1, K, r);
+        }
+    };
+    if ((r + 1) * kRun > K) {
+        asm volatile("");  // a branch: selects would cost every run
+        load(std::true_type{});
+    } else {
+        load(std::false_type{});
     }
     static_assert(T::kLoads % 2 == 0 && T::BN % 16 == 0, "the parity of a load is that of its rows");
     static_assert(T::BM <= 64 * T::NW, "one load of scales a wave");
@@ -153,7 +165,7 @@ __device__ __forceinline__ void tile_stage(const uint8_t *__restrict__ cur, uint
     float f[J];
     const auto read_a = [&](int j, int32x8 (&a)[2]) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) a[kk] = frag(cur + T::BN * kRun, wm + 32 * j + fr, 4 * kk + fc);
+        for (int kk = 0; kk < 2; ++kk) a[kk] = frag(cur + (T::BN + wm + 32 * j) * kRun, fr, 4 * kk + fc);
     };
     const auto fold = [&](floatx16 &sum, const floatx16 &part, float by) {
 #pragma unroll
@@ -172,7 +184,7 @@ __device__ __forceinline__ void tile_stage(const uint8_t *__restrict__ cur, uint
 #pragma unroll
         for (int i = 0; i < I; ++i)
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) w[i][kk] = frag(cur, wn + 32 * i + fr, 4 * kk + fc);
+            for (int kk = 0; kk < 2; ++kk) w[i][kk] = frag(cur + (wn + 32 * i) * kRun, fr, 4 * kk + fc);
 #pragma unroll
         for (int j = 0; j < J; ++j) f[j] = scales[32 * j] * sw;
         static_for<I * J + 1>([&](auto TT) {
@@ -193,7 +205,7 @@ __device__ __forceinline__ void tile_stage(const uint8_t *__restrict__ cur, uint
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) w[i][kk] = frag(cur, wn + 32 * i + fr, 4 * kk + fc);
+        for (int kk = 0; kk < 2; ++kk) w[i][kk] = frag(cur + (wn + 32 * i) * kRun, fr, 4 * kk + fc);
     static_for<J>([&](auto JJ) {
         constexpr int j = decltype(JJ)::value;
         f[j] = scales[32 * j] * sw;
@@ -333,8 +345,16 @@ __device__ __forceinline__ void wait_vm_fence() {
 
 template <int I, int J>
 __device__ __forceinline__ void split_issue(const Panels &p, uint8_t *__restrict__ dst, int lane, int K, int runs, int r) {
+    const auto load = [&](auto tail) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < 4 * (I + J); ++t) panel_load(t < 4 * I ? p.w : p.a, p, dst + t * 1024, t < 4 * I ? t : t - 4 * I, t & 1, K, r);
+        for (int t = 0; t < 4 * (I + J); ++t) panel_load<decltype(tail)::value>(t < 4 * I ? p.w : p.a, p, dst + t * 1024, t < 4 * I ? t : t - 4 * I, t & 1, K, r);
+    };
+    if ((r + 1) * kRun > K) {
+        asm volatile("");  // a branch
+        load(std::true_type{});
+    } else {
+        load(std::false_type{});
+    }
     __builtin_amdgcn_raw_ptr_buffer_load_lds(p.s, (__attribute__((address_space(3))) void *)(dst + 32 * (I + J) * kRun), 4, (lane * runs + r) * 4, 0, 0, 0);
 }
 
@@ -354,9 +374,9 @@ __device__ __forceinline__ void split_step(const uint8_t *__restrict__ cur, uint
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-        for (int i = 0; i < I; ++i) w[i][kk] = frag(cur, 32 * i + fr, 4 * kk + fc);
+        for (int i = 0; i < I; ++i) w[i][kk] = frag(cur + 32 * i * kRun, fr, 4 * kk + fc);
 #pragma unroll
-        for (int j = 0; j < J; ++j) a[j][kk] = frag(cur + 32 * I * kRun, 32 * j + fr, 4 * kk + fc);
+        for (int j = 0; j < J; ++j) a[j][kk] = frag(cur + 32 * (I + j) * kRun, fr, 4 * kk + fc);
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) f[j] = reinterpret_cast<const float *>(cur + P::kPanels)[32 * j + fr] * sw;
