@@ -698,8 +698,8 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
 // wave turns 16 into MFMA operands in LDS (f16: of the keys codes less zero points, exactly; of the values that times c) and all
 // read them back; two stages, one barrier a stage: the operands of the next tokens are made while the present ones are used, and
 // the words of those after that are on their way.
-// A prompt of 4096 tokens, 32 query heads on 8 of 128 channels: 165 us, 137 GFLOP at 834 TFLOP/s.  VALU work and MFMAs hardly overlap on a
-// SIMD (an MFMA of 16 cycles hides one or two instructions), so it is bound by their sum: 37% of the time are MFMAs, 49% the softmax
+// A prompt of 4096 tokens, 32 query heads on 8 of 128 channels: 160 us, 137 GFLOP at 860 TFLOP/s.  VALU work and MFMAs hardly overlap on a
+// SIMD (an MFMA of 16 cycles hides one or two instructions), so it is bound by their sum: 38% of the busy cycles are MFMAs, 47% the softmax
 // and the making of operands; without the latter it takes 145 us, without LDS reads 7 us less, and the products of
 // the next tokens issued among the present ones' exponentials change nothing.
 // Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row tiles from the
@@ -860,7 +860,7 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     if (p.rows) {
         p.mt = most_tiles(c->head_dim, c->group);
         // Eight waves share the making of operands where there are two workgroups of them a CU, the heavy ones to be evened out by the
-        // light ones.  Prompts of 4096 and of 2048 tokens, 8 heads of 128 channels, 4 queries each: 165 and 78 us, with four waves
+        // light ones.  Prompts of 4096 and of 2048 tokens, 8 heads of 128 channels, 4 queries each: 160 and 78 us, with four waves
         // 186 and 73.  With 64 channels four of them take 109 us and eight 120: their registers leave room for four waves a SIMD.
         if (c->head_dim == 128 && rows / (128 * p.mt) * c->kv_heads >= 2 * cus) p.waves = 8;
         p.tiles = tiles(16 * p.waves * p.mt);

@@ -80,8 +80,9 @@ __device__ __forceinline__ uint32_t codes_of_any(const float (&x)[8], float scal
 }
 
 // A workgroup has one token (its slot, position and angles are read once) and up to `share` of its heads, in the order K, V, Q:
-// eight elements a lane, D / 8 lanes a head.  HBM-bound where the tokens are many: 4096 tokens of 32 heads of each kind, all in
-// places of their own, move 170 MB with the cache's partial lines.
+// eight elements a lane, D / 8 lanes a head.  HBM-bound where the tokens are many, its vector instructions about as busy: 4096 tokens of 32 heads
+// of each kind, all in places of their own, move 152 MB, more with the cache's partial lines, in 32 to 34 us (4.5 to 4.7 TB/s);
+// 16 tokens of 8 heads and 32 of the queries take 3.4 us.
 template <int D, int G>
 __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int share) {
     constexpr int kLanes = D / 8, kUnits = 256 / kLanes;
@@ -180,7 +181,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int share
     }
 }
 
-// Rows of the cache as numbers, a workgroup a token, eight elements a lane; a slot outside the cache gives zeros.
+// Rows of the cache as numbers, a workgroup a token, eight elements a lane; a slot outside the cache gives zeros.  HBM-bound: 4096
+// tokens of 32 heads, 85 MB, in 21 us (4.1 TB/s).
 template <int D, int G>
 __global__ __launch_bounds__(256) void kv4_gather_kernel(const uint32_t *__restrict__ k_codes, const uint32_t *__restrict__ k_groups,
                                                          const uint32_t *__restrict__ v_codes, const uint32_t *__restrict__ v_groups,
@@ -220,7 +222,8 @@ __global__ __launch_bounds__(256) void kv4_gather_kernel(const uint32_t *__restr
 }
 
 // Heads a workgroup takes of a token: one round of its lanes where that leaves the card with less than four workgroups a CU, else
-// more of them, for whom the angles and the slot are read once.
+// more of them, for whom the angles and the slot are read once.  16 tokens of 96 heads: 3.3 us, as one workgroup a token 6.2; 4096
+// of them: 32 us, by one round a workgroup 42.
 int share_of(int64_t tokens, int units, int lanes) {
     const int round = 256 / lanes, rounds = (units + round - 1) / round;
     const int64_t wanted = (4 * cu_count() + tokens - 1) / tokens;  // workgroups a token
