@@ -274,8 +274,9 @@ struct Rows {
 
 // Loads the rows.  A row's power of two takes its largest element below 2^14, so that a sixteenth of it keeps bf16's bits down to
 // 2^-24 of the largest.  kShared: all rows take the greatest one's, whose exponent is returned for the tables to hold: a row
-// 2^10 smaller keeps its bits down to 2^-16 of its largest and loses 2^-25 of that below.  Rows smaller still have their own, and
-// `uneven` is set.  most(v): the greatest v of those who read the tables.
+// 2^10 smaller keeps its bits down to 2^-16 of its largest and loses 2^-25 of that below.  Rows smaller still have their own, as
+// have rows above 2^64, whose exponent would take the tables out of f32's range; `uneven` is set then.  most(v): the greatest v of
+// those who read the tables.
 template <bool kShared, int D, int G, int MT, class Most>
 __device__ __forceinline__ int load_rows(const AttnArgs &a, Rows<D, G, MT> &s, const Seq &sq, int head, int row0, const Most &most) {
     constexpr int GR = D / G, W = G / 32, kNone = -1000;
@@ -313,11 +314,11 @@ __device__ __forceinline__ int load_rows(const AttnArgs &a, Rows<D, G, MT> &s, c
         greatest = max(greatest, ex[mt]);
     }
     int all = kShared ? most(max_over_wave(greatest)) : 0;
-    if (all == kNone) all = 0;  // rows of zeros
+    all = all == kNone ? 0 : min(all, 50);  // kNone: rows of zeros
     bool apart = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const bool own = ex[mt] != kNone && (!kShared || ex[mt] < all - 10);
+        const bool own = ex[mt] != kNone && (!kShared || ex[mt] < all - 10 || ex[mt] > all);
         const int at_ex = own ? ex[mt] : all;
         apart |= own;
         s.rel[mt] = __builtin_ldexpf(1.0f, at_ex - all);

@@ -188,14 +188,16 @@ def test_prompts_of_many_heads(cuda, d, group, causal):
 
 @pytest.mark.parametrize("d,group", SHAPES)
 @pytest.mark.parametrize("q_lens,kv_lens", [([1637, 30], [1637, 500]), ([20, 9], [300, 700]), ([200, 9], [300, 700])])
-def test_rows_of_any_size(cuda, d, group, q_lens, kv_lens):
-    """Queries of a tile from 2^-40 to 2^3, and of zeros: a row's products do not suffer from a larger row's."""
+@pytest.mark.parametrize("top", [0, 60, 120])
+def test_rows_of_any_size(cuda, d, group, q_lens, kv_lens, top):
+    """Queries of a tile from 2^-40 to 2^3, of zeros, and a few 2^top times that: a row's products do not suffer from a larger row's."""
     cache = _cache(51, 300, 8, 16, d, group, cuda)
     table = _table(51, [-(-n // 16) for n in kv_lens], 300, -(-max(kv_lens) // 16), cuda)
     g = torch.Generator(device=cuda).manual_seed(52)
     shape = (sum(q_lens), 32, 1)
     q = torch.randn((*shape[:2], d), generator=g, device=cuda) * torch.exp2(torch.randint(-40, 4, shape, generator=g, device=cuda).float())
-    q = (q * (torch.rand(shape, generator=g, device=cuda) > 0.1)).bfloat16()
+    u = torch.rand(shape, generator=g, device=cuda)
+    q = (q * (u > 0.1) * torch.where(u > 0.97, 2.0**top, 1.0)).bfloat16()
     lens = torch.tensor(kv_lens, dtype=torch.int32, device=cuda)
     cu = torch.tensor(np.cumsum([0] + q_lens), dtype=torch.int32, device=cuda)
     for scale in (d ** -0.5, 2.0 ** 20):  # the second makes scores of the small rows, and one heavy token of the large ones'
