@@ -62,6 +62,15 @@ def test_against_float64(cuda, m, n, k, exact, out):
 
 
 @pytest.mark.parametrize("exact", [True, False])
+@pytest.mark.parametrize("m,n,k", [(1, 11008, 4096), (16, 8333, 2064), (40, 5001, 1552), (3, 16000, 784), (100, 4100, 912)])
+def test_tiles_of_64_by_32(cuda, m, n, k, exact):
+    """Few rows of many outputs: K over six waves, more than one turn of each wave's ring."""
+    (qa, sa), (qw, sw) = _inputs(m + n, m, n, k, cuda)
+    y = ops.gemm_fp8_block(qa, sa, qw, sw, out_dtype=torch.float32 if exact else torch.bfloat16, exact=exact)
+    _check(y, qa, sa, qw, sw, exact)
+
+
+@pytest.mark.parametrize("exact", [True, False])
 @pytest.mark.parametrize("m,n,k", [(700, 4096, 4096), (1500, 1408, 1024), (2048, 2049, 512), (4096, 2048, 1088)])
 def test_large(cuda, m, n, k, exact):
     (qa, sa), (qw, sw) = _inputs(5, m, n, k, cuda)
