@@ -243,6 +243,26 @@ def test_masked_places_may_hold_anything(cuda, q_lens):
         assert torch.all((got.double() - want).abs() <= bound)
 
 
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [700, 129]), ([1, 1], [90, 3000]), ([500, 40], [700, 129]), ([900, 300], [900, 300])])
+def test_offsets_past_32_bits(cuda, q_lens, kv_lens):
+    """Pages at the ends of a cache of more than 2^32 words of codes give the bits of a small cache's."""
+    heads, page, d, pages = 16, 128, 128, 140000  # 18 GB of codes each
+    small = _cache(70, 40, heads, page, d, 128, cuda)
+    big = ops.Kv4Cache(*(torch.empty((pages, *t.shape[1:]), dtype=torch.int32, device=cuda)
+                         for t in (small.k_codes, small.k_groups, small.v_codes, small.v_groups)))
+    at = torch.tensor([i if i % 2 else pages - 1 - i for i in range(40)], device=cuda)
+    for a, b in ((big.k_codes, small.k_codes), (big.k_groups, small.k_groups), (big.v_codes, small.v_codes), (big.v_groups, small.v_groups)):
+        a[at] = b
+    table = _table(71, [-(-n // page) for n in kv_lens], 40, -(-max(kv_lens) // page), cuda)
+    far = torch.where(table < 40, at[table.clamp(max=39).long()].int(), table)
+    g = torch.Generator(device=cuda).manual_seed(72)
+    q = torch.randn((sum(q_lens), 4 * heads, d), generator=g, device=cuda).bfloat16()
+    lens = torch.tensor(kv_lens, dtype=torch.int32, device=cuda)
+    cu = None if max(q_lens) == 1 else torch.tensor(np.cumsum([0] + q_lens), dtype=torch.int32, device=cuda)
+    got = ops.kv4_attention(q, big, far, lens, cu_q=cu)
+    assert torch.equal(got, ops.kv4_attention(q, small, table, lens, cu_q=cu)) and torch.isfinite(got).all()
+
+
 def test_length_past_the_table_is_cut(cuda):
     q, cache, table, lens, _, _ = _run(cuda, [1], [160], 2, 4, 128, 128, 16, seed=17)
     assert torch.equal(ops.kv4_attention(q, cache, table, lens + 1000), ops.kv4_attention(q, cache, table, lens))

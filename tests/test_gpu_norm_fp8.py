@@ -122,6 +122,19 @@ def test_block_quantizer_non_finite(cuda):
     assert np.isfinite(c[2:]).all()
 
 
+def test_offsets_past_32_bits(cuda):
+    """Rows at the end of more than 2^32 bytes come out as they do alone."""
+    m, k = 65600, 32768
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(30)
+    x[-3:] = torch.randn((3, k), generator=g, device=cuda).bfloat16()
+    w = torch.ones(k, dtype=torch.bfloat16, device=cuda)
+    for part, whole in ((ops.rms_norm_fp8(x[-3:], w, residual=x[-3:], block=128), ops.rms_norm_fp8(x, w, residual=x, block=128)),
+                        (ops.quantize_fp8_block(x[-3:]), ops.quantize_fp8_block(x))):
+        for a, b in zip(part, whole):
+            assert torch.equal(a, b[-3:])
+
+
 def test_refusals(cuda):
     x, w = torch.zeros((2, 128), device=cuda, dtype=torch.bfloat16), torch.zeros(128, device=cuda)
     for bad in (dict(weight=w[:64]), dict(block=64), dict(residual=x.float()), dict(residual=x[:1]), dict(out=x),
