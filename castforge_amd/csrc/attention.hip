@@ -358,49 +358,57 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const flo
     float y[MT][2][4];  // scores and their tokens' exponents, base 2
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        floatx4 ks[GR], dot[MT][GR];
-#pragma unroll
-        for (int gr = 0; gr < GR; ++gr) ks[gr] = four(tokens.keys[gr], h);
         const floatx4 e = four(tokens.exponent, h);
-#pragma unroll
-        for (int gr = 0; gr < GR; ++gr)
+        const auto product = [&](int gr, floatx4 (&dot)[MT]) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < W; ++u) {
                 const halfx8 k = keys(h, gr, u);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
-                    dot[mt][gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, s.q[mt][gr][u], u ? dot[mt][gr] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    dot[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, s.q[mt][gr][u], u ? dot[mt] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             }
-        if (kShared && s.uneven) {
-            asm volatile("");  // a branch
+        };
+        if constexpr (kShared) {
+            // group by group: two row tiles of four groups fit the registers only so
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) {
+                const floatx4 ks = four(tokens.keys[gr], h);
+                floatx4 dot[MT];
+                product(gr, dot);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[mt][h][r] = __builtin_fmaf(dot[mt][r], ks[r], gr ? y[mt][h][r] : e[r]);
+            }
+        } else {
+            floatx4 ks[GR], dot[GR][MT];
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) ks[gr] = four(tokens.keys[gr], h);
+#pragma unroll
+            for (int gr = 0; gr < GR; ++gr) product(gr, dot[gr]);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int gr = 0; gr < GR; ++gr) dot[mt][gr] *= s.rel[mt];
-        }
+                for (int r = 0; r < 4; ++r) {
+                    float v = dot[0][mt][r] * ks[0][r];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if constexpr (!kShared) {
-                    float v = dot[mt][0][r] * ks[0][r];
-#pragma unroll
-                    for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], v);
+                    for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[gr][mt][r], ks[gr][r], v);
                     y[mt][h][r] = __builtin_fmaf(v, s.rel[mt], e[r]);
-                    continue;
                 }
-                y[mt][h][r] = e[r];
-#pragma unroll
-                for (int gr = 0; gr < GR; ++gr) y[mt][h][r] = __builtin_fmaf(dot[mt][gr][r], ks[gr][r], y[mt][h][r]);
-            }
+        }
     }
-    if (edge) {
+    if (edge || (kShared && s.uneven)) {
         asm volatile("");  // a branch: as selects on a uniform condition these were a quarter of the loop
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (kShared) {
+                    const float e = tokens.exponent[first + 16 * (i / 4) + 4 * g + i % 4];
+                    y[mt][i / 4][i % 4] = e > -INFINITY ? __builtin_fmaf(y[mt][i / 4][i % 4] - e, s.rel[mt], e) : -INFINITY;
+                }
                 if (at + 16 * (i / 4) + 4 * g + i % 4 >= s.limit[mt]) y[mt][i / 4][i % 4] = -INFINITY;
+            }
     }
     constexpr int PG = kShared ? 1 : GR;
     uint32_t p[MT][PG][4];  // weights, times c, as f16 pairs: tokens (0, 1), (2, 3) of both halves
@@ -695,7 +703,7 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
     }
 }
 
-// Many rows: each wave takes 16 MT rows of its own, and the NW of a workgroup share the work on the codes.  Of every 16 NW tokens a
+// Many rows: each wave takes 32 rows of its own, and the NW of a workgroup share the work on the codes.  Of every 16 NW tokens a
 // wave turns 16 into MFMA operands in LDS (f16: of the keys codes less zero points, exactly; of the values that times c) and all
 // read them back; two stages, one barrier a stage: the operands of the next tokens are made while the present ones are used, and
 // the words of those after that are on their way.
@@ -703,6 +711,7 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
 // SIMD (an MFMA of 16 cycles hides one or two instructions), so it is bound by their sum: 38% of the busy cycles are MFMAs, 47% the softmax
 // and the making of operands; without the latter it takes 145 us, without LDS reads 7 us less, and the products of
 // the next tokens issued among the present ones' exponentials change nothing.
+// Two or three waves a SIMD: with 64 channels three take 110 us for 4096 tokens, two 140 and four 121.
 // Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row tiles from the
 // last, which see the most tokens.
 template <int D, int G, int NW>
@@ -713,8 +722,9 @@ struct Stage {
     Tokens<GR, 16 * NW> tokens;
 };
 
-template <int D, int G, int MT, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void kv4_attention_tile_kernel(AttnArgs a, int tiles) {
+template <int D, int G, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 3))) void kv4_attention_tile_kernel(AttnArgs a, int tiles) {
+    constexpr int MT = 2;
     typedef Rows<D, G, MT> S;
     constexpr int GR = D / G, W = G / 32, R = 128 / G, NT = G / 16, kWords = D / 8, VW = KvTile<D, G>::VW, kRow = D + 4, kTokens = 16 * NW;
     extern __shared__ __align__(16) uint8_t lds[];
@@ -835,8 +845,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     }
 }
 
-// Row tiles of 16 a wave at most, by its registers: with groups of 32 in 128 channels two of them no longer fit without
-// spilling, and three or four never do.
+// Row tiles of 16 a wave of the split kernel at most, by its registers: with groups of 32 in 128 channels two of them no longer fit
+// without spilling, and three or four never do.
 constexpr int most_tiles(int64_t d, int64_t g) { return d / g >= 4 ? 1 : 2; }
 
 // How a call is laid out: rows a wave (16 mt), whether waves share rows (splits of the tokens) or have their own, row
@@ -859,10 +869,11 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     // waves a CU), 1536 and 2048 tokens 39, 57 and 74 us; as splits 32, 56 and 85.
     p.rows = varlen && rows / 32 * c->kv_heads >= 6 * cus;
     if (p.rows) {
-        p.mt = most_tiles(c->head_dim, c->group);
+        p.mt = 2;
         // Eight waves share the making of operands where there are two workgroups of them a CU, the heavy ones to be evened out by the
-        // light ones.  Prompts of 4096 and of 2048 tokens, 8 heads of 128 channels, 4 queries each: 160 and 78 us, with four waves
-        // 186 and 73.  With 64 channels four of them take 109 us and eight 120: their registers leave room for four waves a SIMD.
+        // light ones.  Prompts of 4096 and of 2048 tokens, 8 heads of 128 channels, 4 queries each: 158 and 78 us, with four waves
+        // 186 and 73.  With 64 channels four of them take 110 us and eight 120: three waves a SIMD of different workgroups then wait at
+        // different times.
         if (c->head_dim == 128 && rows / (128 * p.mt) * c->kv_heads >= 2 * cus) p.waves = 8;
         p.tiles = tiles(16 * p.waves * p.mt);
         return p;
@@ -902,11 +913,11 @@ void raise_lds_limit(const void *kern, int bytes, std::atomic<uint64_t> &done) {
 
 template <int D, int G, int NW>
 void launch_tile(const AttnArgs &a, const Plan &p, hipStream_t st) {
-    constexpr int MT = most_tiles(D, G), sums = 16 * NW * (D + 4) * 4, stages = 2 * sizeof(Stage<D, G, NW>), lds = stages > sums ? stages : sums;
+    constexpr int sums = 16 * NW * (D + 4) * 4, stages = 2 * sizeof(Stage<D, G, NW>), lds = stages > sums ? stages : sums;
     static_assert(lds + NW * sizeof(Own<D, G, 16, _Float16>) <= NW * 20 * 1024, "two workgroups a CU");
     require(p.tiles * a.heads <= 0x7fffffff, "too many workgroups for one launch");
     static std::atomic<uint64_t> attr_devices{0};
-    const auto kern = kv4_attention_tile_kernel<D, G, MT, NW>;
+    const auto kern = kv4_attention_tile_kernel<D, G, NW>;
     raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
     kern<<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(64 * NW), lds, st>>>(a, static_cast<int>(p.tiles));
     check_launch("kv4_attention_tile");
