@@ -149,7 +149,7 @@ struct KvTile {
 // at a time.
 template <int GR, int N>
 struct Tokens {
-    float keys[GR][N];   // scale times what turns a product into a score
+    float keys[N][GR];   // scale times what turns a product into a score
     float exponent[N];   // of the values' largest scale; -inf where there is no token
     float back[N];       // 2^-exponent
 };
@@ -159,9 +159,11 @@ template <int D, int G, int N, class C>
 struct Own {
     static constexpr int GR = D / G, kRow = N + 4;   // tokens a row of `v`, padded for the banks
     uint32_t v[KvTile<D, G>::kDeal ? 16 * kRow : 4];  // the values' codes: word by word, a token each
-    uint32_t k[GR][N];  // zero point in both halves, as f16 denormals
+    uint32_t k[N][GR];  // zero point in both halves, as f16 denormals
     uint16_t z[GR][N];  // of the values
-    C c[GR][N];         // the values' scales without the exponent, an f16 one times 2^11
+    // the values' scales without the exponent: f32 ones a token's together, f16 ones, times 2^11, in pairs of tokens
+    static constexpr bool kPairs = sizeof(C) == 2;
+    C c[kPairs ? GR : N][kPairs ? N : GR];
 };
 
 template <int D, int G>
@@ -213,19 +215,28 @@ template <int D, int G, int N, int M, class C>
 __device__ __forceinline__ void fill_token(const uint32_t (&words)[D / G], bool value, int token, bool off, float qk, Tokens<D / G, N> &tokens, Own<D, G, M, C> &own, int at) {
     constexpr int GR = D / G;
     float v[GR], top = 0.f;
+    uint32_t z[GR];
 #pragma unroll
     for (int gr = 0; gr < GR; ++gr) {
         const uint32_t w = off ? 0u : words[gr];
         v[gr] = kv4_scale(w);
         top = fmaxf(top, v[gr]);
-        if (value) own.z[gr][at] = static_cast<uint16_t>(kv4_zero(w));
-        else own.k[gr][at] = kv4_zero(w) * 0x00010001u;
+        z[gr] = kv4_zero(w);
     }
     const int ex = __builtin_amdgcn_frexp_expf(top);
+    if (value) {
 #pragma unroll
-    for (int gr = 0; gr < GR; ++gr) {
-        if (value) own.c[gr][at] = static_cast<C>(__builtin_ldexpf(v[gr], (sizeof(C) == 2 ? 11 : 0) - ex));  // f16: exact down to 2^-25
-        else tokens.keys[gr][token] = v[gr] * qk;
+        for (int gr = 0; gr < GR; ++gr) {
+            own.z[gr][at] = static_cast<uint16_t>(z[gr]);
+            v[gr] = __builtin_ldexpf(v[gr], (sizeof(C) == 2 ? 11 : 0) - ex);
+            if constexpr (Own<D, G, M, C>::kPairs) own.c[gr][at] = static_cast<C>(v[gr]);  // exact down to 2^-25
+        }
+        if constexpr (!Own<D, G, M, C>::kPairs) __builtin_memcpy(__builtin_assume_aligned(own.c[at], 4 * GR), v, 4 * GR);
+    } else {
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) v[gr] *= qk, z[gr] *= 0x00010001u;
+        __builtin_memcpy(__builtin_assume_aligned(tokens.keys[token], 4 * GR), v, 4 * GR);
+        __builtin_memcpy(__builtin_assume_aligned(own.k[at], 4 * GR), z, 4 * GR);
     }
     if (value) tokens.exponent[token] = off ? -INFINITY : static_cast<float>(ex), tokens.back[token] = __builtin_ldexpf(1.0f, -ex);
 }
@@ -350,15 +361,24 @@ __device__ __forceinline__ float score_factor(const AttnArgs &a, int ex) { retur
 // turns u into the operand of 16 channels and 32 tokens.  first: the tokens' place in the table.  kShared: the values hold c
 // already, rounded to f16 with it, and the weights are rounded alone; many rows share that work then.
 template <bool kShared, int D, int G, int MT, int N, class Keys, class Values>
-__device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const float (*scales)[32], int first, Rows<D, G, MT> &s, int at, int sure, const Keys &keys, const Values &values) {
+__device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const float (*scales)[D / G], int first, Rows<D, G, MT> &s, int at, int sure, const Keys &keys, const Values &values) {
     constexpr int GR = D / G, W = G / 32, NT = G / 16;
     const int g = (threadIdx.x >> 4) & 3;
     const bool edge = at + 32 > sure;  // uniform: some row does not see some token
     const auto four = [&](const float *p, int h) { return *reinterpret_cast<const floatx4 *>(p + first + 16 * h + 4 * g); };
+    struct Four {
+        float v[4][GR];
+    };
+    const auto four_by = [&](const float (*p)[GR], int h) {  // of tokens with GR numbers each
+        Four f;
+        __builtin_memcpy(&f, __builtin_assume_aligned(p[first + 16 * h + 4 * g], 16), sizeof f);
+        return f;
+    };
     float y[MT][2][4];  // scores and their tokens' exponents, base 2
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const floatx4 e = four(tokens.exponent, h);
+        const Four ks = four_by(tokens.keys, h);
         const auto product = [&](int gr, floatx4 (&dot)[MT]) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < W; ++u) {
@@ -373,13 +393,12 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const flo
             // 198 for a prompt of 4096 tokens in groups of 32, 264 instead of 170 for 512 after 8192)
 #pragma unroll
             for (int gr = 0; gr < GR; ++gr) {
-                const floatx4 ks = four(tokens.keys[gr], h);
                 floatx4 dot[MT];
                 product(gr, dot);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) y[mt][h][r] = gr || kShared ? __builtin_fmaf(dot[mt][r], ks[r], gr ? y[mt][h][r] : e[r]) : dot[mt][r] * ks[r];
+                    for (int r = 0; r < 4; ++r) y[mt][h][r] = gr || kShared ? __builtin_fmaf(dot[mt][r], ks.v[r][gr], gr ? y[mt][h][r] : e[r]) : dot[mt][r] * ks.v[r][gr];
             }
             if constexpr (!kShared)
 #pragma unroll
@@ -387,18 +406,16 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const flo
 #pragma unroll
                     for (int r = 0; r < 4; ++r) y[mt][h][r] = __builtin_fmaf(y[mt][h][r], s.rel[mt], e[r]);
         } else {
-            floatx4 ks[GR], dot[GR][MT];
-#pragma unroll
-            for (int gr = 0; gr < GR; ++gr) ks[gr] = four(tokens.keys[gr], h);
+            floatx4 dot[GR][MT];
 #pragma unroll
             for (int gr = 0; gr < GR; ++gr) product(gr, dot[gr]);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float v = dot[0][mt][r] * ks[0][r];
+                    float v = dot[0][mt][r] * ks.v[r][0];
 #pragma unroll
-                    for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[gr][mt][r], ks[gr][r], v);
+                    for (int gr = 1; gr < GR; ++gr) v = __builtin_fmaf(dot[gr][mt][r], ks.v[r][gr], v);
                     y[mt][h][r] = __builtin_fmaf(v, s.rel[mt], e[r]);
                 }
         }
@@ -419,15 +436,12 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const flo
     constexpr int PG = kShared ? 1 : GR;
     uint32_t p[MT][PG][4];  // weights, times c, as f16 pairs: tokens (0, 1), (2, 3) of both halves
     {
-        floatx4 back[2], c[2][PG];
+        floatx4 back[2];
+        Four c[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             back[h] = four(tokens.back, h);
-#pragma unroll
-            for (int gr = 0; gr < PG; ++gr) {
-                if constexpr (kShared) c[h][gr] = floatx4{1.f, 1.f, 1.f, 1.f};
-                else c[h][gr] = four(scales[gr], h);
-            }
+            if constexpr (!kShared) c[h] = four_by(scales, h);
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -453,7 +467,8 @@ __device__ __forceinline__ void attend(const Tokens<D / G, N> &tokens, const flo
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int h = i / 2, r = i % 2 * 2;
-                    const halfx2 v = {static_cast<_Float16>(w[h][r] * c[h][gr][r]), static_cast<_Float16>(w[h][r + 1] * c[h][gr][r + 1])};
+                    const float c0 = kShared ? 1.f : c[h].v[r][gr], c1 = kShared ? 1.f : c[h].v[r + 1][gr];
+                    const halfx2 v = {static_cast<_Float16>(w[h][r] * c0), static_cast<_Float16>(w[h][r + 1] * c1)};
                     p[mt][gr][i] = __builtin_bit_cast(uint32_t, v);
                 }
         }
@@ -524,7 +539,7 @@ __device__ __forceinline__ void walk(const AttnArgs &a, Tokens<D / G, 32> &token
         }
         wave_order();
         attend<false, D, G, MT>(
-            tokens, own.c, 0, s, at, sure, [&](int h, int gr, int u) { return codes_f16(cur.kc[h][gr][u], own.k[gr][16 * h + n]); },
+            tokens, own.c, 0, s, at, sure, [&](int h, int gr, int u) { return codes_f16(cur.kc[h][gr][u], own.k[16 * h + n][gr]); },
             [&](int gr) {
                 Pairs p[2];
                 uint2 z[2];
@@ -783,7 +798,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 3)))
         wave_order();
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
-            const uint32_t zz = own.k[gr][n];
+            const uint32_t zz = own.k[n][gr];
 #pragma unroll
             for (int u = 0; u < W; ++u) st.keys[wave][gr * W + u][lane] = __builtin_bit_cast(uint4, codes_f16(t.kc[gr][u], zz));
             uint4 w;
