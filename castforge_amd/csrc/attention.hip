@@ -671,15 +671,28 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 
     }
 }
 
-// Joins the splits: 2.7 us for one sequence of a few splits, 5.4 us for 128 splits of 28 rows, and the host's second launch.
-// The splits of a row: a workgroup a (token, query head), D / 8 lanes of eight channels by 2048 / D lanes of splits.
+// Joins the splits: a workgroup a (token, query head), D / 8 lanes of eight channels by 2048 / D lanes of splits, each with a
+// reference of its own until the end: one pass, whose first loads wait for nothing, not even for the number of splits (0.5 us less
+// than a pass for the references first).  By latency: 4.8 us for 1536 rows of two splits, 5.3 us for 28 rows of 128, and the host's
+// second launch.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
     constexpr int kCh = D / 8, kSp = 256 / kCh;
     __shared__ __align__(16) float sums[kSp][D + 4];
-    __shared__ float red[4], ls[kSp];
+    __shared__ float ms[kSp], ls[kSp];
     const int hq = a.heads * a.ratio, token = blockIdx.x / hq;
     const int64_t at = blockIdx.x;
+    const int ch = threadIdx.x % kCh * 8, sl = threadIdx.x / kCh;
+    struct Part {
+        float4 x, y;
+        float2 ml;
+    };
+    const float *part = a.part + at * a.splits * (D + 4);
+    const auto load = [&](int s) {
+        const float *p = part + static_cast<int64_t>(s) * (D + 4);
+        return Part{*reinterpret_cast<const float4 *>(p + ch), *reinterpret_cast<const float4 *>(p + ch + 4), *reinterpret_cast<const float2 *>(p + D)};
+    };
+    Part next = load(min(sl, a.splits - 1));
     int seq = token;
     if (a.cu_q) {
         seq = -1;
@@ -690,37 +703,36 @@ __global__ __launch_bounds__(256) void kv4_attention_join_kernel(AttnArgs a) {
         }
         if (seq < 0) return;
     }
-    const int cap = token_cap(a);
-    const int used = splits_of(a.num_pages > 0 ? min(max(a.kv_lens[seq], 0), cap) : 0, a.splits);
-    const float *part = a.part + at * a.splits * (D + 4);
-    float m = kNoMax;
-    for (int s = threadIdx.x; s < used; s += 256) m = fmaxf(m, part[static_cast<int64_t>(s) * (D + 4) + D]);
-    m = wave_max<64>(m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const int ch = threadIdx.x % kCh * 8, sl = threadIdx.x / kCh;
-    float l = 0.f, v[8];
+    const int used = splits_of(a.num_pages > 0 ? min(max(a.kv_lens[seq], 0), token_cap(a)) : 0, a.splits);
+    float m = kNoMax, l = 0.f, v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
     for (int s = sl; s < used; s += kSp) {
-        const float *p = part + static_cast<int64_t>(s) * (D + 4);
-        const float f = __builtin_amdgcn_exp2f(p[D] - m);
-        const float4 x = *reinterpret_cast<const float4 *>(p + ch), y = *reinterpret_cast<const float4 *>(p + ch + 4);
-        l = __builtin_fmaf(p[D + 1], f, l);
-        v[0] = __builtin_fmaf(x.x, f, v[0]), v[1] = __builtin_fmaf(x.y, f, v[1]), v[2] = __builtin_fmaf(x.z, f, v[2]), v[3] = __builtin_fmaf(x.w, f, v[3]);
-        v[4] = __builtin_fmaf(y.x, f, v[4]), v[5] = __builtin_fmaf(y.y, f, v[5]), v[6] = __builtin_fmaf(y.z, f, v[6]), v[7] = __builtin_fmaf(y.w, f, v[7]);
-    }
+        const Part p = next;
+        if (s + kSp < used) next = load(s + kSp);
+        const float top = fmaxf(m, p.ml.x), f = __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(p.ml.x - top);
+        const float o[8] = {p.x.x, p.x.y, p.x.z, p.x.w, p.y.x, p.y.y, p.y.z, p.y.w};
+        m = top;
+        l = __builtin_fmaf(p.ml.y, g, l * f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[sl][ch + e] = v[e];
-    if (ch == 0) ls[sl] = l;
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(o[e], g, v[e] * f);
+    }
+    if (ch == 0) ms[sl] = m;
+    __syncthreads();
+    float top = ms[0];
+#pragma unroll
+    for (int i = 1; i < kSp; ++i) top = fmaxf(top, ms[i]);
+    const float f = __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[sl][ch + e] = v[e] * f;
+    if (ch == 0) ls[sl] = l * f;
     __syncthreads();
     if (threadIdx.x < D) {
         float t = 0.f, o = 0.f;
 #pragma unroll
         for (int i = 0; i < kSp; ++i) t += ls[i], o += sums[i][threadIdx.x];
         a.out[at * D + threadIdx.x] = f32_to_bf16_rne(t == 0.f ? 0.f : o / t);
-        if (a.lse && threadIdx.x == 0) a.lse[at] = t == 0.f ? -INFINITY : (m + log2f(t)) * 0.693147180559945309f;
+        if (a.lse && threadIdx.x == 0) a.lse[at] = t == 0.f ? -INFINITY : (top + log2f(t)) * 0.693147180559945309f;
     }
 }
 
