@@ -67,6 +67,18 @@ int32_t guarded(char **out_error, F &&body) {
 }
 
 // ----------------------------------------------------------------------------------------
+// device: 16 bytes that are read once, or written for a later kernel, past what others keep in the caches
+// ----------------------------------------------------------------------------------------
+typedef uint32_t nt_uint4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load_once(const void *p) {
+    const nt_uint4 v = __builtin_nontemporal_load(static_cast<const nt_uint4 *>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void store_past(void *p, const uint4 &v) {
+    __builtin_nontemporal_store(nt_uint4{v.x, v.y, v.z, v.w}, static_cast<nt_uint4 *>(p));
+}
+
+// ----------------------------------------------------------------------------------------
 // device: scalar codecs
 // ----------------------------------------------------------------------------------------
 __device__ __forceinline__ float bf16_to_f32(uint16_t b) {

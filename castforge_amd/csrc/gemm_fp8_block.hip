@@ -279,7 +279,8 @@ void fp8_block_tile_kernel(GemmArgs g) {
 
     // acc[i][j] reg 4 t + q holds n = 32 i + 8 t + 4 (lane / 32) + q, m = 32 j + lane % 32
     if (g.y_bf16 && g.N % 8 == 0 && g.y_vec) {
-        // through LDS, so that every global store is a run of 64 I bytes of a row
+        // through LDS, so that every global store is a run of 64 I bytes of a row; past the caches, which hold the panels that other
+        // tiles read (4096 x 11008 x 4096 with its quantizer: 218 -> 202 us)
         constexpr int kChunks = 4 * I, kRows = 64 / kChunks;
         __syncthreads();  // every wave is done with the stages
         uint8_t *eb = lds + wave * 32 * J * T::kEpiRow;
@@ -303,7 +304,7 @@ void fp8_block_tile_kernel(GemmArgs g) {
             const int ml = rb + lane / kChunks;
             const uint4 v = *reinterpret_cast<const uint4 *>(eb + ml * T::kEpiRow + ((cl ^ (ml & (kChunks - 1))) * 16));
             const int m = m0 + wm + ml, n = n0 + wn + cl * 8;
-            if (m < g.M && n < g.N) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(g.Y) + static_cast<int64_t>(m) * g.N + n) = v;
+            if (m < g.M && n < g.N) store_past(static_cast<uint16_t *>(g.Y) + static_cast<int64_t>(m) * g.N + n, v);
         }
         return;
     }

@@ -82,7 +82,8 @@ __device__ __forceinline__ uint32_t codes_of_any(const float (&x)[8], float scal
 // A workgroup has one token (its slot, position and angles are read once) and up to `share` of its heads, in the order K, V, Q:
 // eight elements a lane, D / 8 lanes a head.  HBM-bound where the tokens are many, its vector instructions about as busy: 4096 tokens of 32 heads
 // of each kind, all in places of their own, move 152 MB, more with the cache's partial lines, in 32 to 34 us (4.5 to 4.7 TB/s);
-// 16 tokens of 8 heads and 32 of the queries take 3.4 us.
+// 16 tokens of 8 heads and 32 of the queries take 3.4 us.  Rows are read and queries written past the caches, which keep the cache's
+// partial lines then: 68 -> 56 us with the read-back where outputs are new memory, 56 -> 54 where they are not.
 template <int D, int G>
 __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int share) {
     constexpr int kLanes = D / 8, kUnits = 256 / kLanes;
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int share
     const auto source = [&](int u) { return (u < a.heads ? k + u * D : u < 2 * a.heads ? v + (u - a.heads) * D : q + (u - 2 * a.heads) * D); };
     const auto load = [&](int u, uint4 (&w)[2]) {
         const uint16_t *src = source(u);
-        w[0] = *reinterpret_cast<const uint4 *>(src + 8 * piece);
+        w[0] = load_once(src + 8 * piece);
         if (turns && !a.interleaved && (u < a.heads || u >= 2 * a.heads)) w[1] = *reinterpret_cast<const uint4 *>(src + 8 * other);
     };
     int u = static_cast<int>(blockIdx.y) * share + local;
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a, int share
             uint4 o;
             o.x = f32x2_to_bf16x2_rne(x[0], x[1]), o.y = f32x2_to_bf16x2_rne(x[2], x[3]);
             o.z = f32x2_to_bf16x2_rne(x[4], x[5]), o.w = f32x2_to_bf16x2_rne(x[6], x[7]);
-            *reinterpret_cast<uint4 *>(a.q_out + (token * a.q_heads + u - 2 * a.heads) * D + 8 * piece) = o;
+            store_past(a.q_out + (token * a.q_heads + u - 2 * a.heads) * D + 8 * piece, o);
             continue;
         }
         if (!kept) continue;
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(256) void kv4_gather_kernel(const uint32_t *__restr
             uint4 w;
             w.x = f32x2_to_bf16x2_rne(x[0], x[1]), w.y = f32x2_to_bf16x2_rne(x[2], x[3]);
             w.z = f32x2_to_bf16x2_rne(x[4], x[5]), w.w = f32x2_to_bf16x2_rne(x[6], x[7]);
-            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(is_v ? v_out : k_out) + at) = w;
+            store_past(static_cast<uint16_t *>(is_v ? v_out : k_out) + at, w);
         } else {
             float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(is_v ? v_out : k_out) + at);
             o[0] = make_float4(x[0], x[1], x[2], x[3]);
