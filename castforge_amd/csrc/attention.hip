@@ -180,7 +180,9 @@ __device__ __forceinline__ void load_tile(const AttnArgs &a, KvTile<D, G> &t, in
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
             if constexpr (W == 4) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(kc + gr * (G / 8));
+                // whole cache lines in one instruction, past the caches: 48 sequences of up to 8000 tokens 65 -> 60 us.  (Not so the
+                // values' or smaller groups' words, whose lines several instructions share: up to a fifth slower.)
+                const uint4 v = load_once(kc + gr * (G / 8));
                 t.kc[h][gr][0] = v.x, t.kc[h][gr][1] = v.y, t.kc[h][gr][2] = v.z, t.kc[h][gr][3] = v.w;
             } else if constexpr (W == 2) {
                 const uint2 v = *reinterpret_cast<const uint2 *>(kc + gr * (G / 8));
@@ -584,7 +586,7 @@ __device__ __forceinline__ void settle(Rows<D, G, MT> &s) {
 
 // One workgroup's NW waves take the same rows and every NW-th 32 tokens of a split's share, and are joined through LDS;
 // splits are joined by kv4_attention_join_kernel.  For few rows a sequence: bound by the cache's bytes where they are many (48
-// sequences of up to 8000 tokens, 8 heads: 235 MB in 63 us), by latency where they are few.
+// sequences of up to 8000 tokens, 8 heads: 235 MB in 60 us with the join), by latency where they are few.
 template <int D, int G, int NW>
 struct SplitLds {
     float sums[NW][16][D + 4];
