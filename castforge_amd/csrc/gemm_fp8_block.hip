@@ -112,8 +112,8 @@ __device__ __forceinline__ void store4(const GemmArgs &g, int m, int n, const fl
 //
 // Workgroup tile 32 I WN (n) x 32 J WM (m), WN x WM waves of 32 I x 32 J.  A stage is one run of 128 of both
 // panels and the A rows' scales, brought by buffer loads straight into LDS; two stages, one barrier a stage:
-// a stage is loaded while the other one is computed.  4096 x 11008 x 4096: 206 to 220 us, 1.7 to 1.8 PFLOP/s (2.0 where K is 11008); a
-// third of a CU's last round of tiles is idle, the clock is 2.05 GHz under the load, and of the busy cycles 47% are MFMAs and 32%
+// a stage is loaded while the other one is computed.  4096 x 11008 x 4096: 189 us beside its quantizer, 218 in a row, 1.7 to 1.95 PFLOP/s; a
+// third of a CU's last round of tiles is idle, the clock is 2.05 GHz under the load, and of the busy cycles 47% are MFMAs and 31%
 // the folds and addresses, which hardly overlap on a SIMD.  No faster: a run's first fragments read ahead of its barrier; 128 x
 // 128 a wave at one wave a SIMD, whose sums lie where vector instructions cannot reach them (73 -> 90 us for 4096 x 4096 x 4096).
 template <int I, int J, int WN, int WM>
