@@ -84,7 +84,8 @@ struct Seq {
     int seq, first, n, len, tile;  // first token of its n queries; cached tokens; row tile
 };
 
-// Tokens that a sequence's table holds: so far below 2^31 (check_counts) that offsets past a length do not wrap.
+// Tokens that a sequence's table holds: so far below 2^31 (check_counts) that a round of a workgroup's tokens past a length does not
+// wrap.
 __device__ __forceinline__ int token_cap(const AttnArgs &a) { return a.table_cols << a.page_shift; }
 
 // Splits that share a sequence of len tokens: at least 128 tokens each.
@@ -616,7 +617,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 
     const int used = splits_of(sq.len, a.splits);
     if (split >= used) return;
     const int share = (sq.len / used + 32 * NW) / (32 * NW) * (32 * NW);  // used * share >= len; whole rounds of the waves
-    const int first = split * share, end = min(seen, first + share);
+    // shares are rounded up, each of up to 2 a CU: the end of one may lie past 2^31, so it is not a sum
+    const int first = split * share, end = seen - first > share ? first + share : seen;
     S s;
     load_rows<false>(a, s, sq, head, row0, [](int v) { return v; });
     walk<D, G, MT>(a, sh.tokens[wave], sh.own[wave], s, sq, head, first + 32 * wave, 32 * NW, end);

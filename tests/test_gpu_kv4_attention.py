@@ -326,3 +326,25 @@ def test_empty(cuda):
     assert ops.kv4_attention(q, cache, table[:0], lens[:0]).shape == (0, 8, 128)
     one = torch.ones((1, 8, 128), device=cuda, dtype=torch.bfloat16)
     assert torch.all(ops.kv4_attention(one, cache, table[:, :0], lens) == 0)
+
+
+@pytest.mark.parametrize("heads,pages", [(1, 524272), (2, 524280), (4, 524284), (8, 524286), (1, 524287), (8, 524287)])
+def test_lengths_up_to_the_limit(cuda, heads, pages):
+    """Tables near 2^31 - 4096 tokens, whose entries but the last name a page of zero keys: the last page's keys, of score 60, take
+    all of the weight but 2^31 exp(-60), and so the output is the mean of its values, for whichever split holds it."""
+    page, d = 4096, 64
+    cache = _cache(80, 2, heads, page, d, 64, cuda)
+    cache.k_groups.fill_(0x3C00 | (7 << 16))  # scale 1, zero point 7
+    cache.k_codes[0] = 0x77777777             # zeros
+    cache.k_codes[1] = -0x77777778            # 0x88888888: ones
+    table = torch.zeros((1, pages), dtype=torch.int32, device=cuda)
+    table[0, -1] = 1
+    q = torch.ones((1, heads, d), dtype=torch.bfloat16, device=cuda)
+    lens = torch.tensor([pages * page], dtype=torch.int32, device=cuda)
+    got, lse = ops.kv4_attention(q, cache, table, lens, scale=60 / 64, return_lse=True)
+    v = _numbers(cache.v_codes[1], cache.v_groups[1], 64)
+    want, mag = v.mean(1), v.abs().mean(1)
+    # scores are exact here; the other bounds as above
+    under = page * 15 * 2.0 ** -31 * (v.abs().amax() / page)
+    assert torch.all((got[0].double() - want).abs() <= 1.1 * 2.0 ** -10 * mag + under + 2.0 ** -8 * want.abs())
+    assert torch.all((lse.double() - (60 + math.log(page))).abs() <= 1e-5 * 70)
