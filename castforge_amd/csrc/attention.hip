@@ -151,7 +151,7 @@ struct KvTile {
 template <int GR, int N>
 struct Tokens {
     float keys[N][GR];   // scale times what turns a product into a score
-    float exponent[N];   // of the values' largest scale; -inf where there is no token
+    float exponent[N];   // of the values' largest scale, by magnitude; -inf where there is no token
     float back[N];       // 2^-exponent
 };
 
@@ -223,7 +223,7 @@ __device__ __forceinline__ void fill_token(const uint32_t (&words)[D / G], bool 
     for (int gr = 0; gr < GR; ++gr) {
         const uint32_t w = off ? 0u : words[gr];
         v[gr] = kv4_scale(w);
-        top = fmaxf(top, v[gr]);
+        top = fmaxf(top, fabsf(v[gr]));  // a caller's own cache may hold negative ones
         z[gr] = kv4_zero(w);
     }
     const int ex = __builtin_amdgcn_frexp_expf(top);
@@ -356,7 +356,7 @@ __device__ __forceinline__ int load_rows(const AttnArgs &a, Rows<D, G, MT> &s, c
 __device__ __forceinline__ float score_factor(const AttnArgs &a, int ex) { return __builtin_ldexpf(a.scale * 1.44269504088896341f, ex + 24); }
 
 // 32 tokens at `at`.  A token's weight is held with the exponent of its values' scale: with s_t = c_t 2^e_t (the largest
-// of its groups', c in [0.5, 1)), exp2(score + e_t - m) times c rounds to f16 as what the token adds to the output, whatever
+// of its groups' magnitudes, c in [0.5, 1)), exp2(score + e_t - m) times c rounds to f16 as what the token adds to the output, whatever
 // the scales are; the sum takes the 2^-e_t back.  m is 7 below the largest so far when it moves, and it moves only
 // when something exceeds it by 15: weights stay below 2^15, the largest ones above 2^7 (f16 keeps its 11 bits
 // down to 2^-21 of them), and the rescaling is rare.

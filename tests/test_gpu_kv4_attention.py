@@ -348,3 +348,22 @@ def test_lengths_up_to_the_limit(cuda, heads, pages):
     under = page * 15 * 2.0 ** -31 * (v.abs().amax() / page)
     assert torch.all((got[0].double() - want).abs() <= 1.1 * 2.0 ** -10 * mag + under + 2.0 ** -8 * want.abs())
     assert torch.all((lse.double() - (60 + math.log(page))).abs() <= 1e-5 * 70)
+
+
+@pytest.mark.parametrize("d,group", SHAPES)
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1], [777, 40]), ([3, 40], [300, 90]), ([1637, 30], [1637, 500])])
+@pytest.mark.parametrize("sign", ["both", "below"])
+def test_negative_scales(cuda, d, group, q_lens, kv_lens, sign):
+    """Groups whose scale is negative, up to 2^9: some of a token's, or all of them."""
+    pages, page = [-(-n // 16) for n in kv_lens], 16
+    cache = _cache(81, sum(pages), 8, page, d, group, cuda, base=100.0, spread=0.5)
+    g = torch.Generator(device=cuda).manual_seed(82)
+    for t in (cache.k_groups, cache.v_groups):
+        t |= 0x8000 if sign == "below" else torch.where(torch.rand(t.shape, generator=g, device=cuda) < 0.5, 0x8000, 0)
+    table = _table(83, pages, sum(pages), max(pages), cuda)
+    q = (1e-3 * torch.randn((sum(q_lens), 32, d), generator=g, device=cuda)).bfloat16()
+    lens = torch.tensor(kv_lens, dtype=torch.int32, device=cuda)
+    cu = torch.tensor(np.cumsum([0] + q_lens), dtype=torch.int32, device=cuda)
+    got = ops.kv4_attention(q, cache, table, lens, cu_q=cu)
+    want, _, bound, _ = _reference(q, cache, table, kv_lens, q_lens, True, d ** -0.5)
+    assert torch.all((got.double() - want).abs() <= bound)
