@@ -42,6 +42,10 @@ inline void check_hip(hipError_t e, const char *what) {
 // objects, or an earlier asynchronous fault).
 inline void check_launch(const char *kernel) { check_hip(hipGetLastError(), kernel); }
 
+// Workgroups of `threads` work-items that one launch takes.  HIP counts a dimension's work-items in 32 bits: of more it runs what is
+// left modulo 2^32, and reports an error only where nothing is.
+constexpr int64_t most_workgroups(int64_t threads) { return 0xffffffffll / threads; }
+
 // Compute units of the current device (asked once per device).
 int64_t cu_count();
 

@@ -282,13 +282,13 @@ __global__ __launch_bounds__(256) void rms_norm_fp8_generic_kernel(const void *x
     }
 }
 
-// E4M3 codes and scales of blocks of block_rows x 128: one workgroup a block, two passes.
+// E4M3 codes and scales of blocks of block_rows x 128, from block `first` on: one workgroup a block, two passes.
 __global__ __launch_bounds__(256) void quant_fp8_block_generic_kernel(const void *__restrict__ src, int bf16, int64_t rows,
-                                                                      int64_t cols, int block_rows, uint8_t *__restrict__ codes,
+                                                                      int64_t cols, int block_rows, int64_t first, uint8_t *__restrict__ codes,
                                                                       float *__restrict__ scales) {
     __shared__ float red[4];
-    const int64_t runs = (cols + kRun - 1) / kRun;
-    const int64_t br = blockIdx.x / runs, g = blockIdx.x % runs;
+    const int64_t runs = (cols + kRun - 1) / kRun, block = first + blockIdx.x;
+    const int64_t br = block / runs, g = block % runs;
     const int64_t r0 = br * block_rows, c0 = g * kRun;
     const int n_rows = static_cast<int>(min(static_cast<int64_t>(block_rows), rows - r0));
     const int n_cols = static_cast<int>(min(static_cast<int64_t>(kRun), cols - c0));
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(256) void quant_fp8_block_generic_kernel(const void
     const Quot quot(scale);
     for (int i = threadIdx.x / kRun; i < n_rows; i += 256 / kRun)
         if (c < n_cols) codes[(r0 + i) * cols + c0 + c] = static_cast<uint8_t>(e4m3x4(quot(load_elem(src, bf16, (r0 + i) * cols + c0 + c)), 0.f, 0.f, 0.f));
-    if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+    if (threadIdx.x == 0) scales[block] = scale;
 }
 
 __global__ __launch_bounds__(256) void dequant_fp8_block_kernel(const uint8_t *__restrict__ codes, const float *__restrict__ scales,
@@ -372,25 +372,32 @@ int32_t castforge_hip_rms_norm_fp8(const void *x, int32_t x_dtype, const void *r
         require((residual != nullptr) == (h != nullptr), "residual and h go together: both NULL or neither");
         if (rows == 0 || cols == 0) return;
         require(x && weight && codes && scales, "buffers must not be NULL");
-        require(rows <= 0x7fffffff, "too many rows for one launch");
         hipStream_t st = static_cast<hipStream_t>(stream);
         const bool xb = x_dtype == CFH_DTYPE_BF16, wb = weight_dtype == CFH_DTYPE_BF16;
-        if (cols >= 8) {
-            const bool cut = cols % 8 != 0;
-            const auto go = [&](auto x_bf16, auto w_bf16) {
-                constexpr bool X = decltype(x_bf16)::value, W = decltype(w_bf16)::value;
-                return cut ? launch_norm<X, W, true>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st)
-                           : launch_norm<X, W, false>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st);
-            };
-            if (xb ? (wb ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{}))
-                   : (wb ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{}))) {
-                check_launch("rms_norm_fp8");
-                return;
+        const int64_t runs = block ? (cols + kRun - 1) / kRun : 1;
+        const auto norm = [&](const void *x, const void *residual, int64_t rows, void *h, uint8_t *codes, float *scales) {
+            if (cols >= 8) {
+                const bool cut = cols % 8 != 0;
+                const auto go = [&](auto x_bf16, auto w_bf16) {
+                    constexpr bool X = decltype(x_bf16)::value, W = decltype(w_bf16)::value;
+                    return cut ? launch_norm<X, W, true>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st)
+                               : launch_norm<X, W, false>(x, residual, weight, eps, rows, cols, block, h, codes, scales, st);
+                };
+                if (xb ? (wb ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{}))
+                       : (wb ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{}))) {
+                    check_launch("rms_norm_fp8");
+                    return;
+                }
             }
+            rms_norm_fp8_generic_kernel<<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, st>>>(
+                x, residual, xb, weight, wb, eps, cols, block, h, codes, scales);
+            check_launch("rms_norm_fp8");
+        };
+        // a workgroup a row, of up to 1024
+        for (int64_t row = 0; row < rows; row += most_workgroups(1024)) {
+            const auto from = [&](auto *p) { return p ? reinterpret_cast<decltype(p)>(reinterpret_cast<uintptr_t>(p) + row * cols * (xb ? 2 : 4)) : p; };
+            norm(from(x), from(residual), std::min(rows - row, most_workgroups(1024)), from(h), codes + row * cols, scales + row * runs);
         }
-        rms_norm_fp8_generic_kernel<<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, st>>>(
-            x, residual, xb, weight, wb, eps, cols, block, h, codes, scales);
-        check_launch("rms_norm_fp8");
     });
 }
 
@@ -403,7 +410,6 @@ int32_t castforge_hip_quantize_fp8_block(const void *src, int32_t src_dtype, int
         if (rows == 0 || cols == 0) return;
         require(src && codes && scales, "buffers must not be NULL");
         const int64_t blocks = ((rows + block_rows - 1) / block_rows) * ((cols + kRun - 1) / kRun);
-        require(blocks <= 0x7fffffff, "too many blocks for one launch");
         hipStream_t st = static_cast<hipStream_t>(stream);
         if (block_rows == 1 && cols >= 8 && cols <= 0x7fffff00) {
             const int runs = static_cast<int>((cols + kRun - 1) / kRun);
@@ -416,9 +422,11 @@ int32_t castforge_hip_quantize_fp8_block(const void *src, int32_t src_dtype, int
             check_launch("quant_fp8_block");
             return;
         }
-        quant_fp8_block_generic_kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st>>>(
-            src, src_dtype == CFH_DTYPE_BF16, rows, cols, block_rows, codes, scales);
-        check_launch("quant_fp8_block");
+        for (int64_t first = 0; first < blocks; first += most_workgroups(256)) {
+            const unsigned grid = static_cast<unsigned>(std::min(blocks - first, most_workgroups(256)));
+            quant_fp8_block_generic_kernel<<<dim3(grid), dim3(256), 0, st>>>(src, src_dtype == CFH_DTYPE_BF16, rows, cols, block_rows, first, codes, scales);
+            check_launch("quant_fp8_block");
+        }
     });
 }
 

@@ -156,3 +156,32 @@ def test_empty(cuda):
         codes, scales, h = ops.rms_norm_fp8(x, torch.zeros(shape[1], device=cuda), residual=x, block=128)
         assert codes.shape == shape and h.shape == shape
         assert ops.quantize_fp8_block(x)[0].shape == shape
+
+
+@pytest.mark.parametrize("k", [1032, 7])
+def test_more_rows_than_a_launch_of_workgroups(cuda, k):
+    """2^24 rows and a few, each a workgroup of 256: more than 2^32 work-items.  Rows come out as they do alone."""
+    m = 2**24 + 5
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device=cuda)
+    at = torch.tensor([0, 1, 2**23, 2**24 - 1, 2**24, m - 1], device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(31)
+    x[at] = torch.randn((6, k), generator=g, device=cuda).bfloat16()
+    w = torch.ones(k, dtype=torch.bfloat16, device=cuda)
+    part = ops.rms_norm_fp8(x[at], w, residual=x[at], block=128)
+    for a, b in zip(part, ops.rms_norm_fp8(x, w, residual=x, block=128, out=x)):
+        assert torch.equal(a, b[at])
+
+
+def test_more_blocks_than_a_launch_of_workgroups(cuda):
+    """2^24 blocks and a few of the quantizer's plain kernel, as rows of seven elements and as one long row of 128 x 128 blocks."""
+    g = torch.Generator(device=cuda).manual_seed(32)
+    rows = torch.zeros((2**24 + 5, 7), dtype=torch.bfloat16, device=cuda)
+    rows[-9:] = torch.randn((9, 7), generator=g, device=cuda).bfloat16()
+    for a, b in zip(ops.quantize_fp8_block(rows), ops.quantize_fp8_block(rows[-9:])):
+        assert torch.equal(a[-9:], b)
+    del rows
+    row = torch.zeros((1, 2**31 + 300), dtype=torch.bfloat16, device=cuda)
+    row[:, -700:] = torch.randn((1, 700), generator=g, device=cuda).bfloat16()
+    (codes, scales), tail = ops.quantize_fp8_block(row, 128), ops.quantize_fp8_block(row[:, -(6 * 128 + 44):], 128)
+    assert torch.equal(codes[:, -(6 * 128 + 44):], tail[0]) and torch.equal(scales[:, -7:], tail[1])
+    assert torch.all(scales[:, :2**24 - 10] == 1)
