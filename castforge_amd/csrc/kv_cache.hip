@@ -35,7 +35,7 @@ struct AppendArgs {
     const int64_t *slots, *positions;
     const float *cos, *sin;
     uint16_t *q_out;
-    int64_t tokens, capacity, max_pos;
+    int64_t capacity, max_pos;
     int heads, q_heads, page_shift, rot, interleaved;
     uint32_t *k_codes, *k_groups, *v_codes, *v_groups;
 };
@@ -266,17 +266,21 @@ int32_t castforge_hip_kv4_append(const cfh_kv4_cache_t *cache, const uint16_t *k
             require(aligned(q_out, 16), "q_out must be 16-byte aligned");
         }
         require(rot == 0 || (positions && cos && sin && max_pos >= 1), "positions, cos and sin must be given for a rotation");
-        AppendArgs a{k, v, q, k_stride, v_stride, q_stride, slots, positions, cos, sin, q_out, tokens,
-                     cache->num_pages * cache->page_size, max_pos, static_cast<int>(cache->kv_heads),
-                     q ? static_cast<int>(q_heads) : 0, log2_of(cache->page_size), static_cast<int>(rot), interleaved,
-                     cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups};
         require(rot == 0 || (aligned(cos, 16) && aligned(sin, 16)), "cos and sin must be 16-byte aligned");
-        const int units = 2 * a.heads + a.q_heads, share = share_of(tokens, units, static_cast<int>(cache->head_dim / 8));
-        const dim3 grid(static_cast<unsigned>(tokens), (units + share - 1) / share);
-        kv4_by_shape(cache, [&](auto d, auto g) {
-            kv4_append_kernel<decltype(d)::value, decltype(g)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a, share);
-        });
-        check_launch("kv4_append");
+        const int units = static_cast<int>(2 * cache->kv_heads + (q ? q_heads : 0)), share = share_of(tokens, units, static_cast<int>(cache->head_dim / 8));
+        const int shares = (units + share - 1) / share;  // workgroups a token
+        for (int64_t t = 0, most = most_workgroups(256) / shares; t < tokens; t += most) {
+            const AppendArgs a{k + t * k_stride, v + t * v_stride, q ? q + t * q_stride : nullptr, k_stride, v_stride, q_stride, slots + t,
+                               rot ? positions + t : nullptr, cos, sin, q ? q_out + t * q_heads * cache->head_dim : nullptr,
+                               cache->num_pages * cache->page_size, max_pos, static_cast<int>(cache->kv_heads),
+                               q ? static_cast<int>(q_heads) : 0, log2_of(cache->page_size), static_cast<int>(rot), interleaved,
+                               cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups};
+            const dim3 grid(static_cast<unsigned>(std::min(tokens - t, most)), shares);
+            kv4_by_shape(cache, [&](auto d, auto g) {
+                kv4_append_kernel<decltype(d)::value, decltype(g)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a, share);
+            });
+            check_launch("kv4_append");
+        }
     });
 }
 
@@ -290,13 +294,18 @@ int32_t castforge_hip_kv4_gather(const cfh_kv4_cache_t *cache, const int64_t *sl
         require(slots && k_out && v_out, "buffers must not be NULL");
         require(aligned(k_out, 16) && aligned(v_out, 16), "k_out and v_out must be 16-byte aligned");
         const int units = static_cast<int>(2 * cache->kv_heads), share = share_of(tokens, units, static_cast<int>(cache->head_dim / 8));
-        const dim3 grid(static_cast<unsigned>(tokens), (units + share - 1) / share);
-        kv4_by_shape(cache, [&](auto d, auto g) {
-            kv4_gather_kernel<decltype(d)::value, decltype(g)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
-                cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups, slots, cache->num_pages * cache->page_size,
-                static_cast<int>(cache->kv_heads), log2_of(cache->page_size), k_out, v_out, out_dtype == CFH_DTYPE_BF16, share);
-        });
-        check_launch("kv4_gather");
+        const int shares = (units + share - 1) / share;  // workgroups a token
+        const int64_t row = cache->kv_heads * cache->head_dim * (out_dtype == CFH_DTYPE_BF16 ? 2 : 4);
+        for (int64_t t = 0, most = most_workgroups(256) / shares; t < tokens; t += most) {
+            const dim3 grid(static_cast<unsigned>(std::min(tokens - t, most)), shares);
+            kv4_by_shape(cache, [&](auto d, auto g) {
+                kv4_gather_kernel<decltype(d)::value, decltype(g)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+                    cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups, slots + t, cache->num_pages * cache->page_size,
+                    static_cast<int>(cache->kv_heads), log2_of(cache->page_size), static_cast<char *>(k_out) + t * row,
+                    static_cast<char *>(v_out) + t * row, out_dtype == CFH_DTYPE_BF16, share);
+            });
+            check_launch("kv4_gather");
+        }
     });
 }
 

@@ -214,3 +214,23 @@ def test_empty(cuda):
     one = torch.ones((1, 2, 64), device=cuda, dtype=torch.bfloat16)
     ops.kv4_append(nothing, one, one, torch.zeros(1, dtype=torch.int64, device=cuda))
     assert torch.equal(ops.kv4_gather(nothing, torch.zeros(1, dtype=torch.int64, device=cuda))[0], torch.zeros_like(one))
+
+
+def test_more_tokens_than_a_launch_of_workgroups(cuda):
+    """2^24 tokens and a few, each a workgroup of 256: more than 2^32 work-items.  Those with a slot come out as they do alone."""
+    n, d = 2**24 + 5, 64
+    cache, small = (ops.Kv4Cache.empty(1, 1, 16, d, 64, device=cuda) for _ in range(2))
+    at = torch.tensor([0, 7654321, 2**23 - 1, 2**23, 2**24 - 1, 2**24, n - 1], device=cuda)
+    qkv, pos, cos, sin = _case(11, 7, 1, 1, d, d)
+    few = [qkv[:, i:i + 1].to(cuda).contiguous() for i in range(3)]
+    q, k, v = (torch.zeros((n, 1, d), dtype=torch.bfloat16, device=cuda).index_copy_(0, at, t) for t in few)
+    slots, positions = torch.full((n,), -1, device=cuda), torch.zeros(n, dtype=torch.int64, device=cuda)
+    slots[at], positions[at] = torch.arange(7, device=cuda), pos.to(cuda)
+    got = ops.kv4_append(cache, k, v, slots, positions, cos.to(cuda), sin.to(cuda), q=q)
+    want = ops.kv4_append(small, few[1], few[2], torch.arange(7, device=cuda), pos.to(cuda), cos.to(cuda), sin.to(cuda), q=few[0])
+    assert torch.equal(got[at], want)
+    assert torch.equal(cache.k_codes, small.k_codes) and torch.equal(cache.v_groups, small.v_groups)
+    for a, b in zip(ops.kv4_gather(cache, slots), ops.kv4_gather(small, torch.arange(7, device=cuda))):
+        assert torch.equal(a[at], b)
+        a[at] = 0
+        assert not a.any()
