@@ -476,9 +476,9 @@ __global__ __launch_bounds__(64 * NW) void fp8_block_split_kernel(GemmArgs g) {
     }
 }
 
-// Any shape and alignment: one thread per output, exact E4M3 decode, f32 sums.
-__global__ __launch_bounds__(256) void fp8_block_gemm_generic_kernel(GemmArgs g) {
-    const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+// Any shape and alignment: one thread per output, from output `first` on; exact E4M3 decode, f32 sums.
+__global__ __launch_bounds__(256) void fp8_block_gemm_generic_kernel(GemmArgs g, int64_t first) {
+    const int64_t idx = first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (idx >= static_cast<int64_t>(g.M) * g.N) return;
     const int64_t m = idx / g.N, n = idx - m * g.N;
     const uint8_t *a = g.A + m * g.K, *w = g.W + n * g.K;
@@ -511,7 +511,7 @@ void launch_split(GemmArgs g, hipStream_t st) {
     const auto kern = fp8_block_split_kernel<kExact, I, J, NW, S>;
     raise_lds_limit(reinterpret_cast<const void *>(kern), P::kLds, attr_devices);
     g.tiles_m = (g.M + 32 * J - 1) / (32 * J), g.tiles_n = (g.N + 32 * I - 1) / (32 * I);
-    require(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 8, "too many tiles for one launch");
+    require(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= most_workgroups(64 * NW), "too many tiles for one launch");
     kern<<<dim3(g.tiles_m * g.tiles_n), dim3(64 * NW), P::kLds, st>>>(g);
     check_launch("fp8_block_split");
 }
@@ -523,7 +523,7 @@ void launch_tile(GemmArgs g, hipStream_t st) {
     const auto kern = fp8_block_tile_kernel<kExact, I, J, WN, WM>;
     raise_lds_limit(reinterpret_cast<const void *>(kern), T::kLds, attr_devices);
     g.tiles_m = (g.M + T::BM - 1) / T::BM, g.tiles_n = (g.N + T::BN - 1) / T::BN;
-    require(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= 0x7fffffff / 8, "too many tiles for one launch");
+    require(static_cast<int64_t>(g.tiles_m) * g.tiles_n <= most_workgroups(64 * T::NW), "too many tiles for one launch");
     kern<<<dim3(g.tiles_m * g.tiles_n), dim3(64 * T::NW), T::kLds, st>>>(g);
     check_launch("fp8_block_tile");
 }
@@ -583,8 +583,10 @@ extern "C" int32_t castforge_hip_gemm_fp8_block(const uint8_t *qa, const float *
             return;
         }
         const int64_t tot = m * n;
-        require((tot + 255) / 256 <= 0x7fffffff, "shape too large for the generic FP8 kernel");
-        fp8_block_gemm_generic_kernel<<<dim3(static_cast<unsigned>((tot + 255) / 256)), dim3(256), 0, st>>>(g);
-        check_launch("fp8_block_gemm_generic");
+        for (int64_t first = 0; first < tot; first += most_workgroups(256) * 256) {
+            const int64_t blocks = std::min((tot - first + 255) / 256, most_workgroups(256));
+            fp8_block_gemm_generic_kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st>>>(g, first);
+            check_launch("fp8_block_gemm_generic");
+        }
     });
 }

@@ -533,7 +533,8 @@ int32_t castforge_hip_dequantize_fp8_block(const uint8_t *codes, const float *sc
  * with sw [ceil(n / 128), ceil(k / 128)] (block_rows 128).  y f32 or bf16.
  * exact 0: fp8 MFMA, whose adder keeps about 13 bits below the largest product of each block of eight (see
  * castforge_hip_gemm_fp8; here its sums start anew every 128 columns).  exact 1: the codes widened to f16,
- * exact products and f32 sums, at about half the rate. */
+ * exact products and f32 sums, at about half the rate.
+ * Products of more tiles than one launch holds (one row by more than about 7e8 outputs) are refused. */
 int32_t castforge_hip_gemm_fp8_block(const uint8_t *qa, const float *sa, int64_t m, const uint8_t *qw,
                                      const float *sw, int64_t n, int64_t k, void *y, int32_t y_dtype, int32_t exact,
                                      void *stream, char **out_error);

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from castforge_amd import ops
+from castforge_amd import ffi, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +149,21 @@ def test_empty(cuda):
     e = torch.empty((3, 0), dtype=torch.uint8, device=cuda)
     z = torch.empty((3, 0), device=cuda)
     assert torch.equal(ops.gemm_fp8_block(e, z, e, z[:1]), torch.zeros((3, 3), device=cuda, dtype=torch.bfloat16))
+
+
+def test_more_outputs_than_a_launch_of_work_items(cuda):
+    """2^32 outputs and some of the plain kernel (K is no multiple of 16): rows come out as they do alone."""
+    m, n, k = 2**16 + 3, 2**16, 8
+    g = torch.Generator(device=cuda).manual_seed(33)
+    qa, qw = (torch.randint(0, 120, (r, k), generator=g, device=cuda, dtype=torch.uint8) for r in (m, n))
+    sa, sw = torch.rand((m, 1), generator=g, device=cuda), torch.rand((n // 128, 1), generator=g, device=cuda)
+    y = ops.gemm_fp8_block(qa, sa, qw, sw)
+    for r in (slice(0, 3), slice(2**15 - 1, 2**15 + 2), slice(2**16 - 2, m)):
+        assert torch.equal(y[r], ops.gemm_fp8_block(qa[r].contiguous(), sa[r].contiguous(), qw, sw))
+
+
+def test_refuses_more_tiles_than_a_launch(cuda):
+    n, k = 2**30, 16
+    qw, sw = torch.zeros((n, k), dtype=torch.uint8, device=cuda), torch.zeros((n // 128, 1), device=cuda)
+    with pytest.raises(ffi.CastForgeHipError, match="too many tiles"):
+        ops.gemm_fp8_block(qw[:1], sw[:1], qw, sw)
