@@ -35,6 +35,7 @@ struct AttnArgs {
     float *part;  // splits > 1: [tokens * q heads][splits][D + 2], output sums, reference, sum
     float scale;
     int tokens, batch, heads, ratio, page_shift, table_cols, num_pages, causal, splits;
+    int first_tile;  // of a launch's row tiles, where one launch cannot hold them all
 };
 
 // A uniform word through the scalar cache: no vector load, whose wait would take in the tile loads before it.
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
     const int split = blockIdx.x % a.splits, head = blockIdx.x / a.splits % a.heads;
-    const Seq sq = find_tile(a, blockIdx.x / a.splits / a.heads, 16 * MT);
+    const Seq sq = find_tile(a, a.first_tile + blockIdx.x / a.splits / a.heads, 16 * MT);
     if (sq.seq < 0) return;
     const int row0 = sq.tile * 16 * MT;
     // the last row of the tile sees the most
@@ -771,7 +772,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 3)))
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int n = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % a.heads;
-    const Seq sq = find_tile(a, tiles - 1 - blockIdx.x / a.heads, 16 * NW * MT);
+    const Seq sq = find_tile(a, tiles - 1 - (a.first_tile + blockIdx.x / a.heads), 16 * NW * MT);
     if (sq.seq < 0) return;
     const int total = sq.n * a.ratio, row_of_all = sq.tile * 16 * NW * MT, row0 = row_of_all + wave * 16 * MT;
     const auto seen = [&](int last_row) { return a.causal ? max(0, min(sq.len, sq.len - sq.n + last_row / a.ratio + 1)) : sq.len; };
@@ -944,29 +945,41 @@ void raise_lds_limit(const void *kern, int bytes, std::atomic<uint64_t> &done) {
     }
 }
 
+// launch(workgroups) of as many row tiles as one launch holds, `each` workgroups a tile, until all have run.
+template <class F>
+void for_tiles(AttnArgs &a, const Plan &p, int64_t each, int threads, const F &launch) {
+    require(p.tiles <= 0x7fffffff, "too many rows and sequences for one call");
+    const int64_t most = most_workgroups(threads) / each;
+    for (int64_t t = 0; t < p.tiles; t += most) {
+        a.first_tile = static_cast<int>(t);
+        launch(static_cast<unsigned>(std::min(p.tiles - t, most) * each));
+    }
+}
+
 template <int D, int G, int NW>
-void launch_tile(const AttnArgs &a, const Plan &p, hipStream_t st) {
+void launch_tile(AttnArgs a, const Plan &p, hipStream_t st) {
     constexpr int sums = 16 * NW * (D + 4) * 4, stages = 2 * sizeof(Stage<D, G, NW>), lds = stages > sums ? stages : sums;
     static_assert(lds + NW * sizeof(Own<D, G, 16, _Float16>) <= NW * 20 * 1024, "two workgroups a CU");
-    require(p.tiles * a.heads <= 0x7fffffff, "too many workgroups for one launch");
     static std::atomic<uint64_t> attr_devices{0};
     const auto kern = kv4_attention_tile_kernel<D, G, NW>;
     raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
-    kern<<<dim3(static_cast<unsigned>(p.tiles * a.heads)), dim3(64 * NW), lds, st>>>(a, static_cast<int>(p.tiles));
-    check_launch("kv4_attention_tile");
+    for_tiles(a, p, a.heads, 64 * NW, [&](unsigned grid) {
+        kern<<<dim3(grid), dim3(64 * NW), lds, st>>>(a, static_cast<int>(p.tiles));
+        check_launch("kv4_attention_tile");
+    });
 }
 
 template <int D, int G, int MT, int NW>
-void launch_split(const AttnArgs &a, const Plan &p, hipStream_t st) {
-    const int64_t grid = p.tiles * a.heads * p.splits;
-    require(grid <= 0x7fffffff, "too many workgroups for one launch");
+void launch_split(AttnArgs a, const Plan &p, hipStream_t st) {
     constexpr int lds = sizeof(SplitLds<D, G, NW>);
     static_assert(lds <= 160 * 1024, "LDS budget");
     const auto kern = kv4_attention_split_kernel<D, G, MT, NW>;
     static std::atomic<uint64_t> attr_devices{0};
     if (lds > 64 * 1024) raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
-    kern<<<dim3(static_cast<unsigned>(grid)), dim3(64 * NW), lds, st>>>(a);
-    check_launch("kv4_attention_split");
+    for_tiles(a, p, a.heads * p.splits, 64 * NW, [&](unsigned grid) {
+        kern<<<dim3(grid), dim3(64 * NW), lds, st>>>(a);
+        check_launch("kv4_attention_split");
+    });
     if (p.splits > 1) {
         kv4_attention_join_kernel<D><<<dim3(static_cast<unsigned>(a.tokens * a.heads * a.ratio)), dim3(256), 0, st>>>(a);
         check_launch("kv4_attention_join");
@@ -1020,7 +1033,7 @@ int32_t castforge_hip_kv4_attention(const cfh_kv4_cache_t *cache, const uint16_t
         AttnArgs a{q, q_stride, cache->k_codes, cache->k_groups, cache->v_codes, cache->v_groups, cu_q, page_table, kv_lens, out, lse,
                    static_cast<float *>(workspace), scale, static_cast<int>(tokens), static_cast<int>(batch),
                    static_cast<int>(cache->kv_heads), static_cast<int>(q_heads / cache->kv_heads), log2_of(cache->page_size),
-                   static_cast<int>(table_cols), static_cast<int>(cache->num_pages), causal, static_cast<int>(p.splits)};
+                   static_cast<int>(table_cols), static_cast<int>(cache->num_pages), causal, static_cast<int>(p.splits), 0};
         hipStream_t st = static_cast<hipStream_t>(stream);
         kv4_by_shape(cache, [&](auto d, auto gr) {
             constexpr int D = decltype(d)::value, G = decltype(gr)::value;

@@ -367,3 +367,21 @@ def test_negative_scales(cuda, d, group, q_lens, kv_lens, sign):
     got = ops.kv4_attention(q, cache, table, lens, cu_q=cu)
     want, _, bound, _ = _reference(q, cache, table, kv_lens, q_lens, True, d ** -0.5)
     assert torch.all((got.double() - want).abs() <= bound)
+
+
+def test_more_sequences_than_a_launch_of_workgroups(cuda):
+    """2^21 sequences and a few: with eight heads of keys more than 2^32 work-items."""
+    b, heads, d = 2**21 + 5, 8, 64
+    cache = _cache(84, 3, heads, 16, d, 64, cuda)
+    table = torch.zeros((b, 1), dtype=torch.int32, device=cuda)
+    lens = torch.zeros(b, dtype=torch.int32, device=cuda)
+    at = torch.tensor([0, 12345, 2**21 - 1, 2**21, 2**21 + 4], device=cuda)
+    table[at, 0] = torch.tensor([0, 1, 2, 1, 0], dtype=torch.int32, device=cuda)
+    lens[at] = torch.tensor([3, 16, 9, 1, 15], dtype=torch.int32, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(85)
+    q = torch.ones((b, heads, d), dtype=torch.bfloat16, device=cuda)
+    q[at] = torch.randn((5, heads, d), generator=g, device=cuda).bfloat16()
+    got = ops.kv4_attention(q, cache, table, lens)
+    assert torch.equal(got[at], ops.kv4_attention(q[at], cache, table[at], lens[at]))
+    got[at] = 0
+    assert not got.any()
