@@ -1005,22 +1005,25 @@ def gemm_fp8_block(qa: torch.Tensor, sa: torch.Tensor, qw: torch.Tensor, sw: tor
 
 
 # ------------------------------------------------ a paged cache of 4-bit keys and values ----
-@dataclass
+@dataclass(frozen=True, init=False)
 class Kv4Cache:
     """Paged keys and values as 4-bit codes with an f16 scale and a zero point per group of channels.
 
     codes i32 [pages, kv_heads, page_size, head_dim / 8] (element i in bits 4 (i % 8) of word i / 8), groups i32
     [pages, kv_heads, page_size, head_dim / group] (scale f16 in bits 0..15, zero point in bits 16..19); an
     element stands for (q - z) * scale.  head_dim 64 or 128; group 32, 64 or 128, at most head_dim; page_size a
-    power of two in [16, 4096]."""
+    power of two in [16, 4096].
+
+    The calls take the tensors' addresses from here, where they were checked: fields cannot be set again (make another
+    Kv4Cache of other tensors, as dataclasses.replace does), and the tensors must keep their memory (no resize_ or set_)."""
     k_codes: torch.Tensor
     k_groups: torch.Tensor
     v_codes: torch.Tensor
     v_groups: torch.Tensor
     group: int = 128
 
-    def __post_init__(self):
-        kc, kg, vc, vg, group = self.k_codes, self.k_groups, self.v_codes, self.v_groups, self.group
+    def __init__(self, k_codes: torch.Tensor, k_groups: torch.Tensor, v_codes: torch.Tensor, v_groups: torch.Tensor, group: int = 128):
+        kc, kg, vc, vg = k_codes, k_groups, v_codes, v_groups
         shape, dev, i32 = kc.shape, kc.get_device(), torch.int32
         if len(shape) != 4 or shape[3] not in (8, 16) or group not in (32, 64, 128) or group > 8 * shape[3]:
             raise ValueError("codes must be [pages, kv_heads, page_size, head_dim / 8], head_dim 64 or 128, and group 32, 64 or "
@@ -1032,9 +1035,13 @@ class Kv4Cache:
                 and vg.is_contiguous() and kg.get_device() == dev and vc.get_device() == dev and vg.get_device() == dev):
             _refuse(kc, {"k_codes": kc, "k_groups": kg, "v_codes": vc, "v_groups": vg},
                     f"codes must be int32 {list(shape)} and groups int32 {list(gshape)}")
-        self.num_pages, self.kv_heads, self.page_size, self.head_dim, self._dev = pages, heads, page, 8 * words, dev
-        self._struct = ffi.Kv4CacheStruct(kc.data_ptr(), kg.data_ptr(), vc.data_ptr(), vg.data_ptr(), pages, heads, page, 8 * words, group)
-        self._ref = ctypes.byref(self._struct)
+        held = ffi.Kv4CacheStruct(kc.data_ptr(), kg.data_ptr(), vc.data_ptr(), vg.data_ptr(), pages, heads, page, 8 * words, group)
+        # past the class's __setattr__, which refuses
+        self.__dict__.update(k_codes=kc, k_groups=kg, v_codes=vc, v_groups=vg, group=group, num_pages=pages, kv_heads=heads, page_size=page,
+                             head_dim=8 * words, _dev=dev, _struct=held, _ref=ctypes.byref(held))
+
+    def __reduce__(self):  # copies are made anew: their addresses are their own
+        return type(self), (self.k_codes, self.k_groups, self.v_codes, self.v_groups, self.group)
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, group: int = 128,

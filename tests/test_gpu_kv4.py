@@ -1,5 +1,8 @@
 """Appending to the paged 4-bit cache and reading it back, bit for bit against a numpy restatement in f32, and
 the codes' own error against float64; rows that no slot names keep their bits."""
+import copy
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -234,3 +237,36 @@ def test_more_tokens_than_a_launch_of_workgroups(cuda):
         assert torch.equal(a[at], b)
         a[at] = 0
         assert not a.any()
+
+
+def test_fields_stay_those_the_calls_use(cuda):
+    """A cache's buffers and group cannot be exchanged behind the addresses that its calls take; another cache is made of others."""
+    cache = _random_cache(9, 3, 2, 16, 64, 32, cuda)
+    for name in ("k_codes", "k_groups", "v_codes", "v_groups"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name).clone())
+        with pytest.raises(AttributeError):
+            delattr(cache, name)
+    for name, value in (("group", 64), ("num_pages", 2), ("kv_heads", 1), ("page_size", 32), ("head_dim", 128)):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, value)
+    larger = [torch.cat([t, t]) for t in (cache.k_codes, cache.k_groups, cache.v_codes, cache.v_groups)]
+    grown = dataclasses.replace(cache, **dict(zip(("k_codes", "k_groups", "v_codes", "v_groups"), larger)))
+    assert grown.num_pages == 6 and cache.num_pages == 3 and grown.nbytes() == 2 * cache.nbytes()
+    slots = torch.arange(48, 96, device=cuda)
+    for a, b in zip(ops.kv4_gather(grown, slots), ops.kv4_gather(cache, slots - 48)):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))  # random words hold NaN
+
+
+def test_copies_hold_their_own_rows(cuda):
+    cache = _random_cache(10, 2, 2, 16, 64, 32, cuda)
+    other, same = copy.deepcopy(cache), copy.copy(cache)
+    assert same.k_codes is cache.k_codes and other.k_codes.data_ptr() != cache.k_codes.data_ptr()
+    slots, one = torch.arange(3, device=cuda), torch.ones((3, 2, 64), device=cuda, dtype=torch.bfloat16)
+    before = [t.clone() for t in ops.kv4_gather(cache, slots)]
+    ops.kv4_append(other, one, one, slots)
+    for a, b in zip(ops.kv4_gather(cache, slots), before):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    ops.kv4_append(same, one, one, slots)
+    for a, b in zip(ops.kv4_gather(cache, slots), ops.kv4_gather(other, slots)):
+        assert torch.equal(a, b)
