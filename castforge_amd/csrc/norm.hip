@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void rms_norm_fp8_generic_kernel(const void *x
     }
     const float rstd = 1.0f / sqrtf(over_block(ss, true) / static_cast<float>(cols) + eps);
     const auto y = [&](int64_t i) { return elem(i) * rstd * load_elem(w, w_bf16, i); };
-    const int64_t run = block ? block : cols, runs = (cols + run - 1) / run;
+    const int64_t run = block ? block : cols, runs = block ? (cols + run - 1) / run : 1;
     for (int64_t g = 0; g < runs; ++g) {
         const int64_t end = min(cols, (g + 1) * run);
         float am = 0.f;
@@ -370,8 +370,9 @@ int32_t castforge_hip_rms_norm_fp8(const void *x, int32_t x_dtype, const void *r
         require(block == 0 || block == kRun, "block must be 0 (a scale per row) or 128");
         require(eps >= 0.f, "eps must be non-negative");
         require((residual != nullptr) == (h != nullptr), "residual and h go together: both NULL or neither");
-        if (rows == 0 || cols == 0) return;
-        require(x && weight && codes && scales, "buffers must not be NULL");
+        if (rows == 0 || (cols == 0 && block)) return;
+        // a row without elements still has its scale, 1
+        require(scales && (cols == 0 || (x && weight && codes)), "buffers must not be NULL");
         hipStream_t st = static_cast<hipStream_t>(stream);
         const bool xb = x_dtype == CFH_DTYPE_BF16, wb = weight_dtype == CFH_DTYPE_BF16;
         const int64_t runs = block ? (cols + kRun - 1) / kRun : 1;

@@ -185,3 +185,13 @@ def test_more_blocks_than_a_launch_of_workgroups(cuda):
     (codes, scales), tail = ops.quantize_fp8_block(row, 128), ops.quantize_fp8_block(row[:, -(6 * 128 + 44):], 128)
     assert torch.equal(codes[:, -(6 * 128 + 44):], tail[0]) and torch.equal(scales[:, -7:], tail[1])
     assert torch.all(scales[:, :2**24 - 10] == 1)
+
+
+def test_rows_of_no_elements_have_a_scale(cuda):
+    """The greatest of nothing is zero, and the scale of zeros one; with runs of 128 there is none to give."""
+    x = torch.empty((5, 0), device=cuda, dtype=torch.bfloat16)
+    held = torch.full((5,), 7.0, device=cuda)  # what the scales' memory may hold before
+    del held
+    codes, scales, h = ops.rms_norm_fp8(x, torch.empty(0, device=cuda))
+    assert codes.shape == (5, 0) and h is x and torch.equal(scales, torch.ones(5, device=cuda))
+    assert ops.rms_norm_fp8(x, torch.empty(0, device=cuda), residual=x, block=128)[1].shape == (5, 0)
