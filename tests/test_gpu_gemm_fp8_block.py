@@ -167,3 +167,28 @@ def test_refuses_more_tiles_than_a_launch(cuda):
     qw, sw = torch.zeros((n, k), dtype=torch.uint8, device=cuda), torch.zeros((n // 128, 1), device=cuda)
     with pytest.raises(ffi.CastForgeHipError, match="too many tiles"):
         ops.gemm_fp8_block(qw[:1], sw[:1], qw, sw)
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(3600, 4104, 592), (3700, 4099, 400), (3300, 3500, 912)])
+def test_tiles_of_256(cuda, m, n, k, out):
+    """The tiles of the largest products, cut in M, N and K: more than a round of 128 x 128 ones, at most one of 256 x 256."""
+    (qa, sa), (qw, sw) = _inputs(m + k, m, n, k, cuda)
+    _check(ops.gemm_fp8_block(qa, sa, qw, sw, out_dtype=out), qa, sa, qw, sw, False)
+
+
+@pytest.mark.parametrize("m,n,k,exact", [(1000, 4100, 400, False), (1000, 4100, 400, True), (3600, 4104, 400, False), (3700, 4099, 592, False)])
+def test_large_tiles_keep_rows_apart(cuda, m, n, k, exact):
+    """NaN in a row of x, or in a row of w, stays in its row, or column, of a product by 128 x 128 and 256 x 256 tiles."""
+    (qa, sa), (qw, sw) = _inputs(14, m, n, k, cuda)
+    ref = ops.gemm_fp8_block(qa, sa, qw, sw, exact=exact)
+    qa2, qw2 = qa.clone(), qw.clone()
+    rows, cols = [5, m // 2, m - 1], [0, 1234, n - 1]
+    for i, (r, c) in enumerate(zip(rows, cols)):
+        qa2[r, 130 * i] = 0x7F
+        qw2[c, k - 1 - 100 * i] = 0x7F
+    y = ops.gemm_fp8_block(qa2, sa, qw2, sw, exact=exact)
+    bad = torch.zeros_like(ref, dtype=torch.bool)
+    bad[rows] = True
+    bad[:, cols] = True
+    assert torch.isnan(y[bad]).all() and torch.equal(y[~bad], ref[~bad])
