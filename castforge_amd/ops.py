@@ -1142,7 +1142,10 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, kv
     (those of the call's own queries included).  cu_q int32 [B + 1] gives each sequence's queries; without it every
     sequence has one.  causal: query i of n sees the tokens up to kv_lens - n + i.  scale defaults to
     head_dim ** -0.5.  Queries that see nothing give zeros.  Returns bf16 [T, q_heads, head_dim], and with
-    return_lse the f32 [T, q_heads] logarithms of the sums of exp(scores)."""
+    return_lse the f32 [T, q_heads] logarithms of the sums of exp(scores), -inf of those that see nothing.
+
+    Rows that cu_q gives to no sequence (past its last entry, where a batch is padded, and all of them without a sequence) are
+    not written: they hold whatever the new memory held, and are not to be read."""
     qs = cache._rows(q, None, "q")
     t, hq, d = shape = q.shape
     heads, dev = cache.kv_heads, cache._dev

@@ -5,6 +5,7 @@ Bound of an output: weights are rounded to f16 after their scale, two roundings 
 mantissa: up to 15 2^-31 of the largest p s a token, s the scale of its values; scores are f32 sums of d exact products and a scale, (d + 8) 2^-24 of scale * sum |q k| each,
 which moves a weight by as much of itself, and so the output by twice that of sum p |v|, and the logarithm of
 the sum by as much; a bf16 output rounds by 2^-9 of itself."""
+import ctypes
 import math
 
 import numpy as np
@@ -385,3 +386,28 @@ def test_more_sequences_than_a_launch_of_workgroups(cuda):
     assert torch.equal(got[at], ops.kv4_attention(q[at], cache, table[at], lens[at]))
     got[at] = 0
     assert not got.any()
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [
+    ([1, 1, 1], [300, 17, 777]),         # one launch
+    ([3, 1, 2], [50, 5000, 300]),        # splits and their join
+    ([900, 1, 700], [900, 40, 800])])    # rows of each wave's own
+def test_rows_of_no_sequence_keep_what_they_hold(cuda, q_lens, kv_lens):
+    """Rows of out and lse past the last of cu_q, and all of them without a sequence, are not written; a caller's own buffers show it."""
+    q, cache, table, lens, cu, _ = _run(cuda, q_lens, kv_lens, 8, 4, 128, 128, 16, seed=23, varlen=True)
+    t, more = len(q), 5
+    wide = torch.cat([q, torch.ones((more, *q.shape[1:]), dtype=q.dtype, device=cuda)])
+    for b in (len(q_lens), 0):
+        out = torch.full_like(wide, 7.0)
+        lse = torch.full(wide.shape[:2], 7.0, device=cuda)
+        size = ctypes.c_int64()
+        ffi.call("castforge_hip_kv4_attention_workspace", cache._ref, t + more, 32, b, table.shape[1], 1, ctypes.byref(size))
+        ws = torch.empty(max(size.value, 1), dtype=torch.uint8, device=cuda)
+        ffi.call("castforge_hip_kv4_attention", cache._ref, wide.data_ptr(), 32 * 128, t + more, 32, b, cu.data_ptr(), table.data_ptr(), table.shape[1],
+                 lens.data_ptr(), 1, 128 ** -0.5, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream)
+        n = t if b else 0
+        assert torch.all(out[n:] == 7) and torch.all(lse[n:] == 7)
+        if b:
+            want, want_lse, bound, moved = _reference(q, cache, table, kv_lens, q_lens, True, 128 ** -0.5)
+            assert torch.all((out[:t].double() - want).abs() <= bound)
+            assert torch.all((lse[:t].double() - want_lse).abs() <= 1e-5 * (1 + want_lse.abs()) + moved)
