@@ -32,7 +32,7 @@ struct AttnArgs {
     const int32_t *table, *kv_lens;
     uint16_t *out;
     float *lse;
-    float *part;  // splits > 1: [tokens * q heads][splits][D + 2], output sums, reference, sum
+    float *part;  // splits > 1: [tokens * q heads][splits][D + 4], output sums, reference, sum, two unused
     float scale;
     int tokens, batch, heads, ratio, page_shift, table_cols, num_pages, causal, splits;
     int first_tile;  // of a launch's row tiles, where one launch cannot hold them all
@@ -48,8 +48,8 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return
 
 // Codes as they stand in a word are f16 denormals: pairs 16 bits apart, code times 2^-24, or 2^-20 where it lies 4 bits
 // higher; a zero point held the same way is subtracted from them exactly.  (Subtracting the zero points'
-// share of a sum instead leaves the sum's rounding, in an f16 MFMA about 2^-18 of its largest product, where a
-// heavy token's codes equal its zero point.)
+// share of a sum instead leaves the f32 rounding of sums of up to 15 times a weight, 2^-22 of them each (measured): up to 2^-18 of
+// a heavy token's weight where its codes equal its zero point.)
 __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, a) - __builtin_bit_cast(halfx2, b));
 }
@@ -900,7 +900,8 @@ Plan plan_of(const cfh_kv4_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio;
     const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
     // Enough rows for six waves a CU of 32 rows: every wave its own rows.  8 heads of 128, 4 queries each: prompts of 1024 (four
-    // waves a CU), 1536 and 2048 tokens 39, 57 and 74 us; as splits 32, 56 and 85.
+    // waves a CU), 1536 and 2048 tokens 39, 57 and 74 us; as splits 32, 56 and 85.  The rule is for the call: single queries in it walk
+    // their tokens in one workgroup (2048 rows of a prompt beside 47 queries over 8000 tokens 253 us, in two calls 71 and 88).
     p.rows = varlen && rows / 32 * c->kv_heads >= 6 * cus;
     if (p.rows) {
         p.mt = 2;

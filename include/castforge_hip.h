@@ -542,7 +542,8 @@ int32_t castforge_hip_gemm_fp8_block(const uint8_t *qa, const float *sa, int64_t
 /* A paged cache of 4-bit keys and values (device buffers of the caller, 16-byte aligned).  A page holds
  * page_size tokens of every head: codes u32 [num_pages, kv_heads, page_size, head_dim / 8], element i in bits
  * 4 (i % 8) of word i / 8; groups u32 [num_pages, kv_heads, page_size, head_dim / group], the f16 scale in bits
- * 0..15 (of either sign) and the zero point in bits 16..19.  dequant = (q - z) * f32(scale).
+ * 0..15 (of either sign) and the zero point in bits 16..19.  dequant = (q - z) * f32(scale).  A scale that is not finite makes
+ * NaN or infinity of its group where a query sees its token, and may do so for other queries of the sequence.
  * head_dim 64 or 128; group 32, 64 or 128, at most head_dim; page_size a power of two in [16, 4096]. */
 typedef struct {
     uint32_t *k_codes, *k_groups, *v_codes, *v_groups;
