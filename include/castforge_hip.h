@@ -515,7 +515,8 @@ int32_t castforge_hip_matmul_f32(const float *a, int64_t m, int64_t k, const flo
  * y / scale (OCP E4M3FN, to the nearest even; without the reference codec's 32 exceptions), scale = absmax < 1e-12 ? 1 : absmax * f32(1 / 448) of the row
  * (block 0, scales [rows]) or of each run of 128 columns (block 128, scales [rows, ceil(cols / 128)]).  x, residual and h are of x_dtype (F32 or BF16),
  * weight [cols] of weight_dtype.  residual and h may both be NULL (h = x, not written); h may be x or
- * residual itself.  The sum of squares is f32: it overflows above about 1.8e19 an element. */
+ * residual itself.  The sum of squares is f32: it overflows above about 1.8e19 an element.  A row of no columns has the
+ * scale 1 with block 0, and none with 128. */
 int32_t castforge_hip_rms_norm_fp8(const void *x, int32_t x_dtype, const void *residual, const void *weight,
                                    int32_t weight_dtype, float eps, int64_t rows, int64_t cols, int32_t block,
                                    void *h, uint8_t *codes, float *scales, void *stream, char **out_error);

@@ -411,3 +411,8 @@ def test_rows_of_no_sequence_keep_what_they_hold(cuda, q_lens, kv_lens):
             want, want_lse, bound, moved = _reference(q, cache, table, kv_lens, q_lens, True, 128 ** -0.5)
             assert torch.all((out[:t].double() - want).abs() <= bound)
             assert torch.all((lse[:t].double() - want_lse).abs() <= 1e-5 * (1 + want_lse.abs()) + moved)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [131072]), ([1, 1], [99991, 70001]), ([5], [60013])])
+def test_long_caches(cuda, q_lens, kv_lens):
+    _run(cuda, q_lens, kv_lens, 4, 7, 128, 32, 64, seed=24)
