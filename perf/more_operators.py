@@ -219,9 +219,9 @@ def _rotate(x, cos, sin, rot, interleaved):
 
 
 def _power(amax):
-    """The least power of two that brings amax to 448 or less."""
+    """The least power of two that brings amax to 448 or less, from 2^-70 to 2^30."""
     m, e = torch.frexp(amax)
-    return torch.ldexp(torch.ones_like(amax), (e - 9 + (m > 0.875)).clamp(-100, 120))
+    return torch.ldexp(torch.ones_like(amax), (e - 9 + (m > 0.875)).clamp(-70, 30))
 
 
 def _store(codes, scales, x, pages, places, touched):
@@ -349,7 +349,7 @@ def exact(case, seed):
         return (x / scale).to(F8).double() * scale
 
     def power(amax):
-        return 2.0 ** math.ceil(math.log2(amax / 448)) if amax else 2.0**-100
+        return 2.0 ** math.ceil(math.log2(amax / 448)) if amax else 2.0**-70
 
     if case["op"] == "evict":
         index, weights, ks_out, vs_out = [], [], [], []
