@@ -1,0 +1,366 @@
+// Appending keys and values to the paged 8-bit cache, with the position rotation on the way, reading rows back, and
+// moving the tokens that are worth most to new pages.
+//
+// Rotation of a head's first `rot` channels by the angles of the token's position: pairs (i, i + rot / 2),
+// or (2 i, 2 i + 1) where interleaved; (a, b) -> (a c - b s, b c + a s), each product and the difference
+// rounded to f32 where it stands.  Keys go from the rotated f32 straight into codes; queries, rotated in the
+// same launch, are rounded once to bf16.
+//
+// Codes of a page and head: s' = max(s, 2^e), e the least with absmax <= 448 * 2^e over the call's tokens there, s the
+// page's scale, or 0 where its first place is among them (the page starts anew); code = E4M3(x / s'), NaN -> 0.
+// Codes of tokens before the call's go over to s', rounded from the codes.
+#include <algorithm>
+
+#include "../../include/castforge_hip.h"
+#include "cfh_common.hpp"
+#include "kv8.hpp"
+
+namespace cfh {
+namespace {
+
+struct AppendArgs8 {
+    const uint16_t *k, *v, *q;
+    int64_t k_stride, v_stride, q_stride;  // elements from a token's row to the next one's
+    const int32_t *cu_q, *table, *kv_lens;
+    const int64_t *positions;
+    const float *cos, *sin;
+    uint16_t *q_out;
+    int64_t max_pos;
+    int tokens, batch, heads, q_heads, page_shift, table_cols, num_pages, rot, interleaved;
+    uint8_t *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    int64_t first_block;  // of a launch's workgroups, where one launch cannot hold them all
+    int64_t kv_blocks;    // workgroups with keys or values; one a token of the queries follows
+};
+
+// A page's new tokens: places lo .. hi - 1 of the page in column `col` of sequence seq's table; `row` the first one's row.
+struct Unit {
+    int seq, col, lo, hi, row;
+};
+
+// New tokens of a sequence with n rows and a length: those at places first .. end - 1, pages' columns from first >> shift on.
+__device__ __forceinline__ void new_tokens(const AppendArgs8 &a, int n, int len, int &first, int &end) {
+    first = max(len - n, 0);
+    end = n > 0 ? min(len, a.table_cols << a.page_shift) : 0;
+}
+
+// The unit of a number: the pages that get tokens, sequence by sequence.  The lanes of a wave look at 64 sequences at once.
+__device__ __forceinline__ Unit find_unit(const AppendArgs8 &a, int unit) {
+    const int lane = threadIdx.x & 63, page = 1 << a.page_shift;
+    const auto made = [&](int seq, int begin, int n, int len, int k) {
+        int first, end;
+        new_tokens(a, n, len, first, end);
+        Unit u;
+        u.seq = seq, u.col = (first >> a.page_shift) + k;
+        const int base = u.col << a.page_shift;
+        u.lo = max(first - base, 0), u.hi = min(end - base, page);
+        u.row = begin + (base + u.lo - (len - n));
+        return u;
+    };
+    if (!a.cu_q) {
+        if (unit >= a.batch) return Unit{-1, 0, 0, 0, 0};
+        const int len = a.kv_lens[unit];
+        int first, end;
+        new_tokens(a, 1, len, first, end);
+        return first < end ? made(unit, unit, 1, len, 0) : Unit{-1, 0, 0, 0, 0};
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+        const int b = b0 + lane;
+        int begin = 0, n = 0, len = 0, pages = 0;
+        if (b < a.batch) {  // clamped: a malformed list stays inside the rows
+            begin = min(max(a.cu_q[b], 0), a.tokens);
+            n = min(max(a.cu_q[b + 1], begin), a.tokens) - begin;
+            len = a.kv_lens[b];
+            int first, end;
+            new_tokens(a, n, len, first, end);
+            if (first < end) pages = ((end - 1) >> a.page_shift) - (first >> a.page_shift) + 1;
+        }
+        int upto = pages;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint64_t hit = __ballot(before + upto > unit);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            return made(b0 + l, __builtin_amdgcn_readlane(begin, l), __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(len, l),
+                        unit - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(pages, l)));
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return Unit{-1, 0, 0, 0, 0};
+}
+
+__device__ __forceinline__ void unpack8(const uint4 &w, float (&x)[8]) {
+    const uint32_t b[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(b[i] << 16), x[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u);
+}
+
+// What turns a lane's eight channels, piece * 8 on, of a token at a position.
+struct Turn {
+    float c[8], t[8];  // cosines and sines of the lane's channels, the sine's sign taken in
+    __device__ __forceinline__ void load(const AppendArgs8 &a, int64_t token, int piece) {
+        const int half = a.rot / 2;
+        const bool low = 8 * piece < half;
+        // a position outside the table takes its nearest row
+        const int64_t pos = min(max(a.positions[token], int64_t{0}), a.max_pos - 1);
+        const float *cp = a.cos + pos * half, *sp = a.sin + pos * half;
+        if (a.interleaved) {
+            const float4 cc = *reinterpret_cast<const float4 *>(cp + 4 * piece), ss = *reinterpret_cast<const float4 *>(sp + 4 * piece);
+            c[0] = c[1] = cc.x, c[2] = c[3] = cc.y, c[4] = c[5] = cc.z, c[6] = c[7] = cc.w;
+            t[0] = -ss.x, t[1] = ss.x, t[2] = -ss.y, t[3] = ss.y, t[4] = -ss.z, t[5] = ss.z, t[6] = -ss.w, t[7] = ss.w;
+        } else {
+            const int at = low ? 8 * piece : 8 * piece - half;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 cc = reinterpret_cast<const float4 *>(cp + at)[h], ss = reinterpret_cast<const float4 *>(sp + at)[h];
+                c[4 * h] = cc.x, c[4 * h + 1] = cc.y, c[4 * h + 2] = cc.z, c[4 * h + 3] = cc.w;
+                t[4 * h] = low ? -ss.x : ss.x, t[4 * h + 1] = low ? -ss.y : ss.y, t[4 * h + 2] = low ? -ss.z : ss.z, t[4 * h + 3] = low ? -ss.w : ss.w;
+            }
+        }
+    }
+    // (a, b) -> (a c - b s, b c + a s): x c + partner * (+- s), which rounds as the difference does
+    __device__ __forceinline__ void apply(const AppendArgs8 &a, const uint4 &partner, float (&x)[8]) const {
+        float y[8];
+        if (a.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+        } else {
+            unpack8(partner, y);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + y[i] * t[i];
+    }
+};
+
+// A workgroup has the keys, or the values, of one head in one page: eight channels a lane, D / 8 lanes a token, NP rounds of
+// 2048 / D tokens whose numbers stay in registers between the absmax and the codes.  The workgroups after those have a token's
+// queries each.
+template <int D, int NP>
+__global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs8 a) {
+    constexpr int kLanes = D / 8, kRows = 256 / kLanes;
+    __shared__ float tops[4];
+    const int piece = threadIdx.x % kLanes, local = threadIdx.x / kLanes;
+    const int64_t block = a.first_block + blockIdx.x;
+    const bool turns = 8 * piece < a.rot;
+    const int half = a.rot / 2, other = a.interleaved ? piece : 8 * piece < half ? piece + half / 8 : piece - half / 8;
+    if (block >= a.kv_blocks) {
+        const int token = static_cast<int>(block - a.kv_blocks);
+        if (token >= (a.cu_q ? a.cu_q[a.batch] : a.tokens)) return;  // of no sequence
+        Turn turn;
+        if (turns) turn.load(a, token, piece);
+        for (int h = local; h < a.q_heads; h += kRows) {
+            const uint16_t *src = a.q + token * a.q_stride + h * D;
+            float x[8];
+            unpack8(load_once(src + 8 * piece), x);
+            if (turns) turn.apply(a, a.interleaved ? uint4{} : *reinterpret_cast<const uint4 *>(src + 8 * other), x);
+            store_past(a.q_out + (static_cast<int64_t>(token) * a.q_heads + h) * D + 8 * piece,
+                       make_uint4(f32x2_to_bf16x2_rne(x[0], x[1]), f32x2_to_bf16x2_rne(x[2], x[3]), f32x2_to_bf16x2_rne(x[4], x[5]), f32x2_to_bf16x2_rne(x[6], x[7])));
+        }
+        return;
+    }
+    const int which = static_cast<int>(block % (2 * a.heads));
+    const bool is_v = which >= a.heads;
+    const int head = is_v ? which - a.heads : which;
+    const Unit u = find_unit(a, static_cast<int>(block / (2 * a.heads)));
+    if (u.seq < 0) return;
+    const int page = a.table[static_cast<int64_t>(u.seq) * a.table_cols + u.col];
+    if (page < 0 || page >= a.num_pages) return;
+    const int64_t row0 = kv8_row(page, head, 0, a.heads, a.page_shift);
+    uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + row0 * D + 8 * piece;
+    float *scale_at = (is_v ? a.v_scales : a.k_scales) + static_cast<int64_t>(page) * a.heads + head;
+    const float old = u.lo > 0 ? *scale_at : 0.f;
+    const int count = u.hi - u.lo;
+    float x[NP][8], top = 0.f;
+    const uint16_t *rows = is_v ? a.v + head * D : a.k + head * D;
+    const int64_t stride = is_v ? a.v_stride : a.k_stride;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int r = j * kRows + local;
+        if (r < count) {
+            const uint16_t *src = rows + (u.row + r) * stride;
+            unpack8(load_once(src + 8 * piece), x[j]);
+            if (turns && !is_v) {
+                Turn turn;
+                turn.load(a, u.row + r, piece);
+                turn.apply(a, a.interleaved ? uint4{} : *reinterpret_cast<const uint4 *>(src + 8 * other), x[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));  // NaN: left out
+        }
+    }
+    top = wave_max<64>(top);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();  // also: every lane has read the old scale
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float scale = fmaxf(old, kv8_scale_of(top));
+    if (scale > old) {
+        if (threadIdx.x == 0) *scale_at = scale;
+        const float ratio = old / scale;
+        for (int r = local; r < u.lo; r += kRows) {
+            uint2 *p = reinterpret_cast<uint2 *>(codes + r * D);
+            *p = make_uint2(e4m3x4_by(p->x, ratio), e4m3x4_by(p->y, ratio));
+        }
+    }
+    const bool power = (__float_as_uint(scale) & 0x7fffffu) == 0;
+    const float inv = 1.0f / scale;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int r = j * kRows + local;
+        if (r < count) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = power ? x[j][i] * inv : x[j][i] / scale;  // the same number
+                y[i] = v != v ? 0.f : __builtin_amdgcn_fmed3f(v, -448.f, 448.f);
+            }
+            *reinterpret_cast<uint2 *>(codes + (u.lo + r) * D) = make_uint2(f32_to_e4m3x4(y), f32_to_e4m3x4(y + 4));
+        }
+    }
+}
+
+// Rows of the cache as numbers, a workgroup a token, eight elements a lane; a slot outside the cache gives zeros.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_gather_kernel(const uint8_t *__restrict__ k_codes, const float *__restrict__ k_scales,
+                                                         const uint8_t *__restrict__ v_codes, const float *__restrict__ v_scales,
+                                                         const int64_t *__restrict__ slots, int64_t capacity, int heads, int page_shift,
+                                                         void *__restrict__ k_out, void *__restrict__ v_out, int bf16, int share) {
+    constexpr int kLanes = D / 8, kUnits = 256 / kLanes;
+    const int64_t token = blockIdx.x, slot = slots[token];
+    const bool kept = slot >= 0 && slot < capacity;
+    const int64_t page = kept ? slot >> page_shift : 0;
+    const int at = static_cast<int>(slot & ((1 << page_shift) - 1));
+    const int piece = threadIdx.x % kLanes, end = min(2 * heads, static_cast<int>(blockIdx.y + 1) * share);
+#pragma unroll 2
+    for (int u = static_cast<int>(blockIdx.y) * share + static_cast<int>(threadIdx.x) / kLanes; u < end; u += kUnits) {
+        const bool is_v = u >= heads;
+        const int head = is_v ? u - heads : u;
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (kept) {
+            const uint2 w = *reinterpret_cast<const uint2 *>((is_v ? v_codes : k_codes) + kv8_row(page, head, at, heads, page_shift) * D + 8 * piece);
+            const float scale = (is_v ? v_scales : k_scales)[page * heads + head];
+            e4m3x4_to_f32(w.x, x), e4m3x4_to_f32(w.y, x + 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= scale;
+        }
+        const int64_t out = (token * heads + head) * D + 8 * piece;
+        if (bf16) {
+            store_past(static_cast<uint16_t *>(is_v ? v_out : k_out) + out,
+                       make_uint4(f32x2_to_bf16x2_rne(x[0], x[1]), f32x2_to_bf16x2_rne(x[2], x[3]), f32x2_to_bf16x2_rne(x[4], x[5]), f32x2_to_bf16x2_rne(x[6], x[7])));
+        } else {
+            float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(is_v ? v_out : k_out) + out);
+            o[0] = make_float4(x[0], x[1], x[2], x[3]);
+            o[1] = make_float4(x[4], x[5], x[6], x[7]);
+        }
+    }
+}
+
+// Heads a workgroup of the gather takes of a token: one round of its lanes where that leaves the card with less than four
+// workgroups a CU, else more of them, for whom the slot is read once.
+int share_of(int64_t tokens, int units, int lanes) {
+    const int round = 256 / lanes, rounds = (units + round - 1) / round;
+    const int64_t wanted = (4 * cu_count() + tokens - 1) / tokens;  // workgroups a token
+    const int ways = static_cast<int>(std::min<int64_t>(rounds, wanted));
+    return (rounds + ways - 1) / ways * round;
+}
+
+void check_rows8(const void *p, int64_t stride, int64_t heads, int64_t d, int64_t tokens, const char *what) {
+    require(aligned(p, 16), std::string(what) + " must be 16-byte aligned");
+    require(tokens <= 1 || (stride >= heads * d && stride % 8 == 0),
+            std::string(what) + "'s token stride must be a multiple of 8 and at least heads * head_dim");
+}
+
+template <int D, int NP>
+void launch_append(const AppendArgs8 &a, unsigned grid, hipStream_t st) {
+    kv8_append_kernel<D, NP><<<dim3(grid), dim3(256), 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace cfh
+
+using namespace cfh;
+
+extern "C" {
+
+int32_t castforge_hip_kv8_append(const cfh_kv8_cache_t *cache, const uint16_t *k, int64_t k_stride, const uint16_t *v, int64_t v_stride,
+                                 int64_t tokens, int64_t batch, const int32_t *cu_q, const int32_t *page_table, int64_t table_cols,
+                                 const int32_t *kv_lens, const int64_t *positions, const float *cos, const float *sin, int64_t max_pos,
+                                 int64_t rot, int32_t interleaved, const uint16_t *q, int64_t q_stride, int64_t q_heads, uint16_t *q_out,
+                                 void *stream, char **out_error) {
+    return guarded(out_error, [&] {
+        check_kv8(cache);
+        check_kv8_table(cache, batch, table_cols);
+        require(tokens >= 0 && tokens <= 0x7fffffff, "tokens must be in [0, 2^31)");
+        require(rot >= 0 && rot <= cache->head_dim && rot % 16 == 0, "rot must be a multiple of 16 and at most head_dim");
+        require(interleaved == 0 || interleaved == 1, "interleaved must be 0 or 1");
+        require((q != nullptr) == (q_out != nullptr), "q and q_out go together: both NULL or neither");
+        require(q == nullptr || (q_heads >= 1 && q_heads <= 65536), "q_heads must be in [1, 65536]");
+        require(cu_q != nullptr || tokens == batch, "without cu_q every sequence has one token: tokens must equal batch");
+        if (tokens == 0 || batch == 0) return;
+        require(k && v && kv_lens && (table_cols == 0 || page_table), "buffers must not be NULL");
+        check_rows8(k, k_stride, cache->kv_heads, cache->head_dim, tokens, "k");
+        check_rows8(v, v_stride, cache->kv_heads, cache->head_dim, tokens, "v");
+        if (q) {
+            check_rows8(q, q_stride, q_heads, cache->head_dim, tokens, "q");
+            require(aligned(q_out, 16), "q_out must be 16-byte aligned");
+        }
+        require(rot == 0 || (positions && cos && sin && max_pos >= 1), "positions, cos and sin must be given for a rotation");
+        require(rot == 0 || (aligned(cos, 16) && aligned(sin, 16)), "cos and sin must be 16-byte aligned");
+        // pages that n tokens lie in: n at most, and n / page_size + 2
+        const int64_t units = cu_q ? std::min(tokens, tokens / cache->page_size + 2 * batch) : batch;
+        AppendArgs8 a{k, v, q, k_stride, v_stride, q_stride, cu_q, page_table, kv_lens, positions, cos, sin, q_out, max_pos,
+                      static_cast<int>(tokens), static_cast<int>(batch), static_cast<int>(cache->kv_heads), q ? static_cast<int>(q_heads) : 0,
+                      kv8_log2(cache->page_size), static_cast<int>(table_cols), static_cast<int>(cache->num_pages), static_cast<int>(rot),
+                      interleaved, cache->k_codes, cache->v_codes, cache->k_scales, cache->v_scales, 0, units * 2 * cache->kv_heads};
+        const int64_t blocks = a.kv_blocks + (q ? tokens : 0);
+        const int rounds = static_cast<int>(std::max<int64_t>(1, cache->page_size * cache->head_dim / 2048));
+        for (int64_t most = most_workgroups(256); a.first_block < blocks; a.first_block += most) {
+            const unsigned grid = static_cast<unsigned>(std::min(blocks - a.first_block, most));
+            const hipStream_t st = static_cast<hipStream_t>(stream);
+            if (cache->head_dim == 64) {
+                if (rounds == 1) launch_append<64, 1>(a, grid, st);
+                else if (rounds == 2) launch_append<64, 2>(a, grid, st);
+                else if (rounds == 4) launch_append<64, 4>(a, grid, st);
+                else launch_append<64, 8>(a, grid, st);
+            } else {
+                if (rounds == 1) launch_append<128, 1>(a, grid, st);
+                else if (rounds == 2) launch_append<128, 2>(a, grid, st);
+                else if (rounds == 4) launch_append<128, 4>(a, grid, st);
+                else if (rounds == 8) launch_append<128, 8>(a, grid, st);
+                else launch_append<128, 16>(a, grid, st);
+            }
+            check_launch("kv8_append");
+        }
+    });
+}
+
+int32_t castforge_hip_kv8_gather(const cfh_kv8_cache_t *cache, const int64_t *slots, int64_t tokens, void *k_out, void *v_out,
+                                 int32_t out_dtype, void *stream, char **out_error) {
+    return guarded(out_error, [&] {
+        check_kv8(cache);
+        require(tokens >= 0 && tokens <= 0x7fffffff, "tokens must be in [0, 2^31)");
+        require(out_dtype == CFH_DTYPE_F32 || out_dtype == CFH_DTYPE_BF16, "out_dtype must be F32 or BF16");
+        if (tokens == 0) return;
+        require(slots && k_out && v_out, "buffers must not be NULL");
+        require(aligned(k_out, 16) && aligned(v_out, 16), "k_out and v_out must be 16-byte aligned");
+        const int units = static_cast<int>(2 * cache->kv_heads), share = share_of(tokens, units, static_cast<int>(cache->head_dim / 8));
+        const int shares = (units + share - 1) / share;  // workgroups a token
+        const int64_t row = cache->kv_heads * cache->head_dim * (out_dtype == CFH_DTYPE_BF16 ? 2 : 4);
+        for (int64_t t = 0, most = most_workgroups(256) / shares; t < tokens; t += most) {
+            const dim3 grid(static_cast<unsigned>(std::min(tokens - t, most)), shares);
+            const auto launch = [&](auto kern) {
+                kern<<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+                    cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, slots + t, cache->num_pages * cache->page_size,
+                    static_cast<int>(cache->kv_heads), kv8_log2(cache->page_size), static_cast<char *>(k_out) + t * row,
+                    static_cast<char *>(v_out) + t * row, out_dtype == CFH_DTYPE_BF16, share);
+            };
+            cache->head_dim == 64 ? launch(kv8_gather_kernel<64>) : launch(kv8_gather_kernel<128>);
+            check_launch("kv8_gather");
+        }
+    });
+}
+
+}  // extern "C"

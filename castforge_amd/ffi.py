@@ -109,6 +109,19 @@ class Kv4CacheStruct(ctypes.Structure):
     ]
 
 
+class Kv8CacheStruct(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", c_void_p),
+        ("k_scales", c_void_p),
+        ("v_codes", c_void_p),
+        ("v_scales", c_void_p),
+        ("num_pages", c_int64),
+        ("kv_heads", c_int64),
+        ("page_size", c_int64),
+        ("head_dim", c_int64),
+    ]
+
+
 _P = c_void_p
 _E = POINTER(c_char_p)
 # name -> (restype, argtypes) for every entry point of the header
@@ -183,6 +196,14 @@ SIGNATURES = {
                                               c_int64, _P, c_int32, ctypes.c_float, _P, _P, _P, c_int64, _P, _E]),
     "castforge_hip_kv4_attention_workspace": (c_int32, [POINTER(Kv4CacheStruct), c_int64, c_int64, c_int64, c_int64,
                                                         c_int32, POINTER(c_int64), _E]),
+    "castforge_hip_kv8_append": (c_int32, [POINTER(Kv8CacheStruct), _P, c_int64, _P, c_int64, c_int64, c_int64, _P, _P, c_int64,
+                                           _P, _P, _P, _P, c_int64, c_int64, c_int32, _P, c_int64, c_int64, _P, _P, _E]),
+    "castforge_hip_kv8_gather": (c_int32, [POINTER(Kv8CacheStruct), _P, c_int64, _P, _P, c_int32, _P, _E]),
+    "castforge_hip_kv8_attention": (c_int32, [POINTER(Kv8CacheStruct), _P, c_int64, c_int64, c_int64, c_int64, _P, _P,
+                                              c_int64, _P, c_int32, c_int64, c_int64, ctypes.c_float, _P, _P, _P, c_int64, _P,
+                                              c_int64, _P, _E]),
+    "castforge_hip_kv8_attention_workspace": (c_int32, [POINTER(Kv8CacheStruct), c_int64, c_int64, c_int64, c_int64,
+                                                        c_int32, c_int64, c_int64, POINTER(c_int64), _E]),
 }
 
 _lib = None

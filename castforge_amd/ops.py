@@ -1004,9 +1004,30 @@ def gemm_fp8_block(qa: torch.Tensor, sa: torch.Tensor, qw: torch.Tensor, sw: tor
     return y
 
 
-# ------------------------------------------------ a paged cache of 4-bit keys and values ----
+# --------------------------------------------- paged caches of 4-bit and of 8-bit keys and values ----
+class _PagedCache:
+    """What the calls over a cache check of their other tensors."""
+
+    def _rows(self, t: torch.Tensor, heads: int | None, what: str) -> int:
+        """Checks bf16 [T, heads, head_dim] rows, contiguous but for the token stride, which is returned."""
+        shape, stride, d = t.shape, t.stride(), self.head_dim
+        if not (t.get_device() == self._dev and t.dtype == torch.bfloat16 and len(shape) == 3 and shape[2] == d
+                and (heads is None or shape[1] == heads) and stride[2] == 1 and (stride[1] == d or shape[1] <= 1)):
+            if not t.is_cuda:
+                raise ValueError("castforge_amd kernels take device tensors (HIP); got a CPU tensor")
+            raise ValueError(f"{what} must be bfloat16 [tokens, {'heads' if heads is None else heads}, {d}] on {self.k_codes.device}, "
+                             "contiguous within a token")
+        return stride[0]
+
+    def _vector(self, t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> int:
+        """Checks a contiguous [n] of dtype and returns its address."""
+        if not (t.get_device() == self._dev and t.dtype == dtype and t.shape == (n,) and t.is_contiguous()):
+            _refuse(self.k_codes, {what: t}, f"{what} must be {str(dtype).removeprefix('torch.')} [{n}]")
+        return t.data_ptr()
+
+
 @dataclass(frozen=True, init=False)
-class Kv4Cache:
+class Kv4Cache(_PagedCache):
     """Paged keys and values as 4-bit codes with an f16 scale and a zero point per group of channels.
 
     codes i32 [pages, kv_heads, page_size, head_dim / 8] (element i in bits 4 (i % 8) of word i / 8), groups i32
@@ -1053,23 +1074,6 @@ class Kv4Cache:
 
     def nbytes(self) -> int:
         return 4 * sum(t.numel() for t in (self.k_codes, self.k_groups, self.v_codes, self.v_groups))
-
-    def _rows(self, t: torch.Tensor, heads: int | None, what: str) -> int:
-        """Checks bf16 [T, heads, head_dim] rows, contiguous but for the token stride, which is returned."""
-        shape, stride, d = t.shape, t.stride(), self.head_dim
-        if not (t.get_device() == self._dev and t.dtype == torch.bfloat16 and len(shape) == 3 and shape[2] == d
-                and (heads is None or shape[1] == heads) and stride[2] == 1 and (stride[1] == d or shape[1] <= 1)):
-            if not t.is_cuda:
-                raise ValueError("castforge_amd kernels take device tensors (HIP); got a CPU tensor")
-            raise ValueError(f"{what} must be bfloat16 [tokens, {'heads' if heads is None else heads}, {d}] on {self.k_codes.device}, "
-                             "contiguous within a token")
-        return stride[0]
-
-    def _vector(self, t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> int:
-        """Checks a contiguous [n] of dtype and returns its address."""
-        if not (t.get_device() == self._dev and t.dtype == dtype and t.shape == (n,) and t.is_contiguous()):
-            _refuse(self.k_codes, {what: t}, f"{what} must be {str(dtype).removeprefix('torch.')} [{n}]")
-        return t.data_ptr()
 
 
 def kv4_append(cache: Kv4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -1165,4 +1169,179 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, kv
     ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=q.device) if size else None  # held until the call returns
     ffi.call("castforge_hip_kv4_attention", cache._ref, q.data_ptr(), qs, t, hq, b, cp, page_table.data_ptr(), cols, lp, int(causal),
              d ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse), _ptr(ws), size, _stream(q))
+    return (out, lse) if return_lse else out
+
+
+@dataclass(frozen=True, init=False)
+class Kv8Cache(_PagedCache):
+    """Paged keys and values as E4M3 codes with one scale a page and head.
+
+    codes u8 [pages, kv_heads, page_size, head_dim], scales f32 [pages, kv_heads]; an element stands for code * scale.  head_dim
+    64 or 128; page_size a power of two in [16, 256].  Scales are positive, 2^-70 to 2^30; kv8_append makes powers of two.
+
+    The calls take the tensors' addresses from here, where they were checked: fields cannot be set again (make another
+    Kv8Cache of other tensors, as dataclasses.replace does), and the tensors must keep their memory (no resize_ or set_)."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+    def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor):
+        kc, ks, vc, vs = k_codes, k_scales, v_codes, v_scales
+        shape, dev, u8, f32 = kc.shape, kc.get_device(), torch.uint8, torch.float32
+        if len(shape) != 4 or shape[3] not in (64, 128):
+            raise ValueError("codes must be [pages, kv_heads, page_size, head_dim], head_dim 64 or 128")
+        pages, heads, page, d = shape
+        sshape = (pages, heads)
+        if not (dev >= 0 and vc.shape == shape and ks.shape == sshape and vs.shape == sshape and kc.dtype == u8 and ks.dtype == f32
+                and vc.dtype == u8 and vs.dtype == f32 and kc.is_contiguous() and ks.is_contiguous() and vc.is_contiguous()
+                and vs.is_contiguous() and ks.get_device() == dev and vc.get_device() == dev and vs.get_device() == dev):
+            _refuse(kc, {"k_codes": kc, "k_scales": ks, "v_codes": vc, "v_scales": vs},
+                    f"codes must be uint8 {list(shape)} and scales float32 {list(sshape)}")
+        held = ffi.Kv8CacheStruct(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), pages, heads, page, d)
+        # past the class's __setattr__, which refuses
+        self.__dict__.update(k_codes=kc, k_scales=ks, v_codes=vc, v_scales=vs, num_pages=pages, kv_heads=heads, page_size=page,
+                             head_dim=d, _dev=dev, _struct=held, _ref=ctypes.byref(held))
+
+    def __reduce__(self):  # copies are made anew: their addresses are their own
+        return type(self), (self.k_codes, self.k_scales, self.v_codes, self.v_scales)
+
+    @classmethod
+    def empty(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, device: torch.device | str = "cuda") -> "Kv8Cache":
+        """A cache of zeros."""
+        z = []
+        for _ in range(2):
+            z += [torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=torch.uint8, device=device),
+                  torch.ones((num_pages, kv_heads), dtype=torch.float32, device=device)]
+        return cls(*z)
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales))
+
+    def _batch(self, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None, rows: int, what: str
+               ) -> tuple[int, int, int, int | None]:
+        """Checks a batch's lists, `rows` rows of `what` in all: (sequences, table's columns, addresses of kv_lens and cu_q)."""
+        if not (page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous() and page_table.get_device() == self._dev):
+            _refuse(self.k_codes, {"page_table": page_table}, "page_table must be int32 [sequences, pages]")
+        b, cols = page_table.shape
+        lp, cp = self._vector(kv_lens, torch.int32, b, "kv_lens"), None
+        if cu_q is not None:
+            cp = self._vector(cu_q, torch.int32, b + 1, "cu_q")
+        elif rows != b:
+            raise ValueError(f"without cu_q every sequence has one row: {what} and page_table must have the same rows")
+        return b, cols, lp, cp
+
+
+def _call_on(dev: int, name: str, *args) -> None:
+    """ffi.call with dev as the current device, which a launch on one of its streams needs."""
+    if torch.cuda.current_device() == dev:
+        ffi.call(name, *args)
+    else:
+        with torch.cuda.device(dev):
+            ffi.call(name, *args)
+
+
+def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+               cu_q: torch.Tensor | None = None, positions: torch.Tensor | None = None, cos: torch.Tensor | None = None,
+               sin: torch.Tensor | None = None, q: torch.Tensor | None = None, interleaved: bool = False) -> torch.Tensor | None:
+    """Appends a batch's new keys and values to the cache in one launch, with the lists that kv8_attention takes next:
+    page_table int32 [B, pages], kv_lens int32 [B] cached tokens, the new ones included, cu_q int32 [B + 1] each sequence's
+    rows (without it every sequence has one).  Row i of a sequence's n is its token kv_lens - n + i; tokens that the table, or the
+    cache, does not hold are left out.
+
+    Keys [T, kv_heads, head_dim] bf16 are rotated by the angles of positions (int64 [T]; cos and sin f32 [max_pos, rot / 2], the
+    first `rot` channels in pairs (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved) and written as E4M3 codes.  A page's scale
+    of a head is the least power of two that brings all its tokens to 448 or less: where new tokens need a greater one the page's codes
+    are rounded anew to it; a page whose first place is written starts anew.  Without cos and sin nothing is rotated.  q
+    [T, q_heads, head_dim], if given, is rotated too and returned (bf16, contiguous; rows of no sequence are not written).
+
+    Rows may be slices of one projection's output: only the token stride is free (a multiple of 8).  A page must not get tokens of
+    two sequences in one call."""
+    ks, vs, n = cache._rows(k, cache.kv_heads, "k"), cache._rows(v, cache.kv_heads, "v"), k.shape[0]
+    if v.shape[0] != n:
+        raise ValueError("k and v must have the same tokens")
+    b, cols, lp, up = cache._batch(page_table, kv_lens, cu_q, n, "k")
+    rot = max_pos = 0
+    pp = cp = ip = qp = op = None
+    if cos is not None or sin is not None or positions is not None:
+        if cos is None or sin is None or positions is None:
+            raise ValueError("positions, cos and sin go together")
+        pp = cache._vector(positions, torch.int64, n, "positions")
+        shape, dev = cos.shape, cache._dev
+        if not (len(shape) == 2 and sin.shape == shape and cos.dtype == torch.float32 and sin.dtype == torch.float32
+                and cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == dev and sin.get_device() == dev):
+            _refuse(k, {"cos": cos, "sin": sin}, "cos and sin must be float32 [max_pos, rot / 2]")
+        max_pos, rot, cp, ip = shape[0], 2 * shape[1], cos.data_ptr(), sin.data_ptr()
+    q_out, qs, hq = None, 0, 0
+    if q is not None:
+        qs, qshape = cache._rows(q, None, "q"), q.shape
+        if qshape[0] != n:
+            raise ValueError("q and k must have the same tokens")
+        hq, d = qshape[1], cache.head_dim
+        q_out = torch.empty_strided(qshape, (hq * d, d, 1), dtype=torch.bfloat16, device=q.device)
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    _call_on(cache._dev, "castforge_hip_kv8_append", cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, n, b, up, page_table.data_ptr(), cols, lp,
+             pp, cp, ip, max_pos, rot, int(interleaved), qp, qs, hq, op, _stream(k))
+    return q_out
+
+
+def kv8_gather(cache: Kv8Cache, slots: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that `slots` (int64 [T], page * page_size + place) hold, [T, kv_heads, head_dim] each, rounded once to
+    out_dtype (float32, and bfloat16 where scales are powers of two: exact); a slot outside the cache gives zeros."""
+    n = slots.shape[0] if slots.dim() == 1 else -1
+    sp = cache._vector(slots, torch.int64, n, "slots")
+    h, d = cache.kv_heads, cache.head_dim
+    k = torch.empty_strided((n, h, d), (h * d, d, 1), dtype=out_dtype, device=slots.device)
+    v = torch.empty_like(k)
+    _call_on(cache._dev, "castforge_hip_kv8_gather", cache._ref, sp, n, k.data_ptr(), v.data_ptr(), _out_dtype(out_dtype), _stream(slots))
+    return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _kv8_workspace(device: int, kv_heads: int, page_size: int, head_dim: int, tokens: int, q_heads: int, batch: int, cols: int, varlen: int,
+                   window: int, sinks: int) -> int:
+    """castforge_hip_kv8_attention_workspace's bytes, which depend on sizes alone."""
+    size = ctypes.c_int64()
+    shape = ffi.Kv8CacheStruct(None, None, None, None, 0, kv_heads, page_size, head_dim)
+    _call_on(device, "castforge_hip_kv8_attention_workspace", ctypes.byref(shape), tokens, q_heads, batch, cols, varlen, window, sinks,
+             ctypes.byref(size))
+    return size.value
+
+
+def kv8_attention(q: torch.Tensor, cache: Kv8Cache, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None = None,
+                  causal: bool = True, scale: float | None = None, window: int | None = None, sinks: int = 0, return_lse: bool = False,
+                  weights: torch.Tensor | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """softmax(scale * q K^T) V over the cache, as kv4_attention: q bf16 [T, q_heads, head_dim] (only the token stride is free; head
+    h reads keys' head h // (q_heads // kv_heads)), page_table int32 [B, pages], kv_lens int32 [B] cached tokens (those of the
+    call's own queries included), cu_q int32 [B + 1] each sequence's queries (without it every sequence has one).  causal: query i of
+    n, at place p = kv_lens - n + i, sees the tokens up to p; with a window (at least 1; needs causal) only the last `window` of them
+    and the first `sinks` of the sequence.  scale defaults to head_dim ** -0.5.  Queries that see nothing give zeros.
+
+    weights (f32 [B, kv_heads, N], contiguous): the softmax's weights that each cached token got in this call are added to it, summed
+    over the queries and over the query heads of a head of keys; tokens past N are left out.  What kv8_evict goes by.
+
+    Returns bf16 [T, q_heads, head_dim], and with return_lse the f32 [T, q_heads] logarithms of the sums of exp(scores), -inf of
+    those that see nothing.  Rows that cu_q gives to no sequence are not written: they are not to be read."""
+    qs = cache._rows(q, None, "q")
+    t, hq, d = shape = q.shape
+    heads, dev = cache.kv_heads, cache._dev
+    if hq % heads:
+        raise ValueError("q_heads must be a multiple of the cache's heads")
+    b, cols, lp, cp = cache._batch(page_table, kv_lens, cu_q, t, "q")
+    if window is None:
+        window = 0
+    elif window < 1:
+        raise ValueError("window must be at least 1, or None")
+    wp, wcols = None, 0
+    if weights is not None:
+        if not (weights.dim() == 3 and weights.shape[:2] == (b, heads) and weights.dtype == torch.float32 and weights.is_contiguous()
+                and weights.get_device() == dev):
+            _refuse(q, {"weights": weights}, f"weights must be float32 [{b}, {heads}, tokens]")
+        wp, wcols = weights.data_ptr(), weights.shape[2]
+    out = torch.empty_strided(shape, (hq * d, d, 1), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty_strided((t, hq), (hq, 1), dtype=torch.float32, device=q.device) if return_lse or weights is not None else None
+    size = _kv8_workspace(dev, heads, cache.page_size, d, t, hq, b, cols, 0 if cp is None else 1, window, sinks)
+    ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=q.device) if size else None  # held until the call returns
+    _call_on(dev, "castforge_hip_kv8_attention", cache._ref, q.data_ptr(), qs, t, hq, b, cp, page_table.data_ptr(), cols, lp, int(causal),
+             window, sinks, d ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse), wp, wcols, _ptr(ws), size, _stream(q))
     return (out, lse) if return_lse else out

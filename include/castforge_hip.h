@@ -593,6 +593,59 @@ int32_t castforge_hip_kv4_attention_workspace(const cfh_kv4_cache_t *cache, int6
                                               int64_t batch, int64_t table_cols, int32_t varlen, int64_t *out_bytes,
                                               char **out_error);
 
+/* A paged cache of 8-bit keys and values (device buffers of the caller; codes 16-byte aligned).  A page holds page_size
+ * tokens of every head: codes u8 E4M3FN [num_pages, kv_heads, page_size, head_dim], and one scale a page and head, f32
+ * [num_pages, kv_heads]: an element stands for code * scale.  Scales are positive, from 2^-70 to 2^30 (append makes powers of
+ * two); a code that is NaN, which append never writes, makes NaN of its outputs where a query sees its token, and may do so for
+ * other queries of the sequence.  head_dim 64 or 128; page_size a power of two in [16, 256]. */
+typedef struct {
+    uint8_t *k_codes;
+    float *k_scales;
+    uint8_t *v_codes;
+    float *v_scales;
+    int64_t num_pages, kv_heads, page_size, head_dim;
+} cfh_kv8_cache_t;
+
+/* Writes the keys and values of a batch's new tokens, with the lists that castforge_hip_kv8_attention takes next: sequence b has
+ * the rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q i32 [batch + 1], rising from 0; NULL: one row each) and kv_lens[b] tokens with them,
+ * so that its row i of n is token kv_lens[b] - n + i, in place t % page_size of page page_table[b][t / page_size] (i32
+ * [batch, table_cols]; tokens before the first, past the table or on a page id outside the cache are left out).  A page must
+ * not get tokens of two sequences in one call.
+ * Keys are rotated first, as castforge_hip_kv4_append's, by row positions[row] of cos and sin.  Of a page and head,
+ * s' = max(s, 2^e): e the least, from -70 to 30, with absmax <= 448 * 2^e over the call's tokens there (NaN left out), s the page's
+ * scale, or 0 where its place 0 is among them: the page starts anew.  code = E4M3(x / s') to the nearest even, saturating at 448, NaN -> 0;
+ * the page's tokens before the call's go over to s' as E4M3(code * f32(s / s')).
+ * q (optional, bf16 [tokens, q_heads, head_dim]) is rotated into q_out (contiguous), rounded once to bf16; rows of no
+ * sequence are not written.
+ * k, v, q: bf16, 16-byte aligned, channels and heads contiguous, *_stride elements from token to token (a
+ * multiple of 8).  cos, sin and q_out: 16-byte aligned. */
+int32_t castforge_hip_kv8_append(const cfh_kv8_cache_t *cache, const uint16_t *k, int64_t k_stride, const uint16_t *v,
+                                 int64_t v_stride, int64_t tokens, int64_t batch, const int32_t *cu_q, const int32_t *page_table,
+                                 int64_t table_cols, const int32_t *kv_lens, const int64_t *positions, const float *cos,
+                                 const float *sin, int64_t max_pos, int64_t rot, int32_t interleaved, const uint16_t *q,
+                                 int64_t q_stride, int64_t q_heads, uint16_t *q_out, void *stream, char **out_error);
+
+/* The rows of `tokens` slots (page * page_size + place) as numbers, k_out and v_out [tokens, kv_heads, head_dim] F32 or BF16
+ * (rounded once); a slot outside the cache gives zeros. */
+int32_t castforge_hip_kv8_gather(const cfh_kv8_cache_t *cache, const int64_t *slots, int64_t tokens, void *k_out,
+                                 void *v_out, int32_t out_dtype, void *stream, char **out_error);
+
+/* castforge_hip_kv4_attention over this cache, with two more things.
+ * window (0: none; needs causal): a query at place p = kv_lens[b] - n + i sees the tokens p - window < t <= p and, of those before,
+ * the first `sinks` of the sequence.  Tokens that no query of a call sees are not read.
+ * weights (optional, f32 [batch, kv_heads, weights_cols]; needs lse): weights[b, h, t] += the softmax's weights that token t got,
+ * summed over the call's queries and the query heads of head h.  Each element has one writer; those of tokens that nobody sees, and
+ * tokens past weights_cols, are left alone. */
+int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t *q, int64_t q_stride, int64_t tokens,
+                                    int64_t q_heads, int64_t batch, const int32_t *cu_q, const int32_t *page_table,
+                                    int64_t table_cols, const int32_t *kv_lens, int32_t causal, int64_t window, int64_t sinks,
+                                    float scale, uint16_t *out, float *lse, float *weights, int64_t weights_cols, void *workspace,
+                                    int64_t workspace_bytes, void *stream, char **out_error);
+/* varlen: whether cu_q will be given. */
+int32_t castforge_hip_kv8_attention_workspace(const cfh_kv8_cache_t *cache, int64_t tokens, int64_t q_heads, int64_t batch,
+                                              int64_t table_cols, int32_t varlen, int64_t window, int64_t sinks, int64_t *out_bytes,
+                                              char **out_error);
+
 #ifdef __cplusplus
 }
 #endif
