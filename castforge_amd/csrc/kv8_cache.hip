@@ -258,6 +258,189 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(const uint8_t *__restri
     }
 }
 
+struct EvictArgs8 {
+    uint8_t *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    const int32_t *table, *kv_lens, *new_table;
+    const float *weights;
+    int32_t *kept, *new_lens;
+    float *new_weights;
+    int heads, page_shift, table_cols, new_cols, num_pages, weights_cols, keep, sinks, recent;
+    int used_cols;        // of new_table: those that keep tokens take
+    int64_t first_block;  // of a launch's workgroups, where one launch cannot hold them all
+};
+
+__device__ __forceinline__ int evict_len(const EvictArgs8 &a, int seq) { return min(max(a.kv_lens[seq], 0), a.table_cols << a.page_shift); }
+
+// A weight as a number that orders alike: greater ones first, -0 as 0, NaN last.
+__device__ __forceinline__ uint32_t rank_of(float w) {
+    const uint32_t b = __float_as_uint(w + 0.f);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// The sums of the lanes before this one, over a workgroup of kWaves waves: of a and b apart.
+template <int kWaves>
+__device__ __forceinline__ uint2 sums_before(uint32_t a, uint32_t b, uint2 *waves, uint2 &all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint2 v = make_uint2(a, b);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(v.x, o), y = __shfl_up(v.y, o);
+        if (lane >= o) v.x += x, v.y += y;
+    }
+    __syncthreads();  // the last call's are read
+    if (lane == 63) waves[wave] = v;
+    __syncthreads();
+    uint2 before = make_uint2(v.x - a, v.y - b);
+    all = make_uint2(0, 0);
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before.x += waves[w].x, before.y += waves[w].y;
+        all.x += waves[w].x, all.y += waves[w].y;
+    }
+    return before;
+}
+
+// Which tokens of a sequence and head are kept: a workgroup each.  The rank of the last one that is comes from its bits, 11, 11 and 10
+// at a time: a histogram in LDS of the ranks that agree so far, and the bin in which the count is reached.  Then one pass in the
+// tokens' order gives each kept one its place: those of higher rank, and the first of the last rank's.
+constexpr int kSelectThreads = 1024, kSelectEach = 4;
+__global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(EvictArgs8 a) {
+    constexpr int kWaves = kSelectThreads / 64;
+    __shared__ uint32_t bins[2048];
+    __shared__ uint2 waves[kWaves];
+    __shared__ uint32_t found[2];
+    const int64_t block = a.first_block + blockIdx.x;
+    const int seq = static_cast<int>(block / a.heads), head = static_cast<int>(block % a.heads), tid = threadIdx.x;
+    const int len = evict_len(a, seq), keep = min(len, a.keep);
+    const float *weights = a.weights + block * a.weights_cols;
+    int32_t *kept = a.kept + block * a.keep;
+    float *new_weights = a.new_weights ? a.new_weights + block * a.keep : nullptr;
+    const auto weight = [&](int t) { return t < a.weights_cols ? weights[t] : 0.f; };
+    if (head == 0 && tid == 0) a.new_lens[seq] = keep;
+    for (int i = keep + tid; i < a.keep; i += kSelectThreads) {
+        kept[i] = -1;
+        if (new_weights) new_weights[i] = 0.f;
+    }
+    if (len <= a.keep) {
+        for (int t = tid; t < len; t += kSelectThreads) {
+            kept[t] = t;
+            if (new_weights) new_weights[t] = weight(t);
+        }
+        return;
+    }
+    // candidates: tokens first .. last - 1, of which `want` stay; fewer than all of them
+    const int first = a.sinks, last = len - a.recent;
+    const uint32_t want = static_cast<uint32_t>(a.keep - a.sinks - a.recent);
+    uint32_t prefix = 0, mask = 0, left = want;  // of the last kept one's rank: its bits so far; candidates still to come with them
+    for (int shift = 21, step = 0; step < 3 && want > 0; ++step) {
+        const int bits = step < 2 ? 11 : 10;
+        for (int i = tid; i < 2048; i += kSelectThreads) bins[i] = 0;
+        __syncthreads();
+        for (int t = first + tid; t < last; t += kSelectThreads) {
+            const uint32_t r = rank_of(weight(t));
+            if ((r & mask) == prefix) atomicAdd(&bins[(r >> shift) & ((1u << bits) - 1)], 1u);
+        }
+        __syncthreads();
+        // bins from the top: lane tid has two of them
+        const uint32_t hi = bins[2047 - 2 * tid], lo = bins[2046 - 2 * tid];
+        uint2 all;
+        const uint32_t before = sums_before<kWaves>(hi + lo, 0, waves, all).x;
+        if (before < left && before + hi + lo >= left) {
+            const bool in_hi = before + hi >= left;
+            found[0] = static_cast<uint32_t>(2047 - 2 * tid - (in_hi ? 0 : 1));
+            found[1] = left - before - (in_hi ? 0 : hi);
+        }
+        __syncthreads();
+        prefix |= found[0] << shift, mask |= ((1u << bits) - 1) << shift, left = found[1];
+        shift -= step == 0 ? 11 : 10;
+    }
+    // in order, kSelectEach tokens a lane
+    uint32_t above = 0, equal = 0;  // kept before this round, those of the last rank apart
+    for (int t0 = 0; t0 < len; t0 += kSelectThreads * kSelectEach) {
+        float w[kSelectEach];
+        uint32_t sure = 0, tie = 0;  // bit masks
+#pragma unroll
+        for (int i = 0; i < kSelectEach; ++i) {
+            const int t = t0 + tid * kSelectEach + i;
+            w[i] = t < len ? weight(t) : 0.f;
+            const uint32_t r = rank_of(w[i]);
+            const bool always = t < first || t >= last;
+            if (t < len && (always || (want > 0 && r > prefix))) sure |= 1u << i;
+            if (t < len && !always && want > 0 && r == prefix) tie |= 1u << i;
+        }
+        uint2 all;
+        const uint2 before = sums_before<kWaves>(__popc(sure), __popc(tie), waves, all);
+        uint32_t s = above + before.x, e = equal + before.y;
+#pragma unroll
+        for (int i = 0; i < kSelectEach; ++i) {
+            const bool is_tie = tie >> i & 1u, in = (sure >> i & 1u) || (is_tie && e < left);
+            if (in) {
+                const uint32_t to = s + min(e, left);
+                kept[to] = t0 + tid * kSelectEach + i;
+                if (new_weights) new_weights[to] = w[i];
+            }
+            s += sure >> i & 1u, e += is_tie;
+        }
+        above += all.x, equal += all.y;
+    }
+}
+
+// Moves the kept tokens: a workgroup the keys, or the values, of one head in one new page; 16 codes a lane.  The new page takes the
+// greatest of its tokens' scales: their codes move as they are, others are rounded to it.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_move_kernel(EvictArgs8 a) {
+    constexpr int kLanes = D / 16, kRows = 256 / kLanes, kMost = 256 / kRows;  // rounds of the largest page
+    __shared__ float tops[4];
+    const int64_t block = a.first_block + blockIdx.x;
+    const int which = static_cast<int>(block % (2 * a.heads)), col = static_cast<int>(block / (2 * a.heads) % a.used_cols);
+    const int seq = static_cast<int>(block / (2 * a.heads) / a.used_cols);
+    const bool is_v = which >= a.heads;
+    const int head = is_v ? which - a.heads : which, page = 1 << a.page_shift;
+    const int count = min(min(evict_len(a, seq), a.keep) - col * page, page);
+    if (count <= 0) return;
+    const int to = a.new_table[static_cast<int64_t>(seq) * a.new_cols + col];
+    if (to < 0 || to >= a.num_pages) return;
+    uint8_t *codes = is_v ? a.v_codes : a.k_codes;
+    float *scales = is_v ? a.v_scales : a.k_scales;
+    const int32_t *kept = a.kept + (static_cast<int64_t>(seq) * a.heads + head) * a.keep + col * page;
+    const int32_t *table = a.table + static_cast<int64_t>(seq) * a.table_cols;
+    const int piece = threadIdx.x % kLanes, local = threadIdx.x / kLanes;
+    uint4 w[kMost];
+    float s[kMost], top = 0.f;
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+        const int r = j * kRows + local;
+        w[j] = uint4{}, s[j] = 0.f;
+        if (r < count) {
+            const int t = kept[r], p = table[t >> a.page_shift];
+            if (p >= 0 && p < a.num_pages) {  // else zeros
+                w[j] = load_once(codes + kv8_row(p, head, t & (page - 1), a.heads, a.page_shift) * D + 16 * piece);
+                s[j] = scales[static_cast<int64_t>(p) * a.heads + head];
+            }
+            top = fmaxf(top, s[j]);
+        }
+    }
+    top = wave_max<64>(top);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    if (!(top > 0.f)) top = 1.f;  // no token's page is one of the cache's
+    if (threadIdx.x == 0) scales[static_cast<int64_t>(to) * a.heads + head] = top;
+    uint8_t *out = codes + kv8_row(to, head, 0, a.heads, a.page_shift) * D + 16 * piece;
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+        const int r = j * kRows + local;
+        if (r < count) {
+            if (s[j] != top) {
+                const float ratio = s[j] / top;
+                w[j] = make_uint4(e4m3x4_by(w[j].x, ratio), e4m3x4_by(w[j].y, ratio), e4m3x4_by(w[j].z, ratio), e4m3x4_by(w[j].w, ratio));
+            }
+            *reinterpret_cast<uint4 *>(out + r * D) = w[j];
+        }
+    }
+}
+
 // Heads a workgroup of the gather takes of a token: one round of its lanes where that leaves the card with less than four
 // workgroups a CU, else more of them, for whom the slot is read once.
 int share_of(int64_t tokens, int units, int lanes) {
@@ -360,6 +543,37 @@ int32_t castforge_hip_kv8_gather(const cfh_kv8_cache_t *cache, const int64_t *sl
             cache->head_dim == 64 ? launch(kv8_gather_kernel<64>) : launch(kv8_gather_kernel<128>);
             check_launch("kv8_gather");
         }
+    });
+}
+
+int32_t castforge_hip_kv8_evict(const cfh_kv8_cache_t *cache, const int32_t *page_table, int64_t table_cols, const int32_t *kv_lens, int64_t batch,
+                                const float *weights, int64_t weights_cols, int64_t keep, int64_t sinks, int64_t recent, const int32_t *new_table,
+                                int64_t new_cols, int32_t *kept, int32_t *new_lens, float *new_weights, void *stream, char **out_error) {
+    return guarded(out_error, [&] {
+        check_kv8(cache);
+        check_kv8_table(cache, batch, table_cols);
+        require(weights_cols >= 0 && weights_cols <= 0x7fffffff, "weights_cols must be in [0, 2^31)");
+        require(keep >= 1 && keep <= 0x7ffff000, "keep must be in [1, 2^31 - 4096]");
+        require(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks, "sinks and recent must not be negative, and at most keep together");
+        require(new_cols >= 0 && new_cols <= 0x7ffff000 / cache->page_size && new_cols * cache->page_size >= keep, "new_table must have room for keep tokens");
+        if (batch == 0) return;
+        require(kv_lens && (table_cols == 0 || page_table) && (weights_cols == 0 || weights) && new_table && kept && new_lens, "buffers must not be NULL");
+        EvictArgs8 a{cache->k_codes, cache->v_codes, cache->k_scales, cache->v_scales, page_table, kv_lens, new_table, weights, kept, new_lens, new_weights,
+                     static_cast<int>(cache->kv_heads), kv8_log2(cache->page_size), static_cast<int>(table_cols), static_cast<int>(new_cols),
+                     static_cast<int>(cache->num_pages), static_cast<int>(weights_cols), static_cast<int>(keep), static_cast<int>(sinks), static_cast<int>(recent),
+                     static_cast<int>((keep + cache->page_size - 1) / cache->page_size), 0};
+        const hipStream_t st = static_cast<hipStream_t>(stream);
+        const auto launches = [&](int64_t blocks, int threads, const char *what, const auto &launch) {
+            for (a.first_block = 0; a.first_block < blocks; a.first_block += most_workgroups(threads)) {
+                launch(dim3(static_cast<unsigned>(std::min(blocks - a.first_block, most_workgroups(threads)))));
+                check_launch(what);
+            }
+        };
+        launches(batch * cache->kv_heads, kSelectThreads, "kv8_select", [&](dim3 grid) { kv8_select_kernel<<<grid, dim3(kSelectThreads), 0, st>>>(a); });
+        launches(batch * a.used_cols * 2 * cache->kv_heads, 256, "kv8_move", [&](dim3 grid) {
+            const auto kern = cache->head_dim == 64 ? kv8_move_kernel<64> : kv8_move_kernel<128>;
+            kern<<<grid, dim3(256), 0, st>>>(a);
+        });
     });
 }
 

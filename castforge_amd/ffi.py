@@ -204,6 +204,8 @@ SIGNATURES = {
                                               c_int64, _P, _E]),
     "castforge_hip_kv8_attention_workspace": (c_int32, [POINTER(Kv8CacheStruct), c_int64, c_int64, c_int64, c_int64,
                                                         c_int32, c_int64, c_int64, POINTER(c_int64), _E]),
+    "castforge_hip_kv8_evict": (c_int32, [POINTER(Kv8CacheStruct), _P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int64,
+                                          _P, c_int64, _P, _P, _P, _P, _E]),
 }
 
 _lib = None

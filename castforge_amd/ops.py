@@ -1345,3 +1345,32 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, page_table: torch.Tensor, kv
     _call_on(dev, "castforge_hip_kv8_attention", cache._ref, q.data_ptr(), qs, t, hq, b, cp, page_table.data_ptr(), cols, lp, int(causal),
              window, sinks, d ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse), wp, wcols, _ptr(ws), size, _stream(q))
     return (out, lse) if return_lse else out
+
+
+def kv8_evict(cache: Kv8Cache, page_table: torch.Tensor, kv_lens: torch.Tensor, weights: torch.Tensor, keep: int, new_table: torch.Tensor,
+              sinks: int = 0, recent: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cuts each sequence and head to `keep` tokens: the first `sinks`, the last `recent`, and of those between the ones of greatest
+    weight (f32 [B, kv_heads, N], what kv8_attention added up; tokens past N have 0; NaN comes last; among equals the first), in their
+    order.  They move to the pages of new_table (int32 [B, pages], room for keep tokens; a page id outside the cache is not written), a
+    page's scale the greatest of its tokens'.  The old pages are as they were: a sequence goes on with new_table once they are given back.
+    Pages of new_table must differ from each other and from all that page_table names.
+
+    Returns (kept int32 [B, kv_heads, keep], the old places, -1 past the last; int32 [B], the new lengths min(kv_lens, keep); f32
+    [B, kv_heads, keep], the kept tokens' weights, 0 past the last).  Keys keep their rotation: positions of later tokens go on from the old
+    length, places (and windows) from the new one."""
+    heads, dev = cache.kv_heads, cache._dev
+    b, cols, lp, _ = cache._batch(page_table, kv_lens, None, page_table.shape[0], "kv_lens")
+    if not (weights.dim() == 3 and weights.shape[:2] == (b, heads) and weights.dtype == torch.float32 and weights.is_contiguous()
+            and weights.get_device() == dev and new_table.dim() == 2 and new_table.shape[0] == b and new_table.dtype == torch.int32
+            and new_table.is_contiguous() and new_table.get_device() == dev):
+        _refuse(cache.k_codes, {"weights": weights, "new_table": new_table},
+                f"weights must be float32 [{b}, {heads}, tokens] and new_table int32 [{b}, pages]")
+    if keep < 1:
+        raise ValueError("keep must be at least 1")
+    shape, strides = (b, heads, keep), (heads * keep, keep, 1)
+    kept = torch.empty_strided(shape, strides, dtype=torch.int32, device=weights.device)
+    lens = torch.empty_strided((b,), (1,), dtype=torch.int32, device=weights.device)
+    new = torch.empty_strided(shape, strides, dtype=torch.float32, device=weights.device)
+    _call_on(dev, "castforge_hip_kv8_evict", cache._ref, page_table.data_ptr(), cols, lp, b, weights.data_ptr(), weights.shape[2], keep, sinks,
+             recent, new_table.data_ptr(), new_table.shape[1], kept.data_ptr(), lens.data_ptr(), new.data_ptr(), _stream(weights))
+    return kept, lens, new

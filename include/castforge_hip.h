@@ -646,6 +646,21 @@ int32_t castforge_hip_kv8_attention_workspace(const cfh_kv8_cache_t *cache, int6
                                               int64_t table_cols, int32_t varlen, int64_t window, int64_t sinks, int64_t *out_bytes,
                                               char **out_error);
 
+/* Cuts each sequence and head to its `keep` tokens of greatest weight.  Of sequence b with L = kv_lens[b] tokens in the pages
+ * of page_table, every head keeps all if L <= keep, else the first `sinks`, the last `recent` and, of those between, the ones of greatest
+ * weights[b, head, t] (f32 [batch, kv_heads, weights_cols], castforge_hip_kv8_attention's; tokens past weights_cols have 0; NaN comes
+ * last; among equals the lowest t), in the order of t.  kept (i32 [batch, kv_heads, keep]): their t, -1 past the last; new_lens (i32
+ * [batch]): min(L, keep); new_weights (optional, f32 [batch, kv_heads, keep]): their weights, 0 past the last.
+ * Kept token i goes to place i % page_size of page new_table[b][i / page_size] (i32 [batch, new_cols]; a page id outside the cache is
+ * not written).  A new page's scale is the greatest of its tokens' scales s: codes become E4M3(code * f32(s / greatest)); tokens
+ * of a page id outside the cache become zeros.  Pages that are written must be none of those that any sequence of the call reads, and
+ * differ from each other: the old ones are as they were, also where sequences share them.  Keys keep their rotation; places count anew.
+ * kept and new_lens are in use until the call's work has run. */
+int32_t castforge_hip_kv8_evict(const cfh_kv8_cache_t *cache, const int32_t *page_table, int64_t table_cols, const int32_t *kv_lens,
+                                int64_t batch, const float *weights, int64_t weights_cols, int64_t keep, int64_t sinks, int64_t recent,
+                                const int32_t *new_table, int64_t new_cols, int32_t *kept, int32_t *new_lens, float *new_weights,
+                                void *stream, char **out_error);
+
 #ifdef __cplusplus
 }
 #endif

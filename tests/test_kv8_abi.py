@@ -30,6 +30,10 @@ def _attention(cache=None, q=16, qs=512, n=1, hq=4, b=1, cu=None, table=16, cols
             ws, size, None)
 
 
+def _evict(cache=None, table=16, cols=4, lens=16, b=1, w=16, wcols=64, keep=20, sinks=0, recent=0, new=16, ncols=2, kept=16, nlens=16, nw=None):
+    return ("castforge_hip_kv8_evict", cache or _cache(), table, cols, lens, b, w, wcols, keep, sinks, recent, new, ncols, kept, nlens, nw, None)
+
+
 @pytest.mark.parametrize("call,needle", [
     (("castforge_hip_kv8_append", None, *_append()[2:]), "cache"),
     (_append(_cache(head_dim=96)), "head_dim"),
@@ -81,6 +85,20 @@ def _attention(cache=None, q=16, qs=512, n=1, hq=4, b=1, cu=None, table=16, cols
     (_attention(n=2, b=2, qs=200), "stride"),
     (_attention(cols=1 << 28), "2^31"),
     (_attention(n=1 << 30, b=1 << 30), "2^31"),
+    (_evict(_cache(page_size=20)), "page_size"),
+    (_evict(b=-1), "batch"),
+    (_evict(cols=1 << 28), "2^31"),
+    (_evict(wcols=-1), "weights_cols"),
+    (_evict(keep=0), "keep"),
+    (_evict(keep=1 << 31), "keep"),
+    (_evict(sinks=-1), "sinks"),
+    (_evict(sinks=11, recent=10), "together"),
+    (_evict(keep=33), "new_table"),
+    (_evict(ncols=1 << 28), "new_table"),
+    (_evict(lens=None), "NULL"),
+    (_evict(w=None), "NULL"),
+    (_evict(kept=None), "NULL"),
+    (_evict(nlens=None), "NULL"),
     (("castforge_hip_kv8_attention_workspace", _cache(), 1, 4, 1, 4, 0, 0, 0, None), "out_bytes"),
 ])
 def test_invalid_arguments_report_status_1(call, needle):
@@ -91,5 +109,5 @@ def test_invalid_arguments_report_status_1(call, needle):
 def test_empty_calls_are_noops():
     nothing = dict(n=0, b=0, lens=None, table=None)
     for call in (_append(**nothing, k=None, v=None, rot=0), _append(n=0, b=3, cu=16), _append(n=3, b=0, cu=16, ks=256), _gather(n=0, slots=None, k=None, v=None),
-                 _attention(**nothing, q=None, out=None), _attention(n=0, b=3, cu=16), _attention(n=3, b=0, cu=16)):
+                 _attention(**nothing, q=None, out=None), _attention(n=0, b=3, cu=16), _attention(n=3, b=0, cu=16), _evict(b=0, lens=None, table=None, kept=None)):
         assert _status(*call)[0] == 0
