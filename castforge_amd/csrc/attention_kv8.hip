@@ -116,6 +116,14 @@ __device__ __forceinline__ bf16x8 keys_bf16(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t low_codes(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05010400u); }
 __device__ __forceinline__ uint32_t high_codes(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07030602u); }
 
+// Code u of four tokens, W words each, as f16.
+template <int u, int W>
+__device__ __forceinline__ uint2 values_f16(const uint32_t (&v)[4][W]) {
+    constexpr int i = u / 4, c = u % 4;
+    const auto pair = [&](int r) { return f16_pair(c < 2 ? low_codes(v[r][i], v[r + 1][i]) : high_codes(v[r][i], v[r + 1][i]), c % 2); };
+    return make_uint2(pair(0), pair(2));
+}
+
 // Rows of a wave: 16 MT of the n * ratio (query, head of the group) pairs of a sequence and a head of keys, row = query *
 // ratio + head; the MFMAs' columns.  With S^T = K Q^T a lane holds the scores of one row and four tokens a
 // half, which is the layout that O^T = V^T P^T takes its second operand in: the weights stay in registers.
@@ -162,60 +170,90 @@ __device__ __forceinline__ Sure seen_by_all(const Rows8<D, MT> &s, int len) {
     return Sure{__builtin_amdgcn_readfirstlane(low), __builtin_amdgcn_readfirstlane(limit)};
 }
 
+// What the tokens of a half's page share: what turns a product into a score, base 2, the exponent e of their values' scale, and 2^-e.
+struct Page {
+    float kf, e, back;
+};
+__device__ __forceinline__ Page page_of(float scale, float ks, float vs) {
+    const float e = exponent_of(vs);
+    return Page{scale * ks, e, __builtin_amdgcn_exp2f(-e)};
+}
+
 // 32 tokens at `at`.  A token's weight is held with the exponent e of its values' scale: exp2(score + e - m) rounds to f16 as what
 // the token adds to the output, whatever the scales are; the sum takes the 2^-e back.  m is 7 below the largest so far when it
 // moves, and it moves only when something exceeds it by 15: weights stay below 2^15, the largest ones above 2^7 (f16 keeps its
 // 11 bits down to 2^-21 of them), and the rescaling is rare.
-// keys(h, i): the MFMA operand of half h's 16 tokens and 32 channels; values(u): that of 16 channels and 32 tokens; kf, e and
-// back of a half's page: what turns a product into a score, e and 2^-e.  live: the half's page is one of the cache's.
-template <int D, int MT, class Keys, class Values>
-__device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int at, bool edge, const float (&kf)[2], const float (&e)[2],
-                                       const float (&back)[2], const bool (&live)[2], const Keys &keys, const Values &values) {
+// keys(h, i): the MFMA operand of half h's 16 tokens and 32 channels; values(u): that of 16 channels and 32 tokens.  gone: a half's
+// page is none of the cache's; edge, uniform: so, or some row does not see some token.
+// kFold: one fma takes a product to an exponent less m; where m moves, they are made from the products again, which stay until then
+// (a register a score: the kernel of few rows has none left).
+template <bool kFold, int D, int MT, class Keys, class Values>
+__device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int at, bool edge, const bool (&gone)[2], const Page (&pages)[2], const Keys &keys, const Values &values) {
     constexpr int KS = D / 32, NT = D / 16;
     const int g = (threadIdx.x >> 4) & 3;
-    float y[MT][2][4];
+    floatx4 dot[MT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        floatx4 dot[MT];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             const bf16x8 k = keys(h, i);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
-                dot[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, s.q[mt][i]), i ? dot[mt] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                dot[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, s.q[mt][i]), i ? dot[mt][h] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
         }
+    float z[MT][2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[mt][h][r] = __builtin_fmaf(dot[mt][r], kf[h], e[h]);
-    }
-    if (edge) {  // uniform: some row does not see some token
-        asm volatile("");  // a branch, not selects in every step
+        for (int h = 0; h < 2; ++h) {
+            const float em = kFold ? pages[h].e - s.m[mt] : pages[h].e;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int r = 0; r < 4; ++r) z[mt][h][r] = __builtin_fmaf(dot[mt][h][r], pages[h].kf, em);
+        }
+    if (edge) {
+        int first = at + 4 * g;
+        asm volatile("" : "+v"(first));  // a branch: the comparisons stay in it
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int t = at + 16 * (i / 4) + 4 * g + i % 4;
-                if (!(live[i / 4] && t < s.limit[mt] && (t >= s.low[mt] || t < a.sinks))) y[mt][i / 4][i % 4] = -INFINITY;
+        for (int i = 0; i < 8; ++i) {
+            const int t = first + 16 * (i / 4) + i % 4;
+            const bool behind = t >= a.sinks;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const bool hidden = gone[i / 4] | (t >= s.limit[mt]) | ((t < s.low[mt]) & behind);
+                z[mt][i / 4][i % 4] = hidden ? -INFINITY : z[mt][i / 4][i % 4];
             }
+        }
     }
     uint32_t p[MT][4];  // weights as f16 pairs: tokens (0, 1), (2, 3) of both halves
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const float (&v)[2][4] = y[mt];
-        const float top = max3(max3(v[0][0], v[0][1], v[0][2]), max3(v[0][3], v[1][0], v[1][1]), max3(v[1][2], v[1][3], v[1][3]));
-        if (__any(top > s.m[mt] + 15.f)) {
+        float (&v)[2][4] = z[mt];
+        const float most = max3(max3(v[0][0], v[0][1], v[0][2]), max3(v[0][3], v[1][0], v[1][1]), max3(v[1][2], v[1][3], v[1][3]));
+        if (__any(most > (kFold ? 15.f : s.m[mt] + 15.f))) {
+            float top = most;
+            if constexpr (kFold) {
+                top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float y = __builtin_fmaf(dot[mt][i / 4][i % 4], pages[i / 4].kf, pages[i / 4].e);
+                    v[i / 4][i % 4] = v[i / 4][i % 4] == -INFINITY ? -INFINITY : y;
+                    top = fmaxf(top, v[i / 4][i % 4]);
+                }
+            }
             const float m = fmaxf(s.m[mt], max_over_g(top) - 7.f), f = __builtin_amdgcn_exp2f(s.m[mt] - m);
             s.m[mt] = m;
             s.l[mt] *= f;
 #pragma unroll
             for (int u = 0; u < NT; ++u) s.o[mt][u] *= f;
+            if constexpr (kFold)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i / 4][i % 4] -= m;
         }
         float w[2][4];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            w[i / 4][i % 4] = __builtin_amdgcn_exp2f(y[mt][i / 4][i % 4] - s.m[mt]);
-            s.l[mt] = __builtin_fmaf(w[i / 4][i % 4], back[i / 4], s.l[mt]);
+            w[i / 4][i % 4] = __builtin_amdgcn_exp2f(kFold ? v[i / 4][i % 4] : v[i / 4][i % 4] - s.m[mt]);
+            s.l[mt] = __builtin_fmaf(w[i / 4][i % 4], pages[i / 4].back, s.l[mt]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -267,27 +305,17 @@ __device__ __forceinline__ void walk(const AttnArgs8 &a, Rows8<D, MT> &s, const 
                     for (int i = 0; i < W; ++i)
                         if (!cur.live[h] || at + 16 * h + 4 * g + r >= sq.len) cur.v[h][r][i] = 0;
         }
-        float kf[2], e[2], back[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            kf[h] = a.scale * cur.ks[h];
-            e[h] = exponent_of(cur.vs[h]);
-            back[h] = __builtin_amdgcn_exp2f(-e[h]);
-        }
-        const bool edge = apart || at + 32 > sure.limit || (at < sure.low && at + 32 > a.sinks);
-        attend<D, MT>(
-            a, s, at, edge, kf, e, back, cur.live,
+        const Page pages_of[2] = {page_of(a.scale, cur.ks[0], cur.vs[0]), page_of(a.scale, cur.ks[1], cur.vs[1])};
+        const bool gone[2] = {!cur.live[0], !cur.live[1]}, edge = apart || at + 32 > sure.limit || (at < sure.low && at + 32 > a.sinks);
+        attend<false, D, MT>(
+            a, s, at, edge, gone, pages_of,
             [&](int h, int i) {
                 const uint4 w = cur.k[h][i / 2];
                 return i % 2 ? keys_bf16(w.z, w.w) : keys_bf16(w.x, w.y);
             },
             [&](auto u) {
-                constexpr int i = u / 4, c = u % 4;
-                const auto pair = [&](int h, int r) {
-                    const uint32_t x = cur.v[h][r][i], y = cur.v[h][r + 1][i];
-                    return f16_pair(c < 2 ? low_codes(x, y) : high_codes(x, y), c % 2);
-                };
-                return __builtin_bit_cast(halfx8, uintx4{pair(0, 0), pair(0, 2), pair(1, 0), pair(1, 2)});
+                const uint2 x = values_f16<u>(cur.v[0]), y = values_f16<u>(cur.v[1]);
+                return __builtin_bit_cast(halfx8, uintx4{x.x, x.y, y.x, y.y});
             });
         cur = next;
     }
@@ -449,6 +477,131 @@ __global__ __launch_bounds__(256) void kv8_attention_join_kernel(AttnArgs8 a) {
     }
 }
 
+// Many rows: each wave takes 32 rows of its own, and the NW of a workgroup share the making of the MFMA operands.  Of every 16 NW
+// tokens a wave turns 16 into operands in LDS and all read them back; two stages, one barrier a stage: the operands of the next tokens
+// are made while the present ones are used, and the codes of those after that are on their way.
+// Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row tiles from the
+// last, which see the most tokens.
+template <int D, int NW>
+struct Stage8 {
+    static constexpr int KS = D / 32, NT = D / 16;
+    uint4 keys[NW][KS][64];        // 16 tokens, 32 channels: a lane's operand
+    uint4 values[NW / 2][NT][64];  // 32 tokens, 16 channels
+    Page pages[NW];
+};
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 3))) void kv8_attention_tile_kernel(AttnArgs8 a, int tiles) {
+    constexpr int MT = 2, KS = D / 32, NT = D / 16, W = D / 64, kSteps = NW / 2;  // steps of 32 tokens a stage
+    extern __shared__ __align__(16) uint8_t lds[];
+    Stage8<D, NW> *stages = reinterpret_cast<Stage8<D, NW> *>(lds);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int n = lane & 15, g = lane >> 4;
+    const int head = blockIdx.x % a.heads;
+    const Seq sq = find_tile(a, tiles - 1 - (a.first_tile + blockIdx.x / a.heads), 16 * NW * MT);
+    if (sq.seq < 0) return;
+    const int total = sq.n * a.ratio, row_of_all = sq.tile * 16 * NW * MT, row0 = row_of_all + wave * 16 * MT;
+    const Span span = span_of(a, sq, row_of_all / a.ratio, (min(row_of_all + 16 * NW * MT, total) - 1) / a.ratio);
+    const int steps = span.steps();
+    // the wave's own rows see tokens below `mine`, and from `from` on or sinks
+    const int mine = row0 < total ? limit_of(a, sq, (min(row0 + 16 * MT, total) - 1) / a.ratio) : 0;
+    const int from = row0 < total ? low_of(a, sq, row0 / a.ratio) : 0;
+    Rows8<D, MT> s;
+    load_rows(a, s, sq, head, row0);
+    const Sure sure = seen_by_all(s, sq.len);
+    const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
+
+    // this wave's 16 tokens of a stage
+    struct Part {
+        uint4 k[W];
+        uint32_t v[4][W];
+        float ks, vs;
+        int at;
+        bool live;
+    };
+    const auto token_at = [&](int step) { return span.token_of(step + wave / 2) + 16 * (wave & 1); };
+    const auto page_at = [&](int step) {
+        const int at = token_at(step);
+        return step + wave / 2 < steps && at < span.end ? scalar_load(table, at >> a.page_shift) : -1;
+    };
+    const auto load = [&](Part &t, int page, int step) {
+        t.at = token_at(step);
+        t.live = page >= 0 && page < a.num_pages;
+        const int p = t.live ? page : 0;
+        const int64_t row = kv8_row(p, head, t.at & ((1 << a.page_shift) - 1), a.heads, a.page_shift), at_scale = static_cast<int64_t>(p) * a.heads + head;
+        const uint8_t *k = a.k_codes + (row + n) * D + 16 * g, *v = a.v_codes + (row + 4 * g) * D + n * (D / 16);
+#pragma unroll
+        for (int i = 0; i < W; ++i) t.k[i] = *reinterpret_cast<const uint4 *>(k + 64 * i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) __builtin_memcpy(t.v[r], __builtin_assume_aligned(v + r * D, D / 16), D / 16);
+        t.ks = scalar_load(a.k_scales, at_scale), t.vs = scalar_load(a.v_scales, at_scale);
+    };
+    const auto make = [&](Part &t, Stage8<D, NW> &st) {
+        if (!t.live || t.at + 16 > sq.len) {  // uniform: bytes that are no token's may be NaN, which a weight of 0 does not take away
+            asm volatile("");
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                if (!t.live) t.k[i] = uint4{};
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!t.live || t.at + 4 * g + r >= sq.len) t.v[r][i] = 0;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            st.keys[wave][2 * i][lane] = __builtin_bit_cast(uint4, keys_bf16(t.k[i].x, t.k[i].y));
+            st.keys[wave][2 * i + 1][lane] = __builtin_bit_cast(uint4, keys_bf16(t.k[i].z, t.k[i].w));
+        }
+        static_for<NT>([&](auto u) __attribute__((always_inline)) { reinterpret_cast<uint2 *>(&st.values[wave / 2][u][lane])[wave & 1] = values_f16<u>(t.v); });
+        // no page of the cache: scores of -inf, by products of zeros
+        if (lane == 0) st.pages[wave] = t.live ? page_of(a.scale, t.ks, t.vs) : Page{0.f, -INFINITY, 0.f};
+    };
+    Part part;
+    if (steps > 0) {
+        load(part, page_at(0), 0);
+        make(part, stages[0]);
+        load(part, page_at(kSteps), kSteps);
+    }
+    int page = page_at(2 * kSteps);
+    // the queries have come: else the compiler waits for them in every stage, and with them for the codes on their way
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    for (int step = 0, i = 0; step < steps; step += kSteps, i ^= 1) {
+        __syncthreads();  // stage i is made, and the other one no longer read
+        if (step + kSteps < steps) {
+            make(part, stages[i ^ 1]);
+            load(part, page, step + 2 * kSteps);
+            page = page_at(step + 3 * kSteps);
+        }
+        const Stage8<D, NW> &st = stages[i];
+#pragma unroll
+        for (int sub = 0; sub < kSteps; ++sub) {
+            const int at = span.token_of(step + sub);
+            if (at >= mine) break;
+            if (at + 32 <= from && at >= a.sinks) continue;
+            const Page pages_of[2] = {st.pages[2 * sub], st.pages[2 * sub + 1]};
+            attend<true, D, MT>(
+                a, s, at, at + 32 > sure.limit || (at < sure.low && at + 32 > a.sinks), {false, false}, pages_of,
+                [&](int h, int k) { return __builtin_bit_cast(bf16x8, st.keys[2 * sub + h][k][lane]); },
+                [&](auto u) { return __builtin_bit_cast(halfx8, st.values[sub][u][lane]); });
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int row = row0 + 16 * mt + n;
+        const float l = sum_over_g(s.l[mt]), inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
+        if (row >= total) continue;
+        const int64_t to = out_row(a, sq, head, row);
+        if (a.lse && g == 0) a.lse[to] = lse_of(s.m[mt], l);
+        // a lane's D / 4 channels lie behind one another
+        uint16_t *out = a.out + to * D + g * (D / 4);
+#pragma unroll
+        for (int c = 0; c < D / 4; c += 8) {
+            const auto v = [&](int e) { return s.o[mt][(c + e) % NT][(c + e) / NT] * inv; };
+            *reinterpret_cast<uint4 *>(out + c) = make_uint4(f32x2_to_bf16x2_rne(v(0), v(1)), f32x2_to_bf16x2_rne(v(2), v(3)), f32x2_to_bf16x2_rne(v(4), v(5)), f32x2_to_bf16x2_rne(v(6), v(7)));
+        }
+    }
+}
+
 // Weights that the cached tokens got, from the logarithms of the rows' sums: weights[seq, head, t] += sum over the head's rows of
 // exp(score - lse).  A wave has 16 tokens' keys, as MFMA operands, and walks over the rows that see some of them; S^T = K Q^T leaves
 // each lane four tokens' sums over its rows, joined over the 16 lanes at the end.  Every sum has one writer.
@@ -511,19 +664,28 @@ __global__ __launch_bounds__(256) void kv8_attention_weights_kernel(AttnArgs8 a,
     }
 }
 
-// How a call is laid out: rows a wave (16 mt), row tiles at most, splits, workspace.
+// How a call is laid out: rows a wave (16 mt), whether waves share rows (splits of the tokens) or have their own, row
+// tiles at most, splits, workspace.
 struct Plan {
-    int mt;
+    int mt, waves;
+    bool rows;
     int64_t tiles, splits, bytes;
 };
 
 Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols, bool varlen, int64_t window, int64_t sinks) {
-    Plan p{1, 0, 1, 0};
+    Plan p{1, 4, false, 0, 1, 0};
     if (tokens == 0 || batch == 0) return p;
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio, each = (rows + batch - 1) / batch;
+    const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
+    p.rows = varlen && rows / 32 * c->kv_heads >= 6 * cus;
+    if (p.rows) {
+        p.mt = 2;
+        if (rows / (128 * p.mt) * c->kv_heads >= 2 * cus) p.waves = 8;
+        p.tiles = tiles(16 * p.waves * p.mt);
+        return p;
+    }
     p.mt = each <= 96 ? 1 : 2;
-    const int64_t per = 16 * p.mt;
-    p.tiles = varlen ? rows / per + batch : batch * ((ratio + per - 1) / per);
+    p.tiles = tiles(16 * p.mt);
     const int64_t tasks = p.tiles * c->kv_heads, len = std::min(table_cols * c->page_size, window + sinks + 64 + tokens);
     p.splits = std::max<int64_t>(1, std::min((2 * cus + tasks - 1) / tasks, (len + 127) / 128));
     const int64_t row = (c->head_dim + 4) * 4;
@@ -555,6 +717,19 @@ void launch_split(AttnArgs8 a, const Plan &p, hipStream_t st) {
         kv8_attention_join_kernel<D><<<dim3(static_cast<unsigned>(static_cast<int64_t>(a.tokens) * a.heads * a.ratio)), dim3(256), 0, st>>>(a);
         check_launch("kv8_attention_join");
     }
+}
+
+template <int D, int NW>
+void launch_tile(AttnArgs8 a, const Plan &p, hipStream_t st) {
+    constexpr int lds = 2 * sizeof(Stage8<D, NW>);
+    static_assert(lds <= NW * 20 * 1024, "eight waves a CU");
+    static std::atomic<uint64_t> attr_devices{0};
+    const auto kern = kv8_attention_tile_kernel<D, NW>;
+    raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
+    for_tiles(a, p, a.heads, 64 * NW, [&](unsigned grid) {
+        kern<<<dim3(grid), dim3(64 * NW), lds, st>>>(a, static_cast<int>(p.tiles));
+        check_launch("kv8_attention_tile");
+    });
 }
 
 // window 0 (none) as one that no place reaches.
@@ -614,8 +789,12 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
                     static_cast<int>(table_cols), static_cast<int>(cache->num_pages), causal, static_cast<int>(p.splits),
                     static_cast<int>(window_of(window)), static_cast<int>(sinks), 0};
         const hipStream_t st = static_cast<hipStream_t>(stream);
-        if (cache->head_dim == 64) p.mt == 1 ? launch_split<64, 1, 4>(a, p, st) : launch_split<64, 2, 4>(a, p, st);
-        else p.mt == 1 ? launch_split<128, 1, 4>(a, p, st) : launch_split<128, 2, 4>(a, p, st);
+        const auto launch = [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            if (p.rows) p.waves == 8 ? launch_tile<D, 8>(a, p, st) : launch_tile<D, 4>(a, p, st);
+            else p.mt == 1 ? launch_split<D, 1, 4>(a, p, st) : launch_split<D, 2, 4>(a, p, st);
+        };
+        cache->head_dim == 64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
         const int64_t reach = std::min(weights ? weights_cols : 0, table_cols * cache->page_size), blocks = (reach + 63) / 64;
         const int64_t all = blocks * batch * cache->kv_heads;
         for (int64_t b = 0, most = most_workgroups(256); b < all; b += most) {
