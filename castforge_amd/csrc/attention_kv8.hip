@@ -31,12 +31,22 @@ struct AttnArgs8 {
     const int32_t *table, *kv_lens;
     uint16_t *out;
     float *lse;
-    float *part;  // splits > 1: [tokens * q heads][splits][D + 4], output sums, reference, sum, two unused
+    float *part;  // splits > 1: [tokens * q heads][splits][D + 4], output sums, reference, sum, how many splits there are (of the first), unused
     float scale;  // of scores, base 2
     int tokens, batch, heads, ratio, page_shift, table_cols, num_pages, causal, splits;
     int window, sinks;  // window 0x7fffffff: none
+    uint32_t ratio_mul;  // query_of's
+    int ratio_shift;
+    float *scores;      // NULL, or where the kernel of few rows leaves its scores: [tokens * q heads][score_cols], base 2
+    int score_cols;
     int first_tile;     // of a launch's row tiles, where one launch cannot hold them all
 };
+
+// row / ratio of a row below 2^31: by ceil(2^(31 + l) / ratio), l = ceil(log2 ratio), which is exact there (a division takes ten times as
+// long, and tiles begin with several).
+__device__ __forceinline__ int query_of(const AttnArgs8 &a, int row) {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(row)) * a.ratio_mul >> a.ratio_shift);
+}
 
 // What a query at a place sees: t < limit, and t >= low or t < sinks.
 __device__ __forceinline__ int limit_of(const AttnArgs8 &a, const Seq &sq, int i) { return a.causal ? min(sq.len, sq.len - sq.n + i + 1) : sq.len; }
@@ -142,7 +152,7 @@ __device__ __forceinline__ void load_rows(const AttnArgs8 &a, Rows8<D, MT> &s, c
     const int n = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const int row = row0 + 16 * mt + n, i = row / a.ratio;
+        const int row = row0 + 16 * mt + n, i = query_of(a, row);
         const bool in = i < sq.n;
         // rows past the sequence's see all: they are not stored, and do not make a tile an edge
         s.limit[mt] = in ? limit_of(a, sq, i) : 0x7fffffff;
@@ -185,10 +195,8 @@ __device__ __forceinline__ Page page_of(float scale, float ks, float vs) {
 // 11 bits down to 2^-21 of them), and the rescaling is rare.
 // keys(h, i): the MFMA operand of half h's 16 tokens and 32 channels; values(u): that of 16 channels and 32 tokens.  gone: a half's
 // page is none of the cache's; edge, uniform: so, or some row does not see some token.
-// kFold: one fma takes a product to an exponent less m; where m moves, they are made from the products again, which stay until then
-// (a register a score: the kernel of few rows has none left).
-template <bool kFold, int D, int MT, class Keys, class Values>
-__device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int at, bool edge, const bool (&gone)[2], const Page (&pages)[2], const Keys &keys, const Values &values) {
+template <int D, int MT, class Keys, class Values>
+__device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int at, bool edge, const bool (&gone)[2], const Page (&pages)[2], float *const (&score_rows)[MT], const Keys &keys, const Values &values) {
     constexpr int KS = D / 32, NT = D / 16;
     const int g = (threadIdx.x >> 4) & 3;
     floatx4 dot[MT][2];
@@ -201,15 +209,13 @@ __device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int 
             for (int mt = 0; mt < MT; ++mt)
                 dot[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, s.q[mt][i]), i ? dot[mt][h] : floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
         }
-    float z[MT][2][4];
+    float y[MT][2][4];  // scores and their values' exponents, base 2
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float em = kFold ? pages[h].e - s.m[mt] : pages[h].e;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) z[mt][h][r] = __builtin_fmaf(dot[mt][h][r], pages[h].kf, em);
-        }
+            for (int r = 0; r < 4; ++r) y[mt][h][r] = __builtin_fmaf(dot[mt][h][r], pages[h].kf, pages[h].e);
     if (edge) {
         int first = at + 4 * g;
         asm volatile("" : "+v"(first));  // a branch: the comparisons stay in it
@@ -220,39 +226,37 @@ __device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int 
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 const bool hidden = gone[i / 4] | (t >= s.limit[mt]) | ((t < s.low[mt]) & behind);
-                z[mt][i / 4][i % 4] = hidden ? -INFINITY : z[mt][i / 4][i % 4];
+                y[mt][i / 4][i % 4] = hidden ? -INFINITY : y[mt][i / 4][i % 4];
             }
         }
+    }
+    if (a.scores) {  // uniform; scores of what a row does not see are not read, but for those of no page: -inf
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                floatx4 v;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = gone[h] ? -INFINITY : dot[mt][h][r] * pages[h].kf;
+                if (score_rows[mt] && at + 16 * h < a.score_cols) *reinterpret_cast<floatx4 *>(score_rows[mt] + at + 16 * h) = v;  // a table may end with a half
+            }
     }
     uint32_t p[MT][4];  // weights as f16 pairs: tokens (0, 1), (2, 3) of both halves
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        float (&v)[2][4] = z[mt];
+        const float (&v)[2][4] = y[mt];
         const float most = max3(max3(v[0][0], v[0][1], v[0][2]), max3(v[0][3], v[1][0], v[1][1]), max3(v[1][2], v[1][3], v[1][3]));
-        if (__any(most > (kFold ? 15.f : s.m[mt] + 15.f))) {
-            float top = most;
-            if constexpr (kFold) {
-                top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float y = __builtin_fmaf(dot[mt][i / 4][i % 4], pages[i / 4].kf, pages[i / 4].e);
-                    v[i / 4][i % 4] = v[i / 4][i % 4] == -INFINITY ? -INFINITY : y;
-                    top = fmaxf(top, v[i / 4][i % 4]);
-                }
-            }
-            const float m = fmaxf(s.m[mt], max_over_g(top) - 7.f), f = __builtin_amdgcn_exp2f(s.m[mt] - m);
+        if (__any(most > s.m[mt] + 15.f)) {
+            const float m = fmaxf(s.m[mt], max_over_g(most) - 7.f), f = __builtin_amdgcn_exp2f(s.m[mt] - m);
             s.m[mt] = m;
             s.l[mt] *= f;
 #pragma unroll
             for (int u = 0; u < NT; ++u) s.o[mt][u] *= f;
-            if constexpr (kFold)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i / 4][i % 4] -= m;
         }
         float w[2][4];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            w[i / 4][i % 4] = __builtin_amdgcn_exp2f(kFold ? v[i / 4][i % 4] : v[i / 4][i % 4] - s.m[mt]);
+            w[i / 4][i % 4] = __builtin_amdgcn_exp2f(v[i / 4][i % 4] - s.m[mt]);
             s.l[mt] = __builtin_fmaf(w[i / 4][i % 4], pages[i / 4].back, s.l[mt]);
         }
 #pragma unroll
@@ -267,14 +271,26 @@ __device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int 
     });
 }
 
+// Where a row's output goes, of the sequence's row tile.
+__device__ __forceinline__ int64_t out_row(const AttnArgs8 &a, const Seq &sq, int head, int row) {
+    const int i = query_of(a, row);
+    return static_cast<int64_t>(sq.first + i) * (a.heads * a.ratio) + head * a.ratio + row - i * a.ratio;
+}
+
 // A wave's walk over steps first, first + by, .. below last of a span, the next tile's loads in flight.
 template <int D, int MT>
-__device__ __forceinline__ void walk(const AttnArgs8 &a, Rows8<D, MT> &s, const Seq &sq, int head, const Span &span, int first, int by, int last) {
+__device__ __forceinline__ void walk(const AttnArgs8 &a, Rows8<D, MT> &s, const Seq &sq, int head, const Span &span, int row0, int first, int by, int last) {
     if (first >= last) return;
     constexpr int W = Tile8<D>::W;
     const int lane = threadIdx.x & 63, g = lane >> 4;
     const Sure sure = seen_by_all(s, sq.len);
     const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
+    float *score_rows[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int row = row0 + 16 * mt + (lane & 15);
+        score_rows[mt] = a.scores && row < sq.n * a.ratio ? a.scores + out_row(a, sq, head, row) * a.score_cols + 4 * g : nullptr;
+    }
     const auto pages = [&](int step, int (&p)[2]) {
         const int at = span.token_of(step);
 #pragma unroll
@@ -307,8 +323,8 @@ __device__ __forceinline__ void walk(const AttnArgs8 &a, Rows8<D, MT> &s, const 
         }
         const Page pages_of[2] = {page_of(a.scale, cur.ks[0], cur.vs[0]), page_of(a.scale, cur.ks[1], cur.vs[1])};
         const bool gone[2] = {!cur.live[0], !cur.live[1]}, edge = apart || at + 32 > sure.limit || (at < sure.low && at + 32 > a.sinks);
-        attend<false, D, MT>(
-            a, s, at, edge, gone, pages_of,
+        attend<D, MT>(
+            a, s, at, edge, gone, pages_of, score_rows,
             [&](int h, int i) {
                 const uint4 w = cur.k[h][i / 2];
                 return i % 2 ? keys_bf16(w.z, w.w) : keys_bf16(w.x, w.y);
@@ -330,11 +346,6 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs8 &a, int seq) {
     }
     sq.len = a.num_pages > 0 ? min(max(scalar_load(a.kv_lens, seq), 0), token_cap(a)) : 0;
     return sq;
-}
-
-// Where a row's output goes, of the sequence's row tile.
-__device__ __forceinline__ int64_t out_row(const AttnArgs8 &a, const Seq &sq, int head, int row) {
-    return static_cast<int64_t>(sq.first + row / a.ratio) * (a.heads * a.ratio) + head * a.ratio + row % a.ratio;
 }
 
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f; }
@@ -359,12 +370,12 @@ __global__ __launch_bounds__(64 * NW) void kv8_attention_split_kernel(AttnArgs8 
     const int row0 = sq.tile * 16 * MT, rows = min(16 * MT, sq.n * a.ratio - row0);
     const int used = splits_of_seq(a, sq);
     if (split >= used) return;
-    const Span span = span_of(a, sq, row0 / a.ratio, (row0 + rows - 1) / a.ratio);
+    const Span span = span_of(a, sq, query_of(a, row0), query_of(a, row0 + rows - 1));
     const int steps = span.steps(), share = (steps + used * NW - 1) / (used * NW) * NW;  // whole rounds of the waves
     Rows8<D, MT> s;
     load_rows(a, s, sq, head, row0);
     // shares are rounded up: the last ones may be empty
-    walk<D, MT>(a, s, sq, head, span, split * share + wave, NW, min(steps, (split + 1) * share));
+    walk<D, MT>(a, s, sq, head, span, row0, split * share + wave, NW, min(steps, (split + 1) * share));
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (16 * mt >= rows) break;
@@ -402,7 +413,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_attention_split_kernel(AttnArgs8 
                 float *p = a.part + (at * a.splits + split) * (D + 4);
                 *reinterpret_cast<float4 *>(p + ch) = make_float4(v[0], v[1], v[2], v[3]);
                 *reinterpret_cast<float4 *>(p + ch + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                if (ch == 0) p[D] = mm, p[D + 1] = l;
+                if (ch == 0) *reinterpret_cast<float4 *>(p + D) = make_float4(mm, l, __int_as_float(used), 0.f);
             } else {
                 const float inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
                 *reinterpret_cast<uint4 *>(a.out + at * D + ch) =
@@ -414,8 +425,46 @@ __global__ __launch_bounds__(64 * NW) void kv8_attention_split_kernel(AttnArgs8 
     }
 }
 
-// Joins the splits: a workgroup a (token, query head), D / 8 lanes of eight channels by 2048 / D lanes of splits, each with a
-// reference of its own until the end.
+// Joins the splits of many rows: D / 4 lanes of four channels a row, which take four splits at a time: 32768 rows of two splits cost a
+// prompt 6 us, by the kernel below 34.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_attention_join_rows_kernel(AttnArgs8 a) {
+    constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes, hq = a.heads * a.ratio;
+    const int ch = threadIdx.x % kLanes * 4;
+    if (at >= (a.cu_q ? min(a.cu_q[a.batch], a.tokens) : a.tokens) * hq) return;  // of no sequence
+    const float *part = a.part + at * a.splits * (D + 4);
+    const int used = min(max(__float_as_int(part[D + 2]), 1), a.splits);
+    float m = kNoMax, l = 0.f;
+    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < used; s += 4) {
+        floatx4 o[4];
+        floatx2 ml[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float *p = part + static_cast<int64_t>(min(s + i, used - 1)) * (D + 4);
+            o[i] = *reinterpret_cast<const floatx4 *>(p + ch), ml[i] = *reinterpret_cast<const floatx2 *>(p + D);
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+        const float f = __builtin_amdgcn_exp2f(m - top);
+        m = top, l *= f, v *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float g = s + i < used ? __builtin_amdgcn_exp2f(ml[i].x - m) : 0.f;
+            l = __builtin_fmaf(ml[i].y, g, l);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(o[i][e], g, v[e]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
+    *reinterpret_cast<uint2 *>(a.out + at * D + ch) = make_uint2(f32x2_to_bf16x2_rne(v[0] * inv, v[1] * inv), f32x2_to_bf16x2_rne(v[2] * inv, v[3] * inv));
+    if (a.lse && ch == 0) a.lse[at] = lse_of(m, l);
+}
+
+// Joins the many splits of few rows: a workgroup a (token, query head), D / 8 lanes of eight channels by 2048 / D lanes of splits, each
+// with a reference of its own until the end.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_attention_join_kernel(AttnArgs8 a) {
     constexpr int kCh = D / 8, kSp = 256 / kCh;
@@ -425,26 +474,17 @@ __global__ __launch_bounds__(256) void kv8_attention_join_kernel(AttnArgs8 a) {
     const int64_t at = blockIdx.x;
     const int token = static_cast<int>(at / hq), ch = threadIdx.x % kCh * 8, sl = threadIdx.x / kCh;
     struct Part {
-        float4 x, y;
-        float2 ml;
+        floatx4 x, y;
+        floatx2 ml;
     };
     const float *part = a.part + at * a.splits * (D + 4);
     const auto load = [&](int s) {
         const float *p = part + static_cast<int64_t>(s) * (D + 4);
-        return Part{*reinterpret_cast<const float4 *>(p + ch), *reinterpret_cast<const float4 *>(p + ch + 4), *reinterpret_cast<const float2 *>(p + D)};
+        return Part{*reinterpret_cast<const floatx4 *>(p + ch), *reinterpret_cast<const floatx4 *>(p + ch + 4), *reinterpret_cast<const floatx2 *>(p + D)};
     };
     Part next = load(min(sl, a.splits - 1));
-    int seq = token;
-    if (a.cu_q) {
-        seq = -1;
-        for (int b0 = 0; b0 < a.batch && seq < 0; b0 += 64) {
-            const int b = b0 + (threadIdx.x & 63);
-            const uint64_t hit = __ballot(b < a.batch && a.cu_q[min(b, a.batch)] <= token && token < a.cu_q[min(b, a.batch - 1) + 1]);
-            if (hit) seq = __builtin_amdgcn_readfirstlane(b0 + __builtin_ctzll(hit));
-        }
-        if (seq < 0) return;
-    }
-    const int used = splits_of_seq(a, seq_of(a, seq));
+    const int used = min(max(__float_as_int(part[D + 2]), 1), a.splits);
+    if (a.cu_q && token >= a.cu_q[a.batch]) return;  // of no sequence
     float m = kNoMax, l = 0.f, v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
@@ -452,11 +492,10 @@ __global__ __launch_bounds__(256) void kv8_attention_join_kernel(AttnArgs8 a) {
         const Part p = next;
         if (s + kSp < used) next = load(s + kSp);
         const float top = fmaxf(m, p.ml.x), f = __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(p.ml.x - top);
-        const float o[8] = {p.x.x, p.x.y, p.x.z, p.x.w, p.y.x, p.y.y, p.y.z, p.y.w};
         m = top;
         l = __builtin_fmaf(p.ml.y, g, l * f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(o[e], g, v[e] * f);
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(e < 4 ? p.x[e % 4] : p.y[e % 4], g, v[e] * f);
     }
     if (ch == 0) ms[sl] = m;
     __syncthreads();
@@ -477,191 +516,539 @@ __global__ __launch_bounds__(256) void kv8_attention_join_kernel(AttnArgs8 a) {
     }
 }
 
-// Many rows: each wave takes 32 rows of its own, and the NW of a workgroup share the making of the MFMA operands.  Of every 16 NW
-// tokens a wave turns 16 into operands in LDS and all read them back; two stages, one barrier a stage: the operands of the next tokens
-// are made while the present ones are used, and the codes of those after that are on their way.
-// Heads are dealt out first (one head's keys and values stay with one XCD where there are eight heads), and row tiles from the
-// last, which see the most tokens.
+// Many rows: each wave takes 32 rows of its own, and the eight of a workgroup share the making of the MFMA operands: of every 128
+// tokens a wave turns 32 tokens' half rows of keys and 16 tokens' values into operands in LDS, and all read them back; two stages, one
+// barrier a stage: the operands of the next tokens are made while the present ones are used, and the codes of those after that are on
+// their way.
+// 32 x 32 x 16 MFMAs: of S^T = K Q^T lane (n = lane % 32, h = lane / 32) holds row n's scores of the tokens 8 j + 4 h + r of 32 (j, r < 4),
+// which is what O^T = V^T P^T takes of 16 tokens (j < 2, then j >= 2) as its second operand.  Row i of a tile of V^T is channel
+// i D / 32 + u.
 template <int D, int NW>
 struct Stage8 {
-    static constexpr int KS = D / 32, NT = D / 16;
-    uint4 keys[NW][KS][64];        // 16 tokens, 32 channels: a lane's operand
-    uint4 values[NW / 2][NT][64];  // 32 tokens, 16 channels
-    Page pages[NW];
+    static constexpr int KS = D / 16, NT = D / 32;
+    uint4 keys[NW / 2][KS][64];       // 32 tokens, 16 channels: a lane's operand
+    uint4 values[NW / 2][2][NT][64];  // 16 tokens, 32 channels
+    Page pages[NW / 2][2];
 };
 
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+// A wave's rows, one a lane and a half of the tokens.
+template <int D>
+struct TileRows {
+    static constexpr int KS = D / 16, NT = D / 32;
+    bf16x8 q[KS];    // channels 32 (i / 2) + 16 h + 8 (i % 2) ..
+    int limit, low;
+    floatx16 o[NT];
+    float m, l;
+};
+
+// Scores of 32 tokens and rows, unscaled.
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 3))) void kv8_attention_tile_kernel(AttnArgs8 a, int tiles) {
-    constexpr int MT = 2, KS = D / 32, NT = D / 16, W = D / 64, kSteps = NW / 2;  // steps of 32 tokens a stage
+__device__ __forceinline__ floatx16 tile_scores(const TileRows<D> &s, const Stage8<D, NW> &st, int sub, int lane) {
+    floatx16 dot;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dot[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) dot = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, st.keys[sub][i][lane]), s.q[i], dot, 0, 0, 0);
+    return dot;
+}
+
+// attend()'s steps: exponents less m by one fma each, which are made from the products again where m moves.
+struct Exponents {
+    float z[16], most;
+};
+__device__ __forceinline__ float most_of(const float (&z)[16]) {
+    const float a = max3(max3(z[0], z[1], z[2]), z[3], z[4]), b = max3(max3(z[5], z[6], z[7]), z[8], z[9]);
+    return max3(max3(a, b, z[10]), max3(z[11], z[12], z[13]), max3(z[14], z[15], z[15]));
+}
+__device__ __forceinline__ Exponents exponents_of(const floatx16 &dot, const Page (&pages)[2], float m) {
+    Exponents e;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float em = pages[h].e - m;
+#pragma unroll
+        for (int i = 8 * h; i < 8 * h + 8; ++i) e.z[i] = __builtin_fmaf(dot[i], pages[h].kf, em);
+    }
+    e.most = most_of(e.z);
+    return e;
+}
+
+// What lies in branches: masks, and moves of m.
+template <int D>
+__device__ __forceinline__ void settle(const AttnArgs8 &a, TileRows<D> &s, Exponents &e, const floatx16 &dot, const Page (&pages)[2], int at, bool edge) {
+    if (edge) {
+        int first = at + 4 * ((threadIdx.x >> 5) & 1);
+        asm volatile("" : "+v"(first));  // a branch: the comparisons stay in it
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int t = first + 8 * (i / 4) + i % 4;
+            e.z[i] = (t >= s.limit) | ((t < s.low) & (t >= a.sinks)) ? -INFINITY : e.z[i];
+        }
+        e.most = most_of(e.z);
+    }
+    if (__any(e.most > 15.f)) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float y = __builtin_fmaf(dot[i], pages[i / 8].kf, pages[i / 8].e);
+            e.z[i] = e.z[i] == -INFINITY ? -INFINITY : y;
+            top = fmaxf(top, e.z[i]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float m = fmaxf(s.m, top - 7.f), f = __builtin_amdgcn_exp2f(s.m - m);
+        s.m = m;
+        s.l *= f;
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) s.o[u] *= f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) e.z[i] -= m;
+    }
+}
+
+// Weights as f16 pairs, and their sum.
+template <int D>
+__device__ __forceinline__ void tile_weights(TileRows<D> &s, const Exponents &e, const Page (&pages)[2], uint32_t (&p)[8]) {
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(e.z[i]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float *v = w + 8 * h;
+        s.l = __builtin_fmaf(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])), pages[h].back, s.l);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{w[2 * i], w[2 * i + 1]}), halfx2));
+}
+
+template <int D, int NW>
+__device__ __forceinline__ void tile_outputs(TileRows<D> &s, const Stage8<D, NW> &st, int sub, int lane, const uint32_t (&p)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u)
+            s.o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, st.values[sub][h][u][lane]),
+                                                            __builtin_bit_cast(halfx8, uintx4{p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]}), s.o[u], 0, 0, 0);
+}
+
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void kv8_attention_tile_kernel(AttnArgs8 a, int tiles) {
+    constexpr int kRows = 32, KS = D / 16, NT = D / 32, W = D / 64, kSteps = NW / 2;  // steps of 32 tokens a stage
     extern __shared__ __align__(16) uint8_t lds[];
     Stage8<D, NW> *stages = reinterpret_cast<Stage8<D, NW> *>(lds);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int n = lane & 15, g = lane >> 4;
-    const int head = blockIdx.x % a.heads;
-    const Seq sq = find_tile(a, tiles - 1 - (a.first_tile + blockIdx.x / a.heads), 16 * NW * MT);
+    const int n = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.heads, split = blockIdx.x / a.heads % a.splits;
+    const Seq sq = find_tile(a, tiles - 1 - (a.first_tile + static_cast<int>(blockIdx.x / a.heads / a.splits)), kRows * NW);
     if (sq.seq < 0) return;
-    const int total = sq.n * a.ratio, row_of_all = sq.tile * 16 * NW * MT, row0 = row_of_all + wave * 16 * MT;
-    const Span span = span_of(a, sq, row_of_all / a.ratio, (min(row_of_all + 16 * NW * MT, total) - 1) / a.ratio);
-    const int steps = span.steps();
+    const int used = splits_of_seq(a, sq);
+    if (split >= used) return;
+    const int total = sq.n * a.ratio, row_of_all = sq.tile * kRows * NW, row0 = row_of_all + wave * kRows, row = row0 + n;
+    const Span span = span_of(a, sq, query_of(a, row_of_all), query_of(a, min(row_of_all + kRows * NW, total) - 1));
+    // the split's steps: whole stages; shares are rounded up, the last ones may be empty
+    const int share = (span.steps() + used * kSteps - 1) / (used * kSteps) * kSteps;
+    const int begin = split * share, steps = min(span.steps(), begin + share);
     // the wave's own rows see tokens below `mine`, and from `from` on or sinks
-    const int mine = row0 < total ? limit_of(a, sq, (min(row0 + 16 * MT, total) - 1) / a.ratio) : 0;
-    const int from = row0 < total ? low_of(a, sq, row0 / a.ratio) : 0;
-    Rows8<D, MT> s;
-    load_rows(a, s, sq, head, row0);
-    const Sure sure = seen_by_all(s, sq.len);
+    const int mine = row0 < total ? limit_of(a, sq, query_of(a, min(row0 + kRows, total) - 1)) : 0;
+    const int from = row0 < total ? low_of(a, sq, query_of(a, row0)) : 0;
+    TileRows<D> s;
+    {
+        const int i = query_of(a, row);
+        const bool in = i < sq.n;
+        // rows past the sequence's see all: they are not stored, and do not make a tile an edge
+        s.limit = in ? limit_of(a, sq, i) : 0x7fffffff;
+        s.low = in ? low_of(a, sq, i) : 0;
+        const uint16_t *p = a.q + (sq.first + (in ? i : 0)) * a.q_stride + (head * a.ratio + (in ? row - i * a.ratio : 0)) * D + 16 * h;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s.q[k] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(p + 32 * (k / 2) + 8 * (k % 2)));
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int i16 = 0; i16 < 16; ++i16) s.o[u][i16] = 0.f;
+        s.m = kNoMax, s.l = 0.f;
+    }
+    int sure_limit = min(sq.len, s.limit), sure_low = s.low;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sure_limit = min(sure_limit, __shfl_xor(sure_limit, o)), sure_low = max(sure_low, __shfl_xor(sure_low, o));
+    sure_limit = __builtin_amdgcn_readfirstlane(sure_limit), sure_low = __builtin_amdgcn_readfirstlane(sure_low);
     const int32_t *table = a.table + static_cast<int64_t>(sq.seq) * a.table_cols;
 
-    // this wave's 16 tokens of a stage
+    // This wave's 16 tokens of a stage: half wave % 2 of step wave / 2.  n16 = lane % 16, g = lane / 16.
+    const int sub_of = wave / 2, half = wave & 1, n16 = lane & 15, g = lane >> 4;
     struct Part {
-        uint4 k[W];
-        uint32_t v[4][W];
+        uint4 k[W];     // token n16: codes 16 (W g + i) ..
+        uint32_t v[8];  // tokens 8 j + 4 h + r: codes n D / 32 ..
         float ks, vs;
-        int at;
-        bool live;
+        int at;         // its first token
+        bool live;      // its page is one of the cache's
     };
-    const auto token_at = [&](int step) { return span.token_of(step + wave / 2) + 16 * (wave & 1); };
+    const uint32_t page_bytes = (static_cast<uint32_t>(a.heads) << a.page_shift) * D;  // below 2^26
+    const int page_mask = (1 << a.page_shift) - 1;
+    const uint32_t head_bytes = (static_cast<uint32_t>(head) << a.page_shift) * D;
+    const auto token_at = [&](int step) { return span.token_of(step + sub_of) + 16 * half; };
     const auto page_at = [&](int step) {
         const int at = token_at(step);
-        return step + wave / 2 < steps && at < span.end ? scalar_load(table, at >> a.page_shift) : -1;
+        return step + sub_of < steps && at < span.end ? scalar_load(table, at >> a.page_shift) : -1;
     };
     const auto load = [&](Part &t, int page, int step) {
         t.at = token_at(step);
-        t.live = page >= 0 && page < a.num_pages;
-        const int p = t.live ? page : 0;
-        const int64_t row = kv8_row(p, head, t.at & ((1 << a.page_shift) - 1), a.heads, a.page_shift), at_scale = static_cast<int64_t>(p) * a.heads + head;
-        const uint8_t *k = a.k_codes + (row + n) * D + 16 * g, *v = a.v_codes + (row + 4 * g) * D + n * (D / 16);
+        t.live = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages);
+        const uint32_t p = t.live ? page : 0;
+        const uint64_t from_codes = static_cast<uint64_t>(p) * page_bytes + head_bytes + static_cast<uint32_t>(t.at & page_mask) * D;
+        const uint8_t *k = a.k_codes + from_codes, *v = a.v_codes + from_codes;
 #pragma unroll
-        for (int i = 0; i < W; ++i) t.k[i] = *reinterpret_cast<const uint4 *>(k + 64 * i);
+        for (int i = 0; i < W; ++i) t.k[i] = *reinterpret_cast<const uint4 *>(k + n16 * D + 16 * (W * g + i));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) __builtin_memcpy(t.v[r], __builtin_assume_aligned(v + r * D, D / 16), D / 16);
+        for (int i = 0; i < 8; ++i) {
+            const uint8_t *q = v + 4 * h * D + n * NT + (8 * (i / 4) + i % 4) * D;
+            if constexpr (D == 128) t.v[i] = *reinterpret_cast<const uint32_t *>(q);
+            else t.v[i] = *reinterpret_cast<const uint16_t *>(q);
+        }
+        const int64_t at_scale = static_cast<int64_t>(static_cast<uint64_t>(p) * static_cast<uint32_t>(a.heads) + static_cast<uint32_t>(head));
         t.ks = scalar_load(a.k_scales, at_scale), t.vs = scalar_load(a.v_scales, at_scale);
     };
     const auto make = [&](Part &t, Stage8<D, NW> &st) {
         if (!t.live || t.at + 16 > sq.len) {  // uniform: bytes that are no token's may be NaN, which a weight of 0 does not take away
-            asm volatile("");
+            int at = t.at;
+            asm volatile("" : "+v"(at));
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
+            for (int i = 0; i < W; ++i)
                 if (!t.live) t.k[i] = uint4{};
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (!t.live || t.at + 4 * g + r >= sq.len) t.v[r][i] = 0;
-            }
+            for (int i = 0; i < 8; ++i)
+                if (!t.live || at + 8 * (i / 4) + 4 * h + i % 4 >= sq.len) t.v[i] = 0;
         }
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            st.keys[wave][2 * i][lane] = __builtin_bit_cast(uint4, keys_bf16(t.k[i].x, t.k[i].y));
-            st.keys[wave][2 * i + 1][lane] = __builtin_bit_cast(uint4, keys_bf16(t.k[i].z, t.k[i].w));
+            const int piece = W * g + i;  // of the MFMAs' 32 channels piece / 2, half piece % 2
+            uint4 *to = &st.keys[sub_of][piece & ~1][32 * (piece & 1) + 16 * half + n16];
+            to[0] = __builtin_bit_cast(uint4, keys_bf16(t.k[i].x, t.k[i].y));
+            to[64] = __builtin_bit_cast(uint4, keys_bf16(t.k[i].z, t.k[i].w));
         }
-        static_for<NT>([&](auto u) __attribute__((always_inline)) { reinterpret_cast<uint2 *>(&st.values[wave / 2][u][lane])[wave & 1] = values_f16<u>(t.v); });
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lo[i] = low_codes(t.v[2 * i], t.v[2 * i + 1]), hi[i] = high_codes(t.v[2 * i], t.v[2 * i + 1]);
+        static_for<NT>([&](auto u) __attribute__((always_inline)) {
+            const auto pair = [&](int i) { return f16_pair(u < 2 ? lo[i] : hi[i], u % 2); };
+            st.values[sub_of][half][u][lane] = make_uint4(pair(0), pair(1), pair(2), pair(3));
+        });
         // no page of the cache: scores of -inf, by products of zeros
-        if (lane == 0) st.pages[wave] = t.live ? page_of(a.scale, t.ks, t.vs) : Page{0.f, -INFINITY, 0.f};
+        if (lane == 0) st.pages[sub_of][half] = t.live ? page_of(a.scale, t.ks, t.vs) : Page{0.f, -INFINITY, 0.f};
+    };
+    // a stage's tokens for the wave's rows
+    const auto walk_stage = [&](int step, int i) {
+        const Stage8<D, NW> &st = stages[i];
+        // the wave's steps of the stage: those below the window of all its rows are left out where no sink is among them
+        const auto at_of = [&](int sub) { return span.token_of(step + sub); };
+        int sub = 0, last = kSteps;
+        if (at_of(0) >= a.sinks)
+            while (sub < kSteps && at_of(sub) + 32 <= from) ++sub;
+        while (last > sub && (step + last > steps || at_of(last - 1) >= mine)) --last;
+        if (sub >= last) return;
+        const auto is_edge = [&](int at) { return at + 32 > sure_limit || (at < sure_low && at + 32 > a.sinks); };
+        // The next step's products are issued among this one's weights: vector work and MFMAs then have each other to run beside.
+        floatx16 dot = tile_scores<D, NW>(s, st, sub, lane);
+        Exponents e;
+        Page pg[2];
+        uint32_t p[8];
+        const auto exponents = [&](int at) {
+            pg[0] = st.pages[sub][0], pg[1] = st.pages[sub][1];
+            e = exponents_of(dot, pg, s.m);
+            settle<D>(a, s, e, dot, pg, at, is_edge(at));
+        };
+        exponents(at_of(sub));
+        for (; sub + 1 < last;) {
+            dot = tile_scores<D, NW>(s, st, sub + 1, lane);
+            tile_weights<D>(s, e, pg, p);
+            tile_outputs<D, NW>(s, st, sub, lane, p);
+            ++sub;
+            exponents(at_of(sub));
+        }
+        tile_weights<D>(s, e, pg, p);
+        tile_outputs<D, NW>(s, st, sub, lane, p);
     };
     Part part;
-    if (steps > 0) {
-        load(part, page_at(0), 0);
+    int page = page_at(begin + kSteps);
+    if (steps > begin) {
+        load(part, page_at(begin), begin);
         make(part, stages[0]);
-        load(part, page_at(kSteps), kSteps);
+        // the queries have come too: else the compiler waits for them in every stage, and with them for the codes on their way
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        load(part, page, begin + kSteps);
     }
-    int page = page_at(2 * kSteps);
-    // the queries have come: else the compiler waits for them in every stage, and with them for the codes on their way
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-    for (int step = 0, i = 0; step < steps; step += kSteps, i ^= 1) {
+    page = page_at(begin + 2 * kSteps);
+    for (int step = begin, i = 0; step < steps; step += kSteps, i ^= 1) {
         __syncthreads();  // stage i is made, and the other one no longer read
+        walk_stage(step, i);
         if (step + kSteps < steps) {
             make(part, stages[i ^ 1]);
             load(part, page, step + 2 * kSteps);
             page = page_at(step + 3 * kSteps);
         }
-        const Stage8<D, NW> &st = stages[i];
-#pragma unroll
-        for (int sub = 0; sub < kSteps; ++sub) {
-            const int at = span.token_of(step + sub);
-            if (at >= mine) break;
-            if (at + 32 <= from && at >= a.sinks) continue;
-            const Page pages_of[2] = {st.pages[2 * sub], st.pages[2 * sub + 1]};
-            attend<true, D, MT>(
-                a, s, at, at + 32 > sure.limit || (at < sure.low && at + 32 > a.sinks), {false, false}, pages_of,
-                [&](int h, int k) { return __builtin_bit_cast(bf16x8, st.keys[2 * sub + h][k][lane]); },
-                [&](auto u) { return __builtin_bit_cast(halfx8, st.values[sub][u][lane]); });
-        }
     }
+    const float l = s.l + __shfl_xor(s.l, 32), inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
+    if (row >= total) return;
+    const int64_t to = out_row(a, sq, head, row);
+    // a lane's channels: D / 8 behind one another for each j
+    if (a.splits > 1) {
+        float *part_to = a.part + (to * a.splits + split) * (D + 4);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const int row = row0 + 16 * mt + n;
-        const float l = sum_over_g(s.l[mt]), inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
-        if (row >= total) continue;
-        const int64_t to = out_row(a, sq, head, row);
-        if (a.lse && g == 0) a.lse[to] = lse_of(s.m[mt], l);
-        // a lane's D / 4 channels lie behind one another
-        uint16_t *out = a.out + to * D + g * (D / 4);
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int c = 0; c < D / 4; c += 8) {
-            const auto v = [&](int e) { return s.o[mt][(c + e) % NT][(c + e) / NT] * inv; };
-            *reinterpret_cast<uint4 *>(out + c) = make_uint4(f32x2_to_bf16x2_rne(v(0), v(1)), f32x2_to_bf16x2_rne(v(2), v(3)), f32x2_to_bf16x2_rne(v(4), v(5)), f32x2_to_bf16x2_rne(v(6), v(7)));
-        }
+            for (int c = 0; c < D / 8; c += 4) {
+                const auto v = [&](int e) { return s.o[(c + e) % NT][4 * j + (c + e) / NT]; };
+                *reinterpret_cast<float4 *>(part_to + (8 * j + 4 * h) * NT + c) = make_float4(v(0), v(1), v(2), v(3));
+            }
+        if (h == 0) *reinterpret_cast<float4 *>(part_to + D) = make_float4(s.m, l, __int_as_float(used), 0.f);
+        return;
     }
+    if (a.lse && h == 0) a.lse[to] = lse_of(s.m, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < D / 8; c += 8) {
+            const auto v = [&](int e) { return s.o[(c + e) % NT][4 * j + (c + e) / NT] * inv; };
+            *reinterpret_cast<uint4 *>(a.out + to * D + (8 * j + 4 * h) * NT + c) =
+                make_uint4(f32x2_to_bf16x2_rne(v(0), v(1)), f32x2_to_bf16x2_rne(v(2), v(3)), f32x2_to_bf16x2_rne(v(4), v(5)), f32x2_to_bf16x2_rne(v(6), v(7)));
+        }
 }
 
 // Weights that the cached tokens got, from the logarithms of the rows' sums: weights[seq, head, t] += sum over the head's rows of
-// exp(score - lse).  A wave has 16 tokens' keys, as MFMA operands, and walks over the rows that see some of them; S^T = K Q^T leaves
-// each lane four tokens' sums over its rows, joined over the 16 lanes at the end.  Every sum has one writer.
-template <int D>
-__global__ __launch_bounds__(256) void kv8_attention_weights_kernel(AttnArgs8 a, float *weights, int cols, int blocks, int64_t first_block) {
-    constexpr int KS = D / 32, W = D / 64;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int64_t block = first_block + blockIdx.x;
-    const int seq = static_cast<int>(block / blocks / a.heads), head = static_cast<int>(block / blocks % a.heads);
-    const int t0 = 64 * static_cast<int>(block % blocks) + 16 * wave;
+// exp(score - lse).  Each sum has one writer.
+struct WeightArgs8 {
+    float *weights;
+    int cols;             // tokens of a row of weights
+    int blocks;           // workgroups a sequence and head
+    int64_t first_block;  // of a launch's workgroups, where one launch cannot hold them all
+};
+
+// The queries of a sequence that see some of the tokens t0 .. t1 - 1.
+struct Queries {
+    int first, end;
+};
+__device__ __forceinline__ Queries queries_that_see(const AttnArgs8 &a, const Seq &sq, int t0, int t1) {
+    const int64_t before = static_cast<int64_t>(sq.len) - sq.n;  // place of the first query
+    const int64_t i0 = a.causal ? max(t0 - before, int64_t{0}) : 0;
+    const int64_t i1 = t0 < a.sinks ? sq.n : min(static_cast<int64_t>(sq.n), static_cast<int64_t>(t1) + a.window - 1 - before);
+    return i0 < i1 ? Queries{static_cast<int>(i0), static_cast<int>(i1)} : Queries{0, 0};
+}
+
+// A workgroup has 64 tokens of a sequence and head, whose keys each wave holds as MFMA operands; its waves take the row tiles of 32 in
+// turn, each through LDS of its own, the next one's queries on their way: no barrier until the end, where the waves' sums are joined.
+// With S^T = K Q^T a lane has one row's 16 of 32 scores: -lse is one number a lane, what turns products into scores one a half of 16
+// tokens, and a score costs an fma, an exponential and an addition.
+// kByHead: a tile is 32 queries of one query head (the last one of a head reaches back over queries that it leaves out), whose rows lie a
+// stride apart; else 32 rows in order, each with a query and a head to be told apart (as many instructions again, but full tiles where
+// a sequence has few queries).
+// Queries are read by rows, 16 lanes each, and stored for operand c and half h of lanes at row r ^ (2 c + h): in order, all 16 pieces of a
+// row would lie in the same banks.
+template <int D, bool kByHead>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void kv8_attention_weights_kernel(AttnArgs8 a, WeightArgs8 wa) {
+    constexpr int KS = D / 16, W = D / 64, kLanes = D / 8, kPer = 64 / kLanes, kLoads = 32 / kPer;  // lanes a row, rows a load, loads a tile
+    __shared__ __align__(16) uintx4 staged[4][KS][64];
+    __shared__ float sums[4][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int64_t block = wa.first_block + blockIdx.x;
+    const int seq = static_cast<int>(block / a.heads / wa.blocks), head = static_cast<int>(block % a.heads);
+    // the first tokens are seen by the most rows: they come first, and the last ones beside them (one head after another: 240 us instead of
+    // 152 for a prompt of 4096 tokens)
+    const int k = static_cast<int>(block / a.heads % wa.blocks), most_heavy = (wa.blocks + 1) / 2;
+    const int t0 = 64 * (k < most_heavy ? k : wa.blocks - 1 - (k - most_heavy));
     const Seq sq = seq_of(a, seq);
-    const int most = min(sq.len, cols);
+    const int most = min(sq.len, wa.cols);
     if (t0 >= most || sq.n == 0) return;
-    const int page = scalar_load(a.table, static_cast<int64_t>(seq) * a.table_cols + (t0 >> a.page_shift));
-    if (page < 0 || page >= a.num_pages) return;
-    const uint8_t *k = a.k_codes + (kv8_row(page, head, t0 & ((1 << a.page_shift) - 1), a.heads, a.page_shift) + n) * D + 16 * g;
-    bf16x8 keys[KS];
+    const Queries who = queries_that_see(a, sq, t0, min(t0 + 64, most));
+    if (who.first >= who.end) return;
+    uintx4 keys[2][KS];
+    float kf[2][2];
+    bool live[2][2];  // of 16 tokens
+    {
+        const int32_t *table = a.table + static_cast<int64_t>(seq) * a.table_cols;
+        uintx4 codes[2][2 * W];
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(k + 64 * i);
-        keys[2 * i] = keys_bf16(w.x, w.y), keys[2 * i + 1] = keys_bf16(w.z, w.w);
+        for (int m = 0; m < 2; ++m) {
+            int64_t row[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int t = t0 + 32 * m + 16 * s, page = t < most ? scalar_load(table, t >> a.page_shift) : -1;
+                live[m][s] = page >= 0 && page < a.num_pages;
+                const int p = live[m][s] ? page : 0;
+                row[s] = kv8_row(p, head, t & ((1 << a.page_shift) - 1), a.heads, a.page_shift);
+                kf[m][s] = a.scale * scalar_load(a.k_scales, static_cast<int64_t>(p) * a.heads + head);
+            }
+            const uint8_t *from = a.k_codes + ((n & 16 ? row[1] : row[0]) + (n & 15)) * D + 16 * h;
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) codes[m][i] = *reinterpret_cast<const uintx4 *>(from + 32 * i);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) {
+                keys[m][2 * i] = __builtin_bit_cast(uintx4, keys_bf16(codes[m][i][0], codes[m][i][1]));
+                keys[m][2 * i + 1] = __builtin_bit_cast(uintx4, keys_bf16(codes[m][i][2], codes[m][i][3]));
+            }
     }
-    const float kf = a.scale * scalar_load(a.k_scales, static_cast<int64_t>(page) * a.heads + head);
-    const int before = sq.len - sq.n;  // place of the first query
-    const int i0 = a.causal ? max(t0 - before, 0) : 0;
-    const int64_t last_place = static_cast<int64_t>(t0) + 15 + a.window - 1;
-    const int i1 = t0 < a.sinks ? sq.n - 1 : static_cast<int>(min<int64_t>(sq.n - 1, last_place - before));
-    const int end = (i1 + 1) * a.ratio, hq = a.heads * a.ratio;
-    float sums[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int row = i0 * a.ratio + n; row - n < end; row += 16) {
-        const bool in = row < end;
-        const int i = in ? row / a.ratio : i1, h = head * a.ratio + (in ? row - i * a.ratio : 0);
-        const uint16_t *q = a.q + (sq.first + i) * a.q_stride + h * D;
-        const float lse = a.lse[static_cast<int64_t>(sq.first + i) * hq + h] * 1.44269504088896341f;
-        const int limit = in ? limit_of(a, sq, i) : 0, low = low_of(a, sq, i);
-        floatx4 dot = {0.f, 0.f, 0.f, 0.f};
+    const int hq = a.heads * a.ratio, of_row = lane / kLanes, piece = lane % kLanes;
+    struct RowTile {
+        uintx4 q[kLoads];
+        float lse;
+        int i;      // the lane's row's query
+        bool in;    // the row is one of the tile's
+        int i0, i1; // uniform: queries of the tile's first and last row
+    };
+    // by heads: tile `tile` of head `x`
+    const int per_head = (who.end - who.first + 31) / 32;
+    int x = 0, tile = wave;
+    int64_t at[kLoads], lse_at;
+    if constexpr (kByHead) {
+        // a sequence of fewer than 32 queries has one tile a head, from its first query on: rows past the last one are that one again
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-            dot = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[s], __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4 *>(q + 64 * (s / 2) + 16 * g + 8 * (s % 2))), dot, 0, 0, 0);
+        for (int c = 0; c < kLoads; ++c) at[c] = min(kPer * c + of_row, sq.n - 1) * a.q_stride + 8 * piece;
+        lse_at = static_cast<int64_t>(min(n, sq.n - 1)) * hq;
+    }
+    // in order: rows that go on by `step`, each a query and a head of the group
+    struct Row {
+        int i, x;
+    };
+    const int step = 32 * waves, queries = query_of(a, step), rest = step - queries * a.ratio;
+    const int first_row = who.first * a.ratio + 32 * wave;
+    const Row last{who.end - 1, a.ratio - 1};
+    Row mine, its[kLoads];
+    const auto row_at = [&](int row) {
+        const int i = query_of(a, row);
+        return Row{i, row - i * a.ratio};
+    };
+    const auto advance = [&](Row &r) {
+        r.i += queries, r.x += rest;
+        const bool over = r.x >= a.ratio;
+        r.x -= over ? a.ratio : 0, r.i += over;
+    };
+    if constexpr (!kByHead) {
+        mine = row_at(first_row + n);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int t = t0 + 4 * g + r;
-            const bool seen = t < limit && (t >= low || t < a.sinks);
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(dot[r], kf, -lse));
-            sums[r] += seen ? w : 0.f;
+        for (int c = 0; c < kLoads; ++c) its[c] = row_at(first_row + kPer * c + of_row);
+    }
+    const auto load = [&](int row0) {  // past the end: the last rows again
+        RowTile p;
+        if constexpr (kByHead) {
+            while (tile >= per_head && x < a.ratio) tile -= per_head, ++x;
+            const int from = who.first + 32 * (x < a.ratio ? tile : 0), i0 = max(min(from, who.end - 32), 0), head_x = head * a.ratio + min(x, a.ratio - 1);
+            const uint16_t *q = a.q + (sq.first + i0) * a.q_stride + head_x * D;
+#pragma unroll
+            for (int c = 0; c < kLoads; ++c) p.q[c] = *reinterpret_cast<const uintx4 *>(q + at[c]);
+            p.lse = a.lse[static_cast<int64_t>(sq.first + i0) * hq + head_x + lse_at];
+            p.i = i0 + n, p.in = p.i >= from && p.i < who.end;
+            p.i0 = i0, p.i1 = min(i0 + 31, sq.n - 1);
+            tile += waves;
+        } else {
+#pragma unroll
+            for (int c = 0; c < kLoads; ++c) {
+                const Row r = its[c].i < who.end ? its[c] : last;
+                p.q[c] = *reinterpret_cast<const uintx4 *>(a.q + (sq.first + r.i) * a.q_stride + (head * a.ratio + r.x) * D + 8 * piece);
+                advance(its[c]);
+            }
+            p.in = mine.i < who.end;
+            const Row r = p.in ? mine : last;
+            p.lse = a.lse[static_cast<int64_t>(sq.first + r.i) * hq + head * a.ratio + r.x];
+            p.i = r.i;
+            p.i0 = query_of(a, row0), p.i1 = min(query_of(a, row0 + 31), who.end - 1);
+            advance(mine);
+        }
+        return p;
+    };
+    // this wave's tiles
+    const int tiles = kByHead ? per_head * a.ratio : ((who.end - who.first) * a.ratio + 31) / 32;
+    float sum[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) sum[i] = 0.f;
+    RowTile next = load(first_row);
+    for (int done = wave, row0 = first_row; done < tiles; done += waves) {
+        wave_order();
+        // channels 8 e ..: of the MFMAs' 32 channels e / 4, half e / 2 % 2, the first or second of two
+        const int c_of = piece / 4 * 2 + piece % 2, h_of = piece / 2 % 2;
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) staged[wave][c_of][32 * h_of + ((kPer * c + of_row) ^ (2 * c_of + h_of))] = next.q[c];
+        const float minus_lse = next.in ? next.lse * -1.44269504088896341f : -INFINITY;  // rows past the end: no weight
+        const int limit = limit_of(a, sq, next.i), low = low_of(a, sq, next.i);
+        // uniform: every row of the tile sees every token
+        const bool all = t0 + 64 <= limit_of(a, sq, next.i0) && (t0 >= low_of(a, sq, next.i1) || t0 + 64 <= a.sinks);
+        row0 += step;
+        next = load(row0);
+        wave_order();
+        uintx4 q[KS];
+#pragma unroll
+        for (int c = 0; c < KS; ++c) q[c] = staged[wave][c][32 * h + (n ^ (2 * c + h))];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            floatx16 dot;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dot[i] = 0.f;
+#pragma unroll
+            for (int c = 0; c < KS; ++c) dot = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, keys[m][c]), __builtin_bit_cast(bf16x8, q[c]), dot, 0, 0, 0);
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(dot[i], kf[m][i / 8], minus_lse));
+            if (!all) {
+                int first = t0 + 32 * m + 4 * h;
+                asm volatile("" : "+v"(first));  // a branch: the comparisons stay in it
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int t = first + 8 * (i / 4) + i % 4;
+                    w[i] = (t >= limit) | ((t < low) & (t >= a.sinks)) ? 0.f : w[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[16 * m + i] += w[i];
         }
     }
+    // over the 32 lanes of a half: each step halves the sums a lane has; lane n keeps number n
+    static_for<5>([&](auto s) __attribute__((always_inline)) {
+        constexpr int o = 16 >> s;
+        const bool up = n & o;
+        static_for<o>([&](auto i) __attribute__((always_inline)) {
+            const float kept = up ? sum[i + o] : sum[i], given = up ? sum[i] : sum[i + o];
+            sum[i] = kept + __shfl_xor(given, o);
+        });
+    });
+    const int of = 32 * (n / 16) + 8 * (n / 4 % 4) + 4 * h + n % 4;  // its token
+    sums[wave][of] = sum[0];
+    __syncthreads();
+    const int t = t0 + static_cast<int>(threadIdx.x);
+    if (threadIdx.x < 64 && t < most && (threadIdx.x < 32 ? threadIdx.x < 16 ? live[0][0] : live[0][1] : threadIdx.x < 48 ? live[1][0] : live[1][1])) {
+        float v = 0.f;
+        for (int w = 0; w < waves; ++w) v += sums[w][threadIdx.x];
+        float *p = wa.weights + (static_cast<int64_t>(seq) * a.heads + head) * wa.cols + t;
+        *p += v;
+    }
+}
+
+// The same where the kernel of few rows has left its scores (base 2), [rows][score_cols] from the first row of the sequence and head on:
+// four tokens a lane.
+__global__ __launch_bounds__(256) void kv8_attention_scored_kernel(AttnArgs8 a, WeightArgs8 wa) {
+    const int64_t block = wa.first_block + blockIdx.x;
+    const int seq = static_cast<int>(block / wa.blocks / a.heads), head = static_cast<int>(block / wa.blocks % a.heads);
+    const Seq sq = seq_of(a, seq);
+    const int most = min(sq.len, wa.cols), t = 1024 * static_cast<int>(block % wa.blocks) + 4 * static_cast<int>(threadIdx.x), hq = a.heads * a.ratio;
+    if (t >= most || sq.n == 0) return;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    bool seen = false;
+    for (int i = 0; i < sq.n; ++i) {
+        const int limit = limit_of(a, sq, i), low = low_of(a, sq, i);
+        if (t >= limit || (t + 4 <= low && t >= a.sinks)) continue;
+        seen = true;
+        for (int x = 0; x < a.ratio; ++x) {
+            const int64_t row = static_cast<int64_t>(sq.first + i) * hq + head * a.ratio + x;
+            const floatx4 y = *reinterpret_cast<const floatx4 *>(a.scores + row * a.score_cols + t);
+            const float lse = a.lse[row] * 1.44269504088896341f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        float v = sums[r];
-        v += lane_xor<1>(v);
-        v += lane_xor<2>(v);
-        v += lane_xor<4>(v);
-        v += lane_xor<8>(v);
-        const int t = t0 + 4 * g + r;
-        if (n == 0 && t < most) {
-            float *p = weights + (static_cast<int64_t>(seq) * a.heads + head) * cols + t;
-            *p += v;
+            for (int r = 0; r < 4; ++r)
+                sum[r] += (t + r >= limit) | ((t + r < low) & (t + r >= a.sinks)) ? 0.f : __builtin_amdgcn_exp2f(y[r] - lse);
         }
     }
+    float *p = wa.weights + (static_cast<int64_t>(seq) * a.heads + head) * wa.cols + t;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (seen && t + r < most) p[r] += sum[r];
 }
 
 // How a call is laid out: rows a wave (16 mt), whether waves share rows (splits of the tokens) or have their own, row
@@ -670,27 +1057,38 @@ struct Plan {
     int mt, waves;
     bool rows;
     int64_t tiles, splits, bytes;
+    bool scored;           // weights: the kernel of few rows leaves its scores in the workspace, behind the splits' sums
+    int64_t score_cols, scores_at;  // scores_at: bytes before them
 };
 
-Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols, bool varlen, int64_t window, int64_t sinks) {
-    Plan p{1, 4, false, 0, 1, 0};
+Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols, bool varlen, int64_t window, int64_t sinks, bool weights) {
+    Plan p{1, 4, false, 0, 1, 0, false, 0, 0};
     if (tokens == 0 || batch == 0) return p;
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio, each = (rows + batch - 1) / batch;
     const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
-    p.rows = varlen && rows / 32 * c->kv_heads >= 6 * cus;
+    const int64_t len = std::min(table_cols * c->page_size, window + sinks + 64 + tokens), row = (c->head_dim + 4) * 4;
+    const auto split_to = [&](int64_t splits, int64_t least) {
+        p.splits = std::max<int64_t>(1, std::min(splits, len / least));
+        p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
+        if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
+    };
+    p.rows = varlen && each >= (c->head_dim == 128 ? 64 : 512);
     if (p.rows) {
-        p.mt = 2;
-        if (rows / (128 * p.mt) * c->kv_heads >= 2 * cus) p.waves = 8;
-        p.tiles = tiles(16 * p.waves * p.mt);
+        const int64_t tasks = batch * ((each + 255) / 256) * c->kv_heads, splits = cus / tasks;
+        p.waves = 8;
+        split_to(splits > 2 ? splits : 1, 256);
+        if (p.splits == 1 && tasks < cus && each > 128) p.waves = 4;
+        p.tiles = tiles(32 * p.waves);
         return p;
     }
     p.mt = each <= 96 ? 1 : 2;
     p.tiles = tiles(16 * p.mt);
-    const int64_t tasks = p.tiles * c->kv_heads, len = std::min(table_cols * c->page_size, window + sinks + 64 + tokens);
-    p.splits = std::max<int64_t>(1, std::min((2 * cus + tasks - 1) / tasks, (len + 127) / 128));
-    const int64_t row = (c->head_dim + 4) * 4;
-    p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
-    if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
+    const int64_t tasks = p.tiles * c->kv_heads;
+    split_to((2 * cus + tasks - 1) / tasks, 128);
+    p.score_cols = table_cols * c->page_size;
+    p.scored = weights && each <= 8 && tokens * q_heads * p.score_cols <= int64_t{64} << 20;
+    p.scores_at = p.bytes;
+    if (p.scored) p.bytes += 4 * tokens * q_heads * p.score_cols;
     return p;
 }
 
@@ -713,10 +1111,18 @@ void launch_split(AttnArgs8 a, const Plan &p, hipStream_t st) {
         kv8_attention_split_kernel<D, MT, NW><<<dim3(grid), dim3(64 * NW), lds, st>>>(a);
         check_launch("kv8_attention_split");
     });
-    if (p.splits > 1) {
-        kv8_attention_join_kernel<D><<<dim3(static_cast<unsigned>(static_cast<int64_t>(a.tokens) * a.heads * a.ratio)), dim3(256), 0, st>>>(a);
-        check_launch("kv8_attention_join");
+}
+
+template <int D>
+void launch_join(const AttnArgs8 &a, hipStream_t st) {
+    const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads * a.ratio;
+    if (rows >= 1024) {
+        constexpr int per = 1024 / D;
+        kv8_attention_join_rows_kernel<D><<<dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, st>>>(a);
+    } else {
+        kv8_attention_join_kernel<D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, st>>>(a);
     }
+    check_launch("kv8_attention_join");
 }
 
 template <int D, int NW>
@@ -726,7 +1132,7 @@ void launch_tile(AttnArgs8 a, const Plan &p, hipStream_t st) {
     static std::atomic<uint64_t> attr_devices{0};
     const auto kern = kv8_attention_tile_kernel<D, NW>;
     raise_lds_limit(reinterpret_cast<const void *>(kern), lds, attr_devices);
-    for_tiles(a, p, a.heads, 64 * NW, [&](unsigned grid) {
+    for_tiles(a, p, a.heads * p.splits, 64 * NW, [&](unsigned grid) {
         kern<<<dim3(grid), dim3(64 * NW), lds, st>>>(a, static_cast<int>(p.tiles));
         check_launch("kv8_attention_tile");
     });
@@ -754,12 +1160,13 @@ using namespace cfh;
 extern "C" {
 
 int32_t castforge_hip_kv8_attention_workspace(const cfh_kv8_cache_t *cache, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols,
-                                              int32_t varlen, int64_t window, int64_t sinks, int64_t *out_bytes, char **out_error) {
+                                              int32_t varlen, int64_t window, int64_t sinks, int32_t weights,
+                                              int64_t *out_bytes, char **out_error) {
     if (out_bytes) *out_bytes = 0;
     return guarded(out_error, [&] {
         check_attention(cache, tokens, q_heads, batch, table_cols, window, sinks);
         require(out_bytes != nullptr, "out_bytes must not be NULL");
-        *out_bytes = plan_of(cache, tokens, q_heads, batch, table_cols, varlen != 0, window_of(window), sinks).bytes;
+        *out_bytes = plan_of(cache, tokens, q_heads, batch, table_cols, varlen != 0, window_of(window), sinks, weights != 0).bytes;
     });
 }
 
@@ -780,28 +1187,40 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
         require(tokens <= 1 || (q_stride >= q_heads * cache->head_dim && q_stride % 8 == 0),
                 "q's token stride must be a multiple of 8 and at least q_heads * head_dim");
         if (batch == 0) return;
-        const Plan p = plan_of(cache, tokens, q_heads, batch, table_cols, cu_q != nullptr, window_of(window), sinks);
+        const Plan p = plan_of(cache, tokens, q_heads, batch, table_cols, cu_q != nullptr, window_of(window), sinks, weights != nullptr);
         require(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 16)),
                 "workspace must be 16-byte aligned and hold the bytes that castforge_hip_kv8_attention_workspace gives");
         AttnArgs8 a{q, q_stride, cache->k_codes, cache->v_codes, cache->k_scales, cache->v_scales, cu_q, page_table, kv_lens, out, lse,
                     static_cast<float *>(workspace), scale * 1.44269504088896341f, static_cast<int>(tokens), static_cast<int>(batch),
                     static_cast<int>(cache->kv_heads), static_cast<int>(q_heads / cache->kv_heads), kv8_log2(cache->page_size),
                     static_cast<int>(table_cols), static_cast<int>(cache->num_pages), causal, static_cast<int>(p.splits),
-                    static_cast<int>(window_of(window)), static_cast<int>(sinks), 0};
+                    static_cast<int>(window_of(window)), static_cast<int>(sinks), 0, 0,
+                    p.scored ? static_cast<float *>(workspace) + p.scores_at / 4 : nullptr, static_cast<int>(p.score_cols), 0};
+        const int l = a.ratio > 1 ? kv8_log2(a.ratio - 1) + 1 : 0;  // ceil(log2 ratio)
+        a.ratio_shift = 31 + l, a.ratio_mul = static_cast<uint32_t>(((uint64_t{1} << a.ratio_shift) + a.ratio - 1) / a.ratio);
         const hipStream_t st = static_cast<hipStream_t>(stream);
         const auto launch = [&](auto d) {
             constexpr int D = decltype(d)::value;
             if (p.rows) p.waves == 8 ? launch_tile<D, 8>(a, p, st) : launch_tile<D, 4>(a, p, st);
             else p.mt == 1 ? launch_split<D, 1, 4>(a, p, st) : launch_split<D, 2, 4>(a, p, st);
+            if (p.splits > 1) launch_join<D>(a, st);
         };
         cache->head_dim == 64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
-        const int64_t reach = std::min(weights ? weights_cols : 0, table_cols * cache->page_size), blocks = (reach + 63) / 64;
-        const int64_t all = blocks * batch * cache->kv_heads;
-        for (int64_t b = 0, most = most_workgroups(256); b < all; b += most) {
-            const dim3 grid(static_cast<unsigned>(std::min(all - b, most)));
-            const auto kern = cache->head_dim == 64 ? kv8_attention_weights_kernel<64> : kv8_attention_weights_kernel<128>;
-            kern<<<grid, dim3(256), 0, st>>>(a, weights, static_cast<int>(weights_cols), static_cast<int>(blocks), b);
-            check_launch("kv8_attention_weights");
+        if (weights) {
+            const int64_t each = p.scored ? 1024 : 64, blocks = (std::min(weights_cols, table_cols * cache->page_size) + each - 1) / each;
+            WeightArgs8 wa{weights, static_cast<int>(weights_cols), static_cast<int>(blocks), 0};
+            // a wave for each tile of 32 rows that a sequence has, up to four
+            const int64_t rows = (tokens * a.ratio + batch - 1) / batch, threads = p.scored || rows > 64 ? 256 : rows > 32 ? 128 : 64;
+            const int64_t all = blocks * batch * cache->kv_heads, most = most_workgroups(threads);
+            for (; wa.first_block < all; wa.first_block += most) {
+                const dim3 grid(static_cast<unsigned>(std::min(all - wa.first_block, most)));
+                const bool by_head = tokens >= 32 * batch;
+                const auto kern = p.scored ? kv8_attention_scored_kernel
+                    : cache->head_dim == 64 ? by_head ? kv8_attention_weights_kernel<64, true> : kv8_attention_weights_kernel<64, false>
+                    : by_head ? kv8_attention_weights_kernel<128, true> : kv8_attention_weights_kernel<128, false>;
+                kern<<<grid, dim3(static_cast<unsigned>(threads)), 0, st>>>(a, wa);
+                check_launch("kv8_attention_weights");
+            }
         }
     });
 }

@@ -203,7 +203,7 @@ SIGNATURES = {
                                               c_int64, _P, c_int32, c_int64, c_int64, ctypes.c_float, _P, _P, _P, c_int64, _P,
                                               c_int64, _P, _E]),
     "castforge_hip_kv8_attention_workspace": (c_int32, [POINTER(Kv8CacheStruct), c_int64, c_int64, c_int64, c_int64,
-                                                        c_int32, c_int64, c_int64, POINTER(c_int64), _E]),
+                                                        c_int32, c_int64, c_int64, c_int32, POINTER(c_int64), _E]),
     "castforge_hip_kv8_evict": (c_int32, [POINTER(Kv8CacheStruct), _P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int64,
                                           _P, c_int64, _P, _P, _P, _P, _E]),
 }

@@ -1299,12 +1299,12 @@ def kv8_gather(cache: Kv8Cache, slots: torch.Tensor, out_dtype: torch.dtype = to
 
 @functools.lru_cache(maxsize=4096)
 def _kv8_workspace(device: int, kv_heads: int, page_size: int, head_dim: int, tokens: int, q_heads: int, batch: int, cols: int, varlen: int,
-                   window: int, sinks: int) -> int:
+                   window: int, sinks: int, weights: int) -> int:
     """castforge_hip_kv8_attention_workspace's bytes, which depend on sizes alone."""
     size = ctypes.c_int64()
     shape = ffi.Kv8CacheStruct(None, None, None, None, 0, kv_heads, page_size, head_dim)
     _call_on(device, "castforge_hip_kv8_attention_workspace", ctypes.byref(shape), tokens, q_heads, batch, cols, varlen, window, sinks,
-             ctypes.byref(size))
+             weights, ctypes.byref(size))
     return size.value
 
 
@@ -1340,7 +1340,7 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, page_table: torch.Tensor, kv
         wp, wcols = weights.data_ptr(), weights.shape[2]
     out = torch.empty_strided(shape, (hq * d, d, 1), dtype=torch.bfloat16, device=q.device)
     lse = torch.empty_strided((t, hq), (hq, 1), dtype=torch.float32, device=q.device) if return_lse or weights is not None else None
-    size = _kv8_workspace(dev, heads, cache.page_size, d, t, hq, b, cols, 0 if cp is None else 1, window, sinks)
+    size = _kv8_workspace(dev, heads, cache.page_size, d, t, hq, b, cols, 0 if cp is None else 1, window, sinks, 0 if wp is None else 1)
     ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=q.device) if size else None  # held until the call returns
     _call_on(dev, "castforge_hip_kv8_attention", cache._ref, q.data_ptr(), qs, t, hq, b, cp, page_table.data_ptr(), cols, lp, int(causal),
              window, sinks, d ** -0.5 if scale is None else scale, out.data_ptr(), _ptr(lse), wp, wcols, _ptr(ws), size, _stream(q))

@@ -641,10 +641,10 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
                                     int64_t table_cols, const int32_t *kv_lens, int32_t causal, int64_t window, int64_t sinks,
                                     float scale, uint16_t *out, float *lse, float *weights, int64_t weights_cols, void *workspace,
                                     int64_t workspace_bytes, void *stream, char **out_error);
-/* varlen: whether cu_q will be given. */
+/* varlen, weights: whether cu_q and weights will be given. */
 int32_t castforge_hip_kv8_attention_workspace(const cfh_kv8_cache_t *cache, int64_t tokens, int64_t q_heads, int64_t batch,
-                                              int64_t table_cols, int32_t varlen, int64_t window, int64_t sinks, int64_t *out_bytes,
-                                              char **out_error);
+                                              int64_t table_cols, int32_t varlen, int64_t window, int64_t sinks, int32_t weights,
+                                              int64_t *out_bytes, char **out_error);
 
 /* Cuts each sequence and head to its `keep` tokens of greatest weight.  Of sequence b with L = kv_lens[b] tokens in the pages
  * of page_table, every head keeps all if L <= keep, else the first `sinks`, the last `recent` and, of those between, the ones of greatest

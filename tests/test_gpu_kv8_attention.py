@@ -272,7 +272,7 @@ def test_rows_of_no_sequence_are_left_alone(cuda):
         padded = torch.cat([q, torch.full((5, *q.shape[1:]), math.nan, dtype=q.dtype, device=cuda)])
         t, hq, d = padded.shape
         out, lse = torch.full_like(padded, 7.0), torch.full((t, hq), 7.0, device=cuda)
-        size = ops._kv8_workspace(0, 8, 16, 64, t, hq, 2, table.shape[1], 1, 0, 0)
+        size = ops._kv8_workspace(0, 8, 16, 64, t, hq, 2, table.shape[1], 1, 0, 0, 0)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=cuda)
         ffi.call("castforge_hip_kv8_attention", cache._ref, padded.data_ptr(), hq * d, t, hq, 2, cu.data_ptr(), table.data_ptr(), table.shape[1],
                  lens.data_ptr(), 1, 0, 0, d ** -0.5, out.data_ptr(), lse.data_ptr(), None, 0, ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)

@@ -99,7 +99,7 @@ def _evict(cache=None, table=16, cols=4, lens=16, b=1, w=16, wcols=64, keep=20, 
     (_evict(w=None), "NULL"),
     (_evict(kept=None), "NULL"),
     (_evict(nlens=None), "NULL"),
-    (("castforge_hip_kv8_attention_workspace", _cache(), 1, 4, 1, 4, 0, 0, 0, None), "out_bytes"),
+    (("castforge_hip_kv8_attention_workspace", _cache(), 1, 4, 1, 4, 0, 0, 0, 0, None), "out_bytes"),
 ])
 def test_invalid_arguments_report_status_1(call, needle):
     rc, msg = _status(*call)
