@@ -195,7 +195,7 @@ __device__ __forceinline__ Page page_of(float scale, float ks, float vs) {
 // 11 bits down to 2^-21 of them), and the rescaling is rare.
 // keys(h, i): the MFMA operand of half h's 16 tokens and 32 channels; values(u): that of 16 channels and 32 tokens.  gone: a half's
 // page is none of the cache's; edge, uniform: so, or some row does not see some token.
-template <int D, int MT, class Keys, class Values>
+template <bool kScored, int D, int MT, class Keys, class Values>
 __device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int at, bool edge, const bool (&gone)[2], const Page (&pages)[2], float *const (&score_rows)[MT], const Keys &keys, const Values &values) {
     constexpr int KS = D / 32, NT = D / 16;
     const int g = (threadIdx.x >> 4) & 3;
@@ -230,7 +230,7 @@ __device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int 
             }
         }
     }
-    if (a.scores) {  // uniform; scores of what a row does not see are not read, but for those of no page: -inf
+    if constexpr (kScored) {  // scores of what a row does not see are not read, but for those of no page: -inf
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -278,7 +278,7 @@ __device__ __forceinline__ int64_t out_row(const AttnArgs8 &a, const Seq &sq, in
 }
 
 // A wave's walk over steps first, first + by, .. below last of a span, the next tile's loads in flight.
-template <int D, int MT>
+template <bool kScored, int D, int MT>
 __device__ __forceinline__ void walk(const AttnArgs8 &a, Rows8<D, MT> &s, const Seq &sq, int head, const Span &span, int row0, int first, int by, int last) {
     if (first >= last) return;
     constexpr int W = Tile8<D>::W;
@@ -289,7 +289,7 @@ __device__ __forceinline__ void walk(const AttnArgs8 &a, Rows8<D, MT> &s, const 
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int row = row0 + 16 * mt + (lane & 15);
-        score_rows[mt] = a.scores && row < sq.n * a.ratio ? a.scores + out_row(a, sq, head, row) * a.score_cols + 4 * g : nullptr;
+        score_rows[mt] = kScored && row < sq.n * a.ratio ? a.scores + out_row(a, sq, head, row) * a.score_cols + 4 * g : nullptr;
     }
     const auto pages = [&](int step, int (&p)[2]) {
         const int at = span.token_of(step);
@@ -323,7 +323,7 @@ __device__ __forceinline__ void walk(const AttnArgs8 &a, Rows8<D, MT> &s, const 
         }
         const Page pages_of[2] = {page_of(a.scale, cur.ks[0], cur.vs[0]), page_of(a.scale, cur.ks[1], cur.vs[1])};
         const bool gone[2] = {!cur.live[0], !cur.live[1]}, edge = apart || at + 32 > sure.limit || (at < sure.low && at + 32 > a.sinks);
-        attend<D, MT>(
+        attend<kScored, D, MT>(
             a, s, at, edge, gone, pages_of, score_rows,
             [&](int h, int i) {
                 const uint4 w = cur.k[h][i / 2];
@@ -358,8 +358,8 @@ struct SplitLds8 {
     float m[NW][16], l[NW][16];
 };
 
-template <int D, int MT, int NW>
-__global__ __launch_bounds__(64 * NW) void kv8_attention_split_kernel(AttnArgs8 a) {
+template <bool kScored, int D, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(MT == 1 ? 3 : 2))) void kv8_attention_split_kernel(AttnArgs8 a) {
     extern __shared__ __align__(16) uint8_t lds[];
     SplitLds8<D, NW> &sh = *reinterpret_cast<SplitLds8<D, NW> *>(lds);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * NW) void kv8_attention_split_kernel(AttnArgs8 
     Rows8<D, MT> s;
     load_rows(a, s, sq, head, row0);
     // shares are rounded up: the last ones may be empty
-    walk<D, MT>(a, s, sq, head, span, row0, split * share + wave, NW, min(steps, (split + 1) * share));
+    walk<kScored, D, MT>(a, s, sq, head, span, row0, split * share + wave, NW, min(steps, (split + 1) * share));
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (16 * mt >= rows) break;
@@ -1103,12 +1103,12 @@ void for_tiles(AttnArgs8 &a, const Plan &p, int64_t each, int threads, const F &
     }
 }
 
-template <int D, int MT, int NW>
+template <bool kScored, int D, int MT, int NW>
 void launch_split(AttnArgs8 a, const Plan &p, hipStream_t st) {
     constexpr int lds = sizeof(SplitLds8<D, NW>);
     static_assert(lds <= 64 * 1024, "LDS budget");
     for_tiles(a, p, a.heads * p.splits, 64 * NW, [&](unsigned grid) {
-        kv8_attention_split_kernel<D, MT, NW><<<dim3(grid), dim3(64 * NW), lds, st>>>(a);
+        kv8_attention_split_kernel<kScored, D, MT, NW><<<dim3(grid), dim3(64 * NW), lds, st>>>(a);
         check_launch("kv8_attention_split");
     });
 }
@@ -1202,7 +1202,8 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
         const auto launch = [&](auto d) {
             constexpr int D = decltype(d)::value;
             if (p.rows) p.waves == 8 ? launch_tile<D, 8>(a, p, st) : launch_tile<D, 4>(a, p, st);
-            else p.mt == 1 ? launch_split<D, 1, 4>(a, p, st) : launch_split<D, 2, 4>(a, p, st);
+            else if (p.scored) launch_split<true, D, 1, 4>(a, p, st);  // 8 rows a sequence and head: one row tile
+            else p.mt == 1 ? launch_split<false, D, 1, 4>(a, p, st) : launch_split<false, D, 2, 4>(a, p, st);
             if (p.splits > 1) launch_join<D>(a, st);
         };
         cache->head_dim == 64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
