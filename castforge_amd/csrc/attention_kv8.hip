@@ -359,7 +359,7 @@ struct SplitLds8 {
 };
 
 template <bool kScored, int D, int MT, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(MT == 1 ? 3 : 2))) void kv8_attention_split_kernel(AttnArgs8 a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW > 4 ? NW / 4 : MT == 1 ? 3 : 2))) void kv8_attention_split_kernel(AttnArgs8 a) {
     extern __shared__ __align__(16) uint8_t lds[];
     SplitLds8<D, NW> &sh = *reinterpret_cast<SplitLds8<D, NW> *>(lds);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1055,14 +1055,14 @@ __global__ __launch_bounds__(256) void kv8_attention_scored_kernel(AttnArgs8 a, 
 // tiles at most, splits, workspace.
 struct Plan {
     int mt, waves;
-    bool rows;
+    bool rows, wide;       // wide: more waves a workgroup in place of splits
     int64_t tiles, splits, bytes;
     bool scored;           // weights: the kernel of few rows leaves its scores in the workspace, behind the splits' sums
     int64_t score_cols, scores_at;  // scores_at: bytes before them
 };
 
 Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t batch, int64_t table_cols, bool varlen, int64_t window, int64_t sinks, bool weights) {
-    Plan p{1, 4, false, 0, 1, 0, false, 0, 0};
+    Plan p{1, 4, false, false, 0, 1, 0, false, 0, 0};
     if (tokens == 0 || batch == 0) return p;
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio, each = (rows + batch - 1) / batch;
     const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
@@ -1084,9 +1084,14 @@ Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     p.mt = each <= 96 ? 1 : 2;
     p.tiles = tiles(16 * p.mt);
     const int64_t tasks = p.tiles * c->kv_heads;
-    split_to((2 * cus + tasks - 1) / tasks, 128);
     p.score_cols = table_cols * c->page_size;
     p.scored = weights && each <= 8 && tokens * q_heads * p.score_cols <= int64_t{64} << 20;
+    // A short table and few workgroups: one launch of wide workgroups, four rounds of 32 tokens a wave at most, no partial sums.  One
+    // sequence of 1009 tokens, 8 heads of 128: 11.7 us a call against 15.7 with splits and their join, whose second launch costs the host more
+    // than the longer walk costs the GPU (10.3 against 7.4 us there); 32 sequences of 1000 16.3 against 18.2 there.  At 2000 tokens one
+    // sequence takes 16.1 against 8.0 there.  (Sixteen waves spill: 14.5 for 1009 tokens.)
+    p.wide = p.mt == 1 && tasks <= cus && len <= 1024;
+    if (!p.wide) split_to((2 * cus + tasks - 1) / tasks, 128);
     p.scores_at = p.bytes;
     if (p.scored) p.bytes += 4 * tokens * q_heads * p.score_cols;
     return p;
@@ -1106,7 +1111,9 @@ void for_tiles(AttnArgs8 &a, const Plan &p, int64_t each, int threads, const F &
 template <bool kScored, int D, int MT, int NW>
 void launch_split(AttnArgs8 a, const Plan &p, hipStream_t st) {
     constexpr int lds = sizeof(SplitLds8<D, NW>);
-    static_assert(lds <= 64 * 1024, "LDS budget");
+    static_assert(lds <= 160 * 1024, "LDS budget");
+    static std::atomic<uint64_t> attr_devices{0};
+    if (lds > 64 * 1024) raise_lds_limit(reinterpret_cast<const void *>(kv8_attention_split_kernel<kScored, D, MT, NW>), lds, attr_devices);
     for_tiles(a, p, a.heads * p.splits, 64 * NW, [&](unsigned grid) {
         kv8_attention_split_kernel<kScored, D, MT, NW><<<dim3(grid), dim3(64 * NW), lds, st>>>(a);
         check_launch("kv8_attention_split");
@@ -1202,6 +1209,7 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
         const auto launch = [&](auto d) {
             constexpr int D = decltype(d)::value;
             if (p.rows) p.waves == 8 ? launch_tile<D, 8>(a, p, st) : launch_tile<D, 4>(a, p, st);
+            else if (p.wide) p.scored ? launch_split<true, D, 1, 8>(a, p, st) : launch_split<false, D, 1, 8>(a, p, st);
             else if (p.scored) launch_split<true, D, 1, 4>(a, p, st);  // 8 rows a sequence and head: one row tile
             else p.mt == 1 ? launch_split<false, D, 1, 4>(a, p, st) : launch_split<false, D, 2, 4>(a, p, st);
             if (p.splits > 1) launch_join<D>(a, st);
