@@ -102,11 +102,11 @@ __device__ __forceinline__ void unpack8(const uint4 &w, float (&x)[8]) {
 // What turns a lane's eight channels, piece * 8 on, of a token at a position.
 struct Turn {
     float c[8], t[8];  // cosines and sines of the lane's channels, the sine's sign taken in
-    __device__ __forceinline__ void load(const AppendArgs8 &a, int64_t token, int piece) {
+    __device__ __forceinline__ void load(const AppendArgs8 &a, int64_t position, int piece) {
         const int half = a.rot / 2;
         const bool low = 8 * piece < half;
         // a position outside the table takes its nearest row
-        const int64_t pos = min(max(a.positions[token], int64_t{0}), a.max_pos - 1);
+        const int64_t pos = min(max(position, int64_t{0}), a.max_pos - 1);
         const float *cp = a.cos + pos * half, *sp = a.sin + pos * half;
         if (a.interleaved) {
             const float4 cc = *reinterpret_cast<const float4 *>(cp + 4 * piece), ss = *reinterpret_cast<const float4 *>(sp + 4 * piece);
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs8 a) {
         const int token = static_cast<int>(block - a.kv_blocks);
         if (token >= (a.cu_q ? a.cu_q[a.batch] : a.tokens)) return;  // of no sequence
         Turn turn;
-        if (turns) turn.load(a, token, piece);
+        if (turns) turn.load(a, a.positions[token], piece);
         for (int h = local; h < a.q_heads; h += kRows) {
             const uint16_t *src = a.q + token * a.q_stride + h * D;
             float x[8];
@@ -175,22 +175,27 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs8 a) {
     const float old = u.lo > 0 ? *scale_at : 0.f;
     const int count = u.hi - u.lo;
     float x[NP][8], top = 0.f;
-    const uint16_t *rows = is_v ? a.v + head * D : a.k + head * D;
+    const uint16_t *rows = (is_v ? a.v + head * D : a.k + head * D) + 8 * piece;
     const int64_t stride = is_v ? a.v_stride : a.k_stride;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int r = j * kRows + local;
-        if (r < count) {
-            const uint16_t *src = rows + (u.row + r) * stride;
-            unpack8(load_once(src + 8 * piece), x[j]);
-            if (turns && !is_v) {
-                Turn turn;
-                turn.load(a, u.row + r, piece);
-                turn.apply(a, a.interleaved ? uint4{} : *reinterpret_cast<const uint4 *>(src + 8 * other), x[j]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));  // NaN: left out
+        // rows past the last one are that one again: under a branch each load would wait for itself (prompt of 4096 tokens 64 -> 57 us with
+        // the read-back; four rounds' loads at once: 73, three waves a SIMD instead of seven)
+        const int r = j * kRows + local, at = u.row + min(r, count - 1);
+        if (j * kRows >= count) break;
+        const uint4 own = load_once(rows + at * stride);
+        if (turns && !is_v) {
+            const int64_t position = a.positions[at];
+            const uint4 partner = a.interleaved ? uint4{} : *reinterpret_cast<const uint4 *>(rows + at * stride + 8 * (other - piece));
+            Turn turn;
+            turn.load(a, position, piece);
+            unpack8(own, x[j]);
+            turn.apply(a, partner, x[j]);
+        } else {
+            unpack8(own, x[j]);
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));  // NaN: left out
     }
     top = wave_max<64>(top);
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
@@ -205,21 +210,24 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs8 a) {
             *p = make_uint2(e4m3x4_by(p->x, ratio), e4m3x4_by(p->y, ratio));
         }
     }
-    const bool power = (__float_as_uint(scale) & 0x7fffffu) == 0;
-    const float inv = 1.0f / scale;
+    const auto store = [&](const auto &quotient) {
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int r = j * kRows + local;
-        if (r < count) {
-            float y[8];
+        for (int j = 0; j < NP; ++j) {
+            const int r = j * kRows + local;
+            if (r < count) {
+                float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = power ? x[j][i] * inv : x[j][i] / scale;  // the same number
-                y[i] = v != v ? 0.f : __builtin_amdgcn_fmed3f(v, -448.f, 448.f);
+                for (int i = 0; i < 8; ++i) {
+                    const float v = quotient(x[j][i]);
+                    y[i] = v != v ? 0.f : __builtin_amdgcn_fmed3f(v, -448.f, 448.f);
+                }
+                *reinterpret_cast<uint2 *>(codes + (u.lo + r) * D) = make_uint2(f32_to_e4m3x4(y), f32_to_e4m3x4(y + 4));
             }
-            *reinterpret_cast<uint2 *>(codes + (u.lo + r) * D) = make_uint2(f32_to_e4m3x4(y), f32_to_e4m3x4(y + 4));
         }
-    }
+    };
+    const float inv = 1.0f / scale;
+    if ((__float_as_uint(scale) & 0x7fffffu) == 0) store([&](float v) { return v * inv; });  // a power of two: the same number
+    else store([&](float v) { return v / scale; });
 }
 
 // Rows of the cache as numbers, a workgroup a token, eight elements a lane; a slot outside the cache gives zeros.
@@ -240,7 +248,9 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(const uint8_t *__restri
         const int head = is_v ? u - heads : u;
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (kept) {
-            const uint2 w = *reinterpret_cast<const uint2 *>((is_v ? v_codes : k_codes) + kv8_row(page, head, at, heads, page_shift) * D + 8 * piece);
+            // past the caches, which hold what is written: 61006 tokens of 8 heads after their move 155 -> 125 us together
+            typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+            const uintx2 w = __builtin_nontemporal_load(reinterpret_cast<const uintx2 *>((is_v ? v_codes : k_codes) + kv8_row(page, head, at, heads, page_shift) * D + 8 * piece));
             const float scale = (is_v ? v_scales : k_scales)[page * heads + head];
             e4m3x4_to_f32(w.x, x), e4m3x4_to_f32(w.y, x + 4);
 #pragma unroll
@@ -304,9 +314,12 @@ __device__ __forceinline__ uint2 sums_before(uint32_t a, uint32_t b, uint2 *wave
 // Which tokens of a sequence and head are kept: a workgroup each.  The rank of the last one that is comes from its bits, 11, 11 and 10
 // at a time: a histogram in LDS of the ranks that agree so far, and the bin in which the count is reached.  Then one pass in the
 // tokens' order gives each kept one its place: those of higher rank, and the first of the last rank's.
-constexpr int kSelectThreads = 1024, kSelectEach = 4;
+// kEach: tokens a lane whose weights stay in registers, where the table holds no more (one sequence of 4001 tokens 11.7 -> 9.9 us); 0:
+// they are read in every pass, from the caches (16 in registers took as long for sequences of 8192: 18 us).
+constexpr int kSelectThreads = 1024;
+template <int kEach>
 __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(EvictArgs8 a) {
-    constexpr int kWaves = kSelectThreads / 64;
+    constexpr int kWaves = kSelectThreads / 64, kRound = kEach ? kEach : 4;  // tokens a lane of a round in their order
     __shared__ uint32_t bins[2048];
     __shared__ uint2 waves[kWaves];
     __shared__ uint32_t found[2];
@@ -317,35 +330,48 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(EvictArgs8 a
     int32_t *kept = a.kept + block * a.keep;
     float *new_weights = a.new_weights ? a.new_weights + block * a.keep : nullptr;
     const auto weight = [&](int t) { return t < a.weights_cols ? weights[t] : 0.f; };
+    float held[kRound];
+    const auto hold = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < kRound; ++i) {
+            const int t = t0 + tid * kRound + i;
+            held[i] = t < len ? weight(t) : 0.f;
+        }
+    };
+    if constexpr (kEach > 0) hold(0);
     if (head == 0 && tid == 0) a.new_lens[seq] = keep;
     for (int i = keep + tid; i < a.keep; i += kSelectThreads) {
         kept[i] = -1;
         if (new_weights) new_weights[i] = 0.f;
     }
-    if (len <= a.keep) {
-        for (int t = tid; t < len; t += kSelectThreads) {
-            kept[t] = t;
-            if (new_weights) new_weights[t] = weight(t);
+    // candidates: tokens first .. last - 1, of which `want` stay; fewer than all of them, but where all tokens stay
+    const bool all = len <= a.keep;
+    const int first = all ? len : a.sinks, last = all ? len : len - a.recent;
+    const uint32_t want = all ? 0 : static_cast<uint32_t>(a.keep - a.sinks - a.recent);
+    const auto for_candidates = [&](const auto &f) {
+        if constexpr (kEach > 0) {
+#pragma unroll
+            for (int i = 0; i < kRound; ++i) {
+                const int t = tid * kRound + i;
+                if (t >= first && t < last) f(rank_of(held[i]));
+            }
+        } else {
+            for (int t = first + tid; t < last; t += kSelectThreads) f(rank_of(weight(t)));
         }
-        return;
-    }
-    // candidates: tokens first .. last - 1, of which `want` stay; fewer than all of them
-    const int first = a.sinks, last = len - a.recent;
-    const uint32_t want = static_cast<uint32_t>(a.keep - a.sinks - a.recent);
+    };
     uint32_t prefix = 0, mask = 0, left = want;  // of the last kept one's rank: its bits so far; candidates still to come with them
     for (int shift = 21, step = 0; step < 3 && want > 0; ++step) {
         const int bits = step < 2 ? 11 : 10;
         for (int i = tid; i < 2048; i += kSelectThreads) bins[i] = 0;
         __syncthreads();
-        for (int t = first + tid; t < last; t += kSelectThreads) {
-            const uint32_t r = rank_of(weight(t));
+        for_candidates([&](uint32_t r) {
             if ((r & mask) == prefix) atomicAdd(&bins[(r >> shift) & ((1u << bits) - 1)], 1u);
-        }
+        });
         __syncthreads();
         // bins from the top: lane tid has two of them
         const uint32_t hi = bins[2047 - 2 * tid], lo = bins[2046 - 2 * tid];
-        uint2 all;
-        const uint32_t before = sums_before<kWaves>(hi + lo, 0, waves, all).x;
+        uint2 total;
+        const uint32_t before = sums_before<kWaves>(hi + lo, 0, waves, total).x;
         if (before < left && before + hi + lo >= left) {
             const bool in_hi = before + hi >= left;
             found[0] = static_cast<uint32_t>(2047 - 2 * tid - (in_hi ? 0 : 1));
@@ -355,34 +381,33 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(EvictArgs8 a
         prefix |= found[0] << shift, mask |= ((1u << bits) - 1) << shift, left = found[1];
         shift -= step == 0 ? 11 : 10;
     }
-    // in order, kSelectEach tokens a lane
+    // in order, kRound tokens a lane
     uint32_t above = 0, equal = 0;  // kept before this round, those of the last rank apart
-    for (int t0 = 0; t0 < len; t0 += kSelectThreads * kSelectEach) {
-        float w[kSelectEach];
+    for (int t0 = 0; t0 < len; t0 += kSelectThreads * kRound) {
+        if constexpr (kEach == 0) hold(t0);
         uint32_t sure = 0, tie = 0;  // bit masks
 #pragma unroll
-        for (int i = 0; i < kSelectEach; ++i) {
-            const int t = t0 + tid * kSelectEach + i;
-            w[i] = t < len ? weight(t) : 0.f;
-            const uint32_t r = rank_of(w[i]);
+        for (int i = 0; i < kRound; ++i) {
+            const int t = t0 + tid * kRound + i;
+            const uint32_t r = rank_of(held[i]);
             const bool always = t < first || t >= last;
             if (t < len && (always || (want > 0 && r > prefix))) sure |= 1u << i;
             if (t < len && !always && want > 0 && r == prefix) tie |= 1u << i;
         }
-        uint2 all;
-        const uint2 before = sums_before<kWaves>(__popc(sure), __popc(tie), waves, all);
+        uint2 total;
+        const uint2 before = sums_before<kWaves>(__popc(sure), __popc(tie), waves, total);
         uint32_t s = above + before.x, e = equal + before.y;
 #pragma unroll
-        for (int i = 0; i < kSelectEach; ++i) {
+        for (int i = 0; i < kRound; ++i) {
             const bool is_tie = tie >> i & 1u, in = (sure >> i & 1u) || (is_tie && e < left);
             if (in) {
                 const uint32_t to = s + min(e, left);
-                kept[to] = t0 + tid * kSelectEach + i;
-                if (new_weights) new_weights[to] = w[i];
+                kept[to] = t0 + tid * kRound + i;
+                if (new_weights) new_weights[to] = held[i];
             }
             s += sure >> i & 1u, e += is_tie;
         }
-        above += all.x, equal += all.y;
+        above += total.x, equal += total.y;
     }
 }
 
@@ -569,7 +594,11 @@ int32_t castforge_hip_kv8_evict(const cfh_kv8_cache_t *cache, const int32_t *pag
                 check_launch(what);
             }
         };
-        launches(batch * cache->kv_heads, kSelectThreads, "kv8_select", [&](dim3 grid) { kv8_select_kernel<<<grid, dim3(kSelectThreads), 0, st>>>(a); });
+        const int64_t most = table_cols * cache->page_size;  // tokens a sequence
+        launches(batch * cache->kv_heads, kSelectThreads, "kv8_select", [&](dim3 grid) {
+            const auto kern = most <= 4 * kSelectThreads ? kv8_select_kernel<4> : kv8_select_kernel<0>;
+            kern<<<grid, dim3(kSelectThreads), 0, st>>>(a);
+        });
         launches(batch * a.used_cols * 2 * cache->kv_heads, 256, "kv8_move", [&](dim3 grid) {
             const auto kern = cache->head_dim == 64 ? kv8_move_kernel<64> : kv8_move_kernel<128>;
             kern<<<grid, dim3(256), 0, st>>>(a);
