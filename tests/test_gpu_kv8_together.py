@@ -1,0 +1,100 @@
+"""The operators of the paged 8-bit cache one after another, as a server runs them: prompts appended, attended and observed, cut to
+a budget, then tokens appended behind what was kept, each way against float64 over the cache's own numbers; and the example of a
+layer that does so, by calls and by graph replay."""
+import importlib.util
+from pathlib import Path
+
+import pytest
+import torch
+
+from castforge_amd import ops
+from test_gpu_kv8_attention import _check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d,hkv,ratio,page,window,sinks", [(128, 2, 4, 16, None, 0), (64, 3, 1, 32, None, 0), (128, 1, 7, 64, 300, 4), (64, 2, 3, 16, 50, 20)])
+def test_prompt_eviction_and_tokens(cuda, d, hkv, ratio, page, window, sinks):
+    """After the eviction the cache holds exactly what it held of the kept tokens (scales of random numbers of one size are alike or a
+    power of two apart, which rounds codes: so the attention is checked over what lies there now, and the kept rows against those before
+    to a step of E4M3), and the attention over it is the softmax over those tokens."""
+    prompts, keep, first, recent, tokens = [700, 37, 300], 128, 4, 24, 20
+    g = torch.Generator(device=cuda).manual_seed(d + ratio)
+    batch, hq, cols, new_cols = len(prompts), hkv * ratio, -(-max(prompts) // page), -(-(keep + tokens) // page)
+    pages = torch.randperm(batch * (cols + new_cols), generator=g, device=cuda).int()
+    table, new = pages[:batch * cols].view(batch, cols), pages[batch * cols:].view(batch, new_cols)
+    cache = ops.Kv8Cache.empty(pages.numel(), hkv, page, d, device=cuda)
+    angle = torch.arange(2048, device=cuda)[:, None] * 10000.0 ** (-torch.arange(d // 2, device=cuda) / (d // 2))
+    cos, sin = angle.cos(), angle.sin()
+    lens = torch.tensor(prompts, dtype=torch.int32, device=cuda)
+    cu = torch.nn.functional.pad(lens.cumsum(0), (1, 0)).int()
+
+    def rows(n):
+        return (1.5 * torch.randn((n, hq + 2 * hkv, d), generator=g, device=cuda)).bfloat16().split((hq, hkv, hkv), 1)
+
+    q, k, v = rows(sum(prompts))
+    at = torch.cat([torch.arange(n, device=cuda) for n in prompts])
+    turned = ops.kv8_append(cache, k, v, table, lens, cu_q=cu, positions=at, cos=cos, sin=sin, q=q)
+    _check(turned, cache, table, prompts, prompts, lens, cu, True, None, window, sinks)
+    weights = torch.zeros((batch, hkv, max(prompts)), device=cuda)
+    ops.kv8_attention(turned, cache, table, lens, cu_q=cu, window=window, sinks=sinks, weights=weights)
+    held = [t.clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)]
+    kept, new_lens, kept_weights = ops.kv8_evict(cache, table, lens, weights, keep, new, sinks=first, recent=recent)
+    before = ops.Kv8Cache(*held)
+    for b, n in enumerate(prompts):
+        m = min(n, keep)
+        assert new_lens[b].item() == m
+        places = torch.arange(m, device=cuda)
+        mine = ops.kv8_gather(cache, new[b, places // page].long() * page + places % page, torch.float32)
+        for h in range(hkv):
+            t = kept[b, h, :m].long()
+            assert torch.equal(weights[b, h][t], kept_weights[b, h, :m])
+            for x, y, s in zip(mine, ops.kv8_gather(before, table[b, t // page].long() * page + t % page, torch.float32), (cache.k_scales, cache.v_scales)):
+                step = s[new[b, places // page].long(), h][:, None]  # below 2^-6 a code's step is 2^-9 of the scale: half a step, or 2^-4 of the number
+                assert torch.all((x[:, h] - y[:, h]).abs() <= torch.maximum(y[:, h].abs() * 2.0 ** -4, step * 2.0 ** -10))
+
+    # single tokens behind the kept ones: positions go on from the old lengths, places from the new ones
+    live = torch.zeros((batch, hkv, new_cols * page), device=cuda)
+    live[..., :keep] = kept_weights
+    now = new_lens.clone()
+    for i in range(tokens):
+        q, k, v = rows(batch)
+        now += 1
+        turned = ops.kv8_append(cache, k, v, new, now, positions=lens.long() + i, cos=cos, sin=sin, q=q)
+        if i in (0, 1, page - 1, tokens - 1):
+            _check(turned, cache, new, now.tolist(), [1] * batch, now, None, True, None, window, sinks)
+        ops.kv8_attention(turned, cache, new, now, window=window, sinks=sinks, weights=live)
+    # a query's weights sum to 1: scores' magnitudes sum |q k| / sqrt(d) stay below 40, each of (d + 8) 2^-24 of which moves a weight by
+    # three times as much of itself (twice by its score, once by the logarithm): 2^-10
+    gained = live.sum((1, 2)) - kept_weights.sum((1, 2))
+    assert torch.all((gained - hq * tokens).abs() <= 2.0 ** -9 * (hq * tokens + kept_weights.sum((1, 2))))
+    # and cut again, into the pages of the prompts
+    kept, lens2, _ = ops.kv8_evict(cache, new, now, live, keep, table, sinks=first, recent=recent)
+    assert lens2.tolist() == [min(n, keep) for n in now.tolist()]
+    assert torch.all(kept[:, :, :first] == torch.arange(first, device=cuda, dtype=torch.int32))
+    _check(turned, cache, table, lens2.tolist(), [1] * batch, lens2, None, True, None, window, sinks)
+
+
+@pytest.fixture(scope="module")
+def example():
+    path = Path(__file__).resolve().parent.parent / "examples" / "long_context.py"
+    spec = importlib.util.spec_from_file_location("long_context", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+@pytest.mark.parametrize("prompts,q_heads,kv_heads,head_dim", [((300, 17, 1), 8, 2, 128), ((40,), 4, 4, 64), ((900, 150), 12, 4, 64)])
+def test_layer(cuda, example, prompts, q_heads, kv_heads, head_dim):
+    """Where nothing is evicted, against float32.  E4M3 rounds numbers spread evenly over a binade by 0.026 of their root mean square.
+    A product of two such operands is off by 0.037: the queries, keys and values, and the output; the cache's keys and values by 0.026
+    more.  In the values, and in the output's product, that is the output's error; in queries and keys that of a score of
+    about one sigma, and so of a weight.  Squared and added, queries 0.037, keys and values 0.037 and 0.026 each, the output 0.037: 0.083;
+    twice that is not exceeded.  Where tokens are evicted, replays give what calls do."""
+    called, replayed, plain, _ = example.run(prompts, 20, 1000, 32, 4, 16, 512, q_heads, kv_heads, head_dim)
+    assert example.distance(called, plain) < 0.17
+    for a, b in zip(called, replayed):
+        assert torch.equal(a, b)
+    called, replayed, _, _ = example.run(prompts, 20, 32, 6, 4, 16, 512, q_heads, kv_heads, head_dim)
+    for a, b in zip(called, replayed):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
