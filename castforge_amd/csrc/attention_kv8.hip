@@ -777,7 +777,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         load(part, page, begin + kSteps);
     }
     page = page_at(begin + 2 * kSteps);
-    for (int step = begin, i = 0; step < steps; step += kSteps, i ^= 1) {
+    int i = 0;
+    for (int step = begin; step < steps; step += kSteps, i ^= 1) {
         __syncthreads();  // stage i is made, and the other one no longer read
         walk_stage(step, i);
         if (step + kSteps < steps) {
@@ -787,30 +788,51 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         }
     }
     const float l = s.l + __shfl_xor(s.l, 32), inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
-    if (row >= total) return;
-    const int64_t to = out_row(a, sq, head, row);
-    // a lane's channels: D / 8 behind one another for each j
+    const int to = static_cast<int>(out_row(a, sq, head, row));
+    // Rows are stored by D / 8 lanes each, through LDS (stage i is no longer read): by the lanes that hold them each store touches 64 lines
+    // (64 queries of 7 heads after 16384 tokens, whose splits leave 30 MB: 60.9 -> 54.2 us).  A lane has D / 8 channels behind one another for
+    // each j; piece p of row r lies at p ^ r: in order, a piece of all rows would lie in the same banks.
+    constexpr int kLanes = D / 8, kPer = 64 / kLanes, kStores = kRows / kPer;  // lanes a row, rows a store, stores
+    const int of_row = lane / kLanes, piece = lane % kLanes;
+    uintx4 *rows = reinterpret_cast<uintx4 *>(stages + i) + wave * kRows * kLanes;
+    const auto put = [&](int at, const uintx4 &v) { rows[n * kLanes + (at ^ (n & (kLanes - 1)))] = v; };
+    const auto for_rows = [&](const auto &store) {
+        wave_order();
+#pragma unroll
+        for (int c = 0; c < kStores; ++c) {
+            const int r = kPer * c + of_row, to_row = __shfl(to, r);
+            const uintx4 v = rows[r * kLanes + (piece ^ (r & (kLanes - 1)))];
+            if (row0 + r < total) store(static_cast<int64_t>(to_row), v);
+        }
+        wave_order();
+    };
     if (a.splits > 1) {
-        float *part_to = a.part + (to * a.splits + split) * (D + 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int half = 0; half < 2; ++half) {  // of the channels
 #pragma unroll
-            for (int c = 0; c < D / 8; c += 4) {
-                const auto v = [&](int e) { return s.o[(c + e) % NT][4 * j + (c + e) / NT]; };
-                *reinterpret_cast<float4 *>(part_to + (8 * j + 4 * h) * NT + c) = make_float4(v(0), v(1), v(2), v(3));
-            }
-        if (h == 0) *reinterpret_cast<float4 *>(part_to + D) = make_float4(s.m, l, __int_as_float(used), 0.f);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int c = 0; c < D / 8; c += 4) {
+                    const auto v = [&](int e) { return __float_as_uint(s.o[(c + e) % NT][4 * (2 * half + j) + (c + e) / NT]); };
+                    put(((8 * j + 4 * h) * NT + c) / 4, uintx4{v(0), v(1), v(2), v(3)});
+                }
+            for_rows([&](int64_t at, const uintx4 &v) {
+                *reinterpret_cast<uintx4 *>(a.part + (at * a.splits + split) * (D + 4) + half * (D / 2) + 4 * piece) = v;
+            });
+        }
+        if (h == 0 && row < total) *reinterpret_cast<float4 *>(a.part + (static_cast<int64_t>(to) * a.splits + split) * (D + 4) + D) = make_float4(s.m, l, __int_as_float(used), 0.f);
         return;
     }
-    if (a.lse && h == 0) a.lse[to] = lse_of(s.m, l);
+    if (a.lse && h == 0 && row < total) a.lse[to] = lse_of(s.m, l);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int c = 0; c < D / 8; c += 8) {
             const auto v = [&](int e) { return s.o[(c + e) % NT][4 * j + (c + e) / NT] * inv; };
-            *reinterpret_cast<uint4 *>(a.out + to * D + (8 * j + 4 * h) * NT + c) =
-                make_uint4(f32x2_to_bf16x2_rne(v(0), v(1)), f32x2_to_bf16x2_rne(v(2), v(3)), f32x2_to_bf16x2_rne(v(4), v(5)), f32x2_to_bf16x2_rne(v(6), v(7)));
+            put(((8 * j + 4 * h) * NT + c) / 8,
+                uintx4{f32x2_to_bf16x2_rne(v(0), v(1)), f32x2_to_bf16x2_rne(v(2), v(3)), f32x2_to_bf16x2_rne(v(4), v(5)), f32x2_to_bf16x2_rne(v(6), v(7))});
         }
+    for_rows([&](int64_t at, const uintx4 &v) { *reinterpret_cast<uintx4 *>(a.out + at * D + 8 * piece) = v; });
 }
 
 // Weights that the cached tokens got, from the logarithms of the rows' sums: weights[seq, head, t] += sum over the head's rows of
@@ -1066,8 +1088,10 @@ Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     if (tokens == 0 || batch == 0) return p;
     const int64_t ratio = q_heads / c->kv_heads, cus = cu_count(), rows = tokens * ratio, each = (rows + batch - 1) / batch;
     const auto tiles = [&](int64_t per) { return varlen ? rows / per + batch : batch * ((ratio + per - 1) / per); };
-    const int64_t len = std::min(table_cols * c->page_size, window + sinks + 64 + tokens), row = (c->head_dim + 4) * 4;
-    const auto split_to = [&](int64_t splits, int64_t least) {
+    const int64_t row = (c->head_dim + 4) * 4;
+    // tokens that the queries of a row tile see: a window's, and one more a query that a tile may have
+    const auto len_of = [&](int64_t per) { return std::min(table_cols * c->page_size, window + sinks + 64 + std::min(tokens, per / ratio + 1)); };
+    const auto split_to = [&](int64_t splits, int64_t len, int64_t least) {
         p.splits = std::max<int64_t>(1, std::min(splits, len / least));
         p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
         if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
@@ -1076,7 +1100,9 @@ Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     if (p.rows) {
         const int64_t tasks = batch * ((each + 255) / 256) * c->kv_heads, splits = cus / tasks;
         p.waves = 8;
-        split_to(splits > 2 ? splits : 1, 256);
+        // two splits where each has 768 tokens: 1024 queries of 32 heads at the end of 1000 tokens 34.6 us against 40.6 with them, of 1500
+        // 48.8 both ways, of 2048 60.5 against 55.6, of 8192 211 against 148; more of them, which fill the card, from 256 tokens on
+        split_to(splits, len_of(256), splits > 2 ? 256 : 768);
         if (p.splits == 1 && tasks < cus && each > 128) p.waves = 4;
         p.tiles = tiles(32 * p.waves);
         return p;
@@ -1085,13 +1111,14 @@ Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     p.tiles = tiles(16 * p.mt);
     const int64_t tasks = p.tiles * c->kv_heads;
     p.score_cols = table_cols * c->page_size;
+    const int64_t len = len_of(16 * p.mt);
     p.scored = weights && each <= 8 && tokens * q_heads * p.score_cols <= int64_t{64} << 20;
     // A short table and few workgroups: one launch of wide workgroups, four rounds of 32 tokens a wave at most, no partial sums.  One
     // sequence of 1009 tokens, 8 heads of 128: 11.7 us a call against 15.7 with splits and their join, whose second launch costs the host more
     // than the longer walk costs the GPU (10.3 against 7.4 us there); 32 sequences of 1000 16.3 against 18.2 there.  At 2000 tokens one
     // sequence takes 16.1 against 8.0 there.  (Sixteen waves spill: 14.5 for 1009 tokens.)
     p.wide = p.mt == 1 && tasks <= cus && len <= 1024;
-    if (!p.wide) split_to((2 * cus + tasks - 1) / tasks, 128);
+    if (!p.wide) split_to((2 * cus + tasks - 1) / tasks, len, 128);
     p.scores_at = p.bytes;
     if (p.scored) p.bytes += 4 * tokens * q_heads * p.score_cols;
     return p;
