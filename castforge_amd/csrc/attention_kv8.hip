@@ -8,6 +8,11 @@
 //
 // The softmax's maximum and sum, the scores and the output sums are f32.  Codes reach the MFMAs exactly, keys as bf16 (as the
 // queries are) and values as f16; weights are rounded to f16, 2^-11 of themselves (bf16 would be 2^-8).
+//
+// Three kernels and what bounds them (8 heads of keys, 32 of queries, 128 channels): few rows a sequence read the cache at HBM's rate (48
+// single queries over up to 8000 tokens 98 us, 4.8 TB/s; a large copy runs at 5.1); many rows are bound by the sum of MFMAs and vector
+// instructions (prompt of 4096 tokens 143 to 152 us by the box, 0.9 to 0.96 PFLOP/s); the weights that tokens got are the keys' half of
+// that again, or a pass over scores that the first kernel left.
 #include <algorithm>
 #include <atomic>
 
@@ -351,7 +356,9 @@ __device__ __forceinline__ Seq seq_of(const AttnArgs8 &a, int seq) {
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f; }
 
 // One workgroup's NW waves take the same rows and every NW-th 32 tokens of a split's share, and are joined through LDS;
-// splits are joined by kv8_attention_join_kernel.
+// splits are joined by kv8_attention_join_kernel.  Codes go from memory to registers, without LDS: each is used once, and a wave has the next
+// 32 tokens' on their way while it works on these.  Three waves a SIMD for 16 rows (48 sequences of up to 8000 tokens 106 -> 100 us; with
+// 32 rows they would spill).
 template <int D, int NW>
 struct SplitLds8 {
     float sums[NW][16][D + 4];
@@ -861,7 +868,9 @@ __device__ __forceinline__ Queries queries_that_see(const AttnArgs8 &a, const Se
 // tokens, and a score costs an fma, an exponential and an addition.
 // kByHead: a tile is 32 queries of one query head (the last one of a head reaches back over queries that it leaves out), whose rows lie a
 // stride apart; else 32 rows in order, each with a query and a head to be told apart (as many instructions again, but full tiles where
-// a sequence has few queries).
+// a sequence has few queries: below 32 a sequence).
+// 64 queries of 28 heads after 16384 tokens: 21 us of that call's 55; 418 us were a prompt's of 4096 tokens whose rows each lane read itself.
+// Bound by a workgroup's start (keys from table to operands) beside four rounds of tiles; 240 registers leave two workgroups a CU.
 // Queries are read by rows, 16 lanes each, and stored for operand c and half h of lanes at row r ^ (2 c + h): in order, all 16 pieces of a
 // row would lie in the same banks.
 template <int D, bool kByHead>
@@ -872,8 +881,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int64_t block = wa.first_block + blockIdx.x;
     const int seq = static_cast<int>(block / a.heads / wa.blocks), head = static_cast<int>(block % a.heads);
-    // the first tokens are seen by the most rows: they come first, and the last ones beside them (one head after another: 240 us instead of
-    // 152 for a prompt of 4096 tokens)
+    // the first tokens are seen by the most rows: they come first, and the last ones beside them (one head after another: a prompt of 4096
+    // tokens took 240 us instead of 174 before rows were staged in LDS, 113 since)
     const int k = static_cast<int>(block / a.heads % wa.blocks), most_heavy = (wa.blocks + 1) / 2;
     const int t0 = 64 * (k < most_heavy ? k : wa.blocks - 1 - (k - most_heavy));
     const Seq sq = seq_of(a, seq);
@@ -1045,7 +1054,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 }
 
 // The same where the kernel of few rows has left its scores (base 2), [rows][score_cols] from the first row of the sequence and head on:
-// four tokens a lane.
+// four tokens a lane.  Up to eight rows a sequence and head, where the scores' 4 bytes a row and token are read back in less time than the
+// keys are multiplied again (32 sequences of up to 8000 tokens, 4 query heads a head of keys: 104 us in all against 140; more rows have
+// more scores than keys), and up to 256 MB of them.
 __global__ __launch_bounds__(256) void kv8_attention_scored_kernel(AttnArgs8 a, WeightArgs8 wa) {
     const int64_t block = wa.first_block + blockIdx.x;
     const int seq = static_cast<int>(block / wa.blocks / a.heads), head = static_cast<int>(block / wa.blocks % a.heads);
@@ -1091,34 +1102,51 @@ Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     const int64_t row = (c->head_dim + 4) * 4;
     // tokens that the queries of a row tile see: a window's, and one more a query that a tile may have
     const auto len_of = [&](int64_t per) { return std::min(table_cols * c->page_size, window + sinks + 64 + std::min(tokens, per / ratio + 1)); };
-    const auto split_to = [&](int64_t splits, int64_t len, int64_t least) {
-        p.splits = std::max<int64_t>(1, std::min(splits, len / least));
-        p.splits = std::max<int64_t>(1, std::min(p.splits, (int64_t{256} << 20) / (tokens * q_heads * row)));
-        if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
+    const int64_t most_splits = std::max<int64_t>(1, (int64_t{256} << 20) / (tokens * q_heads * row));
+    const auto splits_for = [&](int64_t splits, int64_t len, int64_t least) { return std::max<int64_t>(1, std::min({splits, len / least, most_splits})); };
+    // Several queries a sequence: the form and its splits by their cost in us.  A workgroup takes `start`, and `token` for each token that its
+    // rows see, of which causal rows see fewer; `slots` of them run at once; splits cost a launch, and the writing and reading of their
+    // sums at 4 TB/s.  The numbers are fits to 65 shapes a head size (1 to 64 sequences of 16 to 2400 queries after 0 to 16000 tokens, in
+    // every form): over them the choice takes 2 to 3% longer than the best form does, 24% at most.  (128 channels, us, tile kernel and split kernel: prompt of
+    // 512 tokens 22 and 14, of 1600 52 and 57, of 2400 77 and 100; 16 prompts of 100 tokens 14 and 27; 64 queries of 32 heads after 4000
+    // tokens 31 and 23, 128 after 16000 54 and 63, 512 after 16000 147 and 186.  By rows a sequence alone: up to 1.9 times the better one's.)
+    const auto cost = [&](double token, double start, int64_t slots, int64_t tasks, int64_t splits, int64_t len) {
+        const double seen = std::min(len, std::max(table_cols * c->page_size - tokens / batch / 2, int64_t{1})), rounds = static_cast<double>((tasks * splits + slots - 1) / slots);
+        return std::max(len * token / splits + start, rounds * (seen * token / splits + start)) + (splits > 1 ? 5 + 2e-6 * tokens * q_heads * splits * row / 4 : 0);
     };
-    p.rows = varlen && each >= (c->head_dim == 128 ? 64 : 512);
+    const bool large = c->head_dim == 128;
+    const auto tasks_of = [&](int64_t per) { return batch * c->kv_heads * ((each + per - 1) / per); };
+    p.mt = each <= 96 ? 1 : 2;
+    const int64_t len = len_of(16 * p.mt);
+    p.tiles = tiles(16 * p.mt);
+    // two workgroups a CU.  A short table and few workgroups: one launch of wide workgroups, four rounds of 32 tokens a wave at most, no partial
+    // sums.  One sequence of 1009 tokens, 8 heads of 128: 11.7 us a call against 15.7 with splits and their join, whose second launch costs the
+    // host more than the longer walk costs the GPU (10.3 against 7.4 us there); 32 sequences of 1000 16.3 against 18.2 there.  At 2000 tokens
+    // one sequence takes 16.1 against 8.0 there.  (Sixteen waves spill: 14.5 for 1009 tokens.)
+    p.wide = p.mt == 1 && p.tiles * c->kv_heads <= cus && len <= 1024;
+    if (!p.wide) p.splits = splits_for((2 * cus + p.tiles * c->kv_heads - 1) / (p.tiles * c->kv_heads), len, 128);
+    if (varlen && each > 16) {
+        const double token = p.wide ? (large ? .0065 : .005) : p.mt == 1 ? (large ? .0155 : .0095) : large ? .0115 : .0085;
+        const int64_t slots = p.wide ? cus : (p.mt == 1 ? 3 : 2) * cus;
+        const auto split_cost = [&](int64_t s) { return cost(token, large ? 6 : 4.5, slots, tasks_of(16 * p.mt), s, len); };
+        const int64_t fewer = splits_for(p.splits, len, 256);  // from 97 rows on a join has many
+        if (p.mt == 2) p.splits = fewer;
+        double best = split_cost(p.splits);
+        const auto take = [&](double us, bool rows, int waves, int64_t splits) {
+            if (us < best) best = us, p.rows = rows, p.waves = waves, p.splits = splits, p.wide = p.wide && !rows;
+        };
+        take(split_cost(1), false, 4, 1);
+        const int64_t half = tasks_of(128), seen = len_of(256);
+        take(half <= cus ? cost(large ? .0255 : .0205, large ? 6 : 5.5, cus, half, 1, seen) : cost(large ? .037 : .027, large ? 10 : 7, 2 * cus, half, 1, seen), true, 4, 1);
+        for (int64_t s = 1; s <= splits_for(32, seen, 256); ++s) take(cost(large ? .027 : .0205, large ? 9 : 6.5, cus, tasks_of(256), s, seen), true, 8, s);
+    }
+    if (p.splits > 1) p.bytes = tokens * q_heads * p.splits * row;
     if (p.rows) {
-        const int64_t tasks = batch * ((each + 255) / 256) * c->kv_heads, splits = cus / tasks;
-        p.waves = 8;
-        // two splits where each has 768 tokens: 1024 queries of 32 heads at the end of 1000 tokens 34.6 us against 40.6 with them, of 1500
-        // 48.8 both ways, of 2048 60.5 against 55.6, of 8192 211 against 148; more of them, which fill the card, from 256 tokens on
-        split_to(splits, len_of(256), splits > 2 ? 256 : 768);
-        if (p.splits == 1 && tasks < cus && each > 128) p.waves = 4;
         p.tiles = tiles(32 * p.waves);
         return p;
     }
-    p.mt = each <= 96 ? 1 : 2;
-    p.tiles = tiles(16 * p.mt);
-    const int64_t tasks = p.tiles * c->kv_heads;
     p.score_cols = table_cols * c->page_size;
-    const int64_t len = len_of(16 * p.mt);
     p.scored = weights && each <= 8 && tokens * q_heads * p.score_cols <= int64_t{64} << 20;
-    // A short table and few workgroups: one launch of wide workgroups, four rounds of 32 tokens a wave at most, no partial sums.  One
-    // sequence of 1009 tokens, 8 heads of 128: 11.7 us a call against 15.7 with splits and their join, whose second launch costs the host more
-    // than the longer walk costs the GPU (10.3 against 7.4 us there); 32 sequences of 1000 16.3 against 18.2 there.  At 2000 tokens one
-    // sequence takes 16.1 against 8.0 there.  (Sixteen waves spill: 14.5 for 1009 tokens.)
-    p.wide = p.mt == 1 && tasks <= cus && len <= 1024;
-    if (!p.wide) split_to((2 * cus + tasks - 1) / tasks, len, 128);
     p.scores_at = p.bytes;
     if (p.scored) p.bytes += 4 * tokens * q_heads * p.score_cols;
     return p;

@@ -138,7 +138,8 @@ struct Turn {
 
 // A workgroup has the keys, or the values, of one head in one page: eight channels a lane, D / 8 lanes a token, NP rounds of
 // 2048 / D tokens whose numbers stay in registers between the absmax and the codes.  The workgroups after those have a token's
-// queries each.
+// queries each.  HBM: 4096 tokens of 32 + 8 + 8 heads of 128 with their read-back 56 us a call, 4.8 TB/s (a large copy runs at 5.1); 16 tokens
+// of as many sequences 6 us on the GPU and 22 a call, which is the host's for two calls.
 template <int D, int NP>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs8 a) {
     constexpr int kLanes = D / 8, kRows = 256 / kLanes;
@@ -316,6 +317,9 @@ __device__ __forceinline__ uint2 sums_before(uint32_t a, uint32_t b, uint2 *wave
 // tokens' order gives each kept one its place: those of higher rank, and the first of the last rank's.
 // kEach: tokens a lane whose weights stay in registers, where the table holds no more (one sequence of 4001 tokens 11.7 -> 9.9 us); 0:
 // they are read in every pass, from the caches (16 in registers took as long for sequences of 8192: 18 us).
+// Bound by one CU's vector instructions: 131072 tokens take 150 us, half of it the last pass, whatever the number of sequences up to one a CU.
+// Batches of eight loads, a ballot for the histogram's additions, other runs of tokens a lane: slower.  Several workgroups a sequence would
+// take four to seven launches.
 constexpr int kSelectThreads = 1024;
 template <int kEach>
 __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(EvictArgs8 a) {
@@ -412,7 +416,8 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(EvictArgs8 a
 }
 
 // Moves the kept tokens: a workgroup the keys, or the values, of one head in one new page; 16 codes a lane.  The new page takes the
-// greatest of its tokens' scales: their codes move as they are, others are rounded to it.
+// greatest of its tokens' scales: their codes move as they are, others are rounded to it.  HBM: 32 sequences of up to 8000 tokens to 2048, with
+// the selection and the read-back, 125 us, 5 TB/s.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_move_kernel(EvictArgs8 a) {
     constexpr int kLanes = D / 16, kRows = 256 / kLanes, kMost = 256 / kRows;  // rounds of the largest page

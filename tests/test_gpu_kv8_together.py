@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from castforge_amd import ops
-from test_gpu_kv8_attention import _check
+from test_gpu_kv8_attention import _check, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -73,6 +73,15 @@ def test_prompt_eviction_and_tokens(cuda, d, hkv, ratio, page, window, sinks):
     assert lens2.tolist() == [min(n, keep) for n in now.tolist()]
     assert torch.all(kept[:, :, :first] == torch.arange(first, device=cuda, dtype=torch.int32))
     _check(turned, cache, table, lens2.tolist(), [1] * batch, lens2, None, True, None, window, sinks)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("q_lens,kv_lens,window", [([100] * 16, [100] * 16, None), ([32] * 64, [32] * 64, None), ([24] * 48, [900] * 48, None), ([1000], [4000], None),
+                                                   ([1000], [4000], 2500), ([300, 301, 299, 1], [2500, 2400, 300, 2000], None), ([256], [6000], None), ([512], [512], None),
+                                                   ([2400], [2400], None), ([130, 2], [9000, 9000], None)])
+def test_every_form_of_attention(cuda, d, q_lens, kv_lens, window):
+    """Few rows, many, each with splits and without, as the sizes choose."""
+    _run(cuda, q_lens, kv_lens, 4, 4, d, 32, seed=len(q_lens), window=window, sinks=4 if window else 0)
 
 
 @pytest.fixture(scope="module")
