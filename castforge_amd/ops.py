@@ -1255,8 +1255,8 @@ def kv8_append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, page_table: to
     are rounded anew to it; a page whose first place is written starts anew.  Without cos and sin nothing is rotated.  q
     [T, q_heads, head_dim], if given, is rotated too and returned (bf16, contiguous; rows of no sequence are not written).
 
-    Rows may be slices of one projection's output: only the token stride is free (a multiple of 8).  A page must not get tokens of
-    two sequences in one call."""
+    Rows may be slices of one projection's output: only the token stride is free (a multiple of 8).  No page may get tokens of two
+    entries of the table in one call."""
     ks, vs, n = cache._rows(k, cache.kv_heads, "k"), cache._rows(v, cache.kv_heads, "v"), k.shape[0]
     if v.shape[0] != n:
         raise ValueError("k and v must have the same tokens")

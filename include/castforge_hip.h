@@ -609,8 +609,8 @@ typedef struct {
 /* Writes the keys and values of a batch's new tokens, with the lists that castforge_hip_kv8_attention takes next: sequence b has
  * the rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q i32 [batch + 1], rising from 0; NULL: one row each) and kv_lens[b] tokens with them,
  * so that its row i of n is token kv_lens[b] - n + i, in place t % page_size of page page_table[b][t / page_size] (i32
- * [batch, table_cols]; tokens before the first, past the table or on a page id outside the cache are left out).  A page must
- * not get tokens of two sequences in one call.
+ * [batch, table_cols]; tokens before the first, past the table or on a page id outside the cache are left out).  No page may
+ * get tokens of two entries of the table in one call.
  * Keys are rotated first, as castforge_hip_kv4_append's, by row positions[row] of cos and sin.  Of a page and head,
  * s' = max(s, 2^e): e the least, from -70 to 30, with absmax <= 448 * 2^e over the call's tokens there (NaN left out), s the page's
  * scale, or 0 where its place 0 is among them: the page starts anew.  code = E4M3(x / s') to the nearest even, saturating at 448, NaN -> 0;

@@ -84,6 +84,61 @@ def test_every_form_of_attention(cuda, d, q_lens, kv_lens, window):
     _run(cuda, q_lens, kv_lens, 4, 4, d, 32, seed=len(q_lens), window=window, sinks=4 if window else 0)
 
 
+def test_sequences_that_share_pages(cuda):
+    """A prefix that three sequences have in the same pages: attention, weights and eviction as with copies of their own."""
+    q, cache, table, lens, cu, _ = _run(cuda, [3, 1, 20], [200, 180, 220], 2, 3, 64, 16, seed=5)
+    shared = table.clone()
+    shared[1:, :8] = table[0, :8]
+    copies = ops.Kv8Cache(*[t.clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)])
+    for t in (copies.k_codes, copies.k_scales, copies.v_codes, copies.v_scales):
+        for b in (1, 2):
+            t[table[b, :8].long()] = t[table[0, :8].long()]
+    free = cache.num_pages
+    both = []
+    for c, tab in ((cache, shared), (copies, table)):
+        more = ops.Kv8Cache(*[torch.cat([t, torch.zeros_like(t[:12])]) for t in (c.k_codes, c.k_scales, c.v_codes, c.v_scales)])
+        w = torch.zeros((3, 2, 224), device=cuda)
+        o = ops.kv8_attention(q, more, tab, lens, cu_q=cu, weights=w)
+        new = torch.arange(free, free + 12, dtype=torch.int32, device=cuda).view(3, 4)
+        kept, new_lens, kept_w = ops.kv8_evict(more, tab, lens, w, 64, new, sinks=4, recent=8)
+        both.append((o, w, kept, new_lens, kept_w, more.k_codes[free:], more.k_scales[free:], more.v_codes[free:], more.v_scales[free:]))
+    for a, b in zip(*both):
+        assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    """Two batches on pages of their own in one cache, appended, attended and cut on two streams at the same time."""
+    g, d, page, keep = torch.Generator(device=cuda).manual_seed(1), 128, 32, 100
+    lens = [torch.tensor([700, 90], dtype=torch.int32, device=cuda), torch.tensor([300, 800], dtype=torch.int32, device=cuda)]
+    tables = [torch.arange(50, dtype=torch.int32, device=cuda).view(2, 25) + 50 * i for i in range(2)]
+    news = [torch.arange(8, dtype=torch.int32, device=cuda).view(2, 4) + 100 + 8 * i for i in range(2)]
+    rows = [torch.randn((int(n.sum()), 12, d), generator=g, device=cuda).bfloat16() for n in lens]
+    cus = [torch.nn.functional.pad(n.cumsum(0), (1, 0)).int() for n in lens]
+
+    def work(cache, i):
+        q, k, v = rows[i].split((8, 2, 2), 1)
+        q = ops.kv8_append(cache, k, v, tables[i], lens[i], cu_q=cus[i], q=q)
+        w = torch.zeros((2, 2, 800), device=cuda)
+        o = ops.kv8_attention(q, cache, tables[i], lens[i], cu_q=cus[i], weights=w)
+        return (o, w, *ops.kv8_evict(cache, tables[i], lens[i], w, keep, news[i]))
+
+    one, two = (ops.Kv8Cache.empty(116, 2, page, d, device=cuda) for _ in range(2))
+    want = [work(one, i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(work(two, i))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
+        for a, b in ((one.k_codes, two.k_codes), (one.k_scales, two.k_scales), (one.v_codes, two.v_codes), (one.v_scales, two.v_scales)):
+            assert torch.equal(a, b)
+
+
 @pytest.fixture(scope="module")
 def example():
     path = Path(__file__).resolve().parent.parent / "examples" / "long_context.py"
