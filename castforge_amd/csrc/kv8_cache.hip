@@ -99,67 +99,70 @@ __device__ __forceinline__ void unpack8(const uint4 &w, float (&x)[8]) {
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(b[i] << 16), x[2 * i + 1] = __uint_as_float(b[i] & 0xffff0000u);
 }
 
-// What turns a lane's eight channels, piece * 8 on, of a token at a position.
-struct Turn {
-    float c[8], t[8];  // cosines and sines of the lane's channels, the sine's sign taken in
-    __device__ __forceinline__ void load(const AppendArgs8 &a, int64_t position, int piece) {
-        const int half = a.rot / 2;
-        const bool low = 8 * piece < half;
-        // a position outside the table takes its nearest row
-        const int64_t pos = min(max(position, int64_t{0}), a.max_pos - 1);
-        const float *cp = a.cos + pos * half, *sp = a.sin + pos * half;
-        if (a.interleaved) {
-            const float4 cc = *reinterpret_cast<const float4 *>(cp + 4 * piece), ss = *reinterpret_cast<const float4 *>(sp + 4 * piece);
-            c[0] = c[1] = cc.x, c[2] = c[3] = cc.y, c[4] = c[5] = cc.z, c[6] = c[7] = cc.w;
-            t[0] = -ss.x, t[1] = ss.x, t[2] = -ss.y, t[3] = ss.y, t[4] = -ss.z, t[5] = ss.z, t[6] = -ss.w, t[7] = ss.w;
-        } else {
-            const int at = low ? 8 * piece : 8 * piece - half;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float4 cc = reinterpret_cast<const float4 *>(cp + at)[h], ss = reinterpret_cast<const float4 *>(sp + at)[h];
-                c[4 * h] = cc.x, c[4 * h + 1] = cc.y, c[4 * h + 2] = cc.z, c[4 * h + 3] = cc.w;
-                t[4 * h] = low ? -ss.x : ss.x, t[4 * h + 1] = low ? -ss.y : ss.y, t[4 * h + 2] = low ? -ss.z : ss.z, t[4 * h + 3] = low ? -ss.w : ss.w;
-            }
-        }
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+
+// Four elements and four more.  Read through the caches, for a row's halves share no lines with their loads: past them 52.3 us, not 49.6,
+// where 4096 tokens of 32 heads are appended and read back.
+__device__ __forceinline__ uint4 load8(const uint16_t *lo, const uint16_t *hi) {
+    const uint2 a = *reinterpret_cast<const uint2 *>(lo), b = *reinterpret_cast<const uint2 *>(hi);
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void store4_past(uint16_t *p, uint32_t a, uint32_t b) { __builtin_nontemporal_store(uintx2{a, b}, reinterpret_cast<uintx2 *>(p)); }
+
+// A lane's eight channels of a row, lo .. lo + 3 and hi .. hi + 3: both of each pair that is turned together, so that a lane reads an angle
+// once and no channel twice (by eight channels in a row a lane: 96 bytes for eight, not 48).
+struct Channels {
+    int lo, hi;
+    bool turned;
+    __device__ __forceinline__ Channels(const AppendArgs8 &a, int piece) : lo(8 * piece), hi(8 * piece + 4), turned(8 * piece < a.rot) {
+        if (turned && !a.interleaved) lo = 4 * piece, hi = a.rot / 2 + 4 * piece;
     }
-    // (a, b) -> (a c - b s, b c + a s): x c + partner * (+- s), which rounds as the difference does
-    __device__ __forceinline__ void apply(const AppendArgs8 &a, const uint4 &partner, float (&x)[8]) const {
-        float y[8];
-        if (a.interleaved) {
+};
+
+// The angles of a lane's four pairs, of a token at a position.
+struct Turn {
+    float c[4], s[4];
+    __device__ __forceinline__ void load(const AppendArgs8 &a, int64_t position, int piece) {
+        // a position outside the table takes its nearest row
+        const int64_t at = min(max(position, int64_t{0}), a.max_pos - 1) * (a.rot / 2) + 4 * piece;
+        const float4 cc = *reinterpret_cast<const float4 *>(a.cos + at), ss = *reinterpret_cast<const float4 *>(a.sin + at);
+        c[0] = cc.x, c[1] = cc.y, c[2] = cc.z, c[3] = cc.w;
+        s[0] = ss.x, s[1] = ss.y, s[2] = ss.z, s[3] = ss.w;
+    }
+    __device__ __forceinline__ void apply(const AppendArgs8 &a, float (&x)[8]) const {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        } else {
-            unpack8(partner, y);
+        for (int i = 0; i < 4; ++i) {
+            const float p = a.interleaved ? x[2 * i] : x[i], q = a.interleaved ? x[2 * i + 1] : x[4 + i];
+            const float u = p * c[i] - q * s[i], v = q * c[i] + p * s[i];
+            (a.interleaved ? x[2 * i] : x[i]) = u, (a.interleaved ? x[2 * i + 1] : x[4 + i]) = v;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + y[i] * t[i];
     }
 };
 
 // A workgroup has the keys, or the values, of one head in one page: eight channels a lane, D / 8 lanes a token, NP rounds of
 // 2048 / D tokens whose numbers stay in registers between the absmax and the codes.  The workgroups after those have a token's
-// queries each.  HBM: 4096 tokens of 32 + 8 + 8 heads of 128 with their read-back 56 us a call, 4.8 TB/s (a large copy runs at 5.1); 16 tokens
-// of as many sequences 6 us on the GPU and 22 a call, which is the host's for two calls.
+// queries each.  HBM: 4096 tokens of 32 heads of each kind, 128 channels, with their read-back 49 us a call, 5.5 TB/s (a large copy runs at
+// 5.1: part of this stays in the last-level cache).  16 tokens of as many sequences 6 us on the GPU and 22 a call, the host's for two calls.
 template <int D, int NP>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs8 a) {
     constexpr int kLanes = D / 8, kRows = 256 / kLanes;
     __shared__ float tops[4];
     const int piece = threadIdx.x % kLanes, local = threadIdx.x / kLanes;
     const int64_t block = a.first_block + blockIdx.x;
-    const bool turns = 8 * piece < a.rot;
-    const int half = a.rot / 2, other = a.interleaved ? piece : 8 * piece < half ? piece + half / 8 : piece - half / 8;
+    const Channels ch(a, piece);
     if (block >= a.kv_blocks) {
         const int token = static_cast<int>(block - a.kv_blocks);
         if (token >= (a.cu_q ? a.cu_q[a.batch] : a.tokens)) return;  // of no sequence
         Turn turn;
-        if (turns) turn.load(a, a.positions[token], piece);
+        if (ch.turned) turn.load(a, a.positions[token], piece);
         for (int h = local; h < a.q_heads; h += kRows) {
             const uint16_t *src = a.q + token * a.q_stride + h * D;
             float x[8];
-            unpack8(load_once(src + 8 * piece), x);
-            if (turns) turn.apply(a, a.interleaved ? uint4{} : *reinterpret_cast<const uint4 *>(src + 8 * other), x);
-            store_past(a.q_out + (static_cast<int64_t>(token) * a.q_heads + h) * D + 8 * piece,
-                       make_uint4(f32x2_to_bf16x2_rne(x[0], x[1]), f32x2_to_bf16x2_rne(x[2], x[3]), f32x2_to_bf16x2_rne(x[4], x[5]), f32x2_to_bf16x2_rne(x[6], x[7])));
+            unpack8(load8(src + ch.lo, src + ch.hi), x);
+            if (ch.turned) turn.apply(a, x);
+            uint16_t *to = a.q_out + (static_cast<int64_t>(token) * a.q_heads + h) * D;
+            store4_past(to + ch.lo, f32x2_to_bf16x2_rne(x[0], x[1]), f32x2_to_bf16x2_rne(x[2], x[3]));
+            store4_past(to + ch.hi, f32x2_to_bf16x2_rne(x[4], x[5]), f32x2_to_bf16x2_rne(x[6], x[7]));
         }
         return;
     }
@@ -171,64 +174,79 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs8 a) {
     const int page = a.table[static_cast<int64_t>(u.seq) * a.table_cols + u.col];
     if (page < 0 || page >= a.num_pages) return;
     const int64_t row0 = kv8_row(page, head, 0, a.heads, a.page_shift);
-    uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + row0 * D + 8 * piece;
+    uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + row0 * D;
     float *scale_at = (is_v ? a.v_scales : a.k_scales) + static_cast<int64_t>(page) * a.heads + head;
     const float old = u.lo > 0 ? *scale_at : 0.f;
     const int count = u.hi - u.lo;
     float x[NP][8], top = 0.f;
-    const uint16_t *rows = (is_v ? a.v + head * D : a.k + head * D) + 8 * piece;
+    const uint16_t *rows = is_v ? a.v + head * D : a.k + head * D;
     const int64_t stride = is_v ? a.v_stride : a.k_stride;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        // rows past the last one are that one again: under a branch each load would wait for itself (prompt of 4096 tokens 64 -> 57 us with
-        // the read-back; four rounds' loads at once: 73, three waves a SIMD instead of seven)
+        // rows past the last one are that one again: under a branch each load would wait for itself (4096 tokens 64 -> 57 us with their
+        // read-back when it was done; four rounds' loads at once: 73, three waves a SIMD instead of seven)
         const int r = j * kRows + local, at = u.row + min(r, count - 1);
         if (j * kRows >= count) break;
-        const uint4 own = load_once(rows + at * stride);
-        if (turns && !is_v) {
-            const int64_t position = a.positions[at];
-            const uint4 partner = a.interleaved ? uint4{} : *reinterpret_cast<const uint4 *>(rows + at * stride + 8 * (other - piece));
-            Turn turn;
-            turn.load(a, position, piece);
-            unpack8(own, x[j]);
-            turn.apply(a, partner, x[j]);
+        const uint16_t *row = rows + at * stride;
+        if (is_v) {
+            unpack8(load_once(row + 8 * piece), x[j]);
         } else {
-            unpack8(own, x[j]);
+            unpack8(load8(row + ch.lo, row + ch.hi), x[j]);
+            if (ch.turned) {
+                Turn turn;
+                turn.load(a, a.positions[at], piece);
+                turn.apply(a, x[j]);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));  // NaN: left out
+        for (int i = 0; i < 8; ++i) top = __builtin_elementwise_maximum(top, fabsf(x[j][i]));  // NaN stays
     }
-    top = wave_max<64>(top);
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();  // also: every lane has read the old scale
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const auto most = [&](float lane_top, bool nan) {
+        lane_top = wave_max<64>(lane_top);
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = nan ? __builtin_nanf("") : lane_top;
+        __syncthreads();  // also: every lane has read the old scale
+        return __builtin_elementwise_maximum(__builtin_elementwise_maximum(tops[0], tops[1]), __builtin_elementwise_maximum(tops[2], tops[3]));
+    };
+    top = most(top, __any(top != top));
+    const bool nan = top != top;
+    if (nan) {  // uniform: once more, NaN left out
+        __syncthreads();
+        top = 0.f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = j * kRows < count ? fmaxf(top, fabsf(x[j][i])) : top;
+        top = most(top, false);
+    }
     const float scale = fmaxf(old, kv8_scale_of(top));
     if (scale > old) {
         if (threadIdx.x == 0) *scale_at = scale;
         const float ratio = old / scale;
         for (int r = local; r < u.lo; r += kRows) {
-            uint2 *p = reinterpret_cast<uint2 *>(codes + r * D);
+            uint2 *p = reinterpret_cast<uint2 *>(codes + r * D + 8 * piece);
             *p = make_uint2(e4m3x4_by(p->x, ratio), e4m3x4_by(p->y, ratio));
         }
     }
-    const auto store = [&](const auto &quotient) {
+    const auto store = [&](const auto &code_of) {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int r = j * kRows + local;
             if (r < count) {
                 float y[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = quotient(x[j][i]);
-                    y[i] = v != v ? 0.f : __builtin_amdgcn_fmed3f(v, -448.f, 448.f);
-                }
-                *reinterpret_cast<uint2 *>(codes + (u.lo + r) * D) = make_uint2(f32_to_e4m3x4(y), f32_to_e4m3x4(y + 4));
+                for (int i = 0; i < 8; ++i) y[i] = code_of(x[j][i]);
+                uint8_t *to = codes + (u.lo + r) * D;
+                const uint32_t one = f32_to_e4m3x4(y), two = f32_to_e4m3x4(y + 4);
+                if (is_v) *reinterpret_cast<uint2 *>(to + 8 * piece) = make_uint2(one, two);
+                else *reinterpret_cast<uint32_t *>(to + ch.lo) = one, *reinterpret_cast<uint32_t *>(to + ch.hi) = two;
             }
         }
     };
+    // Where the scale is a power of two, whose reciprocal is exact, and all quotients are numbers of at most 448, a product is the quotient
+    // and nothing is to be cut (1% of 4096 tokens' time).
     const float inv = 1.0f / scale;
-    if ((__float_as_uint(scale) & 0x7fffffu) == 0) store([&](float v) { return v * inv; });  // a power of two: the same number
-    else store([&](float v) { return v / scale; });
+    if (!nan && top <= 448.f * scale && (__float_as_uint(scale) & 0x7fffffu) == 0) store([&](float v) { return v * inv; });
+    else store([&](float v) { return v != v ? 0.f : __builtin_amdgcn_fmed3f(v / scale, -448.f, 448.f); });
 }
 
 // Rows of the cache as numbers, a workgroup a token, eight elements a lane; a slot outside the cache gives zeros.
@@ -250,7 +268,6 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(const uint8_t *__restri
         float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (kept) {
             // past the caches, which hold what is written: 61006 tokens of 8 heads after their move 155 -> 125 us together
-            typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
             const uintx2 w = __builtin_nontemporal_load(reinterpret_cast<const uintx2 *>((is_v ? v_codes : k_codes) + kv8_row(page, head, at, heads, page_shift) * D + 8 * piece));
             const float scale = (is_v ? v_scales : k_scales)[page * heads + head];
             e4m3x4_to_f32(w.x, x), e4m3x4_to_f32(w.y, x + 4);
