@@ -862,23 +862,25 @@ __device__ __forceinline__ Queries queries_that_see(const AttnArgs8 &a, const Se
     return i0 < i1 ? Queries{static_cast<int>(i0), static_cast<int>(i1)} : Queries{0, 0};
 }
 
-// A workgroup has 64 tokens of a sequence and head, whose keys each wave holds as MFMA operands; its waves take the row tiles of 32 in
-// turn, each through LDS of its own, the next one's queries on their way: no barrier until the end, where the waves' sums are joined.
+// A workgroup has 64 tokens of a sequence and head, whose keys each wave holds as MFMA operands; its one to eight waves take the row tiles of
+// 32 in turn, each through LDS of its own, the next one's queries on their way: no barrier until the end, where the waves' sums are joined.
 // With S^T = K Q^T a lane has one row's 16 of 32 scores: -lse is one number a lane, what turns products into scores one a half of 16
 // tokens, and a score costs an fma, an exponential and an addition.
 // kByHead: a tile is 32 queries of one query head (the last one of a head reaches back over queries that it leaves out), whose rows lie a
 // stride apart; else 32 rows in order, each with a query and a head to be told apart (as many instructions again, but full tiles where
 // a sequence has few queries: below 32 a sequence).
-// 64 queries of 28 heads after 16384 tokens: 21 us of that call's 55; 418 us were a prompt's of 4096 tokens whose rows each lane read itself.
-// Bound by a workgroup's start (keys from table to operands) beside four rounds of tiles; 240 registers leave two workgroups a CU.
+// 64 queries of 28 heads after 16384 tokens: 20 us of that call's 55; a prompt's of 4096 tokens 113, and 418 when each lane read its rows itself.
+// Bound by its vector instructions (an exponential of 16 cycles a score), and by a workgroup's start, from table to operands; 240 registers
+// leave two waves a SIMD.
 // Queries are read by rows, 16 lanes each, and stored for operand c and half h of lanes at row r ^ (2 c + h): in order, all 16 pieces of a
 // row would lie in the same banks.
 template <int D, bool kByHead>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void kv8_attention_weights_kernel(AttnArgs8 a, WeightArgs8 wa) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void kv8_attention_weights_kernel(AttnArgs8 a, WeightArgs8 wa) {
     constexpr int KS = D / 16, W = D / 64, kLanes = D / 8, kPer = 64 / kLanes, kLoads = 32 / kPer;  // lanes a row, rows a load, loads a tile
-    __shared__ __align__(16) uintx4 staged[4][KS][64];
-    __shared__ float sums[4][64];
+    extern __shared__ __align__(16) uint8_t lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    uintx4(*staged)[64] = reinterpret_cast<uintx4(*)[64]>(lds) + wave * KS;
+    const auto sums_of = [&](int w) { return reinterpret_cast<float *>(lds + w * KS * sizeof(*staged)); };  // 64, once its rows are done with
     const int64_t block = wa.first_block + blockIdx.x;
     const int seq = static_cast<int>(block / a.heads / wa.blocks), head = static_cast<int>(block % a.heads);
     // the first tokens are seen by the most rows: they come first, and the last ones beside them (one head after another: a prompt of 4096
@@ -998,7 +1000,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         // channels 8 e ..: of the MFMAs' 32 channels e / 4, half e / 2 % 2, the first or second of two
         const int c_of = piece / 4 * 2 + piece % 2, h_of = piece / 2 % 2;
 #pragma unroll
-        for (int c = 0; c < kLoads; ++c) staged[wave][c_of][32 * h_of + ((kPer * c + of_row) ^ (2 * c_of + h_of))] = next.q[c];
+        for (int c = 0; c < kLoads; ++c) staged[c_of][32 * h_of + ((kPer * c + of_row) ^ (2 * c_of + h_of))] = next.q[c];
         const float minus_lse = next.in ? next.lse * -1.44269504088896341f : -INFINITY;  // rows past the end: no weight
         const int limit = limit_of(a, sq, next.i), low = low_of(a, sq, next.i);
         // uniform: every row of the tile sees every token
@@ -1008,7 +1010,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         wave_order();
         uintx4 q[KS];
 #pragma unroll
-        for (int c = 0; c < KS; ++c) q[c] = staged[wave][c][32 * h + (n ^ (2 * c + h))];
+        for (int c = 0; c < KS; ++c) q[c] = staged[c][32 * h + (n ^ (2 * c + h))];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             floatx16 dot;
@@ -1042,12 +1044,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         });
     });
     const int of = 32 * (n / 16) + 8 * (n / 4 % 4) + 4 * h + n % 4;  // its token
-    sums[wave][of] = sum[0];
+    wave_order();
+    sums_of(wave)[of] = sum[0];
     __syncthreads();
     const int t = t0 + static_cast<int>(threadIdx.x);
     if (threadIdx.x < 64 && t < most && (threadIdx.x < 32 ? threadIdx.x < 16 ? live[0][0] : live[0][1] : threadIdx.x < 48 ? live[1][0] : live[1][1])) {
         float v = 0.f;
-        for (int w = 0; w < waves; ++w) v += sums[w][threadIdx.x];
+        for (int w = 0; w < waves; ++w) v += sums_of(w)[threadIdx.x];
         float *p = wa.weights + (static_cast<int64_t>(seq) * a.heads + head) * wa.cols + t;
         *p += v;
     }
@@ -1273,8 +1276,13 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
         if (weights) {
             const int64_t each = p.scored ? 1024 : 64, blocks = (std::min(weights_cols, table_cols * cache->page_size) + each - 1) / each;
             WeightArgs8 wa{weights, static_cast<int>(weights_cols), static_cast<int>(blocks), 0};
-            // a wave for each tile of 32 rows that a sequence has, up to four
-            const int64_t rows = (tokens * a.ratio + batch - 1) / batch, threads = p.scored || rows > 64 ? 256 : rows > 32 ? 128 : 64;
+            // Waves a workgroup, which share its rows: as many as fill the card once, two a SIMD, for a workgroup's start costs as much as
+            // several tiles of rows.  A call with its weights, us: 64 queries of 32 heads after 4000 tokens, four sequences: one wave 60, two
+            // 63, four 70; of 28 heads after 16384 tokens two 55, one 61, four 57; prompt of 512 tokens eight 31, four 35, two 47.
+            const int64_t rows = (tokens * a.ratio + batch - 1) / batch;
+            int64_t waves = 1;
+            while (waves < 8 && 32 * waves < rows && 2 * waves * blocks * batch * cache->kv_heads <= 8 * cu_count()) waves *= 2;
+            const int64_t threads = p.scored ? 256 : 64 * waves, lds = p.scored ? 0 : waves * 64 * cache->head_dim;
             const int64_t all = blocks * batch * cache->kv_heads, most = most_workgroups(threads);
             for (; wa.first_block < all; wa.first_block += most) {
                 const dim3 grid(static_cast<unsigned>(std::min(all - wa.first_block, most)));
@@ -1282,7 +1290,7 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
                 const auto kern = p.scored ? kv8_attention_scored_kernel
                     : cache->head_dim == 64 ? by_head ? kv8_attention_weights_kernel<64, true> : kv8_attention_weights_kernel<64, false>
                     : by_head ? kv8_attention_weights_kernel<128, true> : kv8_attention_weights_kernel<128, false>;
-                kern<<<grid, dim3(static_cast<unsigned>(threads)), 0, st>>>(a, wa);
+                kern<<<grid, dim3(static_cast<unsigned>(threads)), static_cast<size_t>(lds), st>>>(a, wa);
                 check_launch("kv8_attention_weights");
             }
         }
