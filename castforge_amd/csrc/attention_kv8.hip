@@ -1122,12 +1122,15 @@ Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     p.mt = each <= 96 ? 1 : 2;
     const int64_t len = len_of(16 * p.mt);
     p.tiles = tiles(16 * p.mt);
-    // two workgroups a CU.  A short table and few workgroups: one launch of wide workgroups, four rounds of 32 tokens a wave at most, no partial
-    // sums.  One sequence of 1009 tokens, 8 heads of 128: 11.7 us a call against 15.7 with splits and their join, whose second launch costs the
-    // host more than the longer walk costs the GPU (10.3 against 7.4 us there); 32 sequences of 1000 16.3 against 18.2 there.  At 2000 tokens
-    // one sequence takes 16.1 against 8.0 there.  (Sixteen waves spill: 14.5 for 1009 tokens.)
-    p.wide = p.mt == 1 && p.tiles * c->kv_heads <= cus && len <= 1024;
-    if (!p.wide) p.splits = splits_for((2 * cus + p.tiles * c->kv_heads - 1) / (p.tiles * c->kv_heads), len, 128);
+    // Two workgroups of four waves a CU, or one of eight, which needs no partial sums and no second launch.  The latter for short tables: one
+    // sequence of 1009 tokens, 8 heads of 128, takes 11.7 us a call against 15.7 with splits and their join, whose launch costs the host more
+    // than the longer walk costs the GPU (10.3 against 7.4 us there; of 2000 tokens 16.1 against 8.0; 64 channels 1500 tokens 10.2 against 7.8
+    // there and 11.7 against 14.8 a call; sixteen waves 11.0).  And where it fills half the card with walks that are short or, through a
+    // window, alike: on the GPU 24 sequences of 2000 tokens 20.4 us against 25.3, of 500 to 2000 18.0 against 19.1, 32 through a window of 4096
+    // 55.3 against 58.1.  (Of up to 8000 tokens the longest one is waited for: 24 sequences 59.2 against 56.4.)
+    const int64_t tasks = p.tiles * c->kv_heads;
+    p.wide = p.mt == 1 && tasks <= cus && (len <= (large ? 1024 : 1536) || (2 * tasks > cus && (len <= 2048 || 2 * len <= table_cols * c->page_size)));
+    if (!p.wide) p.splits = splits_for((2 * cus + tasks - 1) / tasks, len, 128);
     if (varlen && each > 16) {
         const double token = p.wide ? (large ? .0065 : .005) : p.mt == 1 ? (large ? .0155 : .0095) : large ? .0115 : .0085;
         const int64_t slots = p.wide ? cus : (p.mt == 1 ? 3 : 2) * cus;
