@@ -774,24 +774,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         tile_weights<D>(s, e, pg, p);
         tile_outputs<D, NW>(s, st, sub, lane, p);
     };
-    Part part;
-    int page = page_at(begin + kSteps);
+    int i = 0;
     if (steps > begin) {
+        Part part;
+        int page = page_at(begin + kSteps);
         load(part, page_at(begin), begin);
         make(part, stages[0]);
-        // the queries have come too: else the compiler waits for them in every stage, and with them for the codes on their way
+        // the queries have come too: else the compiler waits for them in every stage, and with them for the codes on their way (as it would
+        // with the loop behind this branch, not in it)
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         load(part, page, begin + kSteps);
-    }
-    page = page_at(begin + 2 * kSteps);
-    int i = 0;
-    for (int step = begin; step < steps; step += kSteps, i ^= 1) {
-        __syncthreads();  // stage i is made, and the other one no longer read
-        walk_stage(step, i);
-        if (step + kSteps < steps) {
-            make(part, stages[i ^ 1]);
-            load(part, page, step + 2 * kSteps);
-            page = page_at(step + 3 * kSteps);
+        page = page_at(begin + 2 * kSteps);
+        for (int step = begin; step < steps; step += kSteps, i ^= 1) {
+            __syncthreads();  // stage i is made, and the other one no longer read
+            walk_stage(step, i);
+            if (step + kSteps < steps) {
+                make(part, stages[i ^ 1]);
+                load(part, page, step + 2 * kSteps);
+                page = page_at(step + 3 * kSteps);
+            }
         }
     }
     const float l = s.l + __shfl_xor(s.l, 32), inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
