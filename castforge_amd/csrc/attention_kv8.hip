@@ -11,7 +11,7 @@
 //
 // Three kernels and what bounds them (8 heads of keys, 32 of queries, 128 channels): few rows a sequence read the cache at HBM's rate (48
 // single queries over up to 8000 tokens 98 us, 4.8 TB/s; a large copy runs at 5.1); many rows are bound by the sum of MFMAs and vector
-// instructions (prompt of 4096 tokens 143 to 152 us by the box, 0.9 to 0.96 PFLOP/s); the weights that tokens got are the keys' half of
+// instructions (prompt of 4096 tokens 141 to 152 us by the card, 0.9 to 0.97 PFLOP/s); the weights that tokens got are the keys' half of
 // that again, or a pass over scores that the first kernel left.
 #include <algorithm>
 #include <atomic>

@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(EvictArgs8 a
         shift -= step == 0 ? 11 : 10;
     }
     // in order, kRound tokens a lane
-    uint32_t above = 0, equal = 0;  // kept before this round, those of the last rank apart
+    uint32_t above = 0, equal = 0;  // kept before these tokens, those of the last rank apart
     for (int t0 = 0; t0 < len; t0 += kSelectThreads * kRound) {
         if constexpr (kEach == 0) hold(t0);
         uint32_t sure = 0, tie = 0;  // bit masks
