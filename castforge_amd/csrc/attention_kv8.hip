@@ -526,7 +526,16 @@ __global__ __launch_bounds__(256) void kv8_attention_join_kernel(AttnArgs8 a) {
 // Many rows: each wave takes 32 rows of its own, and the eight of a workgroup share the making of the MFMA operands: of every 128
 // tokens a wave turns 32 tokens' half rows of keys and 16 tokens' values into operands in LDS, and all read them back; two stages, one
 // barrier a stage: the operands of the next tokens are made while the present ones are used, and the codes of those after that are on
-// their way.
+// their way.  Eight waves, one workgroup a CU: a prompt of 4096 tokens takes 147 us, by four waves a workgroup, two a CU, which make every
+// operand twice as often, 171.  Each wave for itself (the kernel above) 384.
+// Of the busy cycles MFMAs are 44% and vector instructions 41%, hardly beside each other: 32 x 32 x 16 MFMAs alone, on registers with
+// random numbers, run at 1.5 to 1.65 PFLOP/s here (power), with six fmas each at 1.3, which would be 105 us, and a score costs more than
+// that (an fma, an exponential of 16 cycles, an addition, half a conversion and half a maximum).  The operands' making costs 15 us, the
+// exponentials 7, the reading of keys 9.  16 x 16 x 32 MFMAs: 153 us.  Keys read a step ahead, raised wave priority, other orders of the
+// instructions: no faster.  A workgroup's start (lists, table, first codes, first operands) takes 12000 cycles, a stage 8200: four rounds
+// of workgroups in a prompt of 8192 tokens through a window of 1024 (168 us).  Queries fetched into L2 for the workgroup that follows: no faster.
+// One workgroup a CU that goes through several tiles, the next one's codes on their way under the last one's stores, needs all 256
+// registers, and reads LDS no longer ahead: 177.
 // 32 x 32 x 16 MFMAs: of S^T = K Q^T lane (n = lane % 32, h = lane / 32) holds row n's scores of the tokens 8 j + 4 h + r of 32 (j, r < 4),
 // which is what O^T = V^T P^T takes of 16 tokens (j < 2, then j >= 2) as its second operand.  Row i of a tile of V^T is channel
 // i D / 32 + u.
