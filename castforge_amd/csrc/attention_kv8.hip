@@ -235,14 +235,14 @@ __device__ __forceinline__ void attend(const AttnArgs8 &a, Rows8<D, MT> &s, int 
             }
         }
     }
-    if constexpr (kScored) {  // scores of what a row does not see are not read, but for those of no page: -inf
+    if constexpr (kScored) {  // scores of what a row does not see, and of no page, are not read
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 floatx4 v;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = gone[h] ? -INFINITY : dot[mt][h][r] * pages[h].kf;
+                for (int r = 0; r < 4; ++r) v[r] = dot[mt][h][r] * pages[h].kf;
                 if (score_rows[mt] && at + 16 * h < a.score_cols) *reinterpret_cast<floatx4 *>(score_rows[mt] + at + 16 * h) = v;  // a table may end with a half
             }
     }
@@ -1076,6 +1076,10 @@ __global__ __launch_bounds__(256) void kv8_attention_scored_kernel(AttnArgs8 a, 
     const Seq sq = seq_of(a, seq);
     const int most = min(sq.len, wa.cols), t = 1024 * static_cast<int>(block % wa.blocks) + 4 * static_cast<int>(threadIdx.x), hq = a.heads * a.ratio;
     if (t >= most || sq.n == 0) return;
+    // Tokens of no page are left out as such, not by their scores of -inf: a row that sees no others has -inf as its logarithm too, and their
+    // difference is NaN.  The lane's four lie in one page.
+    const int page = a.table[static_cast<int64_t>(seq) * a.table_cols + (t >> a.page_shift)];
+    if (page < 0 || page >= a.num_pages) return;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     bool seen = false;
     for (int i = 0; i < sq.n; ++i) {
