@@ -117,6 +117,17 @@ def test_windows_over_missing_pages(cuda, q_lens, kv_lens, sinks):
     assert empty[q_lens[0] - 1].all() == (sinks == 0)
 
 
+@pytest.mark.parametrize("q_lens,kv_lens", FORMS)
+def test_what_page_0_holds_is_not_read(cuda, q_lens, kv_lens):
+    missing = [(0, 32, 48), (0, 80, 112), (len(kv_lens) - 1, 0, 16)]
+    case = Case(cuda, q_lens, kv_lens, missing, seed=7)
+    for a, b in zip(case.call(), case.call(case.clean)):
+        assert torch.equal(a, b)
+    case = Case(cuda, q_lens, kv_lens, missing, seed=7, causal=False)
+    for a, b in zip(case.call(), case.call(case.clean)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 @pytest.mark.parametrize("q_lens,kv_lens", FORMS)
 def test_a_query_of_nan_leaves_missing_tokens_alone(cuda, q_lens, kv_lens, value):
