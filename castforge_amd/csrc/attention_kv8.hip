@@ -804,7 +804,26 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             }
         }
     }
-    const float l = s.l + __shfl_xor(s.l, 32), inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
+    float l = s.l + __shfl_xor(s.l, 32);
+    // The zeros that stand for a missing page's keys make NaN with a query of NaN or infinity.  A row that sees missing pages alone gives nothing
+    // all the same; asked here, for such rows only (masked in the loop: 0.6% of a prompt of 128 channels, 3% of one of 64).
+    if (__any(l != l && row < total)) {
+        bool seen = false;
+        for (int step = begin; step < steps; ++step)
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                const int at = span.token_of(step) + 16 * part, page = at < span.end ? scalar_load(table, at >> a.page_shift) : -1;
+                seen |= static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_pages) && at < s.limit && (at + 16 > s.low || at < a.sinks);
+            }
+        if (!seen) {
+            l = 0.f, s.m = kNoMax;
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s.o[u][e] = 0.f;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // 0: no token was seen
     const int to = static_cast<int>(out_row(a, sq, head, row));
     // Rows are stored by D / 8 lanes each, through LDS (stage i is no longer read): by the lanes that hold them each store touches 64 lines
     // (64 queries of 7 heads after 16384 tokens, whose splits leave 30 MB: 60.9 -> 54.2 us).  A lane has D / 8 channels behind one another for

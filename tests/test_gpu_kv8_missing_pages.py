@@ -12,7 +12,8 @@ from test_gpu_kv8_attention import _cache, _reference, _table
 
 pytestmark = pytest.mark.gpu
 
-# queries and lengths that take every form: few rows in one launch and split, with saved scores and without; many rows, split too
+# queries and lengths that take every form: few rows in one launch and split, with saved scores and without; many rows (of eight heads, see
+# Case), by four waves, by eight, and split
 FORMS = [
     ([1, 1, 1], [200, 64, 130]),
     ([1, 1], [9000, 40]),
@@ -24,6 +25,8 @@ FORMS = [
     ([60, 4], [9000, 200]),
     ([900, 700], [1000, 900]),
     ([256], [6000]),
+    ([128] * 8, [200] * 8),
+    ([1000], [4000]),
 ]
 
 
@@ -31,8 +34,9 @@ class Case:
     """Sequences in pages 1 .. of a cache whose page 0 holds NaN, codes and scales; page ids of `missing` ([(sequence, first token,
     end)], whole pages) are outside the cache."""
 
-    def __init__(self, cuda, q_lens, kv_lens, missing, hkv=2, ratio=2, d=128, page=16, seed=0, window=None, sinks=0, causal=True):
+    def __init__(self, cuda, q_lens, kv_lens, missing, d=128, page=16, seed=0, window=None, sinks=0, causal=True):
         self.q_lens, self.kv_lens, self.page = q_lens, kv_lens, page
+        hkv, ratio = (8, 4) if sum(q_lens) > 300 else (2, 2)
         self.args = dict(causal=causal, window=window, sinks=sinks)
         need = [-(-kv // page) for kv in kv_lens]
         tensors = _cache(seed, sum(need) + 1, hkv, page, d, cuda)
@@ -136,3 +140,19 @@ def test_a_query_of_nan_leaves_missing_tokens_alone(cuda, q_lens, kv_lens, value
     q, row = case.q.clone(), q_lens[0] - 1
     q[row, 1] = value
     case.check(case.call(q=q), but=(row, 1))
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("q_lens,kv_lens", FORMS)
+def test_a_query_of_nan_that_sees_nothing_gives_zeros(cuda, q_lens, kv_lens, value):
+    """The padding of a batch holds anything: the last sequence, whose pages are all missing, and the first queries of the first, or those whose
+    window is missing.  Their queries reach nothing: neither their rows nor others'."""
+    b, kv = len(kv_lens) - 1, kv_lens[0]
+    for missing, window in (((0, 0, 48 if b else kv), None), ((0, max(kv - 128, 0) // 16 * 16, kv), 60)):
+        case = Case(cuda, q_lens, kv_lens, [missing, (b, 0, kv_lens[b])] if b else [missing], seed=11, window=window)
+        want, empty = case.check()
+        q = case.q.clone()
+        q[empty] = value
+        for x, y in zip(case.call(q=q), want):
+            assert torch.equal(x, y)
+        assert empty[-q_lens[b] if b or not window else -1:].all()
