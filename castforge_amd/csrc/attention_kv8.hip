@@ -1030,7 +1030,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
         const int c_of = piece / 4 * 2 + piece % 2, h_of = piece / 2 % 2;
 #pragma unroll
         for (int c = 0; c < kLoads; ++c) staged[c_of][32 * h_of + ((kPer * c + of_row) ^ (2 * c_of + h_of))] = next.q[c];
-        const float minus_lse = next.in ? next.lse * -1.44269504088896341f : -INFINITY;  // rows past the end: no weight
+        // no weight for rows past the end, and for those whose scores are all -inf: less their logarithm, which is -inf too, NaN
+        const float minus_lse = next.in && next.lse != -INFINITY ? next.lse * -1.44269504088896341f : -INFINITY;
         const int limit = limit_of(a, sq, next.i), low = low_of(a, sq, next.i);
         // uniform: every row of the tile sees every token
         const bool all = t0 + 64 <= limit_of(a, sq, next.i0) && (t0 >= low_of(a, sq, next.i1) || t0 + 64 <= a.sinks);
@@ -1107,8 +1108,9 @@ __global__ __launch_bounds__(256) void kv8_attention_scored_kernel(AttnArgs8 a, 
         seen = true;
         for (int x = 0; x < a.ratio; ++x) {
             const int64_t row = static_cast<int64_t>(sq.first + i) * hq + head * a.ratio + x;
-            const floatx4 y = *reinterpret_cast<const floatx4 *>(a.scores + row * a.score_cols + t);
             const float lse = a.lse[row] * 1.44269504088896341f;
+            if (lse == -INFINITY) continue;  // all scores are -inf, and their difference is NaN
+            const floatx4 y = *reinterpret_cast<const floatx4 *>(a.scores + row * a.score_cols + t);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 sum[r] += (t + r >= limit) | ((t + r < low) & (t + r >= a.sinks)) ? 0.f : __builtin_amdgcn_exp2f(y[r] - lse);

@@ -1315,7 +1315,8 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, page_table: torch.Tensor, kv
     h reads keys' head h // (q_heads // kv_heads)), page_table int32 [B, pages], kv_lens int32 [B] cached tokens (those of the
     call's own queries included), cu_q int32 [B + 1] each sequence's queries (without it every sequence has one).  causal: query i of
     n, at place p = kv_lens - n + i, sees the tokens up to p; with a window (at least 1; needs causal) only the last `window` of them
-    and the first `sinks` of the sequence.  scale defaults to head_dim ** -0.5.  Queries that see nothing give zeros.
+    and the first `sinks` of the sequence.  Tokens of a page id outside the cache are left out.  scale defaults to head_dim ** -0.5.
+    Queries that see nothing, or whose scores are all -inf, give zeros and no weights.
 
     weights (f32 [B, kv_heads, N], contiguous): the softmax's weights that each cached token got in this call are added to it, summed
     over the queries and over the query heads of a head of keys; tokens past N are left out.  What kv8_evict goes by.

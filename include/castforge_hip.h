@@ -634,8 +634,9 @@ int32_t castforge_hip_kv8_gather(const cfh_kv8_cache_t *cache, const int64_t *sl
  * window (0: none; needs causal): a query at place p = kv_lens[b] - n + i sees the tokens p - window < t <= p and, of those before,
  * the first `sinks` of the sequence.  Tokens that no query of a call sees are not read.
  * weights (optional, f32 [batch, kv_heads, weights_cols]; needs lse): weights[b, h, t] += the softmax's weights that token t got,
- * summed over the call's queries and the query heads of head h.  Each element has one writer; those of tokens that nobody sees, and
- * tokens past weights_cols, are left alone. */
+ * summed over the call's queries and the query heads of head h.  Each element has one writer; those of tokens that nobody sees, of
+ * pages outside the cache, and tokens past weights_cols, are left alone.
+ * A query whose scores are all -inf (they are f32) counts as one that sees nothing. */
 int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t *q, int64_t q_stride, int64_t tokens,
                                     int64_t q_heads, int64_t batch, const int32_t *cu_q, const int32_t *page_table,
                                     int64_t table_cols, const int32_t *kv_lens, int32_t causal, int64_t window, int64_t sinks,

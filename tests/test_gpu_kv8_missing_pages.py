@@ -156,3 +156,23 @@ def test_a_query_of_nan_that_sees_nothing_gives_zeros(cuda, q_lens, kv_lens, val
         for x, y in zip(case.call(q=q), want):
             assert torch.equal(x, y)
         assert empty[-q_lens[b] if b or not window else -1:].all()
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", FORMS)
+def test_queries_whose_scores_are_all_minus_infinity(cuda, q_lens, kv_lens):
+    """-inf times positive keys: as if they saw nothing, for the weights too."""
+    case = Case(cuda, q_lens, kv_lens, [], seed=13)
+    k = case.cache.k_codes
+    k.copy_((k & 0x7F).clamp(1, 0x7E))
+    want = case.call()
+    q, n = case.q.clone(), q_lens[0]
+    q[:n] = -math.inf
+    out, lse, weights = case.call(q=q)
+    assert torch.all(out[:n] == 0) and torch.all(lse[:n] == -math.inf) and torch.equal(weights[0], case.before[0])
+    assert torch.equal(out[n:], want[0][n:]) and torch.equal(lse[n:], want[1][n:]) and torch.equal(weights[1:], want[2][1:])
+    q = case.q.clone()
+    q[n - 1] = -math.inf  # beside others
+    out, lse, weights = case.call(q=q)
+    assert torch.all(out[n - 1] == 0) and torch.all(lse[n - 1] == -math.inf) and torch.isfinite(out).all() and torch.isfinite(weights).all()
+    if n == 1:
+        assert torch.equal(weights[0], case.before[0])
