@@ -1153,7 +1153,7 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, kv
     qs = cache._rows(q, None, "q")
     t, hq, d = shape = q.shape
     heads, dev = cache.kv_heads, cache._dev
-    if hq % heads:
+    if heads < 1 or hq % heads:
         raise ValueError("q_heads must be a multiple of the cache's heads")
     if not (page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous() and page_table.get_device() == dev):
         _refuse(q, {"page_table": page_table}, "page_table must be int32 [sequences, pages]")
@@ -1326,7 +1326,7 @@ def kv8_attention(q: torch.Tensor, cache: Kv8Cache, page_table: torch.Tensor, kv
     qs = cache._rows(q, None, "q")
     t, hq, d = shape = q.shape
     heads, dev = cache.kv_heads, cache._dev
-    if hq % heads:
+    if heads < 1 or hq % heads:
         raise ValueError("q_heads must be a multiple of the cache's heads")
     b, cols, lp, cp = cache._batch(page_table, kv_lens, cu_q, t, "q")
     if window is None:
