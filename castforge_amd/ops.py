@@ -1218,16 +1218,16 @@ class Kv8Cache(_PagedCache):
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales))
 
-    def _batch(self, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None, rows: int, what: str
+    def _batch(self, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor | None, rows: int | None, what: str
                ) -> tuple[int, int, int, int | None]:
-        """Checks a batch's lists, `rows` rows of `what` in all: (sequences, table's columns, addresses of kv_lens and cu_q)."""
+        """Checks a batch's lists, `rows` rows of `what` in all (None: no rows): (sequences, table's columns, addresses of kv_lens and cu_q)."""
         if not (page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous() and page_table.get_device() == self._dev):
             _refuse(self.k_codes, {"page_table": page_table}, "page_table must be int32 [sequences, pages]")
         b, cols = page_table.shape
         lp, cp = self._vector(kv_lens, torch.int32, b, "kv_lens"), None
         if cu_q is not None:
             cp = self._vector(cu_q, torch.int32, b + 1, "cu_q")
-        elif rows != b:
+        elif rows is not None and rows != b:
             raise ValueError(f"without cu_q every sequence has one row: {what} and page_table must have the same rows")
         return b, cols, lp, cp
 
@@ -1360,7 +1360,7 @@ def kv8_evict(cache: Kv8Cache, page_table: torch.Tensor, kv_lens: torch.Tensor, 
     [B, kv_heads, keep], the kept tokens' weights, 0 past the last).  Keys keep their rotation: positions of later tokens go on from the old
     length, places (and windows) from the new one."""
     heads, dev = cache.kv_heads, cache._dev
-    b, cols, lp, _ = cache._batch(page_table, kv_lens, None, page_table.shape[0], "kv_lens")
+    b, cols, lp, _ = cache._batch(page_table, kv_lens, None, None, "")
     if not (weights.dim() == 3 and weights.shape[:2] == (b, heads) and weights.dtype == torch.float32 and weights.is_contiguous()
             and weights.get_device() == dev and new_table.dim() == 2 and new_table.shape[0] == b and new_table.dtype == torch.int32
             and new_table.is_contiguous() and new_table.get_device() == dev):

@@ -66,3 +66,9 @@ def test_caches_of_no_heads_are_refused(cuda):
     for call, cache in ((ops.kv8_attention, ops.Kv8Cache.empty(1, 0, 16, 64, device=cuda)), (ops.kv4_attention, ops.Kv4Cache.empty(1, 0, 16, 64, 32, device=cuda))):
         with pytest.raises(ValueError, match="heads"):
             call(q, cache, table, lens)
+
+
+def test_a_table_of_no_dimensions_is_refused(cuda):
+    cache, i32 = ops.Kv8Cache.empty(1, 1, 16, 64, device=cuda), dict(dtype=torch.int32, device=cuda)
+    with pytest.raises(ValueError, match="page_table"):
+        ops.kv8_evict(cache, torch.tensor(0, **i32), torch.ones(1, **i32), torch.ones((1, 1, 16), device=cuda), 4, torch.zeros((1, 1), **i32))
