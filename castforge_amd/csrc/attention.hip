@@ -423,6 +423,32 @@ __device__ __forceinline__ int seen_by_all(const Rows<D, G, MT> &s, int len) {
     return __builtin_amdgcn_readfirstlane(sure);
 }
 
+// The zeros that stand for a missing page's tokens make NaN with a query of NaN or infinity.  A row that sees missing pages alone, of the
+// tokens first, first + step, .. (of 32) below end that the wave had, gives nothing all the same; asked for such rows only.
+template <int D, int G, int MT>
+__device__ __forceinline__ void drop_unseeing(const AttnArgs &a, Rows<D, G, MT> &s, const int32_t *table, int first, int step, int end) {
+    bool nan = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) nan |= s.l[mt] != s.l[mt];
+    if (!__any(nan)) return;
+    bool seen[MT] = {};
+    for (int at = first; at < end; at += step)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int t = at + 16 * h, page = t < end ? scalar_load(table, t >> a.page_shift) : -1;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) seen[mt] |= page >= 0 && page < a.num_pages && t < s.limit[mt];
+        }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+        if (!seen[mt]) {
+            s.m[mt] = kNoMax, s.l[mt] = 0.f;
+#pragma unroll
+            for (int gr = 0; gr < Rows<D, G, MT>::GR; ++gr)
+#pragma unroll
+                for (int u = 0; u < Rows<D, G, MT>::NT; ++u) s.o[mt][gr][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+}
 
 // A wave's walk over tokens first, first + step, .. (of 32) below end, the next tile's loads in flight.
 template <int D, int G, int MT>
@@ -480,6 +506,7 @@ __device__ __forceinline__ void walk(const AttnArgs &a, Tokens<D / G, 32> &token
             });
         cur = next;
     }
+    drop_unseeing<D, G, MT>(a, s, table, first, step, end);
 }
 
 // Channel of element (r of a lane's four, group gr, tile u) of O^T.
@@ -769,6 +796,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 3)))
                 [&](int gr) { return [&st, gr, sub, lane](int u) { return __builtin_bit_cast(halfx8, st.values[sub][gr * NT + u][lane]); }; });
         }
     }
+    drop_unseeing<D, G, MT>(a, s, table, 0, 32, mine);
     settle<true>(s);
     __syncthreads();  // the stages' LDS now holds outputs, each wave's own part
     if (row0 >= total) return;
