@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import test_gpu_kv8 as append
 import test_gpu_kv8_attention as attention
 from castforge_amd import ffi, ops
 from test_gpu_kv8_missing_pages import FORMS, Case
@@ -72,3 +73,37 @@ def test_a_table_of_no_dimensions_is_refused(cuda):
     cache, i32 = ops.Kv8Cache.empty(1, 1, 16, 64, device=cuda), dict(dtype=torch.int32, device=cuda)
     with pytest.raises(ValueError, match="page_table"):
         ops.kv8_evict(cache, torch.tensor(0, **i32), torch.ones(1, **i32), torch.ones((1, 1, 16), device=cuda), 4, torch.zeros((1, 1), **i32))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_queries_of_nan_and_infinity_are_rotated_as_others(cuda, interleaved):
+    """NaN wherever f32 gives it (whatever its bits), every other number bit for bit, where the cache holds what it holds without queries."""
+    g = torch.Generator().manual_seed(1)
+    rows = torch.randn((40, 7, 128), generator=g)
+    at = torch.rand(rows.shape, generator=g)
+    for i, value in enumerate((float("nan"), float("inf"), -float("inf"), 3e38, 1e-38, -0.0)):
+        rows[:, :5][(at[:, :5] > 0.03 * i) & (at[:, :5] < 0.03 * i + 0.01)] = value
+    rows = rows.bfloat16()
+    angle = torch.arange(50)[:, None] * 10000.0 ** (-torch.arange(64) / 64)
+    i32, dev = dict(dtype=torch.int32, device=cuda), rows.to(cuda)
+    caches, lists = [ops.Kv8Cache.empty(3, 1, 16, 128, device=cuda) for _ in range(2)], (torch.tensor([[2, 0, 1]], **i32), torch.tensor([40], **i32))
+    turn = dict(cu_q=torch.tensor([0, 40], **i32), positions=torch.arange(40, device=cuda), cos=angle.cos().to(cuda), sin=angle.sin().to(cuda), interleaved=interleaved)
+    got = ops.kv8_append(caches[0], dev[:, 5:6], dev[:, 6:], *lists, q=dev[:, :5], **turn).cpu()
+    assert ops.kv8_append(caches[1], dev[:, 5:6], dev[:, 6:], *lists, **turn) is None
+    want = append._rotate(rows[:, :5].float(), angle.cos()[:40], angle.sin()[:40], 128, interleaved).bfloat16()
+    nan = torch.isnan(want)
+    assert nan.any() and torch.equal(torch.isnan(got), nan)
+    assert torch.equal(got.view(torch.int16)[~nan], want.view(torch.int16)[~nan])
+    for name in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        assert torch.equal(getattr(caches[0], name), getattr(caches[1], name))
+
+
+@pytest.mark.parametrize("extra", [60, 250, 2040])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [1009]), ([1] * 24, [500] * 24), ([1, 1], [0, 1]), ([5, 2], [300, 9]), ([512], [512]), ([900, 3], [1600, 3])])
+def test_tables_wider_than_the_lengths(cuda, monkeypatch, q_lens, kv_lens, extra):
+    """Which form a call takes goes by the table's width; what it gives, by the lengths."""
+    def case(cuda):
+        attention._run(cuda, q_lens, kv_lens, 8, 4, 128, 64, seed=extra, extra_cols=extra)
+        attention._run(cuda, q_lens, kv_lens, 2, 3, 64, 64, seed=extra, extra_cols=extra, window=100, sinks=4)
+
+    test_weights_are_numbers(cuda, monkeypatch, case)
