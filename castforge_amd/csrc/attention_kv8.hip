@@ -1087,9 +1087,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
 }
 
 // The same where the kernel of few rows has left its scores (base 2), [rows][score_cols] from the first row of the sequence and head on:
-// four tokens a lane.  Up to eight rows a sequence and head, where the scores' 4 bytes a row and token are read back in less time than the
+// four tokens a lane.  Up to eight rows a sequence and head on average, where the scores' 4 bytes a row and token are read back in less time than the
 // keys are multiplied again (32 sequences of up to 8000 tokens, 4 query heads a head of keys: 104 us in all against 140; more rows have
-// more scores than keys), and up to 256 MB of them.
+// more scores than keys), and up to 256 MB of them, by the table's width (behind one of 131072 tokens those sequences take 122 us, not 99).
 __global__ __launch_bounds__(256) void kv8_attention_scored_kernel(AttnArgs8 a, WeightArgs8 wa) {
     const int64_t block = wa.first_block + blockIdx.x;
     const int seq = static_cast<int>(block / wa.blocks / a.heads), head = static_cast<int>(block / wa.blocks % a.heads);
@@ -1144,10 +1144,14 @@ Plan plan_of(const cfh_kv8_cache_t *c, int64_t tokens, int64_t q_heads, int64_t 
     const auto splits_for = [&](int64_t splits, int64_t len, int64_t least) { return std::max<int64_t>(1, std::min({splits, len / least, most_splits})); };
     // Several queries a sequence: the form and its splits by their cost in us.  A workgroup takes `start`, and `token` for each token that its
     // rows see, of which causal rows see fewer; `slots` of them run at once; splits cost a launch, and the writing and reading of their
-    // sums at 4 TB/s.  The numbers are fits to 65 shapes a head size (1 to 64 sequences of 16 to 2400 queries after 0 to 16000 tokens, in
-    // every form): over them the choice takes 2 to 3% longer than the best form does, 24% at most.  (128 channels, us, tile kernel and split kernel: prompt of
-    // 512 tokens 22 and 14, of 1600 52 and 57, of 2400 77 and 100; 16 prompts of 100 tokens 14 and 27; 64 queries of 32 heads after 4000
-    // tokens 31 and 23, 128 after 16000 54 and 63, 512 after 16000 147 and 186.  By rows a sequence alone: up to 1.9 times the better one's.)
+    // sums at 4 TB/s.  The numbers are fits to 69 shapes a head size (1 to 64 sequences of 16 to 2400 queries after 0 to 16000 tokens, in
+    // every form): over them the choice takes 3% (128 channels) and 1% (64) longer than the best form does, 24% at most.  (128 channels, us, tile
+    // kernel and split kernel: prompt of 512 tokens 22 and 14, of 1600 52 and 57, of 2400 77 and 100; 16 prompts of 100 tokens 14 and 27; 64 queries
+    // of 32 heads after 4000 tokens 31 and 23, 128 after 16000 54 and 63, 512 after 16000 147 and 186.  By rows a sequence alone: up to 1.9 times
+    // the better one's.)
+    // The host does not know the lengths: the table's width stands for them, here and below, and those shapes' tables were as wide as their
+    // lengths.  Behind one of 16384 tokens a prompt of 512 takes 28 us (14), of 1600 77 (52); behind one of 131072 64 queries after 4000 tokens
+    // 29 (21), and a call of one query over 1009, which loses the one launch below, 13.8 (10.5).
     const auto cost = [&](double token, double start, int64_t slots, int64_t tasks, int64_t splits, int64_t len) {
         const double seen = std::min(len, std::max(table_cols * c->page_size - tokens / batch / 2, int64_t{1})), rounds = static_cast<double>((tasks * splits + slots - 1) / slots);
         return std::max(len * token / splits + start, rounds * (seen * token / splits + start)) + (splits > 1 ? 5 + 2e-6 * tokens * q_heads * splits * row / 4 : 0);
@@ -1306,7 +1310,7 @@ int32_t castforge_hip_kv8_attention(const cfh_kv8_cache_t *cache, const uint16_t
             constexpr int D = decltype(d)::value;
             if (p.rows) p.waves == 8 ? launch_tile<D, 8>(a, p, st) : launch_tile<D, 4>(a, p, st);
             else if (p.wide) p.scored ? launch_split<true, D, 1, 8>(a, p, st) : launch_split<false, D, 1, 8>(a, p, st);
-            else if (p.scored) launch_split<true, D, 1, 4>(a, p, st);  // 8 rows a sequence and head: one row tile
+            else if (p.scored) launch_split<true, D, 1, 4>(a, p, st);  // 8 rows a sequence and head on average: tiles of 16
             else p.mt == 1 ? launch_split<false, D, 1, 4>(a, p, st) : launch_split<false, D, 2, 4>(a, p, st);
             if (p.splits > 1) launch_join<D>(a, st);
         };
